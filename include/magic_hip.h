@@ -567,6 +567,87 @@ int magic_knn_merge(int64_t n_query, int32_t k, int32_t n_parts,
                     const double *part_dist /* [n_parts,Q,k] */, const int64_t *part_idx,
                     double *dist, int64_t *idx, void *stream);
 
+/* ------------------------------------------------------------------------------------
+ * Attention of every node over all nodes of its own component graph (no counterpart in the
+ * reference, whose GATConv attends along edges): softmax attention inside segments.  Rows of q
+ * and of k / v are cut into segments (the component graphs of a batch); row i of a segment
+ * attends the unmasked keys of the same segment:
+ *   s = scale <q_i, k_j>;  c = cap > 0 ? cap tanh(s / cap) : s;
+ *   l = c - slopes[h] |q_pos[i] - k_pos[j]|   (slopes != NULL);   p = softmax_j(l);   o_i = sum_j p v_j
+ * q [n_q, q_heads, head_dim], k and v [n_k, kv_heads, head_dim]; query head h reads key head
+ * h / (q_heads / kv_heads).  Row strides ld_*, head strides hs_*, unit stride along head_dim
+ * (head_dim % 8 == 0, at most MAGIC_ATTN_MAX_DIM).  dtype: MAGIC_F32 (products fp32-grade) or
+ * MAGIC_BF16 (products of bf16 values, probabilities and score gradients rounded to bf16 before
+ * their products; every sum and statistic in fp32).  key_mask [n_k]: 0 = the key takes no part
+ * (whatever its rows hold).  A row that sees no key gets o = 0, lse = -inf and zero gradients.
+ * The work comes as two device tables of the segments' tiles, four int32 each:
+ *   q_tiles: {first q row, rows (1..MAGIC_ATTN_TILE), first key row of the segment, its keys}
+ *   k_tiles: {first key row, keys (1..MAGIC_ATTN_TILE), first q row of the segment, its rows}
+ * that cover every row of q (k) exactly once.
+ * lse [q_heads, n_q] (natural logarithm) is what _bwd needs beside out.  dq [n_q,q_heads,D],
+ * dk, dv [n_k,kv_heads,D] contiguous in the operands' type; d_slopes [q_heads] or NULL.  dq may be NULL when it (and
+ * d_slopes) is not wanted, dk and dv together likewise.
+ * Fixed summation order.
+ * ---------------------------------------------------------------------------------- */
+#define MAGIC_F32 0
+#define MAGIC_BF16 1
+#define MAGIC_ATTN_MAX_DIM 128
+#define MAGIC_ATTN_TILE 128
+typedef struct magic_attn {
+    int32_t dtype, q_heads, kv_heads, head_dim;
+    int64_t n_q, n_k;
+    const void *q;  int64_t ld_q, hs_q;
+    const void *k;  int64_t ld_k, hs_k;
+    const void *v;  int64_t ld_v, hs_v;
+    float scale, cap;
+    const float *slopes;               /* [q_heads] or NULL */
+    const int32_t *q_pos, *k_pos;      /* [n_q], [n_k]; needed with slopes */
+    const uint8_t *key_mask;           /* [n_k] or NULL */
+    const int32_t *q_tiles, *k_tiles;
+    int32_t n_q_tiles, n_k_tiles;
+} magic_attn;
+size_t magic_attn_fwd_workspace_bytes(const magic_attn *args /* host */);
+int magic_attn_fwd(const magic_attn *args /* host struct of device pointers */, void *out, int64_t ld_out, int64_t hs_out,
+                   float *lse, void *workspace, size_t workspace_bytes, void *stream);
+size_t magic_attn_bwd_workspace_bytes(const magic_attn *args);
+int magic_attn_bwd(const magic_attn *args, const void *out, int64_t ld_out, int64_t hs_out, const float *lse,
+                   const void *d_out, int64_t ld_do, int64_t hs_do, void *dq, void *dk, void *dv, float *d_slopes,
+                   void *workspace, size_t workspace_bytes, void *stream);
+
+/* RMS norm of every head of q and k with the position rotation in the same pass:
+ *   u = x rsqrt(mean(x^2) + eps) w;  columns (i, i + R/2), i < R/2, turned by pos * base^(-2i/R); R = rotary_dim
+ * (even, 0 = norm only), columns from R on are left as normed.  wq, wk [head_dim] float32; yq, yk contiguous, type of
+ * the operands.  _bwd: dq, dk contiguous, dwq, dwk [head_dim] float32. */
+int magic_head_norm_rope_fwd(int64_t n_rows, int32_t q_heads, int32_t kv_heads, int32_t head_dim, int32_t rotary_dim,
+                             int32_t dtype, const void *q, int64_t ld_q, int64_t hs_q, const void *k, int64_t ld_k,
+                             int64_t hs_k, const float *wq, const float *wk, const int32_t *pos, double eps, double base,
+                             void *yq, void *yk, void *stream);
+size_t magic_head_norm_rope_bwd_workspace_bytes(int64_t n_rows, int32_t head_dim);
+int magic_head_norm_rope_bwd(int64_t n_rows, int32_t q_heads, int32_t kv_heads, int32_t head_dim, int32_t rotary_dim,
+                             int32_t dtype, const void *q, int64_t ld_q, int64_t hs_q, const void *k, int64_t ld_k,
+                             int64_t hs_k, const float *wq, const float *wk, const int32_t *pos, double eps, double base,
+                             const void *dyq, int64_t ld_dyq, int64_t hs_dyq, const void *dyk, int64_t ld_dyk,
+                             int64_t hs_dyk, void *dq, void *dk, float *dwq, float *dwk, void *workspace,
+                             size_t workspace_bytes, void *stream);
+
+/* ------------------------------------------------------------------------------------
+ * Activations kept for the backward pass in 8 bits: blocks of 32 columns of a row share a
+ * power-of-two scale, x ~ code 2^(exp - 127), |code| <= 127, rounded to nearest even.  exp is
+ * the smallest (>= 1) for which no code of the block exceeds 127; 255 marks a block that held
+ * an infinity or a NaN and reads back as NaN.  codes [n_rows, magic_act8_code_stride(n_cols)]
+ * (columns behind n_cols are zero; 16-byte aligned), exps [n_rows, ceil(n_cols / 32)].
+ * magic_act8_weight_grad: dW[m,f] = dY[n,m]^T . Xhat[n,f] read from the codes (fp32-grade
+ * products, fixed summation order).
+ * ---------------------------------------------------------------------------------- */
+int64_t magic_act8_code_stride(int32_t n_cols);
+int magic_act8_pack(int64_t n_rows, int32_t n_cols, const float *x, int64_t ld_x, int8_t *codes, uint8_t *exps,
+                    void *stream);
+int magic_act8_unpack(int64_t n_rows, int32_t n_cols, const int8_t *codes, const uint8_t *exps, float *x, int64_t ld_x,
+                      void *stream);
+size_t magic_act8_weight_grad_workspace_bytes(int64_t n_rows, int32_t m, int32_t f);
+int magic_act8_weight_grad(int64_t n_rows, int32_t m, int32_t f, const float *dy, int64_t ld_dy, const int8_t *codes,
+                           const uint8_t *exps, float *dw, void *workspace, size_t workspace_bytes, void *stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -33,6 +33,15 @@ class MagicCodedInput(C.Structure):
                 ("scale", c_f32)]
 
 
+class MagicAttn(C.Structure):
+    """``magic_attn`` of include/magic_hip.h."""
+    _fields_ = [("dtype", c_i32), ("q_heads", c_i32), ("kv_heads", c_i32), ("head_dim", c_i32), ("n_q", c_i64),
+                ("n_k", c_i64), ("q", c_vp), ("ld_q", c_i64), ("hs_q", c_i64), ("k", c_vp), ("ld_k", c_i64),
+                ("hs_k", c_i64), ("v", c_vp), ("ld_v", c_i64), ("hs_v", c_i64), ("scale", c_f32), ("cap", c_f32),
+                ("slopes", c_vp), ("q_pos", c_vp), ("k_pos", c_vp), ("key_mask", c_vp), ("q_tiles", c_vp),
+                ("k_tiles", c_vp), ("n_q_tiles", c_i32), ("n_k_tiles", c_i32)]
+
+
 # name -> (restype, argtypes); must list every symbol include/magic_hip.h declares
 SYMBOLS = {
     "magic_abi_version": (c_i32, []),
@@ -104,6 +113,21 @@ SYMBOLS = {
                                          c_vp, c_vp, c_vp, c_vp]),
     "magic_readout_workspace_bytes": (c_sz, [c_i64, c_i32, c_i32]),
     "magic_readout": (c_i32, [c_i64, c_i32, c_vp, c_i64, c_vp, c_i32, c_i32, c_vp, c_vp, c_sz, c_vp]),
+    "magic_attn_fwd_workspace_bytes": (c_sz, [C.POINTER(MagicAttn)]),
+    "magic_attn_fwd": (c_i32, [C.POINTER(MagicAttn), c_vp, c_i64, c_i64, c_vp, c_vp, c_sz, c_vp]),
+    "magic_attn_bwd_workspace_bytes": (c_sz, [C.POINTER(MagicAttn)]),
+    "magic_attn_bwd": (c_i32, [C.POINTER(MagicAttn), c_vp, c_i64, c_i64, c_vp, c_vp, c_i64, c_i64, c_vp, c_vp, c_vp,
+                               c_vp, c_vp, c_sz, c_vp]),
+    "magic_head_norm_rope_fwd": (c_i32, [c_i64] + [c_i32] * 5 + [c_vp, c_i64, c_i64] * 2 + [c_vp, c_vp, c_vp, C.c_double,
+                                         C.c_double, c_vp, c_vp, c_vp]),
+    "magic_head_norm_rope_bwd_workspace_bytes": (c_sz, [c_i64, c_i32]),
+    "magic_head_norm_rope_bwd": (c_i32, [c_i64] + [c_i32] * 5 + [c_vp, c_i64, c_i64] * 2 + [c_vp, c_vp, c_vp, C.c_double,
+                                         C.c_double] + [c_vp, c_i64, c_i64] * 2 + [c_vp] * 5 + [c_sz, c_vp]),
+    "magic_act8_code_stride": (c_i64, [c_i32]),
+    "magic_act8_pack": (c_i32, [c_i64, c_i32, c_vp, c_i64, c_vp, c_vp, c_vp]),
+    "magic_act8_unpack": (c_i32, [c_i64, c_i32, c_vp, c_vp, c_vp, c_i64, c_vp]),
+    "magic_act8_weight_grad_workspace_bytes": (c_sz, [c_i64, c_i32, c_i32]),
+    "magic_act8_weight_grad": (c_i32, [c_i64, c_i32, c_i32, c_vp, c_i64, c_vp, c_vp, c_vp, c_vp, c_sz, c_vp]),
     "magic_knn_workspace_bytes": (c_sz, [c_i64, c_i64, c_i32, c_i32]),
     "magic_knn_topk": (c_i32, [c_i64, c_i64, c_i32, c_i32, c_vp, c_i64, c_vp, c_i64, c_i64, c_vp, c_vp,
                                c_vp, c_sz, c_vp]),
@@ -901,3 +925,268 @@ def knn_merge(part_dist: torch.Tensor, part_idx: torch.Tensor):
                                _dev(part_idx, torch.int64, "part_idx"), _dev(dist), _dev(idx), _stream()),
            "magic_knn_merge")
     return dist, idx
+
+
+# ------------------------------------------------------------------------------------- segment attention
+# These operators take their scratch from torch's allocator at every call (not from ``workspace``): calls on several
+# streams, and captured graphs, never share it.
+ATTN_MAX_DIM, ATTN_TILE = 128, 128
+_ATTN_DTYPE = {torch.float32: 0, torch.bfloat16: 1}
+
+
+class _on_device:
+    """Makes ``device`` the current one for a launch when it is not already."""
+
+    def __init__(self, device):
+        self.dev = device.index
+        self.prev = None
+
+    def __enter__(self):
+        cur = torch.cuda.current_device()
+        if self.dev is not None and self.dev != cur:
+            self.prev = cur
+            torch.cuda.set_device(self.dev)
+
+    def __exit__(self, *exc):
+        if self.prev is not None:
+            torch.cuda.set_device(self.prev)
+
+
+def _scratch(nbytes: int, device) -> torch.Tensor:
+    return torch.empty(int(nbytes), dtype=torch.uint8, device=device)
+
+
+def _head_rows(t: torch.Tensor) -> torch.Tensor:
+    """[rows, heads, head_dim] operand with unit inner stride, other strides and address in whole 16 bytes."""
+    per = 16 // t.element_size()
+    if t.stride(2) == 1 and t.stride(0) % per == 0 and t.stride(1) % per == 0 and t.data_ptr() % 16 == 0:
+        return t
+    t = t.contiguous()
+    return t if t.data_ptr() % 16 == 0 else t.clone()
+
+
+def _heads_check(t: torch.Tensor, name: str, like: Optional[torch.Tensor] = None):
+    if not isinstance(t, torch.Tensor) or t.dim() != 3:
+        raise MagicHipError(f"{name} must be a [rows, heads, head_dim] tensor")
+    if t.device.type != "cuda":
+        raise MagicHipError(f"{name} must live on the GPU (got {t.device}); there is no CPU fallback")
+    if t.dtype not in _ATTN_DTYPE:
+        raise MagicHipError(f"{name} must be float32 or bfloat16 (got {t.dtype})")
+    if like is not None and (t.dtype != like.dtype or t.device != like.device):
+        raise MagicHipError(f"{name} must have the type and device of the other operands ({like.dtype}, {like.device}), "
+                            f"got {t.dtype}, {t.device}")
+
+
+def _vec_check(t: Optional[torch.Tensor], name: str, n: int, dtypes, device):
+    if t is None:
+        return
+    if t.dim() != 1 or t.numel() != n or t.dtype not in dtypes or t.device != device:
+        raise MagicHipError(f"{name} must be a tensor of {n} elements of {' / '.join(map(str, dtypes))} on {device}, got "
+                            f"{tuple(t.shape)} {t.dtype} on {t.device}")
+
+
+def attn_check(q, k, v, n_q, n_k, plan_device, cap, slopes, q_pos, k_pos, key_mask):
+    """Argument checks of ``attn_fwd``: types, shapes, devices (host only)."""
+    _heads_check(q, "q")
+    _heads_check(k, "k", q)
+    _heads_check(v, "v", q)
+    if k.shape != v.shape or k.shape[2] != q.shape[2]:
+        raise MagicHipError(f"k and v must agree, and have q's head_dim: {tuple(q.shape)}, {tuple(k.shape)}, {tuple(v.shape)}")
+    hq, hk, d = q.shape[1], k.shape[1], q.shape[2]
+    if hk < 1 or hq < 1 or hq % hk:
+        raise MagicHipError(f"the query heads ({hq}) must be a multiple of the key heads ({hk})")
+    if d < 8 or d % 8 or d > ATTN_MAX_DIM:
+        raise MagicHipError(f"head_dim must be a multiple of 8 up to {ATTN_MAX_DIM} (got {d})")
+    if q.shape[0] != n_q or k.shape[0] != n_k:
+        raise MagicHipError(f"the plan is for {n_q} query and {n_k} key rows, got {q.shape[0]} and {k.shape[0]}")
+    if plan_device != q.device:
+        raise MagicHipError(f"the plan lives on {plan_device}, the operands on {q.device}")
+    if not cap >= 0.0 or cap == float("inf"):
+        raise MagicHipError(f"cap must be finite and >= 0, 0 for none (got {cap})")
+    _vec_check(slopes, "slopes", hq, (torch.float32,), q.device)
+    if slopes is not None and (q_pos is None or k_pos is None):
+        raise MagicHipError("slopes need q_pos and k_pos")
+    _vec_check(q_pos, "q_pos", n_q, (torch.int32,), q.device)
+    _vec_check(k_pos, "k_pos", n_k, (torch.int32,), q.device)
+    _vec_check(key_mask, "key_mask", n_k, (torch.bool, torch.uint8), q.device)
+
+
+def _attn_args(q, k, v, plan, scale, cap, slopes, q_pos, k_pos, key_mask) -> MagicAttn:
+    a = MagicAttn()
+    a.dtype, a.q_heads, a.kv_heads, a.head_dim = _ATTN_DTYPE[q.dtype], q.shape[1], k.shape[1], q.shape[2]
+    a.n_q, a.n_k = q.shape[0], k.shape[0]
+    a.q, a.ld_q, a.hs_q = q.data_ptr(), q.stride(0), q.stride(1)
+    a.k, a.ld_k, a.hs_k = k.data_ptr(), k.stride(0), k.stride(1)
+    a.v, a.ld_v, a.hs_v = v.data_ptr(), v.stride(0), v.stride(1)
+    a.scale, a.cap = float(scale), float(cap)
+    if slopes is not None:
+        a.slopes, a.q_pos, a.k_pos = slopes.data_ptr(), q_pos.data_ptr(), k_pos.data_ptr()
+    if key_mask is not None:
+        a.key_mask = key_mask.data_ptr()
+    a.q_tiles, a.n_q_tiles = plan.q_tiles.data_ptr(), plan.q_tiles.shape[0]
+    a.k_tiles, a.n_k_tiles = plan.k_tiles.data_ptr(), plan.k_tiles.shape[0]
+    return a
+
+
+def attn_operands(q, k, v, slopes, q_pos, k_pos, key_mask):
+    """The operands as the kernels read them (copies only where strides or addresses ask for one)."""
+    c = lambda t: None if t is None else t.contiguous()  # noqa: E731
+    return _head_rows(q), _head_rows(k), _head_rows(v), c(slopes), c(q_pos), c(k_pos), c(key_mask)
+
+
+def attn_fwd(q, k, v, plan, scale: float, cap: float = 0.0, slopes=None, q_pos=None, k_pos=None, key_mask=None):
+    """Segment attention forward: (out [n_q, q_heads, head_dim], lse [q_heads, n_q] float32)."""
+    lib = load()
+    attn_check(q, k, v, plan.n_q, plan.n_k, plan.device, cap, slopes, q_pos, k_pos, key_mask)
+    q, k, v, slopes, q_pos, k_pos, key_mask = attn_operands(q, k, v, slopes, q_pos, k_pos, key_mask)
+    out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+    lse = torch.empty(q.shape[1], q.shape[0], dtype=torch.float32, device=q.device)
+    a = _attn_args(q, k, v, plan, scale, cap, slopes, q_pos, k_pos, key_mask)
+    with _on_device(q.device):
+        ws = _scratch(lib.magic_attn_fwd_workspace_bytes(C.byref(a)), q.device)
+        _check(lib.magic_attn_fwd(C.byref(a), out.data_ptr(), out.stride(0), out.stride(1), lse.data_ptr(), ws.data_ptr(),
+                                  ws.numel(), _stream()), "magic_attn_fwd")
+    return out, lse
+
+
+def attn_bwd(q, k, v, plan, scale: float, out, lse, d_out, cap: float = 0.0, slopes=None, q_pos=None, k_pos=None,
+             key_mask=None, need_dq: bool = True, need_dkv: bool = True, need_dslopes: bool = False):
+    """Gradients of ``attn_fwd``: (dq | None, dk | None, dv | None, d_slopes | None)."""
+    lib = load()
+    attn_check(q, k, v, plan.n_q, plan.n_k, plan.device, cap, slopes, q_pos, k_pos, key_mask)
+    _heads_check(d_out, "d_out", q)
+    _heads_check(out, "out", q)
+    if d_out.shape != q.shape or out.shape != q.shape:
+        raise MagicHipError(f"out and d_out must have q's shape {tuple(q.shape)}")
+    if lse.shape != (q.shape[1], q.shape[0]) or lse.dtype != torch.float32 or not lse.is_contiguous() \
+            or lse.device != q.device:
+        raise MagicHipError("lse must be the float32 [q_heads, n_q] tensor of the forward pass")
+    q, k, v, slopes, q_pos, k_pos, key_mask = attn_operands(q, k, v, slopes, q_pos, k_pos, key_mask)
+    out, d_out = _head_rows(out), _head_rows(d_out)
+    need_dslopes = need_dslopes and slopes is not None
+    new = lambda t: torch.empty(t.shape, dtype=t.dtype, device=t.device)  # noqa: E731
+    dq = new(q) if need_dq or need_dslopes else None
+    dk, dv = (new(k), new(v)) if need_dkv else (None, None)
+    ds = torch.empty(q.shape[1], dtype=torch.float32, device=q.device) if need_dslopes else None
+    a = _attn_args(q, k, v, plan, scale, cap, slopes, q_pos, k_pos, key_mask)
+    with _on_device(q.device):
+        ws = _scratch(lib.magic_attn_bwd_workspace_bytes(C.byref(a)), q.device)
+        _check(lib.magic_attn_bwd(C.byref(a), out.data_ptr(), out.stride(0), out.stride(1), lse.data_ptr(),
+                                  d_out.data_ptr(), d_out.stride(0), d_out.stride(1), _dev(dq), _dev(dk), _dev(dv), _dev(ds),
+                                  ws.data_ptr(), ws.numel(), _stream()), "magic_attn_bwd")
+    return dq, dk, dv, ds
+
+
+# ------------------------------------------------------------------------------------- head norm + rotation
+def _head_norm_check(q, k, wq, wk, pos, rotary_dim, eps, base):
+    _heads_check(q, "q")
+    _heads_check(k, "k", q)
+    n, d = q.shape[0], q.shape[2]
+    if k.shape[0] != n or k.shape[2] != d or q.shape[1] < 1 or k.shape[1] < 1:
+        raise MagicHipError(f"q and k must have the same rows and head_dim, and heads: {tuple(q.shape)}, {tuple(k.shape)}")
+    if d < 1 or d > ATTN_MAX_DIM:
+        raise MagicHipError(f"head_dim must be 1 to {ATTN_MAX_DIM} (got {d})")
+    if rotary_dim < 0 or rotary_dim > d or rotary_dim % 2:
+        raise MagicHipError(f"rotary_dim must be even and 0 to head_dim {d} (got {rotary_dim})")
+    if not eps >= 0.0 or not 0.0 < base < float("inf"):
+        raise MagicHipError(f"eps must be >= 0 and base > 0 (got {eps}, {base})")
+    _vec_check(wq, "q_weight", d, (torch.float32,), q.device)
+    _vec_check(wk, "k_weight", d, (torch.float32,), q.device)
+    _vec_check(pos, "pos", n, (torch.int32,), q.device)
+
+
+def _unit_inner(t):
+    return t if t.stride(2) == 1 else t.contiguous()
+
+
+def head_norm_rope_fwd(q, k, wq, wk, pos, rotary_dim: int, eps: float, base: float):
+    """(yq, yk), contiguous: per-head RMS norm and position rotation."""
+    lib = load()
+    _head_norm_check(q, k, wq, wk, pos, rotary_dim, eps, base)
+    q, k, wq, wk, pos = _unit_inner(q), _unit_inner(k), wq.contiguous(), wk.contiguous(), pos.contiguous()
+    yq = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+    yk = torch.empty(k.shape, dtype=q.dtype, device=q.device)
+    with _on_device(q.device):
+        _check(lib.magic_head_norm_rope_fwd(q.shape[0], q.shape[1], k.shape[1], q.shape[2], rotary_dim, _ATTN_DTYPE[q.dtype],
+                                            q.data_ptr(), q.stride(0), q.stride(1), k.data_ptr(), k.stride(0), k.stride(1),
+                                            wq.data_ptr(), wk.data_ptr(), pos.data_ptr(), float(eps), float(base),
+                                            yq.data_ptr(), yk.data_ptr(), _stream()), "magic_head_norm_rope_fwd")
+    return yq, yk
+
+
+def head_norm_rope_bwd(q, k, wq, wk, pos, rotary_dim: int, eps: float, base: float, dyq, dyk):
+    """(dq, dk, dwq, dwk) of ``head_norm_rope_fwd``."""
+    lib = load()
+    _head_norm_check(q, k, wq, wk, pos, rotary_dim, eps, base)
+    _heads_check(dyq, "dyq", q)
+    _heads_check(dyk, "dyk", q)
+    if dyq.shape != q.shape or dyk.shape != k.shape:
+        raise MagicHipError("the gradients must have the shapes of the outputs")
+    q, k, wq, wk, pos = _unit_inner(q), _unit_inner(k), wq.contiguous(), wk.contiguous(), pos.contiguous()
+    dyq, dyk = _unit_inner(dyq), _unit_inner(dyk)
+    dev = q.device
+    dq, dk = (torch.empty(t.shape, dtype=t.dtype, device=dev) for t in (q, k))
+    dwq, dwk = (torch.empty(q.shape[2], dtype=torch.float32, device=dev) for _ in range(2))
+    with _on_device(dev):
+        ws = _scratch(lib.magic_head_norm_rope_bwd_workspace_bytes(q.shape[0], q.shape[2]), dev)
+        _check(lib.magic_head_norm_rope_bwd(q.shape[0], q.shape[1], k.shape[1], q.shape[2], rotary_dim, _ATTN_DTYPE[q.dtype],
+                                            q.data_ptr(), q.stride(0), q.stride(1), k.data_ptr(), k.stride(0), k.stride(1),
+                                            wq.data_ptr(), wk.data_ptr(), pos.data_ptr(), float(eps), float(base),
+                                            dyq.data_ptr(), dyq.stride(0), dyq.stride(1), dyk.data_ptr(), dyk.stride(0),
+                                            dyk.stride(1), dq.data_ptr(), dk.data_ptr(), dwq.data_ptr(), dwk.data_ptr(),
+                                            ws.data_ptr(), ws.numel(), _stream()), "magic_head_norm_rope_bwd")
+    return dq, dk, dwq, dwk
+
+
+# ------------------------------------------------------------------------------------- 8-bit activation checkpoints
+def act8_pack(x: torch.Tensor):
+    """(codes int8 [N, stride], exps uint8 [N, ceil(F / 32)]) of a float32 [N, F] matrix."""
+    lib = load()
+    if x.dim() != 2 or x.shape[1] < 1:
+        raise MagicHipError(f"x must be a matrix with at least one column (got {tuple(x.shape)})")
+    _dev(x, torch.float32, "x")
+    x = _rows(x)
+    n, f = x.shape
+    codes = torch.empty(n, lib.magic_act8_code_stride(f), dtype=torch.int8, device=x.device)
+    exps = torch.empty(n, (f + 31) // 32, dtype=torch.uint8, device=x.device)
+    with _on_device(x.device):
+        _check(lib.magic_act8_pack(n, f, x.data_ptr(), max(x.stride(0), f), codes.data_ptr(), exps.data_ptr(), _stream()),
+               "magic_act8_pack")
+    return codes, exps
+
+
+def _act8_check(codes, exps, n_cols):
+    n = codes.shape[0]
+    if codes.dim() != 2 or exps.dim() != 2 or codes.dtype != torch.int8 or exps.dtype != torch.uint8 or n_cols < 1 \
+            or codes.shape[1] != load().magic_act8_code_stride(n_cols) or exps.shape != (n, (n_cols + 31) // 32) \
+            or not codes.is_contiguous() or not exps.is_contiguous() or codes.device != exps.device:
+        raise MagicHipError("codes / exps are not what act8_pack returns for this many columns")
+    _dev(codes, torch.int8, "codes")
+
+
+def act8_unpack(codes: torch.Tensor, exps: torch.Tensor, n_cols: int) -> torch.Tensor:
+    lib = load()
+    _act8_check(codes, exps, n_cols)
+    x = torch.empty(codes.shape[0], n_cols, dtype=torch.float32, device=codes.device)
+    with _on_device(x.device):
+        _check(lib.magic_act8_unpack(x.shape[0], n_cols, codes.data_ptr(), exps.data_ptr(), x.data_ptr(), n_cols, _stream()),
+               "magic_act8_unpack")
+    return x
+
+
+def act8_weight_grad(dy: torch.Tensor, codes: torch.Tensor, exps: torch.Tensor, n_cols: int) -> torch.Tensor:
+    """dW [M, n_cols] = dy.T @ unpack(codes, exps)."""
+    lib = load()
+    _act8_check(codes, exps, n_cols)
+    if dy.dim() != 2 or dy.shape[0] != codes.shape[0] or dy.shape[1] < 1 or dy.device != codes.device:
+        raise MagicHipError(f"dy must be a [{codes.shape[0]}, M] matrix on {codes.device}")
+    _dev(dy, torch.float32, "dy")
+    dy = _rows(dy)
+    n, m = dy.shape
+    dw = torch.empty(m, n_cols, dtype=torch.float32, device=dy.device)
+    with _on_device(dy.device):
+        ws = _scratch(lib.magic_act8_weight_grad_workspace_bytes(n, m, n_cols), dy.device)
+        _check(lib.magic_act8_weight_grad(n, m, n_cols, dy.data_ptr(), max(dy.stride(0), m), codes.data_ptr(),
+                                          exps.data_ptr(), dw.data_ptr(), ws.data_ptr(), ws.numel(), _stream()),
+               "magic_act8_weight_grad")
+    return dw

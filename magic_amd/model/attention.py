@@ -1,0 +1,133 @@
+"""Attention of a node over all nodes of its own component graph.
+
+``GATConv`` (``gat.py``) reaches as far as its layers hop along edges; the operators here let every node of a batch of
+component graphs see all nodes of its own graph:
+
+* ``head_norm_rope``: RMS norm of every head of the queries and keys, with the rotation by a node's position (its
+  order of appearance), in one pass;
+* ``segment_attention``: softmax attention inside segments (the component graphs), with scores capped by a tanh, a
+  bias that falls with the distance of two positions, a mask over keys and grouped heads, and its gradients;
+* ``GlobalAttention``: the block ``x + W_o attention(norm_rope(W_q x), norm_rope(W_k x), W_v x)`` that
+  ``GMAEModel(global_attention=True)`` puts behind its encoder.
+
+No counterpart in the reference, whose only attention is the one along edges (``model/gat.py:302-312``).
+"""
+from __future__ import annotations
+
+import math
+from typing import Optional, Sequence
+
+import numpy as np
+import torch
+import torch.nn as nn
+
+from .. import _lib
+from ..graph import Graph
+from .gat import linear_nobias
+
+
+class AttentionPlan:
+    """Segments of ``segment_attention`` and the tables of tiles its kernels walk (on the device)."""
+
+    def __init__(self, q_lens, kv_lens, q_tiles, k_tiles):
+        self.q_lens, self.kv_lens = q_lens, kv_lens
+        self.n_q, self.n_k = sum(q_lens), sum(kv_lens)
+        self.q_tiles, self.k_tiles = q_tiles, k_tiles
+
+    @property
+    def device(self):
+        return self.q_tiles.device
+
+
+def _tiles(rows, others):
+    """int32 [tiles, 4]: {first row, rows, first row of the other side, its rows} of every tile of up to
+    ``_lib.ATTN_TILE`` rows, longest segments' tiles first (they take longest; results do not depend on the order)."""
+    rows, others = np.asarray(rows, np.int64), np.asarray(others, np.int64)
+    n = -(-rows // _lib.ATTN_TILE)
+    seg = np.repeat(np.arange(rows.size), n)
+    at = (np.arange(seg.size) - np.repeat(np.cumsum(n) - n, n)) * _lib.ATTN_TILE
+    r0, o0 = np.cumsum(rows) - rows, np.cumsum(others) - others
+    t = np.stack([r0[seg] + at, np.minimum(rows[seg] - at, _lib.ATTN_TILE), o0[seg], others[seg]], 1)
+    return t[np.argsort(-others[seg], kind="stable")].astype(np.int32)
+
+
+def attention_plan(q_lens: Sequence[int], kv_lens: Optional[Sequence[int]] = None, device="cuda") -> AttentionPlan:
+    """Plan for segments of ``q_lens[i]`` query rows over ``kv_lens[i]`` key rows (host integers, in row order; keys =
+    queries when ``kv_lens`` is None).  Lengths may be zero.  A plan serves any heads, types and options, and can be
+    kept as long as the lengths stay the same (all layers of a step, all calls against one stored graph)."""
+    q_lens = [int(x) for x in q_lens]
+    kv_lens = q_lens if kv_lens is None else [int(x) for x in kv_lens]
+    if len(q_lens) != len(kv_lens):
+        raise _lib.MagicHipError(f"{len(q_lens)} query segments but {len(kv_lens)} key segments")
+    if any(x < 0 for x in q_lens + kv_lens):
+        raise _lib.MagicHipError("segment lengths must not be negative")
+    if max(sum(q_lens), sum(kv_lens)) >= 1 << 31:
+        raise _lib.MagicHipError("segment attention serves up to 2^31 - 1 rows")
+    device = torch.device(device)
+    if device.type == "cuda" and device.index is None:
+        device = torch.device("cuda", torch.cuda.current_device())
+    tabs = [torch.from_numpy(_tiles(a, b)) for a, b in ((q_lens, kv_lens), (kv_lens, q_lens))]
+    if device.type == "cuda":
+        tabs = [t.pin_memory().to(device, non_blocking=True) for t in tabs]
+    return AttentionPlan(q_lens, kv_lens, *tabs)
+
+
+class _SegmentAttentionFn(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, q, k, v, slopes, plan, scale, cap, q_pos, k_pos, key_mask):
+        out, lse = _lib.attn_fwd(q, k, v, plan, scale, cap, slopes, q_pos, k_pos, key_mask)
+        ctx.save_for_backward(q, k, v, slopes, q_pos, k_pos, key_mask, out, lse)
+        ctx.plan, ctx.scale, ctx.cap = plan, scale, cap
+        return out
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, d_out):
+        q, k, v, slopes, q_pos, k_pos, key_mask, out, lse = ctx.saved_tensors
+        need = ctx.needs_input_grad
+        dq, dk, dv, ds = _lib.attn_bwd(q, k, v, ctx.plan, ctx.scale, out, lse, d_out, ctx.cap, slopes, q_pos, k_pos,
+                                       key_mask, need_dq=need[0], need_dkv=need[1] or need[2], need_dslopes=need[3])
+        return (dq if need[0] else None, dk if need[1] else None, dv if need[2] else None, ds) + (None,) * 6
+
+
+def segment_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, plan: AttentionPlan, *,
+                      scale: Optional[float] = None, cap: float = 0.0, slopes: Optional[torch.Tensor] = None,
+                      q_pos: Optional[torch.Tensor] = None, k_pos: Optional[torch.Tensor] = None,
+                      key_mask: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """Softmax attention of the rows of every segment over the keys of the same segment.
+
+    q [n_q, q_heads, head_dim]; k, v [n_k, kv_heads, head_dim], query head h reads key head h // (q_heads //
+    kv_heads).  float32 or bfloat16, any row and head strides, head_dim a multiple of 8 up to 128.
+    ``s = scale q.k`` (scale: 1 / sqrt(head_dim)); ``cap > 0``: ``cap tanh(s / cap)``; ``slopes`` [q_heads] float32:
+    minus ``slopes[h] |q_pos[i] - k_pos[j]|`` (int32 positions); ``key_mask`` [n_k] bool: False = the key takes no part,
+    whatever its rows hold.  A row that sees no key gets zeros, and zero gradients.
+    Differentiable in q, k, v and slopes; the sums have a fixed order."""
+    if scale is None:
+        scale = 1.0 / math.sqrt(q.shape[-1])
+    if not math.isfinite(scale):
+        raise _lib.MagicHipError(f"scale must be finite (got {scale})")
+    return _SegmentAttentionFn.apply(q, k, v, slopes, plan, float(scale), float(cap), q_pos, k_pos, key_mask)
+
+
+class _HeadNormRopeFn(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, q, k, wq, wk, pos, rotary_dim, eps, base):
+        ctx.save_for_backward(q, k, wq, wk, pos)
+        ctx.opts = (rotary_dim, eps, base)
+        return _lib.head_norm_rope_fwd(q, k, wq, wk, pos, rotary_dim, eps, base)
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dyq, dyk):
+        q, k, wq, wk, pos = ctx.saved_tensors
+        return _lib.head_norm_rope_bwd(q, k, wq, wk, pos, *ctx.opts, dyq, dyk) + (None,) * 4
+
+
+def head_norm_rope(q: torch.Tensor, k: torch.Tensor, q_weight: torch.Tensor, k_weight: torch.Tensor, pos: torch.Tensor, *,
+                   rotary_dim: Optional[int] = None, eps: float = 1e-6, base: float = 10000.0):
+    """``(q', k')``: every head of q [n, q_heads, head_dim] and k [n, kv_heads, head_dim] divided by its root mean
+    square (``rsqrt(mean(x^2) + eps)``), times ``q_weight`` / ``k_weight`` [head_dim] float32, and its column pairs
+    (i, i + R/2), i < R/2, turned by ``pos * base^(-2i/R)``; R = ``rotary_dim`` (head_dim unless given; 0: norm only).
+    float32 or bfloat16, any strides, head_dim up to 128, ``pos`` [n] int32.  Differentiable in q, k and the weights."""
+    rotary_dim = q.shape[-1] if rotary_dim is None else int(rotary_dim)
+    return _HeadNormRopeFn.apply(q, k, q_weight, k_weight, pos, rotary_dim, float(eps), float(base))

@@ -211,9 +211,37 @@ class _LinearFn(torch.autograd.Function):
         return dx, dw, db
 
 
-def linear_nobias(x: torch.Tensor, w: torch.Tensor) -> torch.Tensor:
-    """``torch.nn.functional.linear(x, w)`` for GPU tensors with up to 320 output features."""
-    return _LinearNoBiasFn.apply(x, w)
+class _LinearAct8Fn(torch.autograd.Function):
+    """``_LinearNoBiasFn`` that keeps its input for the backward pass as 8-bit codes (``act8.py``): the forward value
+    and the input gradient are those of the float32 layer, the weight gradient reads the codes."""
+
+    @staticmethod
+    def forward(ctx, x, w):
+        y, _, _ = ops.proj_fwd(x, w, w.shape[0], 0, 0)
+        codes = exps = None
+        if ctx.needs_input_grad[1]:
+            codes, exps = _lib.act8_pack(x)
+        ctx.save_for_backward(codes, exps, w)
+        return y
+
+    @staticmethod
+    def backward(ctx, dy):
+        codes, exps, w = ctx.saved_tensors
+        dx = ops.proj_bwd_input(dy, w)[0] if ctx.needs_input_grad[0] else None
+        dw = _lib.act8_weight_grad(dy, codes, exps, w.shape[1]) if ctx.needs_input_grad[1] else None
+        return dx, dw
+
+
+def linear_nobias(x: torch.Tensor, w: torch.Tensor, act_bits: int = 32) -> torch.Tensor:
+    """``torch.nn.functional.linear(x, w)`` for float32 matrices on the GPU.  ``act_bits=8`` keeps ``x`` for the
+    backward pass as 8-bit codes (a quarter of the memory; only the weight gradient sees the rounding)."""
+    if act_bits == 32:
+        return _LinearNoBiasFn.apply(x, w)
+    if act_bits != 8:
+        raise _lib.MagicHipError(f"act_bits must be 32 or 8 (got {act_bits})")
+    if x.dim() != 2 or w.dim() != 2 or x.shape[1] != w.shape[1]:
+        raise _lib.MagicHipError(f"x [N, F] and w [M, F] expected, got {tuple(x.shape)} and {tuple(w.shape)}")
+    return _LinearAct8Fn.apply(x, w)
 
 
 class GATConv(nn.Module):

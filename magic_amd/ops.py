@@ -464,3 +464,50 @@ _register("knn_merge", "(Tensor part_dist, Tensor part_idx) -> (Tensor, Tensor)"
 _register("readout", "(Tensor feat, Tensor? node_type, int n_types, bool mean) -> Tensor",
           lambda feat, node_type, n_types, mean: _lib.readout(feat, node_type, n_types, mean),
           lambda feat, node_type, n_types, mean: feat.new_empty(1, max(n_types, 1) * feat.shape[1]))
+
+
+# ------------------------------------------------------------------------------------- global-attention block
+# The plan of segment attention travels as its two tile tables; operands and results as in ``_lib.attn_fwd``.
+def _attn_plan(q, k, q_tiles, k_tiles):
+    return SimpleNamespace(q_tiles=q_tiles, k_tiles=k_tiles, n_q=q.shape[0], n_k=k.shape[0], device=q_tiles.device)
+
+
+_ATTN = "Tensor q, Tensor k, Tensor v, Tensor q_tiles, Tensor k_tiles, float scale, float cap, Tensor? slopes, " \
+        "Tensor? q_pos, Tensor? k_pos, Tensor? key_mask"
+_register("attn_fwd", f"({_ATTN}) -> (Tensor, Tensor)",
+          lambda q, k, v, q_tiles, k_tiles, scale, cap, slopes, q_pos, k_pos, key_mask:
+          _lib.attn_fwd(q, k, v, _attn_plan(q, k, q_tiles, k_tiles), scale, cap, slopes, q_pos, k_pos, key_mask),
+          lambda q, k, v, q_tiles, k_tiles, scale, cap, slopes, q_pos, k_pos, key_mask:
+          (q.new_empty(q.shape), q.new_empty((q.shape[1], q.shape[0]), dtype=torch.float32)))
+
+
+def _attn_bwd(q, k, v, q_tiles, k_tiles, scale: float, cap: float, slopes, q_pos, k_pos, key_mask, out, lse, d_out):
+    dq, dk, dv, ds = _lib.attn_bwd(q, k, v, _attn_plan(q, k, q_tiles, k_tiles), scale, out, lse, d_out, cap, slopes, q_pos,
+                                   k_pos, key_mask, need_dslopes=slopes is not None)
+    return dq, dk, dv, ds if ds is not None else _empty(q)
+
+
+_register("attn_bwd", f"({_ATTN}, Tensor out, Tensor lse, Tensor d_out) -> (Tensor, Tensor, Tensor, Tensor)", _attn_bwd,
+          lambda q, k, v, q_tiles, k_tiles, scale, cap, slopes, q_pos, k_pos, key_mask, out, lse, d_out:
+          (q.new_empty(q.shape), k.new_empty(k.shape), v.new_empty(v.shape),
+           q.new_empty(q.shape[1] if slopes is not None else 0, dtype=torch.float32)))
+
+_NORM = "Tensor q, Tensor k, Tensor wq, Tensor wk, Tensor pos, int rotary_dim, float eps, float base"
+_register("head_norm_rope_fwd", f"({_NORM}) -> (Tensor, Tensor)",
+          lambda q, k, wq, wk, pos, rotary_dim, eps, base: _lib.head_norm_rope_fwd(q, k, wq, wk, pos, rotary_dim, eps, base),
+          lambda q, k, wq, wk, pos, rotary_dim, eps, base: (q.new_empty(q.shape), k.new_empty(k.shape)))
+_register("head_norm_rope_bwd", f"({_NORM}, Tensor dyq, Tensor dyk) -> (Tensor, Tensor, Tensor, Tensor)",
+          lambda q, k, wq, wk, pos, rotary_dim, eps, base, dyq, dyk:
+          _lib.head_norm_rope_bwd(q, k, wq, wk, pos, rotary_dim, eps, base, dyq, dyk),
+          lambda q, k, wq, wk, pos, rotary_dim, eps, base, dyq, dyk:
+          (q.new_empty(q.shape), k.new_empty(k.shape), wq.new_empty(wq.shape), wk.new_empty(wk.shape)))
+
+_register("act8_pack", "(Tensor x) -> (Tensor, Tensor)", lambda x: _lib.act8_pack(x),
+          lambda x: (x.new_empty((x.shape[0], (x.shape[1] + 15) // 16 * 16), dtype=torch.int8),
+                     x.new_empty((x.shape[0], (x.shape[1] + 31) // 32), dtype=torch.uint8)))
+_register("act8_unpack", "(Tensor codes, Tensor exps, int n_cols) -> Tensor",
+          lambda codes, exps, n_cols: _lib.act8_unpack(codes, exps, n_cols),
+          lambda codes, exps, n_cols: codes.new_empty((codes.shape[0], n_cols), dtype=torch.float32))
+_register("act8_weight_grad", "(Tensor dy, Tensor codes, Tensor exps, int n_cols) -> Tensor",
+          lambda dy, codes, exps, n_cols: _lib.act8_weight_grad(dy, codes, exps, n_cols),
+          lambda dy, codes, exps, n_cols: dy.new_empty((dy.shape[1], n_cols)))

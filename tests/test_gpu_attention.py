@@ -1,0 +1,386 @@
+"""Segment attention, head norm + rotation: against plain 64-bit implementations, element by element.
+
+The bounds are worst cases of the arithmetic the header promises, formed from the inputs.  u = 2^-24 (half a step of
+float32), r = 2^-8 (half a step of bfloat16, relative), 0 for float32 operands.  With w = sum |q||k| scale, a score is
+off by at most (D + 8) u w (products and sums in float32), a logit by delta = that + 4 u |l| + 4 u cap (tanh, bias,
+subtraction); a probability exp(l - lse) by a factor 1 +- e_p, e_p = 2 delta + (nk + 16) u (both logits, the sum over the
+keys), and the p of a product by r more where it is rounded to bfloat16.  The rest follows by the product rule."""
+import math
+
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+U = 2.0 ** -24
+
+
+def _half_step(dtype):
+    return torch.finfo(dtype).eps / 2 if dtype != torch.float32 else 0.0
+
+
+def reference(q, k, v, q_lens, kv_lens, scale, cap, slopes, q_pos, k_pos, key_mask, d_out):
+    """float64 outputs, gradients and the elementwise bounds of the float32 / bfloat16 kernels."""
+    r = _half_step(q.dtype)
+    dev = q.device
+    q, k, v, d_out = (t.detach().double() for t in (q, k, v, d_out))
+    hq, hk, D = q.shape[1], k.shape[1], q.shape[2]
+    g = hq // hk
+    res = {n: torch.zeros_like(t) for n, t in (("out", q), ("dq", q), ("dk", k), ("dv", v))}
+    tol = {n: torch.zeros_like(t) for n, t in res.items()}
+    res["ds"], tol["ds"] = (torch.zeros(hq, dtype=torch.float64, device=dev) for _ in range(2))
+    a = b = 0
+    for nq, nk in zip(q_lens, kv_lens):
+        rows = torch.arange(a, a + nq, device=dev)
+        cols = torch.arange(b, b + nk, device=dev)
+        a, b = a + nq, b + nk
+        if key_mask is not None:
+            cols = cols[key_mask[cols].bool()]
+        if rows.numel() == 0 or cols.numel() == 0:
+            continue
+        n = cols.numel()
+        for h in range(hq):
+            j = h // g
+            Q, K, V, G = q[rows, h], k[cols, j], v[cols, j], d_out[rows, h]
+            s = scale * Q @ K.T
+            w = abs(scale) * Q.abs() @ K.abs().T
+            t = torch.tanh(s / cap) if cap else torch.zeros_like(s)
+            c = cap * t if cap else s
+            dist = torch.zeros_like(s)
+            if slopes is not None:
+                dist = (q_pos[rows].double()[:, None] - k_pos[cols].double()[None]).abs()
+                l = c - slopes[h].double() * dist
+            else:
+                l = c
+            delta = ((D + 8) * U * w).amax(1, keepdim=True) + 4 * U * l.abs().amax(1, keepdim=True) + 4 * U * cap
+            if slopes is not None:
+                delta = delta + 4 * U * (slopes[h].abs().double() * dist).amax(1, keepdim=True)
+            p = torch.softmax(l, 1)
+            ep = 2 * delta + (n + 16) * U
+            O = p @ V
+            res["out"][rows, h] = O
+            tol["out"][rows, h] = (ep + r + (n + 16) * U) * (p @ V.abs()) + r * O.abs()
+            # gradients
+            res["dv"][cols, j] += p.T @ G
+            tol["dv"][cols, j] += ((ep + r) * p).T @ G.abs() + (len(rows) + 16) * U * (p.T @ G.abs())
+            dp, ad = G @ V.T, G.abs() @ V.abs().T
+            dd, add = (G * O).sum(1, keepdim=True), (G.abs() * O.abs()).sum(1, keepdim=True)
+            e_dp = (D + 8) * U * (ad + add) + (G.abs() * (tol["out"][rows, h] + r * O.abs())).sum(1, keepdim=True)
+            dl = p * (dp - dd)
+            e_dl = ep * dl.abs() + p * e_dp
+            f = 1 - t * t if cap else torch.ones_like(t)
+            ef = (2 * delta / cap + 8 * U) if cap else 0.0
+            ds = scale * dl * f
+            e_ds = abs(scale) * (e_dl * f + dl.abs() * ef) + r * ds.abs() + 8 * U * ds.abs()
+            res["dq"][rows, h] = ds @ K
+            tol["dq"][rows, h] = e_ds @ K.abs() + (n + 16) * U * (ds.abs() @ K.abs())
+            res["dk"][cols, j] += ds.T @ Q
+            tol["dk"][cols, j] += e_ds.T @ Q.abs() + (g * len(rows) + 16) * U * (ds.abs().T @ Q.abs())
+            if slopes is not None:
+                res["ds"][h] -= (dl * dist).sum()
+                tol["ds"][h] += (e_dl * dist).sum() + (n + len(rows) + 64) * U * (dl.abs() * dist).sum()
+    for name in ("dq", "dk", "dv"):
+        tol[name] += r * res[name].abs()
+    for name in tol:
+        tol[name] += 2.0 ** -120
+    return res, tol
+
+
+def make(cuda, q_lens, kv_lens, hq, hk, D, dtype, seed=0, slopes=False, mask=None, std=1.0):
+    gen = torch.Generator(device=cuda).manual_seed(seed)
+    rn = lambda *s: torch.randn(*s, generator=gen, device=cuda)  # noqa: E731
+    nq, nk = sum(q_lens), sum(kv_lens)
+    q, k, v = (rn(nq, hq, D) * std).to(dtype), (rn(nk, hk, D) * std).to(dtype), rn(nk, hk, D).to(dtype)
+    d = (rn(nq, hq, D) * 0.1).to(dtype)
+    kw = {}
+    if slopes:
+        kw = dict(slopes=2.0 ** -(3.0 + 4.0 * torch.rand(hq, generator=gen, device=cuda)),
+                  q_pos=torch.randint(0, 500, (nq,), generator=gen, device=cuda, dtype=torch.int32),
+                  k_pos=torch.randint(0, 500, (nk,), generator=gen, device=cuda, dtype=torch.int32))
+    if mask is not None:
+        kw["key_mask"] = torch.rand(nk, generator=gen, device=cuda) < mask
+    return q, k, v, d, kw
+
+
+def run(q, k, v, d, q_lens, kv_lens, cap=0.0, scale=None, **kw):
+    from magic_amd.model.attention import attention_plan, segment_attention
+    plan = attention_plan(q_lens, kv_lens, q.device)
+    leaves = [t.detach().requires_grad_(True) for t in (q, k, v)]
+    if kw.get("slopes") is not None:
+        kw = dict(kw, slopes=kw["slopes"].detach().requires_grad_(True))
+        leaves.append(kw["slopes"])
+    out = segment_attention(*leaves[:3], plan, scale=scale, cap=cap, **kw)
+    got = dict(zip(("dq", "dk", "dv", "ds"), torch.autograd.grad(out, leaves, d)))
+    got["out"] = out.detach()
+    return got
+
+
+def check(got, q, k, v, d, q_lens, kv_lens, cap=0.0, scale=None, slopes=None, q_pos=None, k_pos=None, key_mask=None):
+    scale = 1.0 / math.sqrt(q.shape[2]) if scale is None else scale
+    want, tol = reference(q, k, v, q_lens, kv_lens, scale, cap, slopes, q_pos, k_pos, key_mask, d)
+    for name, g in got.items():
+        err = (g.double() - want[name]).abs()
+        bad = ~(err <= tol[name])
+        assert not bad.any(), (name, int(bad.sum()), float(err.max()), float((err / tol[name]).nan_to_num(1e9).max()),
+                               bad.nonzero()[0].tolist())
+
+
+LENS = {
+    "one": ([1], [1]),
+    "tiny": ([3, 0, 1, 2], [1, 4, 0, 5]),
+    "tile_edges": ([31, 32, 33, 64], [63, 64, 65, 33]),
+    "ragged": ([1, 127, 129, 0, 257, 70], [1, 127, 129, 0, 257, 70]),
+    "cross": ([5, 200, 130], [333, 1, 129]),
+    "few_rows": ([1, 2, 1], [700, 1500, 3]),
+}
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=["f32", "bf16"])
+@pytest.mark.parametrize("hq,hk,D", [(4, 4, 16), (4, 4, 64), (4, 2, 24), (6, 2, 128), (1, 1, 8), (2, 1, 40)])
+@pytest.mark.parametrize("lens", list(LENS))
+def test_attention_forward_and_gradients(cuda, lens, hq, hk, D, dtype):
+    q_lens, kv_lens = LENS[lens]
+    q, k, v, d, kw = make(cuda, q_lens, kv_lens, hq, hk, D, dtype, seed=len(lens) + D)
+    check(run(q, k, v, d, q_lens, kv_lens, **kw), q, k, v, d, q_lens, kv_lens, **kw)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=["f32", "bf16"])
+@pytest.mark.parametrize("cap,slopes,mask", [(20.0, False, None), (0.0, True, None), (3.0, True, 0.4), (0.0, False, 0.1),
+                                             (0.0, False, 0.0), (50.0, True, 0.9)])
+@pytest.mark.parametrize("lens,D", [("ragged", 64), ("few_rows", 16), ("cross", 128)])
+def test_attention_cap_bias_mask(cuda, lens, D, cap, slopes, mask, dtype):
+    q_lens, kv_lens = LENS[lens]
+    q, k, v, d, kw = make(cuda, q_lens, kv_lens, 4, 2, D, dtype, seed=3, slopes=slopes, mask=mask, std=2.0)
+    check(run(q, k, v, d, q_lens, kv_lens, cap=cap, **kw), q, k, v, d, q_lens, kv_lens, cap=cap, **kw)
+
+
+def test_attention_scale_signs_and_large_scores(cuda):
+    q_lens, kv_lens = LENS["ragged"]
+    q, k, v, d, kw = make(cuda, q_lens, kv_lens, 4, 4, 32, torch.float32, seed=5, std=4.0)
+    for scale in (0.0, -0.3, 2.0):
+        check(run(q, k, v, d, q_lens, kv_lens, scale=scale), q, k, v, d, q_lens, kv_lens, scale=scale)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=["f32", "bf16"])
+def test_rows_without_a_visible_key_and_what_masked_keys_hold(cuda, dtype):
+    """Masked keys may hold NaN, infinities and the type's lowest value; rows behind a segment's end may too (they
+    belong to the next segment); a row that sees nothing gives zeros."""
+    from magic_amd.model.attention import attention_plan, segment_attention
+    q_lens = kv_lens = [40, 70, 5, 33]
+    q, k, v, d, _ = make(cuda, q_lens, kv_lens, 4, 2, 64, dtype, seed=9)
+    mask = torch.rand(148, device=cuda) < 0.6
+    mask[110:115] = False                                     # the third segment sees nothing
+    clean = run(q, k, v, d, q_lens, kv_lens, key_mask=mask)
+    check(clean, q, k, v, d, q_lens, kv_lens, key_mask=mask)
+    assert not clean["out"][110:115].any() and not clean["dq"][110:115].any()
+    assert not clean["dk"][~mask].any() and not clean["dv"][~mask].any()
+    for poison in (float("nan"), float("inf"), -float("inf"), torch.finfo(dtype).min):
+        k2, v2 = k.clone(), v.clone()
+        k2[~mask], v2[~mask] = poison, poison
+        dirty = run(q, k2, v2, d, q_lens, kv_lens, key_mask=mask)
+        for name in clean:
+            assert torch.equal(clean[name], dirty[name]), (name, poison)
+    # a NaN row stays inside its own segment and head group
+    k3 = k.clone()
+    k3[45, 0] = float("nan")
+    out = segment_attention(q, k3, v, attention_plan(q_lens, None, cuda))
+    ref = segment_attention(q, k, v, attention_plan(q_lens, None, cuda))
+    hit = torch.zeros(148, 4, dtype=torch.bool, device=cuda)
+    hit[40:110, :2] = True
+    assert torch.equal(out[~hit], ref[~hit]) and torch.isnan(out[hit]).all()
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=["f32", "bf16"])
+def test_attention_strides(cuda, dtype):
+    """Views of one projection output, head-major storage, rows off 16-byte addresses, expanded gradients."""
+    lens = [50, 91]
+    n, h, D = 141, 4, 32
+    qkv = torch.randn(n, 3 * h * D, device=cuda).to(dtype)
+    q, k, v = (qkv[:, i * h * D:(i + 1) * h * D].view(n, h, D) for i in range(3))
+    d = torch.randn(n, h, D, device=cuda).to(dtype)
+    want = run(q.contiguous(), k.contiguous(), v.contiguous(), d, lens, lens)
+    forms = {"view": (q, k, v),
+             "head_major": tuple(t.transpose(0, 1).contiguous().transpose(0, 1) for t in (q, k, v)),
+             "unaligned": tuple(torch.empty(n * h * D + 1, device=cuda, dtype=dtype)[1:].view(n, h, D).copy_(t)
+                                for t in (q, k, v)),
+             "inner_stride": tuple(t.transpose(1, 2).contiguous().transpose(1, 2) for t in (q, k, v))}
+    for name, (a, b, c) in forms.items():
+        got = run(a, b, c, d.transpose(0, 1).contiguous().transpose(0, 1), lens, lens)
+        for key in want:
+            assert torch.equal(got[key], want[key]), (name, key)
+    one = run(q, k, v, torch.ones((), device=cuda, dtype=dtype).expand(n, h, D), lens, lens)
+    check(one, q, k, v, torch.ones(n, h, D, device=cuda, dtype=dtype), lens, lens)
+
+
+def test_attention_gradient_against_differences(cuda):
+    """Central differences of the 64-bit definition along random directions against the kernel's gradients."""
+    lens = [37, 66]
+    q, k, v, d, kw = make(cuda, lens, lens, 4, 2, 16, torch.float32, seed=21, slopes=True, mask=0.8)
+    got = run(q, k, v, d, lens, lens, cap=5.0, **kw)
+
+    def value(q, k, v, slopes):
+        kw2 = dict(kw, slopes=slopes)
+        want, _ = reference(q, k, v, lens, lens, 0.25, 5.0, d_out=d, **kw2)
+        return float((want["out"] * d.double()).sum())
+
+    gen = torch.Generator(device=cuda).manual_seed(4)
+    base = [q.double(), k.double(), v.double(), kw["slopes"].double()]
+    for i, name in enumerate(("dq", "dk", "dv", "ds")):
+        e = torch.randn(base[i].shape, generator=gen, device=cuda, dtype=torch.float64) * (0.01 if name == "ds" else 1.0)
+        step = 1e-5
+        hi, lo = ([t + s * step * e if j == i else t for j, t in enumerate(base)] for s in (1.0, -1.0))
+        diff = (value(*hi) - value(*lo)) / (2 * step)
+        mine = float((got[name].double() * e).sum())
+        # second-order term of the difference (step^2) and the rounding of the float32 gradient
+        size = float((got[name].double() * e).abs().sum())
+        assert abs(diff - mine) <= 1e-4 * size + 1e-9, (name, diff, mine)
+
+
+def test_attention_is_reproducible_and_partial_gradients(cuda):
+    from magic_amd.model.attention import attention_plan, segment_attention
+    lens = [700, 33, 1200]
+    q, k, v, d, kw = make(cuda, lens, lens, 4, 4, 64, torch.float32, seed=2, slopes=True)
+    a, b = (run(q, k, v, d, lens, lens, **kw) for _ in range(2))
+    for name in a:
+        assert torch.equal(a[name], b[name]), name
+    plan = attention_plan(lens, device=cuda)
+    for want in (("dq",), ("dk",), ("dv",), ("ds",)):
+        ts = {"dq": q.clone(), "dk": k.clone(), "dv": v.clone(), "ds": kw["slopes"].clone()}
+        for n in want:
+            ts[n].requires_grad_(True)
+        out = segment_attention(ts["dq"], ts["dk"], ts["dv"], plan, **dict(kw, slopes=ts["ds"]))
+        g, = torch.autograd.grad(out, [ts[want[0]]], d)
+        assert torch.equal(g, a[want[0]]), want
+
+
+def test_attention_streams_and_captured_graph(cuda):
+    """Two calls in flight on two streams, and forward + backward replayed from a captured graph on new inputs."""
+    from magic_amd import _lib
+    from magic_amd.model.attention import attention_plan
+    lens = [300, 41]
+    q, k, v, d, kw = make(cuda, lens, lens, 4, 4, 64, torch.float32, seed=12)
+    plan = attention_plan(lens, device=cuda)
+
+    def step(q, k, v, d):
+        out, lse = _lib.attn_fwd(q, k, v, plan, 0.125)
+        return (out,) + _lib.attn_bwd(q, k, v, plan, 0.125, out, lse, d)[:3]
+
+    want = step(q, k, v, d)
+    torch.cuda.synchronize()
+    side = [torch.cuda.Stream() for _ in range(2)]
+    outs = []
+    for s in side:
+        s.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(s):
+            for _ in range(3):
+                outs.append(step(q, k, v, d))
+    for s in side:
+        torch.cuda.current_stream().wait_stream(s)
+    torch.cuda.synchronize()
+    for got in outs:
+        for x, y in zip(got, want):
+            assert torch.equal(x, y)
+    ins = [t.clone() for t in (q, k, v, d)]
+    graphs = []
+    for _ in range(2):                                       # two graphs, replayed in turn
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            res = step(*ins)
+        graphs.append((g, res))
+    for rep in range(3):
+        new = make(cuda, lens, lens, 4, 4, 64, torch.float32, seed=100 + rep)[:4]
+        for a, b in zip(ins, new):
+            a.copy_(b)
+        eager = step(*new)
+        for g, res in graphs:
+            g.replay()
+            torch.cuda.synchronize()
+            for x, y in zip(res, eager):
+                assert torch.equal(x, y)
+
+
+def test_registered_attention_operators(cuda):
+    from magic_amd.model.attention import attention_plan
+    lens = [45, 80]
+    q, k, v, d, kw = make(cuda, lens, lens, 4, 2, 32, torch.float32, seed=31, slopes=True, mask=0.7)
+    plan = attention_plan(lens, device=cuda)
+    args = (q, k, v, plan.q_tiles, plan.k_tiles, 32 ** -0.5, 4.0, kw["slopes"], kw["q_pos"], kw["k_pos"], kw["key_mask"])
+    out, lse = torch.ops.magic.attn_fwd(*args)
+    grads = torch.ops.magic.attn_bwd(*args, out, lse, d)
+    want = run(q, k, v, d, lens, lens, cap=4.0, **kw)
+    for x, name in zip((out,) + tuple(grads), ("out", "dq", "dk", "dv", "ds")):
+        assert torch.equal(x, want[name]), name
+
+
+# ------------------------------------------------------------------------------------------- head norm + rotation
+def rope_reference(x, w, pos, rot, eps, base, dy):
+    r = _half_step(x.dtype)
+    x, w, dy = x.detach().double(), w.detach().double(), dy.double()
+    d, half = x.shape[-1], rot // 2
+    inv = base ** (-torch.arange(half, dtype=torch.float64, device=x.device) * 2 / max(rot, 1))
+    ang = (pos.double()[:, None] * inv)[:, None]
+    c, s = torch.cos(ang), torch.sin(ang)
+
+    def turn(y, s):
+        return torch.cat([y[..., :half] * c - y[..., half:rot] * s, y[..., half:rot] * c + y[..., :half] * s,
+                          y[..., rot:]], -1)
+
+    q = 1 / torch.sqrt((x * x).mean(-1, keepdim=True) + eps)
+    u = x * q * w
+    mag = torch.cat([u[..., :half].abs() + u[..., half:rot].abs()] * 2 + [u[..., rot:].abs()], -1)
+    y = turn(u, s)
+    # rsqrt of a float32 sum of D squares: (D / 2 + 4) u; sine and cosine of an angle reduced in double: 8 u absolute
+    ty = (d / 2 + 24) * U * mag + r * y.abs()
+    gu = turn(dy, -s)
+    gmag = torch.cat([dy[..., :half].abs() + dy[..., half:rot].abs()] * 2 + [dy[..., rot:].abs()], -1)
+    dw = (gu * x * q).sum((0, 1))
+    n = x.shape[0] * x.shape[1]
+    tw = ((d / 2 + 32) * U + min(n, 4096) * U) * (gmag * x.abs() * q).sum((0, 1))
+    g = gu * w
+    dx = q * (g - x * q * q * (g * x).mean(-1, keepdim=True))
+    am = q * (gmag * w.abs() + x.abs() * q * q * (gmag * w.abs() * x.abs()).mean(-1, keepdim=True))
+    tx = (2.5 * d + 48) * U * am + r * dx.abs()
+    return (y, ty + 1e-30), (dx, tx + 1e-30), (dw, tw + 1e-30)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=["f32", "bf16"])
+@pytest.mark.parametrize("n,hq,hk,D,rot", [(1, 4, 4, 64, 64), (77, 4, 2, 16, 16), (1000, 8, 2, 128, 64), (33, 3, 1, 24, 12),
+                                           (50, 2, 2, 63, 62), (129, 1, 1, 128, 2), (64, 4, 4, 64, 0), (9, 2, 1, 1, 0),
+                                           (5000, 4, 4, 64, 64)])
+def test_head_norm_rope(cuda, n, hq, hk, D, rot, dtype):
+    from magic_amd.model.attention import head_norm_rope
+    gen = torch.Generator(device=cuda).manual_seed(n + D)
+    rn = lambda *s: torch.randn(*s, generator=gen, device=cuda)  # noqa: E731
+    qkv = rn(n, (hq + 2 * hk) * D).to(dtype)
+    q, k = qkv[:, :hq * D].view(n, hq, D), qkv[:, hq * D:(hq + hk) * D].view(n, hk, D)
+    wq, wk = 1 + 0.2 * rn(D), 1 + 0.2 * rn(D)
+    pos = torch.randint(-5, 700000, (n,), generator=gen, device=cuda, dtype=torch.int32)
+    dq, dk = rn(n, hq, D).to(dtype), rn(n, hk, D).to(dtype)
+    leaves = [t.detach().requires_grad_(True) for t in (q, k, wq, wk)]
+    yq, yk = head_norm_rope(*leaves, pos, rotary_dim=rot)
+    gq, gk, gwq, gwk = torch.autograd.grad((yq, yk), leaves, (dq, dk))
+    for x, w, dy, y, g, gw in ((q, wq, dq, yq, gq, gwq), (k, wk, dk, yk, gk, gwk)):
+        for got, (want, tol) in zip((y, g, gw), rope_reference(x, w, pos, rot, 1e-6, 10000.0, dy)):
+            err = (got.double() - want).abs()
+            assert (err <= tol).all(), (float(err.max()), float((err / tol).max()))
+    again = torch.autograd.grad(head_norm_rope(*leaves, pos, rotary_dim=rot), leaves, (dq, dk))
+    for a, b in zip(again, (gq, gk, gwq, gwk)):
+        assert torch.equal(a, b)
+
+
+def test_head_norm_rope_strides_and_operators(cuda):
+    from magic_amd.model.attention import head_norm_rope
+    n, h, D = 91, 4, 32
+    x = torch.randn(n, h, D, device=cuda)
+    w = torch.rand(D, device=cuda) + 0.5
+    pos = torch.arange(n, device=cuda, dtype=torch.int32)
+    want = head_norm_rope(x, x, w, w, pos)
+    odd = torch.empty(n * h * D + 1, device=cuda)[1:].view(n, h, D).copy_(x)
+    for form in (x.transpose(0, 1).contiguous().transpose(0, 1), x.transpose(1, 2).contiguous().transpose(1, 2), odd):
+        for a, b in zip(head_norm_rope(form, x, w, w, pos), want):
+            assert (a - b).abs().max() <= 2e-6 * b.abs().max()           # (another order of the same sum)
+    assert torch.equal(torch.ops.magic.head_norm_rope_fwd(x, x, w, w, pos, D, 1e-6, 10000.0)[0], want[0])
+    empty = head_norm_rope(x[:0], x[:0], w, w, pos[:0])
+    assert empty[0].shape == (0, h, D)
+    lw = w.clone().requires_grad_(True)
+    y = head_norm_rope(x[:0], x[:0], lw, w, pos[:0])[0]
+    assert not torch.autograd.grad(y.sum(), lw)[0].any()
