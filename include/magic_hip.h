@@ -575,7 +575,8 @@ int magic_knn_merge(int64_t n_query, int32_t k, int32_t n_parts,
  *   s = scale <q_i, k_j>;  c = cap > 0 ? cap tanh(s / cap) : s;
  *   l = c - slopes[h] |q_pos[i] - k_pos[j]|   (slopes != NULL);   p = softmax_j(l);   o_i = sum_j p v_j
  * q [n_q, q_heads, head_dim], k and v [n_k, kv_heads, head_dim]; query head h reads key head
- * h / (q_heads / kv_heads).  Row strides ld_*, head strides hs_*, unit stride along head_dim
+ * h / (q_heads / kv_heads).  Row strides ld_*, head strides hs_*, unit stride along head_dim, rows and heads on 16-byte
+ * addresses (out, d_out and the gradients too)
  * (head_dim % 8 == 0, at most MAGIC_ATTN_MAX_DIM).  dtype: MAGIC_F32 (products fp32-grade) or
  * MAGIC_BF16 (products of bf16 values, probabilities and score gradients rounded to bf16 before
  * their products; every sum and statistic in fp32).  key_mask [n_k]: 0 = the key takes no part
@@ -605,6 +606,7 @@ typedef struct magic_attn {
     const uint8_t *key_mask;           /* [n_k] or NULL */
     const int32_t *q_tiles, *k_tiles;
     int32_t n_q_tiles, n_k_tiles;
+    int32_t max_q, max_k;              /* the longest segment's rows and keys */
 } magic_attn;
 size_t magic_attn_fwd_workspace_bytes(const magic_attn *args /* host */);
 int magic_attn_fwd(const magic_attn *args /* host struct of device pointers */, void *out, int64_t ld_out, int64_t hs_out,

@@ -1,0 +1,173 @@
+// Building blocks of the segment-attention kernels (attn_fwd.hip, attn_bwd.hip).
+//
+// All products run on v_mfma_f32_32x32x16_bf16.  float32 operands are split into three bf16 planes and take the six
+// leading cross products (bf16_split.h: fp32-grade); bfloat16 operands are one plane and one product.
+// Lane l of a wavefront, li = l & 31, hf = l >> 5:
+//   A [32 x 16]: row li, columns 8 hf .. + 7        B [16 x 32]: rows 8 hf .. + 7, column li
+//   C [32 x 32]: column li, rows 8 (r / 4) + 4 hf + (r & 3), r = 0 .. 15
+// The 16 rows of a product's inner dimension may come in any order as long as A and B agree, so the accumulators of one
+// product serve as the B operand of the next without leaving their registers: registers 8 s .. 8 s + 7 of a C tile are
+// the inner rows {4 hf + j, 8 + 4 hf + j}, j < 4, of its 16-row slice s.  The other operand of that product is the
+// transpose of a tile that lies row-major in LDS; ds_read_tr16_b64 delivers it: the 16 lanes of a group name a 4 x 16
+// block (lane i: row i / 4, columns 4 (i & 3) .. + 3) and lane i receives column i of it.
+#pragma once
+#include "common.h"
+#include "bf16_split.h"
+#include "lowp.h"
+
+namespace magic {
+namespace attn {
+
+typedef float f32x16_t __attribute__((ext_vector_type(16)));
+typedef float f32x4_t __attribute__((ext_vector_type(4)));
+typedef int i32x4_t __attribute__((ext_vector_type(4)));
+typedef short s16x4_t __attribute__((ext_vector_type(4)));
+typedef __bf16 bf16x4_t __attribute__((ext_vector_type(4)));
+
+constexpr float LOG2E = 1.44269504088896340736f;
+constexpr float LN2 = 0.69314718055994530942f;
+
+template <typename T> struct Planes;
+template <> struct Planes<float> { static constexpr int N = 3; };
+template <> struct Planes<bf16_t> { static constexpr int N = 1; };
+
+// eight consecutive elements of an operand row as they lie in memory
+template <typename T> struct Raw;
+template <> struct Raw<float> {
+    f32x4_t a, b;
+    __device__ __forceinline__ void load(const float *p) {
+        a = *reinterpret_cast<const f32x4_t *>(p);
+        b = *reinterpret_cast<const f32x4_t *>(p + 4);
+    }
+    __device__ __forceinline__ void zero() { a = b = f32x4_t{0.f, 0.f, 0.f, 0.f}; }
+    __device__ __forceinline__ void planes(bf16x8_t (&p)[3]) const {
+        split8(make_float4(a[0], a[1], a[2], a[3]), make_float4(b[0], b[1], b[2], b[3]), p[0], p[1], p[2]);
+    }
+    __device__ __forceinline__ void floats(float (&x)[8]) const {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) x[e] = a[e], x[4 + e] = b[e];
+    }
+};
+template <> struct Raw<bf16_t> {
+    bf16x8_t v;
+    __device__ __forceinline__ void load(const bf16_t *p) { v = *reinterpret_cast<const bf16x8_t *>(p); }
+    __device__ __forceinline__ void zero() {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] = (bf16_t)0.f;
+    }
+    __device__ __forceinline__ void planes(bf16x8_t (&p)[1]) const { p[0] = v; }
+    __device__ __forceinline__ void floats(float (&x)[8]) const {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) x[e] = (float)v[e];
+    }
+};
+
+// eight float32 values -> operand planes of the next product: three exact pieces, or one rounding to bfloat16
+__device__ __forceinline__ void to_planes(const float (&x)[8], bf16x8_t (&p)[3]) {
+    split8(make_float4(x[0], x[1], x[2], x[3]), make_float4(x[4], x[5], x[6], x[7]), p[0], p[1], p[2]);
+}
+__device__ __forceinline__ void to_planes(const float (&x)[8], bf16x8_t (&p)[1]) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) p[0][e] = (bf16_t)x[e];
+}
+
+__device__ __forceinline__ void mma(f32x16_t &c, const bf16x8_t (&a)[3], const bf16x8_t (&b)[3]) {
+    mfma_split6(c, a[0], a[1], a[2], b[0], b[1], b[2]);
+}
+__device__ __forceinline__ void mma(f32x16_t &c, const bf16x8_t (&a)[1], const bf16x8_t (&b)[1]) {
+    c = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a[0], b[0], c, 0, 0, 0);
+}
+
+// A tile of ROWS operand rows in LDS: planes of [ROWS][LDW] bf16, rows padded by 16 bytes (reads of one column range by
+// 32 rows then spread over the banks).
+template <typename T, int DP, int ROWS> struct Tile {
+    static constexpr int NP = Planes<T>::N;
+    static constexpr int W = DP < 32 ? 32 : DP;      // a transposed read covers 32 columns
+    static constexpr int LDW = W + 8;
+    static constexpr int PLANE = ROWS * LDW;
+    static constexpr size_t BYTES = (size_t)NP * PLANE * 2;
+
+    static __device__ __forceinline__ void frag(const bf16_t *t, int row, int col, bf16x8_t (&f)[NP]) {
+#pragma unroll
+        for (int p = 0; p < NP; ++p) f[p] = *reinterpret_cast<const bf16x8_t *>(t + p * PLANE + row * LDW + col);
+    }
+    // transpose of rows r0 .. r0 + 15, columns c0 .. c0 + 31, inner order as described above
+    static __device__ __forceinline__ void frag_t(const bf16_t *t, int r0, int c0, int lane, bf16x8_t (&f)[NP]) {
+        const int off = (r0 + 4 * (lane >> 5) + ((lane & 15) >> 2)) * LDW + c0 + 16 * ((lane >> 4) & 1) + 4 * (lane & 3);
+#pragma unroll
+        for (int p = 0; p < NP; ++p) {
+            typedef __attribute__((address_space(3))) s16x4_t *lds_ptr;
+            union {
+                s16x4_t s[2];
+                bf16x8_t h;
+            } u;
+            u.s[0] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_ptr)(t + p * PLANE + off));
+            u.s[1] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_ptr)(t + p * PLANE + off + 8 * LDW));
+            f[p] = u.h;
+        }
+    }
+};
+
+// Staging of a tile by NT threads: rows of DP columns (zeros behind D) in chunks of eight elements.
+template <typename T, int DP, int ROWS, int NT> struct Stage {
+    typedef Tile<T, DP, ROWS> tile;
+    static constexpr int CPR = DP / 8;                          // chunks of a row
+    static constexpr int TOTAL = ROWS * CPR;
+    static constexpr int N = (TOTAL + NT - 1) / NT;
+    Raw<T> r[N];
+
+    // rows row0 .. of an operand with `n` valid rows behind `base` (n >= 1): rows past the end are read as the last one
+    __device__ __forceinline__ void load(const T *base, int64_t ld, int row0, int n, int D, int tid) {
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            const int c = tid + i * NT;
+            const int row = row0 + c / CPR, col = (c % CPR) * 8;
+            const int rc = row < n ? row : n - 1, cc = col < D ? col : 0;
+            r[i].load(base + (int64_t)rc * ld + cc);
+        }
+    }
+    // keep(row of the tile): false -> zeros, whatever was read
+    template <typename Keep> __device__ __forceinline__ void store(bf16_t *t, int D, int tid, Keep keep) {
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            const int c = tid + i * NT;
+            const int row = c / CPR, col = (c % CPR) * 8;
+            if (TOTAL % NT != 0 && c >= TOTAL) break;
+            if (!(keep(i, row) && col < D)) r[i].zero();
+            bf16x8_t p[tile::NP];
+            r[i].planes(p);
+#pragma unroll
+            for (int k = 0; k < tile::NP; ++k)
+                *reinterpret_cast<bf16x8_t *>(t + k * tile::PLANE + row * tile::LDW + col) = p[k];
+        }
+    }
+    __device__ __forceinline__ static int row_of(int i, int tid) { return (tid + i * NT) / CPR; }
+};
+
+// tanh to a few units of float32 relative: odd series near zero, (1 - e) / (1 + e) elsewhere
+__device__ __forceinline__ float tanh_f(float x) {
+    const float a = fabsf(x), z = x * x;
+    const float s = x * (1.f + z * (-0.333333333f + z * (0.133333333f + z * (-0.0539682540f + z * (0.0218694885f - z * 0.00886323553f)))));
+    const float e = __builtin_amdgcn_exp2f(-2.f * LOG2E * a);
+    const float b = (1.f - e) * __builtin_amdgcn_rcpf(1.f + e);
+    return a < 0.35f ? s : copysignf(b, x);
+}
+
+// distance of two positions whose sign bit was flipped (order and differences of the unsigned values are theirs)
+__device__ __forceinline__ uint32_t flip(int32_t pos) { return (uint32_t)pos ^ 0x80000000u; }
+__device__ __forceinline__ float dist_of(uint32_t a, uint32_t b) { return (float)(max(a, b) - min(a, b)); }
+
+__device__ __forceinline__ float other_half(float x) { return __shfl_xor(x, 32, 64); }
+
+// Block b of a launch runs on XCD b % 8.  Runs of GS consecutive work items (tiles of one segment and head: they read
+// the same keys) go to one XCD, whose L2 then serves all but the first of them; the runs go round the XCDs in order.
+__device__ __forceinline__ int64_t xcd_item(int64_t b, int GS) {
+    const int64_t x = b & 7, i = b >> 3;
+    return ((i / GS) * 8 + x) * GS + i % GS;
+}
+inline int64_t xcd_grid(int64_t items, int GS) { return (items + 8 * GS - 1) / (8 * GS) * (8 * GS); }
+
+int check(const magic_attn *a);  // argument checks shared by the entry points
+
+}  // namespace attn
+}  // namespace magic

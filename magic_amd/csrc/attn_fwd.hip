@@ -1,0 +1,420 @@
+// Softmax attention of the rows of a segment over the keys of the same segment, forward (magic_attn_fwd).
+//   s = scale q.k,  c = cap tanh(s / cap) (cap > 0),  l = c - slope_h |pos_q - pos_k|,  p = softmax of l over the
+//   unmasked keys,  o = sum p v;   lse = log sum exp(l), -inf for a row that sees no key (o = 0 then).
+// One pass over the keys with a running maximum and sum per row; scores are formed transposed (keys x rows), so that a
+// lane owns ONE row's statistics and the probabilities feed the second product from their registers (attn_common.h).
+#include "attn_common.h"
+
+namespace magic {
+namespace attn {
+
+int check(const magic_attn *a) {
+    if (!a) return MAGIC_ERR_INVALID_ARG;
+    if (a->dtype != MAGIC_F32 && a->dtype != MAGIC_BF16) return MAGIC_ERR_UNSUPPORTED;
+    if (a->q_heads < 1 || a->kv_heads < 1 || a->q_heads % a->kv_heads || a->head_dim < 1) return MAGIC_ERR_INVALID_ARG;
+    if (a->head_dim > MAGIC_ATTN_MAX_DIM || a->head_dim % 8 || a->q_heads > 65535) return MAGIC_ERR_UNSUPPORTED;
+    if (a->n_q < 0 || a->n_k < 0 || a->n_q > 0x7fffffff || a->n_k > 0x7fffffff) return MAGIC_ERR_INVALID_ARG;
+    if (a->n_q_tiles < 0 || a->n_k_tiles < 0 || a->max_q < 0 || a->max_k < 0) return MAGIC_ERR_INVALID_ARG;
+    if (a->n_q > 0 && (!a->q || a->n_q_tiles < 1 || !a->q_tiles)) return MAGIC_ERR_INVALID_ARG;
+    if (a->n_k > 0 && (!a->k || !a->v)) return MAGIC_ERR_INVALID_ARG;
+    if (a->ld_q < 0 || a->hs_q < 0 || a->ld_k < 0 || a->hs_k < 0 || a->ld_v < 0 || a->hs_v < 0) return MAGIC_ERR_INVALID_ARG;
+    const int per = a->dtype == MAGIC_F32 ? 4 : 8;   // rows and heads start on 16-byte addresses
+    if (((uintptr_t)a->q | (uintptr_t)a->k | (uintptr_t)a->v) & 15) return MAGIC_ERR_INVALID_ARG;
+    if ((a->ld_q | a->hs_q | a->ld_k | a->hs_k | a->ld_v | a->hs_v) % per) return MAGIC_ERR_INVALID_ARG;
+    if (!(a->cap >= 0.f) || !(a->scale == a->scale)) return MAGIC_ERR_INVALID_ARG;
+    if (a->slopes && ((a->n_q > 0 && !a->q_pos) || (a->n_k > 0 && !a->k_pos))) return MAGIC_ERR_INVALID_ARG;
+    return MAGIC_OK;
+}
+
+}  // namespace attn
+}  // namespace magic
+
+namespace {
+
+using namespace magic::attn;
+using magic::bf16_t;
+using magic::bf16x8_t;
+
+struct FwdArgs {
+    magic_attn a;
+    void *out;
+    int64_t ld_o, hs_o;
+    float *lse;
+    int n_split;          // key ranges of a tile (1: results go straight to out / lse)
+    float *part_o;        // [n_split][q_heads][n_q][head_dim], normalised within the range
+    float *part_l;        // [n_split][q_heads][n_q], base-2 log of the range's sum
+    int cols, rows, gc;   // columns of a block's tile = rows x gc heads of one key head
+    int sub;              // blocks that share a 128-row tile of the table
+    int n_hb;             // head blocks: q_heads / gc
+    int64_t items;
+};
+
+// WM groups of 32 columns (rows, or rows x heads of one key head), KG groups of KW keys: a block of WM * KG wavefronts
+template <typename T, int DP, int WM, int KG, int KW>
+__global__ __launch_bounds__(64 * WM *KG, (DP == 128 && Planes<T>::N == 3) ? 1 : 2) void k_attn_fwd(FwdArgs p) {
+    constexpr int NP = Planes<T>::N, KS = DP / 16, DB = (DP + 31) / 32, BK = KG * KW, NT = 64 * WM * KG, KB = KW / 32;
+    typedef Stage<T, DP, BK, NT> stage;
+    typedef Tile<T, DP, BK> tile;
+    extern __shared__ __align__(16) unsigned char smem[];
+    bf16_t *sK = reinterpret_cast<bf16_t *>(smem), *sV = sK + NP * tile::PLANE;
+    uint32_t *sPos = reinterpret_cast<uint32_t *>(smem + 2 * tile::BYTES);
+    float *sMask = reinterpret_cast<float *>(sPos + BK);
+
+    const magic_attn &a = p.a;
+    const int64_t item = xcd_item(blockIdx.x, 16);
+    if (item >= p.items) return;
+    const int D = a.head_dim, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, li = lane & 31, hf = lane >> 5;
+    const int wm = wave % WM, kg = wave / WM;
+    const int64_t per_hb = (int64_t)a.n_q_tiles * p.sub;
+    const int64_t ts = item % per_hb;
+    const int hb = (int)(item / per_hb % p.n_hb), split = (int)(item / (per_hb * p.n_hb));
+    const int32_t *t = a.q_tiles + 4 * (ts / p.sub);
+    const int nq = t[1] - (int)(ts % p.sub) * p.rows;     // rows left for this block and the ones behind it
+    if (nq <= 0) return;
+    const int64_t q0 = (int64_t)t[0] + (ts % p.sub) * p.rows, k0 = t[2];
+    const int nk = t[3];
+    // this block's range of keys, in whole tiles
+    const int tiles = (nk + BK - 1) / BK, per = (tiles + p.n_split - 1) / p.n_split;
+    const int t_beg = split * per, t_end = min(t_beg + per, tiles);
+
+    const int col = wm * 32 + li;
+    const int row = col / p.gc, h = hb * p.gc + col % p.gc;
+    const bool ok = col < p.cols && row < nq && row < p.rows;
+    const int hk = hb * p.gc / (a.q_heads / a.kv_heads);
+    const T *K = (const T *)a.k + k0 * a.ld_k + hk * a.hs_k, *V = (const T *)a.v + k0 * a.ld_v + hk * a.hs_v;
+
+    bf16x8_t qf[KS][NP];
+    {
+        const T *q = (const T *)a.q + (q0 + (ok ? row : 0)) * a.ld_q + (ok ? h : hb * p.gc) * a.hs_q;
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks) {
+            Raw<T> r;
+            const int c = 16 * ks + 8 * hf;
+            r.load(q + (c < D ? c : 0));
+            if (!ok || c >= D) r.zero();
+            r.planes(qf[ks]);
+        }
+    }
+    const bool bias = a.slopes != nullptr;
+    const float slope2 = bias ? a.slopes[ok ? h : hb * p.gc] * LOG2E : 0.f;
+    const uint32_t qpos = bias ? flip(a.q_pos[q0 + (ok ? row : 0)]) : 0u;
+    const float s_in = a.cap > 0.f ? a.scale / a.cap : a.scale * LOG2E, s_out = a.cap * LOG2E;
+
+    f32x16_t o[DB];
+#pragma unroll
+    for (int d = 0; d < DB; ++d)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) o[d][r] = 0.f;
+    float m = -INFINITY, l = 0.f;  // of this lane's keys: the two halves of a wavefront share m and add l at the end
+
+    stage kst, vst;
+    uint8_t keep[stage::N];
+    uint32_t pos = 0;
+    float mk = 0.f;
+    auto load = [&](int tt) {
+        const int j0 = tt * BK;
+        kst.load(K, a.ld_k, j0, nk, D, tid);
+        vst.load(V, a.ld_v, j0, nk, D, tid);
+#pragma unroll
+        for (int i = 0; i < stage::N; ++i) {
+            const int j = j0 + stage::row_of(i, tid);
+            keep[i] = j < nk;
+            if (a.key_mask && j < nk) keep[i] = a.key_mask[k0 + j];
+        }
+        if (tid < BK) {
+            const int j = j0 + tid;
+            const bool in = j < nk;
+            mk = in && (!a.key_mask || a.key_mask[k0 + (in ? j : 0)]) ? 0.f : -INFINITY;
+            pos = bias && in ? flip(a.k_pos[k0 + j]) : 0u;
+        }
+    };
+    if (t_beg < t_end) load(t_beg);
+    for (int tt = t_beg; tt < t_end; ++tt) {
+        __syncthreads();  // the reads of the tile before are done
+        kst.store(sK, D, tid, [&](int i, int) { return keep[i] != 0; });
+        vst.store(sV, D, tid, [&](int i, int) { return keep[i] != 0; });
+        if (tid < BK) sPos[tid] = pos, sMask[tid] = mk;
+        const bool masked = a.key_mask != nullptr || (tt + 1) * BK > nk;
+        __syncthreads();
+        if (tt + 1 < t_end) load(tt + 1);
+
+        f32x16_t s[KB];
+#pragma unroll
+        for (int b = 0; b < KB; ++b)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) s[b][r] = 0.f;
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks)
+#pragma unroll
+            for (int b = 0; b < KB; ++b) {
+                bf16x8_t f[NP];
+                tile::frag(sK, kg * KW + 32 * b + li, 16 * ks + 8 * hf, f);
+                mma(s[b], f, qf[ks]);
+            }
+        // logits in base 2
+        if (a.cap > 0.f) {
+#pragma unroll
+            for (int b = 0; b < KB; ++b)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) s[b][r] = tanh_f(s[b][r] * s_in) * s_out;
+        } else {
+#pragma unroll
+            for (int b = 0; b < KB; ++b)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) s[b][r] *= s_in;
+        }
+        if (bias) {
+#pragma unroll
+            for (int b = 0; b < KB; ++b)
+#pragma unroll
+                for (int g = 0; g < 4; ++g) {
+                    const i32x4_t kp = *reinterpret_cast<const i32x4_t *>(sPos + kg * KW + 32 * b + 8 * g + 4 * hf);
+#pragma unroll
+                    for (int e = 0; e < 4; ++e)
+                        s[b][4 * g + e] -= slope2 * dist_of((uint32_t)kp[e], qpos);
+                }
+        }
+        if (masked) {
+#pragma unroll
+            for (int b = 0; b < KB; ++b)
+#pragma unroll
+                for (int g = 0; g < 4; ++g) {
+                    const f32x4_t km = *reinterpret_cast<const f32x4_t *>(sMask + kg * KW + 32 * b + 8 * g + 4 * hf);
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) s[b][4 * g + e] = km[e] == 0.f ? s[b][4 * g + e] : -INFINITY;
+                }
+        }
+        float mx = m;
+#pragma unroll
+        for (int b = 0; b < KB; ++b)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) mx = fmaxf(mx, s[b][r]);
+        mx = fmaxf(mx, other_half(mx));
+        const float ms = mx == -INFINITY ? 0.f : mx;
+        if (__any(mx != m)) {
+            const float al = __builtin_amdgcn_exp2f(m - ms);
+            l *= al;
+#pragma unroll
+            for (int d = 0; d < DB; ++d)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) o[d][r] *= al;
+            m = mx;
+        }
+#pragma unroll
+        for (int b = 0; b < KB; ++b)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) {
+                s[b][r] = __builtin_amdgcn_exp2f(s[b][r] - ms);
+                l += s[b][r];
+            }
+#pragma unroll
+        for (int b = 0; b < KB; ++b)
+#pragma unroll
+            for (int u = 0; u < 2; ++u) {
+                float x[8];
+#pragma unroll
+                for (int e = 0; e < 8; ++e) x[e] = s[b][8 * u + e];
+                bf16x8_t pf[NP];
+                to_planes(x, pf);
+#pragma unroll
+                for (int d = 0; d < DB; ++d) {
+                    bf16x8_t f[NP];
+                    tile::frag_t(sV, kg * KW + 32 * b + 16 * u, 32 * d, lane, f);
+                    mma(o[d], f, pf);
+                }
+            }
+    }
+    l += other_half(l);
+    if constexpr (KG > 1) {
+        // the key groups' (m, l, o) come together through LDS, in group order
+        __syncthreads();
+        float *sM = reinterpret_cast<float *>(smem), *sL = sM + KG * 32 * WM, *sO = sL + KG * 32 * WM;
+        constexpr int OW = DB * 32 + 1;
+        if (hf == 0) sM[(kg * WM + wm) * 32 + li] = m, sL[(kg * WM + wm) * 32 + li] = l;
+        __syncthreads();
+        float mt = -INFINITY, lt = 0.f;
+#pragma unroll
+        for (int g = 0; g < KG; ++g) mt = fmaxf(mt, sM[(g * WM + wm) * 32 + li]);
+        const float ms = mt == -INFINITY ? 0.f : mt;
+#pragma unroll
+        for (int g = 0; g < KG; ++g) lt += sL[(g * WM + wm) * 32 + li] * __builtin_amdgcn_exp2f(sM[(g * WM + wm) * 32 + li] - ms);
+        const float al = __builtin_amdgcn_exp2f(m - ms);
+        for (int g = KG - 1; g >= 1; --g) {
+            if (kg == g) {
+#pragma unroll
+                for (int d = 0; d < DB; ++d)
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) {
+                        float *q = sO + (wm * 32 + li) * OW + 32 * d + 8 * (r >> 2) + 4 * hf + (r & 3);
+                        *q = (g == KG - 1 ? 0.f : *q) + o[d][r] * al;
+                    }
+            }
+            __syncthreads();
+        }
+        if (kg != 0) return;
+#pragma unroll
+        for (int d = 0; d < DB; ++d)
+#pragma unroll
+            for (int r = 0; r < 16; ++r)
+                o[d][r] = o[d][r] * al + sO[(wm * 32 + li) * OW + 32 * d + 8 * (r >> 2) + 4 * hf + (r & 3)];
+        m = mt, l = lt;
+    }
+    if (!ok) return;
+    const float inv = l > 0.f || l != l ? 1.f / l : 0.f;
+    const float ls = m == -INFINITY && l == 0.f ? -INFINITY : m + __builtin_amdgcn_logf(l);   // base 2
+    if (p.n_split > 1) {
+        const int64_t base = ((int64_t)split * a.q_heads + h) * a.n_q + q0 + row;
+#pragma unroll
+        for (int d = 0; d < DB; ++d)
+#pragma unroll
+            for (int g = 0; g < 4; ++g) {
+                const int c = 32 * d + 8 * g + 4 * hf;
+                if (c < D)
+                    *reinterpret_cast<f32x4_t *>(p.part_o + base * D + c) =
+                        f32x4_t{o[d][4 * g] * inv, o[d][4 * g + 1] * inv, o[d][4 * g + 2] * inv, o[d][4 * g + 3] * inv};
+            }
+        if (hf == 0) p.part_l[base] = ls;
+        return;
+    }
+    T *out = (T *)p.out + (q0 + row) * p.ld_o + h * p.hs_o;
+#pragma unroll
+    for (int d = 0; d < DB; ++d)
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+            const int c = 32 * d + 8 * g + 4 * hf;
+            const float x[4] = {o[d][4 * g] * inv, o[d][4 * g + 1] * inv, o[d][4 * g + 2] * inv, o[d][4 * g + 3] * inv};
+            magic::store_vec<T, 4>(out + c, c < D, x);
+        }
+    if (hf == 0) p.lse[(int64_t)h * a.n_q + q0 + row] = ls * LN2;
+}
+
+// the key ranges of a row joined in order: o = sum_s 2^(l_s - l) o_s
+template <typename T> __global__ __launch_bounds__(256) void k_attn_join(FwdArgs p) {
+    const magic_attn &a = p.a;
+    const int cpr = a.head_dim / 4;
+    const int64_t total = a.n_q * a.q_heads * cpr, plane = a.n_q * a.q_heads;
+    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < total; i += (int64_t)gridDim.x * 256) {
+        const int64_t hr = i / cpr;                     // head * n_q + row
+        const int c = (int)(i - hr * cpr) * 4;
+        float m = -INFINITY;
+        for (int s = 0; s < p.n_split; ++s) {
+            const float x = p.part_l[s * plane + hr];
+            m = x > m || x != x ? x : m;
+        }
+        const float ms = m == -INFINITY ? 0.f : m;
+        float l = 0.f, o[4] = {0.f, 0.f, 0.f, 0.f};
+        for (int s = 0; s < p.n_split; ++s) {
+            const float w = __builtin_amdgcn_exp2f(p.part_l[s * plane + hr] - ms);
+            const f32x4_t x = *reinterpret_cast<const f32x4_t *>(p.part_o + (s * plane + hr) * a.head_dim + c);
+            l += w;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) o[e] += w * x[e];
+        }
+        const float inv = l > 0.f || l != l ? 1.f / l : 0.f;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) o[e] *= inv;
+        const int64_t h = hr / a.n_q, row = hr - h * a.n_q;
+        magic::store_vec<T, 4>((T *)p.out + row * p.ld_o + h * p.hs_o + c, true, o);
+        if (c == 0) p.lse[hr] = m == -INFINITY ? -INFINITY : (ms + __builtin_amdgcn_logf(l)) * LN2;
+    }
+}
+
+struct Shape {
+    int wm, n_split, cols, rows, gc, sub, n_hb;
+    int64_t items;
+};
+
+// How a call is cut: 128 rows of one head a block, or 32 (row, head) columns with the keys dealt to its wavefronts; then
+// key ranges until there are enough blocks.
+Shape shape_of(const magic_attn *a) {
+    Shape s;
+    const int G = a->q_heads / a->kv_heads;
+    const int64_t big = (int64_t)a->n_q_tiles * a->q_heads;
+    s.wm = big >= 256 && a->max_q > 32 ? 4 : 1;
+    if (s.wm == 4) {
+        s.gc = 1, s.cols = s.rows = 128;
+    } else {
+        s.gc = G;
+        while (s.gc > 32 || G % s.gc) --s.gc;          // heads of a key head that share its tile
+        s.rows = 32 / s.gc, s.cols = s.rows * s.gc;
+    }
+    const int longest = a->max_q < MAGIC_ATTN_TILE ? a->max_q : MAGIC_ATTN_TILE;   // rows of the fullest table entry
+    s.sub = (longest + s.rows - 1) / s.rows;
+    if (s.sub < 1) s.sub = 1;
+    s.n_hb = a->q_heads / s.gc;
+    const int64_t blocks = (int64_t)a->n_q_tiles * s.sub * s.n_hb;
+    int64_t split = (512 + blocks - 1) / blocks;
+    const int64_t most = (a->max_k + 511) / 512;
+    if (split > most) split = most;
+    if (split > 256) split = 256;
+    if (split < 1) split = 1;
+    s.n_split = (int)split;
+    s.items = blocks * split;
+    return s;
+}
+
+template <typename T, int DP, int WM, int KG, int KW> int launch(FwdArgs &p, hipStream_t st) {
+    typedef Tile<T, DP, KG * KW> tile;
+    size_t lds = 2 * tile::BYTES + KG * KW * 8;
+    const size_t join = (size_t)KG * 32 * WM * 8 + (size_t)32 * WM * ((DP + 31) / 32 * 32 + 1) * 4;
+    if (KG > 1 && join > lds) lds = join;
+    if (magic::ensure_dynamic_lds((const void *)k_attn_fwd<T, DP, WM, KG, KW>, lds) != MAGIC_OK) return MAGIC_ERR_RUNTIME;
+    const int64_t grid = xcd_grid(p.items, 16);
+    if (grid > 0x7fffffffLL) return MAGIC_ERR_UNSUPPORTED;
+    MAGIC_LAUNCH("attn_fwd", (k_attn_fwd<T, DP, WM, KG, KW>), (int)grid, 64 * WM * KG, lds, st, p);
+    return magic::launch_status();
+}
+
+template <typename T> int run(FwdArgs &p, int wm, hipStream_t st) {
+    const int D = p.a.head_dim;
+    int rc;
+    if (wm == 4) {
+        rc = D <= 16 ? launch<T, 16, 4, 1, 64>(p, st) : D <= 32 ? launch<T, 32, 4, 1, 64>(p, st)
+             : D <= 64 ? launch<T, 64, 4, 1, 64>(p, st) : launch<T, 128, 4, 1, 64>(p, st);
+    } else {
+        // (three planes of 128 keys and 128 columns would not fit the LDS)
+        constexpr int KG128 = Planes<T>::N == 3 ? 2 : 4;
+        rc = D <= 16 ? launch<T, 16, 1, 4, 32>(p, st) : D <= 32 ? launch<T, 32, 1, 4, 32>(p, st)
+             : D <= 64 ? launch<T, 64, 1, 4, 32>(p, st) : launch<T, 128, 1, KG128, 32>(p, st);
+    }
+    if (rc != MAGIC_OK || p.n_split == 1) return rc;
+    const int grid = magic::stride_grid(p.a.n_q * p.a.q_heads * (D / 4), 256);
+    MAGIC_LAUNCH("attn_join", k_attn_join<T>, grid, 256, 0, st, p);
+    return magic::launch_status();
+}
+
+}  // namespace
+
+extern "C" {
+
+size_t magic_attn_fwd_workspace_bytes(const magic_attn *a) {
+    if (check(a) != MAGIC_OK || a->n_q == 0) return 256;
+    const Shape s = shape_of(a);
+    if (s.n_split == 1) return 256;
+    const size_t rows = (size_t)s.n_split * a->q_heads * a->n_q;
+    return magic::align_up(rows * a->head_dim * sizeof(float)) + magic::align_up(rows * sizeof(float)) + 256;
+}
+
+int magic_attn_fwd(const magic_attn *a, void *out, int64_t ld_out, int64_t hs_out, float *lse, void *workspace,
+                   size_t workspace_bytes, void *stream) {
+    const int st = check(a);
+    if (st != MAGIC_OK || a->n_q == 0) return st;
+    const int per = a->dtype == MAGIC_F32 ? 4 : 8;
+    if (!out || !lse || ((uintptr_t)out & 15) || ld_out < 0 || hs_out < 0 || (ld_out | hs_out) % per) return MAGIC_ERR_INVALID_ARG;
+    const Shape s = shape_of(a);
+    FwdArgs p;
+    p.a = *a;
+    p.out = out, p.ld_o = ld_out, p.hs_o = hs_out, p.lse = lse;
+    p.n_split = s.n_split, p.cols = s.cols, p.rows = s.rows, p.gc = s.gc, p.sub = s.sub, p.n_hb = s.n_hb, p.items = s.items;
+    p.part_o = p.part_l = nullptr;
+    if (s.n_split > 1) {
+        magic::Arena ar(workspace, workspace_bytes);
+        const size_t rows = (size_t)s.n_split * a->q_heads * a->n_q;
+        p.part_o = ar.take<float>(rows * a->head_dim);
+        p.part_l = ar.take<float>(rows);
+        if (!ar.ok()) return MAGIC_ERR_WORKSPACE;
+    }
+    return a->dtype == MAGIC_F32 ? run<float>(p, s.wm, (hipStream_t)stream) : run<bf16_t>(p, s.wm, (hipStream_t)stream);
+}
+
+}  // extern "C"

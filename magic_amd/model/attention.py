@@ -32,6 +32,7 @@ class AttentionPlan:
     def __init__(self, q_lens, kv_lens, q_tiles, k_tiles):
         self.q_lens, self.kv_lens = q_lens, kv_lens
         self.n_q, self.n_k = sum(q_lens), sum(kv_lens)
+        self.max_q, self.max_k = max(q_lens, default=0), max(kv_lens, default=0)
         self.q_tiles, self.k_tiles = q_tiles, k_tiles
 
     @property
