@@ -581,9 +581,9 @@ int magic_knn_merge(int64_t n_query, int32_t k, int32_t n_parts,
  * MAGIC_BF16 (products of bf16 values, probabilities and score gradients rounded to bf16 before
  * their products; every sum and statistic in fp32).  key_mask [n_k]: 0 = the key takes no part
  * (whatever its rows hold).  A row that sees no key gets o = 0, lse = -inf and zero gradients.
- * The work comes as two device tables of the segments' tiles, four int32 each:
- *   q_tiles: {first q row, rows (1..MAGIC_ATTN_TILE), first key row of the segment, its keys}
- *   k_tiles: {first key row, keys (1..MAGIC_ATTN_TILE), first q row of the segment, its rows}
+ * The work comes as two device tables of the segments' tiles, eight int32 each (the last three are not read):
+ *   q_tiles: {first q row, rows (1..MAGIC_ATTN_TILE), first key row of the segment, its keys, segment}
+ *   k_tiles: {first key row, keys (1..MAGIC_ATTN_TILE), first q row of the segment, its rows, segment}
  * that cover every row of q (k) exactly once.
  * lse [q_heads, n_q] (natural logarithm) is what _bwd needs beside out.  dq [n_q,q_heads,D],
  * dk, dv [n_k,kv_heads,D] contiguous in the operands' type; d_slopes [q_heads] or NULL.  dq may be NULL when it (and
@@ -607,6 +607,7 @@ typedef struct magic_attn {
     const int32_t *q_tiles, *k_tiles;
     int32_t n_q_tiles, n_k_tiles;
     int32_t max_q, max_k;              /* the longest segment's rows and keys */
+    int32_t n_seg;                     /* segments: 0 .. n_seg - 1 appear in the tables */
 } magic_attn;
 size_t magic_attn_fwd_workspace_bytes(const magic_attn *args /* host */);
 int magic_attn_fwd(const magic_attn *args /* host struct of device pointers */, void *out, int64_t ld_out, int64_t hs_out,

@@ -39,7 +39,7 @@ class MagicAttn(C.Structure):
                 ("n_k", c_i64), ("q", c_vp), ("ld_q", c_i64), ("hs_q", c_i64), ("k", c_vp), ("ld_k", c_i64),
                 ("hs_k", c_i64), ("v", c_vp), ("ld_v", c_i64), ("hs_v", c_i64), ("scale", c_f32), ("cap", c_f32),
                 ("slopes", c_vp), ("q_pos", c_vp), ("k_pos", c_vp), ("key_mask", c_vp), ("q_tiles", c_vp),
-                ("k_tiles", c_vp), ("n_q_tiles", c_i32), ("n_k_tiles", c_i32), ("max_q", c_i32), ("max_k", c_i32)]
+                ("k_tiles", c_vp), ("n_q_tiles", c_i32), ("n_k_tiles", c_i32), ("max_q", c_i32), ("max_k", c_i32), ("n_seg", c_i32)]
 
 
 # name -> (restype, argtypes); must list every symbol include/magic_hip.h declares
@@ -1025,7 +1025,7 @@ def _attn_args(q, k, v, plan, scale, cap, slopes, q_pos, k_pos, key_mask) -> Mag
         a.key_mask = key_mask.data_ptr()
     a.q_tiles, a.n_q_tiles = plan.q_tiles.data_ptr(), plan.q_tiles.shape[0]
     a.k_tiles, a.n_k_tiles = plan.k_tiles.data_ptr(), plan.k_tiles.shape[0]
-    a.max_q, a.max_k = plan.max_q, plan.max_k
+    a.max_q, a.max_k, a.n_seg = plan.max_q, plan.max_k, plan.n_seg
     return a
 
 

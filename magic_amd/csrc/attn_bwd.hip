@@ -10,7 +10,6 @@ namespace {
 
 using namespace magic::attn;
 using magic::bf16_t;
-using magic::bf16x8_t;
 
 struct BwdArgs {
     magic_attn a;
@@ -22,6 +21,9 @@ struct BwdArgs {
     void *dq, *dk, *dv;
     float *slope_part;  // [n_q tiles][q_heads] or NULL
     int64_t items;
+    Ranges rg;
+    int n_split;        // shares of the rows a key tile's sums are cut into (1: they go straight to dk / dv)
+    float *part;        // [n_split][dk | dv][n_k][kv_heads][head_dim]
 };
 
 // lse2 and D of every row: DP / 8 lanes a row and head
@@ -55,23 +57,66 @@ template <typename T, int DP> __global__ __launch_bounds__(256) void k_attn_delt
     }
 }
 
-// p and ds of one 32 x 32 tile in place: s = scores before the scale, dp = do.v; the lane's column carries `cl`-side
-// values, the four registers of a group the row-side ones
-struct Soft {
-    float s_in, s_out, scale, cap;
-    __device__ __forceinline__ void init(const magic_attn &a) {
-        cap = a.cap, scale = a.scale;
-        s_in = cap > 0.f ? a.scale / cap : a.scale * LOG2E, s_out = cap * LOG2E;
+// Powers of two on the operands of a segment and head (1 unless the mode is scaled) and what undoes them
+struct Scales {
+    float q = 1.f, k = 1.f, v = 1.f, g = 1.f;
+    float s_in, s_out, dp_in;
+    // heads h .. h + n - 1, which share key head hk, take one kind and one scale
+    template <typename M>
+    __device__ __forceinline__ bool init(const Ranges &rg, int h, int n, int hk, int seg, const magic_attn &a) {
+        if (rg.q) {
+            const Range rk = rg.k[hk * rg.n_seg + seg], rv = rg.v[hk * rg.n_seg + seg];
+            Range rq = {0u, 0xffffffffu}, rr = rq;
+            for (int i = h; i < h + n; ++i) {
+                const Range x = rg.q[i * rg.n_seg + seg], y = rg.g[i * rg.n_seg + seg];
+                rq.max = max(rq.max, x.max), rq.min = min(rq.min, x.min);
+                rr.max = max(rr.max, y.max), rr.min = min(rr.min, y.min);
+            }
+            if ((range_ok(rq) && range_ok(rk) && range_ok(rv) && range_ok(rr)) != rg.want_safe) return false;
+            if constexpr (M::SCALED) q = range_scale(rq), k = range_scale(rk), v = range_scale(rv), g = range_scale(rr);
+        }
+        s_in = (a.cap > 0.f ? a.scale / a.cap : a.scale * LOG2E) * (1.f / q * (1.f / k));
+        s_out = a.cap * LOG2E;
+        dp_in = 1.f / v * (1.f / g);
+        return true;
     }
 };
 
-constexpr int NT = 256, BK = 64;
+// Score gradients as operand planes.  In the scaled mode a lane (a column of the product's result) carries a power of
+// two `u` that keeps its largest value so far at most 2^14 and its results in units of it; a larger value lowers u and
+// the results with it.
+struct Running {
+    float u = 0.f;   // 0: nothing seen yet
+    template <int DB> __device__ __forceinline__ void step(const float (&x)[16], f32x16_t (&acc)[DB]) {
+        float m = 0.f;
+#pragma unroll
+        for (int e = 0; e < 16; ++e) m = fmaxf(m, fabsf(x[e]));
+        m = fmaxf(m, other_half(m));
+        const bool grow = m > 0.f && (u == 0.f || m * u > 16384.f);
+        if (__any(grow)) {
+            int e = 13 + 127 - (int)(__float_as_uint(m) >> 23);                     // brings m to [2^13, 2^14)
+            e = e > 120 ? 120 : e < -120 ? -120 : e;
+            const float un = grow ? __uint_as_float((uint32_t)(e + 127) << 23) : u;
+            const float f = u == 0.f ? 1.f : un / u;
+            u = un;
+#pragma unroll
+            for (int d = 0; d < DB; ++d)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) acc[d][r] *= f;
+        }
+    }
+    __device__ __forceinline__ float undo() const { return u == 0.f ? 0.f : 1.f / u; }
+};
 
-template <typename T, int DP>
-__global__ __launch_bounds__(NT, (DP == 128 && Planes<T>::N == 3) ? 1 : 2) void k_attn_dq(BwdArgs p) {
-    constexpr int NP = Planes<T>::N, KS = DP / 16, DB = (DP + 31) / 32;
-    typedef Stage<T, DP, BK, NT> stage;
-    typedef Tile<T, DP, BK> tile;
+constexpr int NT = 256;
+
+template <typename M, int DP, int BK>
+__global__ __launch_bounds__(NT, (DP == 128 && M::N > 1) ? 1 : 2) void k_attn_dq(BwdArgs p) {
+    typedef typename M::T T;
+    typedef typename M::vec vec;
+    constexpr int NP = M::N, KS = DP / 16, DB = (DP + 31) / 32;
+    typedef Stage<M, DP, BK, NT> stage;
+    typedef Tile<M, DP, BK> tile;
     extern __shared__ __align__(16) unsigned char smem[];
     bf16_t *sK = reinterpret_cast<bf16_t *>(smem), *sV = sK + NP * tile::PLANE;
     uint32_t *sPos = reinterpret_cast<uint32_t *>(smem + 2 * tile::BYTES);
@@ -83,7 +128,7 @@ __global__ __launch_bounds__(NT, (DP == 128 && Planes<T>::N == 3) ? 1 : 2) void 
     const int D = a.head_dim, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, li = lane & 31, hf = lane >> 5;
     const int64_t tl = item % a.n_q_tiles;
     const int h = (int)(item / a.n_q_tiles), hk = h / (a.q_heads / a.kv_heads);
-    const int32_t *t = a.q_tiles + 4 * tl;
+    const int32_t *t = a.q_tiles + TAB * tl;
     const int64_t q0 = t[0], k0 = t[2];
     const int nq = t[1], nk = t[3];
     const int row = wave * 32 + li;
@@ -93,7 +138,9 @@ __global__ __launch_bounds__(NT, (DP == 128 && Planes<T>::N == 3) ? 1 : 2) void 
     const float ls = ok ? p.lse2[(int64_t)h * a.n_q + qr] : INFINITY, dl0 = ok ? p.delta[(int64_t)h * a.n_q + qr] : 0.f;
     const bool live = ls != INFINITY;
 
-    bf16x8_t qf[KS][NP], gf[KS][NP];
+    Scales sc;
+    if (!sc.init<M>(p.rg, h, 1, hk, t[4], a)) return;          // the other launch's segment
+    vec qf[KS][NP], gf[KS][NP];
 #pragma unroll
     for (int ks = 0; ks < KS; ++ks) {
         const int c = 16 * ks + 8 * hf, cc = c < D ? c : 0;
@@ -102,14 +149,13 @@ __global__ __launch_bounds__(NT, (DP == 128 && Planes<T>::N == 3) ? 1 : 2) void 
         g.load((const T *)p.dout + qr * p.ld_do + h * p.hs_do + cc);
         if (!ok || c >= D) r.zero();
         if (!live || c >= D) g.zero();
-        r.planes(qf[ks]);
-        g.planes(gf[ks]);
+        r.planes(qf[ks], sc.q);
+        g.planes(gf[ks], sc.g);
     }
     const bool bias = a.slopes != nullptr;
     const float slope2 = bias ? a.slopes[h] * LOG2E : 0.f;
     const uint32_t qpos = bias ? flip(a.q_pos[qr]) : 0u;
-    Soft sf;
-    sf.init(a);
+    Running run;
     float dsl = 0.f;
     f32x16_t acc[DB];
 #pragma unroll
@@ -133,73 +179,83 @@ __global__ __launch_bounds__(NT, (DP == 128 && Planes<T>::N == 3) ? 1 : 2) void 
         if (tid < BK) {
             const int j = j0 + tid;
             const bool in = j < nk;
-            mk = in && (!a.key_mask || a.key_mask[k0 + (in ? j : 0)]) ? 1.f : 0.f;
+            mk = in && (!a.key_mask || a.key_mask[k0 + (in ? j : 0)]) ? 0.f : -INFINITY;
             pos = bias && in ? flip(a.k_pos[k0 + j]) : 0u;
         }
     };
     if (nk > 0) load(0);
     for (int j0 = 0; j0 < nk; j0 += BK) {
         __syncthreads();
-        kst.store(sK, D, tid, [&](int i, int) { return keep[i] != 0; });
-        vst.store(sV, D, tid, [&](int i, int) { return keep[i] != 0; });
+        kst.store(sK, D, tid, sc.k, [&](int i, int) { return keep[i] != 0; });
+        vst.store(sV, D, tid, sc.v, [&](int i, int) { return keep[i] != 0; });
         if (tid < BK) sPos[tid] = pos, sMask[tid] = mk;
         const bool masked = a.key_mask != nullptr || j0 + BK > nk;
         __syncthreads();
         if (j0 + BK < nk) load(j0 + BK);
-#pragma unroll
+#pragma unroll 1
         for (int b = 0; b < BK / 32; ++b) {
             f32x16_t s, dp;
 #pragma unroll
             for (int r = 0; r < 16; ++r) s[r] = 0.f, dp[r] = 0.f;
 #pragma unroll
             for (int ks = 0; ks < KS; ++ks) {
-                bf16x8_t f[NP], g[NP];
+                vec f[NP], g[NP];
                 tile::frag(sK, 32 * b + li, 16 * ks + 8 * hf, f);
                 tile::frag(sV, 32 * b + li, 16 * ks + 8 * hf, g);
                 mma(s, f, qf[ks]);
                 mma(dp, g, gf[ks]);
             }
+            if (a.cap > 0.f) tanh_tile(s, sc.s_in);
+            float ds[16];
 #pragma unroll
-            for (int u = 0; u < 2; ++u) {
-                float ds[8];
+            for (int g = 0; g < 4; ++g) {
+                const int jr = 32 * b + 8 * g + 4 * hf;
+                f32x4_t base = {-ls, -ls, -ls, -ls};       // -inf for masked keys: their probabilities are zeros
+                if (masked) base += *reinterpret_cast<const f32x4_t *>(sMask + jr);
+                i32x4_t kp = {0, 0, 0, 0};
+                if (bias) kp = *reinterpret_cast<const i32x4_t *>(sPos + jr);
 #pragma unroll
-                for (int g = 0; g < 2; ++g) {
-                    const int jr = 32 * b + 16 * u + 8 * g + 4 * hf;
-                    f32x4_t km = {1.f, 1.f, 1.f, 1.f};
-                    if (masked) km = *reinterpret_cast<const f32x4_t *>(sMask + jr);
-                    i32x4_t kp = {0, 0, 0, 0};
-                    if (bias) kp = *reinterpret_cast<const i32x4_t *>(sPos + jr);
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        const int r = 8 * u + 4 * g + e;
-                        float x = s[r] * sf.s_in, f = sf.scale, dist = 0.f;
-                        if (sf.cap > 0.f) {
-                            const float th = tanh_f(x);
-                            x = th * sf.s_out;
-                            f *= 1.f - th * th;
-                        }
-                        if (bias) {
-                            dist = dist_of((uint32_t)kp[e], qpos);
-                            x -= slope2 * dist;
-                        }
-                        float pr = __builtin_amdgcn_exp2f(x - ls);
-                        float dl = pr * (dp[r] - dl0);
-                        if (km[e] == 0.f) dl = 0.f;
-                        if (bias) dsl -= dl * dist;
-                        ds[4 * g + e] = dl * f;
+                for (int e = 0; e < 4; ++e) {
+                    const int r = 4 * g + e;
+                    float f = a.scale, x;
+                    if (a.cap > 0.f) {
+                        x = fmaf(s[r], sc.s_out, base[e]);
+                        f -= f * s[r] * s[r];
+                    } else {
+                        x = fmaf(s[r], sc.s_in, base[e]);
                     }
+                    float dist = 0.f;
+                    if (bias) {
+                        dist = dist_of((uint32_t)kp[e], qpos);
+                        x = fmaf(-slope2, dist, x);
+                    }
+                    const float dl = __builtin_amdgcn_exp2f(x) * fmaf(dp[r], sc.dp_in, -dl0);
+                    if (bias) dsl -= dl * dist;
+                    ds[r] = dl * f;
                 }
-                bf16x8_t pf[NP];
-                to_planes(ds, pf);
+            }
+            float u = 1.f;
+            if constexpr (M::SCALED) {
+                run.step<DB>(ds, acc);
+                u = run.u;
+            }
+#pragma unroll
+            for (int w = 0; w < 2; ++w) {
+                float x[8];
+#pragma unroll
+                for (int e = 0; e < 8; ++e) x[e] = M::SCALED ? ds[8 * w + e] * u : ds[8 * w + e];
+                vec pf[NP];
+                to_planes(x, pf);
 #pragma unroll
                 for (int d = 0; d < DB; ++d) {
-                    bf16x8_t f[NP];
-                    tile::frag_t(sK, 32 * b + 16 * u, 32 * d, lane, f);
+                    vec f[NP];
+                    tile::frag_t(sK, 32 * b + 16 * w, 32 * d, lane, f);
                     mma(acc[d], f, pf);
                 }
             }
         }
     }
+    const float undo = M::SCALED ? run.undo() * (1.f / sc.k) : 1.f;
     if (ok) {
         T *o = (T *)p.dq + (qr * a.q_heads + h) * D;
 #pragma unroll
@@ -207,7 +263,7 @@ __global__ __launch_bounds__(NT, (DP == 128 && Planes<T>::N == 3) ? 1 : 2) void 
 #pragma unroll
             for (int g = 0; g < 4; ++g) {
                 const int c = 32 * d + 8 * g + 4 * hf;
-                const float x[4] = {acc[d][4 * g], acc[d][4 * g + 1], acc[d][4 * g + 2], acc[d][4 * g + 3]};
+                const float x[4] = {acc[d][4 * g] * undo, acc[d][4 * g + 1] * undo, acc[d][4 * g + 2] * undo, acc[d][4 * g + 3] * undo};
                 magic::store_vec<T, 4>(o + c, c < D, x);
             }
     }
@@ -222,11 +278,13 @@ __global__ __launch_bounds__(NT, (DP == 128 && Planes<T>::N == 3) ? 1 : 2) void 
     }
 }
 
-template <typename T, int DP, int BQ>
-__global__ __launch_bounds__(NT, (DP == 128 && Planes<T>::N == 3) ? 1 : 2) void k_attn_dkv(BwdArgs p) {
-    constexpr int NP = Planes<T>::N, KS = DP / 16, DB = (DP + 31) / 32;
-    typedef Stage<T, DP, BQ, NT> stage;
-    typedef Tile<T, DP, BQ> tile;
+template <typename M, int DP, int BQ>
+__global__ __launch_bounds__(NT, DP == 128 ? 1 : 2) void k_attn_dkv(BwdArgs p) {
+    typedef typename M::T T;
+    typedef typename M::vec vec;
+    constexpr int NP = M::N, KS = DP / 16, DB = (DP + 31) / 32;
+    typedef Stage<M, DP, BQ, NT> stage;
+    typedef Tile<M, DP, BQ> tile;
     extern __shared__ __align__(16) unsigned char smem[];
     bf16_t *sQ = reinterpret_cast<bf16_t *>(smem), *sG = sQ + NP * tile::PLANE;
     float *sL = reinterpret_cast<float *>(smem + 2 * tile::BYTES), *sD = sL + BQ;
@@ -237,8 +295,9 @@ __global__ __launch_bounds__(NT, (DP == 128 && Planes<T>::N == 3) ? 1 : 2) void 
     if (item >= p.items) return;
     const int D = a.head_dim, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, li = lane & 31, hf = lane >> 5;
     const int64_t tl = item % a.n_k_tiles;
-    const int hk = (int)(item / a.n_k_tiles), G = a.q_heads / a.kv_heads;
-    const int32_t *t = a.k_tiles + 4 * tl;
+    const int hk = (int)(item / a.n_k_tiles % a.kv_heads), G = a.q_heads / a.kv_heads;
+    const int split = (int)(item / ((int64_t)a.n_k_tiles * a.kv_heads));
+    const int32_t *t = a.k_tiles + TAB * tl;
     const int64_t k0 = t[0], q0 = t[2];
     const int nk = t[1], nq = t[3];
     const int col = wave * 32 + li;
@@ -246,7 +305,9 @@ __global__ __launch_bounds__(NT, (DP == 128 && Planes<T>::N == 3) ? 1 : 2) void 
     const int64_t kr = k0 + (in ? col : 0);
     const bool ok = in && (!a.key_mask || a.key_mask[kr]);
 
-    bf16x8_t kf[KS][NP], vf[KS][NP];
+    Scales sc;
+    if (!sc.init<M>(p.rg, hk * G, G, hk, t[4], a)) return;  // the other launch's segment
+    vec kf[KS][NP], vf[KS][NP];
 #pragma unroll
     for (int ks = 0; ks < KS; ++ks) {
         const int c = 16 * ks + 8 * hf, cc = c < D ? c : 0;
@@ -254,13 +315,12 @@ __global__ __launch_bounds__(NT, (DP == 128 && Planes<T>::N == 3) ? 1 : 2) void 
         r.load((const T *)a.k + kr * a.ld_k + hk * a.hs_k + cc);
         g.load((const T *)a.v + kr * a.ld_v + hk * a.hs_v + cc);
         if (!ok || c >= D) r.zero(), g.zero();
-        r.planes(kf[ks]);
-        g.planes(vf[ks]);
+        r.planes(kf[ks], sc.k);
+        g.planes(vf[ks], sc.v);
     }
     const bool bias = a.slopes != nullptr;
     const uint32_t kpos = bias ? flip(a.k_pos[kr]) : 0u;
-    Soft sf;
-    sf.init(a);
+    Running run;
     f32x16_t gk[DB], gv[DB];
 #pragma unroll
     for (int d = 0; d < DB; ++d)
@@ -282,77 +342,108 @@ __global__ __launch_bounds__(NT, (DP == 128 && Planes<T>::N == 3) ? 1 : 2) void 
         }
         if (tid < BQ) {
             const int r = i0 + tid;
-            ls = r < nq ? l2[r] : INFINITY;
-            dl0 = r < nq ? p.delta[(int64_t)h * a.n_q + q0 + r] : 0.f;
+            ls = r < nq ? -l2[r] : -INFINITY;
+            dl0 = r < nq ? -p.delta[(int64_t)h * a.n_q + q0 + r] : 0.f;
             pos = bias && r < nq ? flip(a.q_pos[q0 + r]) : 0u;
         }
     };
-    const int per_h = (nq + BQ - 1) / BQ, steps = per_h * G;
-    if (steps > 0) load(hk * G, 0);
-    int h = hk * G, it = 0;
-    for (int st = 0; st < steps; ++st) {
+    // this block's share of the steps (heads that share the key head, tiles of their rows)
+    const int per_h = (nq + BQ - 1) / BQ, steps = per_h * G, share = (steps + p.n_split - 1) / p.n_split;
+    const int s_beg = min(split * share, steps), s_end = min(s_beg + share, steps);
+    int h = hk * G + (per_h > 0 ? s_beg / per_h : 0), it = per_h > 0 ? s_beg % per_h : 0;
+    if (s_beg < s_end) load(h, it * BQ);
+    for (int st = s_beg; st < s_end; ++st) {
         __syncthreads();
-        qst.store(sQ, D, tid, [&](int i, int) { return keep[i] != 0; });
-        gst.store(sG, D, tid, [&](int i, int) { return keep[i] != 0; });
+        qst.store(sQ, D, tid, sc.q, [&](int i, int) { return keep[i] != 0; });
+        gst.store(sG, D, tid, sc.g, [&](int i, int) { return keep[i] != 0; });
         if (tid < BQ) sL[tid] = ls, sD[tid] = dl0, sPos[tid] = pos;
         const float slope2 = bias ? a.slopes[h] * LOG2E : 0.f;
         __syncthreads();
         if (++it == per_h) it = 0, ++h;
-        if (st + 1 < steps) load(h, it * BQ);
-#pragma unroll
+        if (st + 1 < s_end) load(h, it * BQ);
+#pragma unroll 1
         for (int b = 0; b < BQ / 32; ++b) {
             f32x16_t s, dp;
 #pragma unroll
             for (int r = 0; r < 16; ++r) s[r] = 0.f, dp[r] = 0.f;
 #pragma unroll
             for (int ks = 0; ks < KS; ++ks) {
-                bf16x8_t f[NP], g[NP];
+                vec f[NP], g[NP];
                 tile::frag(sQ, 32 * b + li, 16 * ks + 8 * hf, f);
                 tile::frag(sG, 32 * b + li, 16 * ks + 8 * hf, g);
                 mma(s, f, kf[ks]);
                 mma(dp, g, vf[ks]);
             }
+            if (a.cap > 0.f) tanh_tile(s, sc.s_in);
+            float pr[16], ds[16];
 #pragma unroll
-            for (int u = 0; u < 2; ++u) {
-                float pr[8], ds[8];
+            for (int g = 0; g < 4; ++g) {
+                const int ir = 32 * b + 8 * g + 4 * hf;
+                const f32x4_t l4 = *reinterpret_cast<const f32x4_t *>(sL + ir);      // -lse, -D of the rows
+                const f32x4_t d4 = *reinterpret_cast<const f32x4_t *>(sD + ir);
+                i32x4_t qp = {0, 0, 0, 0};
+                if (bias) qp = *reinterpret_cast<const i32x4_t *>(sPos + ir);
 #pragma unroll
-                for (int g = 0; g < 2; ++g) {
-                    const int ir = 32 * b + 16 * u + 8 * g + 4 * hf;
-                    const f32x4_t l4 = *reinterpret_cast<const f32x4_t *>(sL + ir);
-                    const f32x4_t d4 = *reinterpret_cast<const f32x4_t *>(sD + ir);
-                    i32x4_t qp = {0, 0, 0, 0};
-                    if (bias) qp = *reinterpret_cast<const i32x4_t *>(sPos + ir);
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        const int r = 8 * u + 4 * g + e;
-                        float x = s[r] * sf.s_in, f = sf.scale;
-                        if (sf.cap > 0.f) {
-                            const float th = tanh_f(x);
-                            x = th * sf.s_out;
-                            f *= 1.f - th * th;
-                        }
-                        if (bias) x -= slope2 * dist_of((uint32_t)qp[e], kpos);
-                        const float q = __builtin_amdgcn_exp2f(x - l4[e]);
-                        pr[4 * g + e] = q;
-                        ds[4 * g + e] = q * (dp[r] - d4[e]) * f;
+                for (int e = 0; e < 4; ++e) {
+                    const int r = 4 * g + e;
+                    float f = a.scale, x;
+                    if (a.cap > 0.f) {
+                        x = fmaf(s[r], sc.s_out, l4[e]);
+                        f -= f * s[r] * s[r];
+                    } else {
+                        x = fmaf(s[r], sc.s_in, l4[e]);
                     }
+                    if (bias) x = fmaf(-slope2, dist_of((uint32_t)qp[e], kpos), x);
+                    const float q = __builtin_amdgcn_exp2f(x);
+                    pr[r] = M::SCALED ? q * 16384.f : q;
+                    ds[r] = q * fmaf(dp[r], sc.dp_in, d4[e]) * f;
                 }
-                bf16x8_t pf[NP], sfr[NP];
-                to_planes(pr, pf);
-                to_planes(ds, sfr);
+            }
+            float u = 1.f;
+            if constexpr (M::SCALED) {
+                run.step<DB>(ds, gk);
+                u = run.u;
+            }
+#pragma unroll
+            for (int w = 0; w < 2; ++w) {
+                float x[8], y[8];
+#pragma unroll
+                for (int e = 0; e < 8; ++e) x[e] = pr[8 * w + e], y[e] = M::SCALED ? ds[8 * w + e] * u : ds[8 * w + e];
+                vec pf[NP], sf[NP];
+                to_planes(x, pf);
+                to_planes(y, sf);
 #pragma unroll
                 for (int d = 0; d < DB; ++d) {
-                    bf16x8_t f[NP];
-                    tile::frag_t(sG, 32 * b + 16 * u, 32 * d, lane, f);
+                    vec f[NP];
+                    tile::frag_t(sG, 32 * b + 16 * w, 32 * d, lane, f);
                     mma(gv[d], f, pf);
-                    tile::frag_t(sQ, 32 * b + 16 * u, 32 * d, lane, f);
-                    mma(gk[d], f, sfr);
+                    tile::frag_t(sQ, 32 * b + 16 * w, 32 * d, lane, f);
+                    mma(gk[d], f, sf);
                 }
             }
         }
     }
     if (!in) return;
-    T *ok_ = (T *)p.dk + (kr * a.kv_heads + hk) * D, *ov = (T *)p.dv + (kr * a.kv_heads + hk) * D;
+    const float uk = M::SCALED ? run.undo() * (1.f / sc.q) : 1.f, uv = M::SCALED ? 1.f / 16384.f * (1.f / sc.g) : 1.f;
+    const int64_t at = (kr * a.kv_heads + hk) * D;
+    if (p.n_split > 1) {
+        float *pk = p.part + (int64_t)split * 2 * a.n_k * a.kv_heads * D + at, *pv = pk + a.n_k * a.kv_heads * D;
+#pragma unroll
+        for (int d = 0; d < DB; ++d)
+#pragma unroll
+            for (int g = 0; g < 4; ++g) {
+                const int c = 32 * d + 8 * g + 4 * hf;
+                if (c < D) {
+                    f32x4_t x, y;
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) x[e] = ok ? gk[d][4 * g + e] * uk : 0.f, y[e] = ok ? gv[d][4 * g + e] * uv : 0.f;
+                    *reinterpret_cast<f32x4_t *>(pk + c) = x;
+                    *reinterpret_cast<f32x4_t *>(pv + c) = y;
+                }
+            }
+        return;
+    }
+    T *o_k = (T *)p.dk + at, *o_v = (T *)p.dv + at;
 #pragma unroll
     for (int d = 0; d < DB; ++d)
 #pragma unroll
@@ -360,10 +451,22 @@ __global__ __launch_bounds__(NT, (DP == 128 && Planes<T>::N == 3) ? 1 : 2) void 
             const int c = 32 * d + 8 * g + 4 * hf;
             float x[4], y[4];
 #pragma unroll
-            for (int e = 0; e < 4; ++e) x[e] = ok ? gk[d][4 * g + e] : 0.f, y[e] = ok ? gv[d][4 * g + e] : 0.f;
-            magic::store_vec<T, 4>(ok_ + c, c < D, x);
-            magic::store_vec<T, 4>(ov + c, c < D, y);
+            for (int e = 0; e < 4; ++e) x[e] = ok ? gk[d][4 * g + e] * uk : 0.f, y[e] = ok ? gv[d][4 * g + e] * uv : 0.f;
+            magic::store_vec<T, 4>(o_k + c, c < D, x);
+            magic::store_vec<T, 4>(o_v + c, c < D, y);
         }
+}
+
+// dk and dv from the shares of the rows, in order
+template <typename T> __global__ __launch_bounds__(256) void k_attn_dkv_join(BwdArgs p) {
+    const int64_t plane = p.a.n_k * p.a.kv_heads * p.a.head_dim, n4 = 2 * plane / 4;
+    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n4; i += (int64_t)gridDim.x * 256) {
+        f32x4_t x = {0.f, 0.f, 0.f, 0.f};
+        for (int s = 0; s < p.n_split; ++s) x += *reinterpret_cast<const f32x4_t *>(p.part + s * 2 * plane + 4 * i);
+        const float y[4] = {x[0], x[1], x[2], x[3]};
+        const int64_t e = 4 * i;
+        magic::store_vec<T, 4>(e < plane ? (T *)p.dk + e : (T *)p.dv + (e - plane), true, y);
+    }
 }
 
 // d slope of a head: the tile sums lane by lane, fixed tree, in double
@@ -375,33 +478,56 @@ __global__ __launch_bounds__(64) void k_attn_dslope(const float *part, int n, in
     if (threadIdx.x == 0) out[blockIdx.x] = (float)s;
 }
 
-template <typename T, int DP> int run(BwdArgs &b, hipStream_t st) {
+// rows of a staged tile: the ones that leave the kernels without register spills
+template <typename M, int DP> constexpr int BK_OF = 32;
+template <typename M, int DP> constexpr int BQ_OF = DP == 128 && M::N == 1 ? 64 : 32;
+
+template <typename M, int DP> int sweeps(BwdArgs &b, hipStream_t st) {
     const magic_attn &a = b.a;
-    constexpr int BQ = 64;
-    if (a.n_q > 0) {
-        const int grid = magic::stride_grid(a.n_q * a.q_heads, 256 / (DP / 8));
-        MAGIC_LAUNCH("attn_bwd_delta", (k_attn_delta<T, DP>), grid, 256, 0, st, b);
-    }
+    constexpr int BK = BK_OF<M, DP>, BQ = BQ_OF<M, DP>;
     if (a.n_q > 0 && b.dq) {
-        const size_t lds = 2 * Tile<T, DP, BK>::BYTES + BK * 8;
-        if (magic::ensure_dynamic_lds((const void *)k_attn_dq<T, DP>, lds) != MAGIC_OK) return MAGIC_ERR_RUNTIME;
+        const size_t lds = 2 * Tile<M, DP, BK>::BYTES + BK * 8;
+        if (magic::ensure_dynamic_lds((const void *)k_attn_dq<M, DP, BK>, lds) != MAGIC_OK) return MAGIC_ERR_RUNTIME;
         b.items = (int64_t)a.n_q_tiles * a.q_heads;
         if (xcd_grid(b.items, 16) > 0x7fffffffLL) return MAGIC_ERR_UNSUPPORTED;
-        MAGIC_LAUNCH("attn_bwd_dq", (k_attn_dq<T, DP>), (int)xcd_grid(b.items, 16), NT, lds, st, b);
+        MAGIC_LAUNCH(M::SCALED ? "attn_bwd_dq_f16x2" : "attn_bwd_dq", (k_attn_dq<M, DP, BK>), (int)xcd_grid(b.items, 16), NT,
+                     lds, st, b);
     }
     if (a.n_k > 0 && b.dk) {
-        const size_t lds = 2 * Tile<T, DP, BQ>::BYTES + BQ * 12;
-        if (magic::ensure_dynamic_lds((const void *)k_attn_dkv<T, DP, BQ>, lds) != MAGIC_OK) return MAGIC_ERR_RUNTIME;
-        b.items = (int64_t)a.n_k_tiles * a.kv_heads;
+        const size_t lds = 2 * Tile<M, DP, BQ>::BYTES + BQ * 12;
+        if (magic::ensure_dynamic_lds((const void *)k_attn_dkv<M, DP, BQ>, lds) != MAGIC_OK) return MAGIC_ERR_RUNTIME;
+        b.items = (int64_t)a.n_k_tiles * a.kv_heads * b.n_split;
         if (xcd_grid(b.items, 16) > 0x7fffffffLL) return MAGIC_ERR_UNSUPPORTED;
-        MAGIC_LAUNCH("attn_bwd_dkv", (k_attn_dkv<T, DP, BQ>), (int)xcd_grid(b.items, 16), NT, lds, st, b);
+        MAGIC_LAUNCH(M::SCALED ? "attn_bwd_dkv_f16x2" : "attn_bwd_dkv", (k_attn_dkv<M, DP, BQ>), (int)xcd_grid(b.items, 16), NT,
+                     lds, st, b);
     }
     return magic::launch_status();
 }
 
-template <typename T> int pick(BwdArgs &b, hipStream_t st) {
+template <typename M> int sweeps_of(BwdArgs &b, hipStream_t st) {
     const int D = b.a.head_dim;
-    return D <= 16 ? run<T, 16>(b, st) : D <= 32 ? run<T, 32>(b, st) : D <= 64 ? run<T, 64>(b, st) : run<T, 128>(b, st);
+    return D <= 16 ? sweeps<M, 16>(b, st) : D <= 32 ? sweeps<M, 32>(b, st) : D <= 64 ? sweeps<M, 64>(b, st) : sweeps<M, 128>(b, st);
+}
+
+template <typename T, int DP> int delta(BwdArgs &b, hipStream_t st) {
+    const int grid = magic::stride_grid(b.a.n_q * b.a.q_heads, 256 / (DP / 8));
+    MAGIC_LAUNCH("attn_bwd_delta", (k_attn_delta<T, DP>), grid, 256, 0, st, b);
+    return magic::launch_status();
+}
+template <typename T> int delta_of(BwdArgs &b, hipStream_t st) {
+    const int D = b.a.head_dim;
+    return D <= 16 ? delta<T, 16>(b, st) : D <= 32 ? delta<T, 32>(b, st) : D <= 64 ? delta<T, 64>(b, st) : delta<T, 128>(b, st);
+}
+
+// shares of the rows a key tile is cut into: enough blocks to fill the chip three times over (segments of very different
+// lengths leave long ones running alone otherwise), at least 512 (head, row) steps each
+int splits(const magic_attn *a) {
+    const int64_t blocks = (int64_t)a->n_k_tiles * a->kv_heads;
+    if (blocks <= 0) return 1;
+    int64_t s = (1536 + blocks - 1) / blocks;
+    const int64_t most = ((int64_t)a->max_q * (a->q_heads / a->kv_heads) + 511) / 512;
+    if (s > most) s = most;
+    return (int)(s < 1 ? 1 : s > 16 ? 16 : s);
 }
 
 }  // namespace
@@ -410,7 +536,9 @@ extern "C" {
 
 size_t magic_attn_bwd_workspace_bytes(const magic_attn *a) {
     if (check(a) != MAGIC_OK) return 256;
-    return 2 * magic::align_up((size_t)a->n_q * a->q_heads * sizeof(float)) +
+    const int n = splits(a);
+    const size_t part = n > 1 ? (size_t)n * 2 * a->n_k * a->kv_heads * a->head_dim * sizeof(float) : 0;
+    return magic::align_up(part) + (use_f16(a) ? magic::align_up(range_count(a, true) * sizeof(Range)) : 0) + 2 * magic::align_up((size_t)a->n_q * a->q_heads * sizeof(float)) +
            magic::align_up((size_t)a->n_q_tiles * a->q_heads * sizeof(float)) + 256;
 }
 
@@ -434,10 +562,34 @@ int magic_attn_bwd(const magic_attn *a, const void *out, int64_t ld_out, int64_t
     b.delta = ar.take<float>((size_t)a->n_q * a->q_heads);
     b.lse2 = ar.take<float>((size_t)a->n_q * a->q_heads);
     b.slope_part = ar.take<float>((size_t)a->n_q_tiles * a->q_heads);
+    const bool f16 = use_f16(a);
+    Range *ranges = f16 ? ar.take<Range>(range_count(a, true)) : nullptr;
+    b.n_split = dk ? splits(a) : 1;
+    b.part = b.n_split > 1 ? ar.take<float>((size_t)b.n_split * 2 * a->n_k * a->kv_heads * a->head_dim) : nullptr;
     if (!ar.ok()) return MAGIC_ERR_WORKSPACE;
     if (!d_slopes) b.slope_part = nullptr;
-    const int rc = a->dtype == MAGIC_F32 ? pick<float>(b, stream) : pick<bf16_t>(b, stream);
+    b.rg = Ranges{nullptr, nullptr, nullptr, nullptr, 0, false};
+    const bool f32 = a->dtype == MAGIC_F32;
+    int rc = MAGIC_OK;
+    if (a->n_q > 0) rc = f32 ? delta_of<float>(b, stream) : delta_of<bf16_t>(b, stream);
     if (rc != MAGIC_OK) return rc;
+    if (f16) {
+        rc = prepare_ranges(a, d_out, ld_do, hs_do, ranges, b.rg, stream);
+        if (rc != MAGIC_OK) return rc;
+        b.rg.want_safe = true;
+        rc = sweeps_of<F16x2>(b, stream);
+        if (rc != MAGIC_OK) return rc;
+        b.rg.want_safe = false;                // the segments whose rows differ too much in size
+    }
+    rc = f32 ? sweeps_of<F32x3>(b, stream) : sweeps_of<BF16>(b, stream);
+    if (rc != MAGIC_OK) return rc;
+    if (b.n_split > 1 && a->n_k > 0) {
+        const int grid = magic::stride_grid(a->n_k * a->kv_heads * a->head_dim / 2, 256);
+        if (f32)
+            MAGIC_LAUNCH("attn_dkv_join", k_attn_dkv_join<float>, grid, 256, 0, stream, b);
+        else
+            MAGIC_LAUNCH("attn_dkv_join", k_attn_dkv_join<bf16_t>, grid, 256, 0, stream, b);
+    }
     if (d_slopes)
         MAGIC_LAUNCH("attn_bwd_dslope", k_attn_dslope, a->q_heads, 64, 0, stream, b.slope_part, a->n_q > 0 ? a->n_q_tiles : 0,
                      a->q_heads, d_slopes);

@@ -27,9 +27,55 @@ typedef __bf16 bf16x4_t __attribute__((ext_vector_type(4)));
 constexpr float LOG2E = 1.44269504088896340736f;
 constexpr float LN2 = 0.69314718055994530942f;
 
-template <typename T> struct Planes;
-template <> struct Planes<float> { static constexpr int N = 3; };
-template <> struct Planes<bf16_t> { static constexpr int N = 1; };
+// How operands become matrix operands (16-bit planes):
+//   F32x3  float32 as three bf16 pieces, six products; exact pieces for any magnitude
+//   F16x2  float32 times a power of two as two fp16 pieces, three products (hi hi, hi lo, lo hi).  22 bits: with the
+//          operand's largest magnitude brought to [2^13, 2^14) a value keeps its error below 2^-22 relative or 2^-39 of
+//          that largest magnitude, whichever is more; what the dropped lo lo takes away is below 2^-22 of a product.
+//          Serves where the rows' magnitudes lie within 2^14 of each other (`Ranges`); F32x3 serves the rest.
+//   BF16   bfloat16, one plane, one product
+struct F32x3 {
+    typedef float T;
+    typedef bf16x8_t vec;
+    static constexpr int N = 3;
+    static constexpr bool SCALED = false;
+};
+typedef _Float16 f16x8_t __attribute__((ext_vector_type(8)));
+typedef _Float16 f16x2_t __attribute__((ext_vector_type(2)));
+struct F16x2 {
+    typedef float T;
+    typedef f16x8_t vec;
+    static constexpr int N = 2;
+    static constexpr bool SCALED = true;
+};
+struct BF16 {
+    typedef bf16_t T;
+    typedef bf16x8_t vec;
+    static constexpr int N = 1;
+    static constexpr bool SCALED = false;
+};
+
+__device__ __forceinline__ void split_f16(const float (&x)[8], f16x8_t (&p)[2]) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        const f32x2_t v = {x[2 * j], x[2 * j + 1]};
+        const f16x2_t h = __builtin_convertvector(v, f16x2_t);
+        const f32x2_t r = {v[0] - (float)h[0], v[1] - (float)h[1]};
+        const f16x2_t l = __builtin_convertvector(r, f16x2_t);
+        p[0][2 * j] = h[0], p[0][2 * j + 1] = h[1];
+        p[1][2 * j] = l[0], p[1][2 * j + 1] = l[1];
+    }
+}
+
+// eight float32 values -> operand planes
+__device__ __forceinline__ void to_planes(const float (&x)[8], bf16x8_t (&p)[3]) {
+    split8(make_float4(x[0], x[1], x[2], x[3]), make_float4(x[4], x[5], x[6], x[7]), p[0], p[1], p[2]);
+}
+__device__ __forceinline__ void to_planes(const float (&x)[8], f16x8_t (&p)[2]) { split_f16(x, p); }
+__device__ __forceinline__ void to_planes(const float (&x)[8], bf16x8_t (&p)[1]) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) p[0][e] = (bf16_t)x[e];
+}
 
 // eight consecutive elements of an operand row as they lie in memory
 template <typename T> struct Raw;
@@ -40,8 +86,13 @@ template <> struct Raw<float> {
         b = *reinterpret_cast<const f32x4_t *>(p + 4);
     }
     __device__ __forceinline__ void zero() { a = b = f32x4_t{0.f, 0.f, 0.f, 0.f}; }
-    __device__ __forceinline__ void planes(bf16x8_t (&p)[3]) const {
+    __device__ __forceinline__ void planes(bf16x8_t (&p)[3], float) const {
         split8(make_float4(a[0], a[1], a[2], a[3]), make_float4(b[0], b[1], b[2], b[3]), p[0], p[1], p[2]);
+    }
+    __device__ __forceinline__ void planes(f16x8_t (&p)[2], float scale) const {
+        const float x[8] = {a[0] * scale, a[1] * scale, a[2] * scale, a[3] * scale,
+                            b[0] * scale, b[1] * scale, b[2] * scale, b[3] * scale};
+        split_f16(x, p);
     }
     __device__ __forceinline__ void floats(float (&x)[8]) const {
 #pragma unroll
@@ -55,24 +106,20 @@ template <> struct Raw<bf16_t> {
 #pragma unroll
         for (int e = 0; e < 8; ++e) v[e] = (bf16_t)0.f;
     }
-    __device__ __forceinline__ void planes(bf16x8_t (&p)[1]) const { p[0] = v; }
+    __device__ __forceinline__ void planes(bf16x8_t (&p)[1], float) const { p[0] = v; }
     __device__ __forceinline__ void floats(float (&x)[8]) const {
 #pragma unroll
         for (int e = 0; e < 8; ++e) x[e] = (float)v[e];
     }
 };
 
-// eight float32 values -> operand planes of the next product: three exact pieces, or one rounding to bfloat16
-__device__ __forceinline__ void to_planes(const float (&x)[8], bf16x8_t (&p)[3]) {
-    split8(make_float4(x[0], x[1], x[2], x[3]), make_float4(x[4], x[5], x[6], x[7]), p[0], p[1], p[2]);
-}
-__device__ __forceinline__ void to_planes(const float (&x)[8], bf16x8_t (&p)[1]) {
-#pragma unroll
-    for (int e = 0; e < 8; ++e) p[0][e] = (bf16_t)x[e];
-}
-
 __device__ __forceinline__ void mma(f32x16_t &c, const bf16x8_t (&a)[3], const bf16x8_t (&b)[3]) {
     mfma_split6(c, a[0], a[1], a[2], b[0], b[1], b[2]);
+}
+__device__ __forceinline__ void mma(f32x16_t &c, const f16x8_t (&a)[2], const f16x8_t (&b)[2]) {
+    c = __builtin_amdgcn_mfma_f32_32x32x16_f16(a[1], b[0], c, 0, 0, 0);
+    c = __builtin_amdgcn_mfma_f32_32x32x16_f16(a[0], b[1], c, 0, 0, 0);
+    c = __builtin_amdgcn_mfma_f32_32x32x16_f16(a[0], b[0], c, 0, 0, 0);
 }
 __device__ __forceinline__ void mma(f32x16_t &c, const bf16x8_t (&a)[1], const bf16x8_t (&b)[1]) {
     c = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a[0], b[0], c, 0, 0, 0);
@@ -80,26 +127,27 @@ __device__ __forceinline__ void mma(f32x16_t &c, const bf16x8_t (&a)[1], const b
 
 // A tile of ROWS operand rows in LDS: planes of [ROWS][LDW] bf16, rows padded by 16 bytes (reads of one column range by
 // 32 rows then spread over the banks).
-template <typename T, int DP, int ROWS> struct Tile {
-    static constexpr int NP = Planes<T>::N;
+template <typename M, int DP, int ROWS> struct Tile {
+    typedef typename M::vec vec;
+    static constexpr int NP = M::N;
     static constexpr int W = DP < 32 ? 32 : DP;      // a transposed read covers 32 columns
     static constexpr int LDW = W + 8;
     static constexpr int PLANE = ROWS * LDW;
     static constexpr size_t BYTES = (size_t)NP * PLANE * 2;
 
-    static __device__ __forceinline__ void frag(const bf16_t *t, int row, int col, bf16x8_t (&f)[NP]) {
+    static __device__ __forceinline__ void frag(const bf16_t *t, int row, int col, vec (&f)[NP]) {
 #pragma unroll
-        for (int p = 0; p < NP; ++p) f[p] = *reinterpret_cast<const bf16x8_t *>(t + p * PLANE + row * LDW + col);
+        for (int p = 0; p < NP; ++p) f[p] = *reinterpret_cast<const vec *>(t + p * PLANE + row * LDW + col);
     }
     // transpose of rows r0 .. r0 + 15, columns c0 .. c0 + 31, inner order as described above
-    static __device__ __forceinline__ void frag_t(const bf16_t *t, int r0, int c0, int lane, bf16x8_t (&f)[NP]) {
+    static __device__ __forceinline__ void frag_t(const bf16_t *t, int r0, int c0, int lane, vec (&f)[NP]) {
         const int off = (r0 + 4 * (lane >> 5) + ((lane & 15) >> 2)) * LDW + c0 + 16 * ((lane >> 4) & 1) + 4 * (lane & 3);
 #pragma unroll
         for (int p = 0; p < NP; ++p) {
             typedef __attribute__((address_space(3))) s16x4_t *lds_ptr;
             union {
                 s16x4_t s[2];
-                bf16x8_t h;
+                vec h;
             } u;
             u.s[0] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_ptr)(t + p * PLANE + off));
             u.s[1] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_ptr)(t + p * PLANE + off + 8 * LDW));
@@ -109,8 +157,9 @@ template <typename T, int DP, int ROWS> struct Tile {
 };
 
 // Staging of a tile by NT threads: rows of DP columns (zeros behind D) in chunks of eight elements.
-template <typename T, int DP, int ROWS, int NT> struct Stage {
-    typedef Tile<T, DP, ROWS> tile;
+template <typename M, int DP, int ROWS, int NT> struct Stage {
+    typedef typename M::T T;
+    typedef Tile<M, DP, ROWS> tile;
     static constexpr int CPR = DP / 8;                          // chunks of a row
     static constexpr int TOTAL = ROWS * CPR;
     static constexpr int N = (TOTAL + NT - 1) / NT;
@@ -127,30 +176,50 @@ template <typename T, int DP, int ROWS, int NT> struct Stage {
         }
     }
     // keep(row of the tile): false -> zeros, whatever was read
-    template <typename Keep> __device__ __forceinline__ void store(bf16_t *t, int D, int tid, Keep keep) {
+    template <typename Keep> __device__ __forceinline__ void store(bf16_t *t, int D, int tid, float scale, Keep keep) {
 #pragma unroll
         for (int i = 0; i < N; ++i) {
             const int c = tid + i * NT;
             const int row = c / CPR, col = (c % CPR) * 8;
             if (TOTAL % NT != 0 && c >= TOTAL) break;
             if (!(keep(i, row) && col < D)) r[i].zero();
-            bf16x8_t p[tile::NP];
-            r[i].planes(p);
+            typename M::vec p[tile::NP];
+            r[i].planes(p, scale);
 #pragma unroll
             for (int k = 0; k < tile::NP; ++k)
-                *reinterpret_cast<bf16x8_t *>(t + k * tile::PLANE + row * tile::LDW + col) = p[k];
+                *reinterpret_cast<typename M::vec *>(t + k * tile::PLANE + row * tile::LDW + col) = p[k];
         }
     }
     __device__ __forceinline__ static int row_of(int i, int tid) { return (tid + i * NT) / CPR; }
 };
 
-// tanh to a few units of float32 relative: odd series near zero, (1 - e) / (1 + e) elsewhere
+// tanh to a few units of float32 relative: odd series below TANH_SMALL, (1 - e) / (1 + e) elsewhere
+constexpr float TANH_SMALL = 0.35f;
+__device__ __forceinline__ float tanh_series(float x) {
+    const float z = x * x;
+    return x * (1.f + z * (-0.333333333f + z * (0.133333333f + z * (-0.0539682540f + z * (0.0218694885f - z * 0.00886323553f)))));
+}
 __device__ __forceinline__ float tanh_f(float x) {
-    const float a = fabsf(x), z = x * x;
-    const float s = x * (1.f + z * (-0.333333333f + z * (0.133333333f + z * (-0.0539682540f + z * (0.0218694885f - z * 0.00886323553f)))));
+    const float a = fabsf(x);
     const float e = __builtin_amdgcn_exp2f(-2.f * LOG2E * a);
     const float b = (1.f - e) * __builtin_amdgcn_rcpf(1.f + e);
-    return a < 0.35f ? s : copysignf(b, x);
+    return a < TANH_SMALL ? tanh_series(x) : copysignf(b, x);
+}
+// x[i] = tanh(x[i] * f) of a tile; the series alone where no score of the wavefront leaves it (a cap is far above most scores)
+__device__ __forceinline__ void tanh_tile(f32x16_t &x, float f) {
+    float m = 0.f;
+#pragma unroll
+    for (int r = 0; r < 16; ++r) {
+        x[r] *= f;
+        m = fmaxf(m, fabsf(x[r]));
+    }
+    if (__any(m >= TANH_SMALL)) {
+#pragma unroll
+        for (int r = 0; r < 16; ++r) x[r] = tanh_f(x[r]);
+    } else {
+#pragma unroll
+        for (int r = 0; r < 16; ++r) x[r] = tanh_series(x[r]);
+    }
 }
 
 // distance of two positions whose sign bit was flipped (order and differences of the unsigned values are theirs)
@@ -168,6 +237,36 @@ __device__ __forceinline__ int64_t xcd_item(int64_t b, int GS) {
 inline int64_t xcd_grid(int64_t items, int GS) { return (items + 8 * GS - 1) / (8 * GS) * (8 * GS); }
 
 int check(const magic_attn *a);  // argument checks shared by the entry points
+
+// Largest magnitude of an operand and the smallest of its nonzero rows' largest ones, per head and segment, as the bits
+// of floats (finite values of the rows that take part; masked keys do not).  F16x2 serves a segment where max / min is
+// at most 2^14 in every operand: its absolute error of 2^-39 max is then below 2^-25 of any row's own largest value.
+struct Range {
+    uint32_t max, min;
+};
+struct Ranges {
+    const Range *q, *k, *v, *g;   // [heads][n_seg], NULL: not used
+    int n_seg;
+    bool want_safe;               // which segments this launch serves (NULL arrays: all)
+};
+__device__ __forceinline__ bool range_ok(Range r) {
+    // zero operands are fine; else exponents at most 14 apart
+    return r.max == 0u || ((r.max >> 23) <= (r.min >> 23) + 14u && (r.min >> 23) > 0u);
+}
+// power of two that brings the largest magnitude to [2^13, 2^14)
+__device__ __forceinline__ float range_scale(Range r) {
+    int e = 13 + 127 - (int)(r.max >> 23);       // exponent of the scale
+    if (r.max == 0u) e = 0;
+    e = e > 120 ? 120 : e;
+    return __uint_as_float((uint32_t)(e + 127) << 23);
+}
+
+// For a float32 call: whether F16x2 is tried, the number of Range entries, and the pass that fills them (with the
+// output's gradient g in backward).
+bool use_f16(const magic_attn *a);
+int64_t range_count(const magic_attn *a, bool grad);
+int prepare_ranges(const magic_attn *a, const void *g, int64_t ld_g, int64_t hs_g, Range *r, Ranges &rg, hipStream_t stream);
+constexpr int TAB = 8;            // int32 words of a tile-table entry
 
 }  // namespace attn
 }  // namespace magic

@@ -14,7 +14,7 @@ int check(const magic_attn *a) {
     if (a->q_heads < 1 || a->kv_heads < 1 || a->q_heads % a->kv_heads || a->head_dim < 1) return MAGIC_ERR_INVALID_ARG;
     if (a->head_dim > MAGIC_ATTN_MAX_DIM || a->head_dim % 8 || a->q_heads > 65535) return MAGIC_ERR_UNSUPPORTED;
     if (a->n_q < 0 || a->n_k < 0 || a->n_q > 0x7fffffff || a->n_k > 0x7fffffff) return MAGIC_ERR_INVALID_ARG;
-    if (a->n_q_tiles < 0 || a->n_k_tiles < 0 || a->max_q < 0 || a->max_k < 0) return MAGIC_ERR_INVALID_ARG;
+    if (a->n_q_tiles < 0 || a->n_k_tiles < 0 || a->max_q < 0 || a->max_k < 0 || a->n_seg < 0) return MAGIC_ERR_INVALID_ARG;
     if (a->n_q > 0 && (!a->q || a->n_q_tiles < 1 || !a->q_tiles)) return MAGIC_ERR_INVALID_ARG;
     if (a->n_k > 0 && (!a->k || !a->v)) return MAGIC_ERR_INVALID_ARG;
     if (a->ld_q < 0 || a->hs_q < 0 || a->ld_k < 0 || a->hs_k < 0 || a->ld_v < 0 || a->hs_v < 0) return MAGIC_ERR_INVALID_ARG;
@@ -24,6 +24,95 @@ int check(const magic_attn *a) {
     if (!(a->cap >= 0.f) || !(a->scale == a->scale)) return MAGIC_ERR_INVALID_ARG;
     if (a->slopes && ((a->n_q > 0 && !a->q_pos) || (a->n_k > 0 && !a->k_pos))) return MAGIC_ERR_INVALID_ARG;
     return MAGIC_OK;
+}
+
+namespace {
+
+__global__ __launch_bounds__(256) void k_range_init(Range *r, int64_t n) {
+    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256) r[i] = Range{0u, 0xffffffffu};
+}
+
+struct RangeArgs {
+    magic_attn a;
+    const void *g;
+    int64_t ld_g, hs_g;
+    Range *q, *k, *v, *gr;
+    int n_seg;
+};
+
+// block: a 128-row tile of one head of one operand, eight lanes a row.  Finite values only: an infinity or a NaN becomes
+// one in the planes whatever the scale.  (max and min do not depend on the order of the atomics.)
+__global__ __launch_bounds__(256) void k_range(RangeArgs r) {
+    const magic_attn &a = r.a;
+    int y = blockIdx.y;
+    const float *base;
+    int64_t ld, hs;
+    Range *out;
+    bool key = false;
+    if (y < a.q_heads) {
+        base = (const float *)a.q, ld = a.ld_q, hs = a.hs_q, out = r.q;
+    } else if ((y -= a.q_heads) < a.kv_heads) {
+        base = (const float *)a.k, ld = a.ld_k, hs = a.hs_k, out = r.k, key = true;
+    } else if ((y -= a.kv_heads) < a.kv_heads) {
+        base = (const float *)a.v, ld = a.ld_v, hs = a.hs_v, out = r.v, key = true;
+    } else {
+        y -= a.kv_heads;
+        base = (const float *)r.g, ld = r.ld_g, hs = r.hs_g, out = r.gr;
+    }
+    if ((int)blockIdx.x >= (key ? a.n_k_tiles : a.n_q_tiles)) return;
+    const int32_t *t = (key ? a.k_tiles : a.q_tiles) + TAB * (int64_t)blockIdx.x;
+    const int lane = threadIdx.x & 7;
+    uint32_t mx = 0u, mn = 0xffffffffu;
+    for (int i = threadIdx.x >> 3; i < t[1]; i += 32) {
+        const int64_t row = (int64_t)t[0] + i;
+        if (key && a.key_mask && !a.key_mask[row]) continue;
+        uint32_t m = 0u;
+        for (int c = 4 * lane; c < a.head_dim; c += 32) {
+            const f32x4_t x = *reinterpret_cast<const f32x4_t *>(base + row * ld + y * hs + c);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const uint32_t b = __float_as_uint(x[e]) & 0x7fffffffu;
+                m = b < 0x7f800000u && b > m ? b : m;
+            }
+        }
+#pragma unroll
+        for (int o = 4; o > 0; o >>= 1) m = max(m, (uint32_t)__shfl_xor((int)m, o, 8));
+        mx = max(mx, m);
+        if (m != 0u) mn = min(mn, m);
+    }
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) {
+        mx = max(mx, (uint32_t)__shfl_xor((int)mx, o, 64));
+        mn = min(mn, (uint32_t)__shfl_xor((int)mn, o, 64));
+    }
+    if ((threadIdx.x & 63) == 0 && mx != 0u) {
+        Range *d = out + (int64_t)y * r.n_seg + t[4];
+        atomicMax(&d->max, mx);
+        atomicMin(&d->min, mn);
+    }
+}
+
+}  // namespace
+
+// F16x2 needs a pass over the operands first: for float32 calls of enough work to pay for it (measured: see attn_fwd)
+bool use_f16(const magic_attn *a) { return a->dtype == MAGIC_F32 && a->head_dim > 32 && a->max_k >= 512 && a->n_seg > 0; }
+
+int64_t range_count(const magic_attn *a, bool grad) {
+    return ((grad ? 2 : 1) * (int64_t)a->q_heads + 2 * (int64_t)a->kv_heads) * a->n_seg;
+}
+
+int prepare_ranges(const magic_attn *a, const void *g, int64_t ld_g, int64_t hs_g, Range *r, Ranges &rg, hipStream_t stream) {
+    const int64_t n = range_count(a, g != nullptr);
+    RangeArgs ra;
+    ra.a = *a, ra.g = g, ra.ld_g = ld_g, ra.hs_g = hs_g, ra.n_seg = a->n_seg;
+    ra.q = r, ra.k = r + (int64_t)a->q_heads * a->n_seg, ra.v = ra.k + (int64_t)a->kv_heads * a->n_seg,
+    ra.gr = ra.v + (int64_t)a->kv_heads * a->n_seg;
+    rg = Ranges{ra.q, ra.k, ra.v, g ? ra.gr : nullptr, a->n_seg, true};
+    MAGIC_LAUNCH("attn_range_init", k_range_init, magic::stride_grid(n, 256), 256, 0, stream, r, n);
+    const int x = a->n_q_tiles > a->n_k_tiles ? a->n_q_tiles : a->n_k_tiles;
+    const int y = a->q_heads * (g ? 2 : 1) + 2 * a->kv_heads;
+    if (x > 0) MAGIC_LAUNCH("attn_range", k_range, dim3(x, y), 256, 0, stream, ra);
+    return magic::launch_status();
 }
 
 }  // namespace attn
@@ -47,14 +136,19 @@ struct FwdArgs {
     int sub;              // blocks that share a 128-row tile of the table
     int n_hb;             // head blocks: q_heads / gc
     int64_t items;
+    Ranges rg;
 };
 
+__device__ __forceinline__ int h_of(const FwdArgs &p, int hb) { return hb * p.gc; }
+
 // WM groups of 32 columns (rows, or rows x heads of one key head), KG groups of KW keys: a block of WM * KG wavefronts
-template <typename T, int DP, int WM, int KG, int KW>
-__global__ __launch_bounds__(64 * WM *KG, (DP == 128 && Planes<T>::N == 3) ? 1 : 2) void k_attn_fwd(FwdArgs p) {
-    constexpr int NP = Planes<T>::N, KS = DP / 16, DB = (DP + 31) / 32, BK = KG * KW, NT = 64 * WM * KG, KB = KW / 32;
-    typedef Stage<T, DP, BK, NT> stage;
-    typedef Tile<T, DP, BK> tile;
+template <typename M, int DP, int WM, int KG, int KW>
+__global__ __launch_bounds__(64 * WM *KG, (DP == 128 && M::N == 3) ? 1 : 2) void k_attn_fwd(FwdArgs p) {
+    typedef typename M::T T;
+    typedef typename M::vec vec;
+    constexpr int NP = M::N, KS = DP / 16, DB = (DP + 31) / 32, BK = KG * KW, NT = 64 * WM * KG, KB = KW / 32;
+    typedef Stage<M, DP, BK, NT> stage;
+    typedef Tile<M, DP, BK> tile;
     extern __shared__ __align__(16) unsigned char smem[];
     bf16_t *sK = reinterpret_cast<bf16_t *>(smem), *sV = sK + NP * tile::PLANE;
     uint32_t *sPos = reinterpret_cast<uint32_t *>(smem + 2 * tile::BYTES);
@@ -68,7 +162,7 @@ __global__ __launch_bounds__(64 * WM *KG, (DP == 128 && Planes<T>::N == 3) ? 1 :
     const int64_t per_hb = (int64_t)a.n_q_tiles * p.sub;
     const int64_t ts = item % per_hb;
     const int hb = (int)(item / per_hb % p.n_hb), split = (int)(item / (per_hb * p.n_hb));
-    const int32_t *t = a.q_tiles + 4 * (ts / p.sub);
+    const int32_t *t = a.q_tiles + TAB * (ts / p.sub);
     const int nq = t[1] - (int)(ts % p.sub) * p.rows;     // rows left for this block and the ones behind it
     if (nq <= 0) return;
     const int64_t q0 = (int64_t)t[0] + (ts % p.sub) * p.rows, k0 = t[2];
@@ -83,7 +177,14 @@ __global__ __launch_bounds__(64 * WM *KG, (DP == 128 && Planes<T>::N == 3) ? 1 :
     const int hk = hb * p.gc / (a.q_heads / a.kv_heads);
     const T *K = (const T *)a.k + k0 * a.ld_k + hk * a.hs_k, *V = (const T *)a.v + k0 * a.ld_v + hk * a.hs_v;
 
-    bf16x8_t qf[KS][NP];
+    float sq = 1.f, sk = 1.f, sv = 1.f;
+    if (p.rg.q) {
+        const Range rq = p.rg.q[h_of(p, hb) * p.rg.n_seg + t[4]], rk = p.rg.k[hk * p.rg.n_seg + t[4]],
+                    rv = p.rg.v[hk * p.rg.n_seg + t[4]];
+        if ((range_ok(rq) && range_ok(rk) && range_ok(rv)) != p.rg.want_safe) return;   // the other launch's segment
+        if constexpr (M::SCALED) sq = range_scale(rq), sk = range_scale(rk), sv = range_scale(rv);
+    }
+    vec qf[KS][NP];
     {
         const T *q = (const T *)a.q + (q0 + (ok ? row : 0)) * a.ld_q + (ok ? h : hb * p.gc) * a.hs_q;
 #pragma unroll
@@ -92,13 +193,15 @@ __global__ __launch_bounds__(64 * WM *KG, (DP == 128 && Planes<T>::N == 3) ? 1 :
             const int c = 16 * ks + 8 * hf;
             r.load(q + (c < D ? c : 0));
             if (!ok || c >= D) r.zero();
-            r.planes(qf[ks]);
+            r.planes(qf[ks], sq);
         }
     }
     const bool bias = a.slopes != nullptr;
     const float slope2 = bias ? a.slopes[ok ? h : hb * p.gc] * LOG2E : 0.f;
     const uint32_t qpos = bias ? flip(a.q_pos[q0 + (ok ? row : 0)]) : 0u;
-    const float s_in = a.cap > 0.f ? a.scale / a.cap : a.scale * LOG2E, s_out = a.cap * LOG2E;
+    const float unscale = 1.f / sq * (1.f / sk);
+    const float s_in = (a.cap > 0.f ? a.scale / a.cap : a.scale * LOG2E) * unscale, s_out = a.cap * LOG2E;
+    constexpr float P_EXP = M::SCALED ? 14.f : 0.f;       // probabilities are formed times 2^14
 
     f32x16_t o[DB];
 #pragma unroll
@@ -131,8 +234,8 @@ __global__ __launch_bounds__(64 * WM *KG, (DP == 128 && Planes<T>::N == 3) ? 1 :
     if (t_beg < t_end) load(t_beg);
     for (int tt = t_beg; tt < t_end; ++tt) {
         __syncthreads();  // the reads of the tile before are done
-        kst.store(sK, D, tid, [&](int i, int) { return keep[i] != 0; });
-        vst.store(sV, D, tid, [&](int i, int) { return keep[i] != 0; });
+        kst.store(sK, D, tid, sk, [&](int i, int) { return keep[i] != 0; });
+        vst.store(sV, D, tid, sv, [&](int i, int) { return keep[i] != 0; });
         if (tid < BK) sPos[tid] = pos, sMask[tid] = mk;
         const bool masked = a.key_mask != nullptr || (tt + 1) * BK > nk;
         __syncthreads();
@@ -147,42 +250,34 @@ __global__ __launch_bounds__(64 * WM *KG, (DP == 128 && Planes<T>::N == 3) ? 1 :
         for (int ks = 0; ks < KS; ++ks)
 #pragma unroll
             for (int b = 0; b < KB; ++b) {
-                bf16x8_t f[NP];
+                vec f[NP];
                 tile::frag(sK, kg * KW + 32 * b + li, 16 * ks + 8 * hf, f);
                 mma(s[b], f, qf[ks]);
             }
-        // logits in base 2
-        if (a.cap > 0.f) {
+        // logits in base 2; a masked key's zero score gets -inf
 #pragma unroll
-            for (int b = 0; b < KB; ++b)
-#pragma unroll
-                for (int r = 0; r < 16; ++r) s[b][r] = tanh_f(s[b][r] * s_in) * s_out;
-        } else {
-#pragma unroll
-            for (int b = 0; b < KB; ++b)
-#pragma unroll
-                for (int r = 0; r < 16; ++r) s[b][r] *= s_in;
-        }
-        if (bias) {
-#pragma unroll
-            for (int b = 0; b < KB; ++b)
-#pragma unroll
-                for (int g = 0; g < 4; ++g) {
-                    const i32x4_t kp = *reinterpret_cast<const i32x4_t *>(sPos + kg * KW + 32 * b + 8 * g + 4 * hf);
-#pragma unroll
-                    for (int e = 0; e < 4; ++e)
-                        s[b][4 * g + e] -= slope2 * dist_of((uint32_t)kp[e], qpos);
-                }
-        }
-        if (masked) {
-#pragma unroll
-            for (int b = 0; b < KB; ++b)
+        for (int b = 0; b < KB; ++b) {
+            const float f = a.cap > 0.f ? s_out : s_in;
+            if (a.cap > 0.f) tanh_tile(s[b], s_in);
+            if (masked) {
 #pragma unroll
                 for (int g = 0; g < 4; ++g) {
                     const f32x4_t km = *reinterpret_cast<const f32x4_t *>(sMask + kg * KW + 32 * b + 8 * g + 4 * hf);
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) s[b][4 * g + e] = km[e] == 0.f ? s[b][4 * g + e] : -INFINITY;
+                    for (int e = 0; e < 4; ++e) s[b][4 * g + e] = fmaf(s[b][4 * g + e], f, km[e]);
                 }
+            } else {
+#pragma unroll
+                for (int r = 0; r < 16; ++r) s[b][r] *= f;
+            }
+            if (bias) {
+#pragma unroll
+                for (int g = 0; g < 4; ++g) {
+                    const i32x4_t kp = *reinterpret_cast<const i32x4_t *>(sPos + kg * KW + 32 * b + 8 * g + 4 * hf);
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) s[b][4 * g + e] = fmaf(-slope2, dist_of((uint32_t)kp[e], qpos), s[b][4 * g + e]);
+                }
+            }
         }
         float mx = m;
 #pragma unroll
@@ -200,11 +295,12 @@ __global__ __launch_bounds__(64 * WM *KG, (DP == 128 && Planes<T>::N == 3) ? 1 :
                 for (int r = 0; r < 16; ++r) o[d][r] *= al;
             m = mx;
         }
+        const float mo = ms - P_EXP;
 #pragma unroll
         for (int b = 0; b < KB; ++b)
 #pragma unroll
             for (int r = 0; r < 16; ++r) {
-                s[b][r] = __builtin_amdgcn_exp2f(s[b][r] - ms);
+                s[b][r] = __builtin_amdgcn_exp2f(s[b][r] - mo);
                 l += s[b][r];
             }
 #pragma unroll
@@ -214,11 +310,11 @@ __global__ __launch_bounds__(64 * WM *KG, (DP == 128 && Planes<T>::N == 3) ? 1 :
                 float x[8];
 #pragma unroll
                 for (int e = 0; e < 8; ++e) x[e] = s[b][8 * u + e];
-                bf16x8_t pf[NP];
+                vec pf[NP];
                 to_planes(x, pf);
 #pragma unroll
                 for (int d = 0; d < DB; ++d) {
-                    bf16x8_t f[NP];
+                    vec f[NP];
                     tile::frag_t(sV, kg * KW + 32 * b + 16 * u, 32 * d, lane, f);
                     mma(o[d], f, pf);
                 }
@@ -260,8 +356,8 @@ __global__ __launch_bounds__(64 * WM *KG, (DP == 128 && Planes<T>::N == 3) ? 1 :
         m = mt, l = lt;
     }
     if (!ok) return;
-    const float inv = l > 0.f || l != l ? 1.f / l : 0.f;
-    const float ls = m == -INFINITY && l == 0.f ? -INFINITY : m + __builtin_amdgcn_logf(l);   // base 2
+    const float inv = l > 0.f || l != l ? 1.f / (l * sv) : 0.f;
+    const float ls = m == -INFINITY && l == 0.f ? -INFINITY : m + __builtin_amdgcn_logf(l) - P_EXP;   // base 2
     if (p.n_split > 1) {
         const int64_t base = ((int64_t)split * a.q_heads + h) * a.n_q + q0 + row;
 #pragma unroll
@@ -321,6 +417,7 @@ template <typename T> __global__ __launch_bounds__(256) void k_attn_join(FwdArgs
 
 struct Shape {
     int wm, n_split, cols, rows, gc, sub, n_hb;
+    bool f16;
     int64_t items;
 };
 
@@ -350,36 +447,46 @@ Shape shape_of(const magic_attn *a) {
     if (split < 1) split = 1;
     s.n_split = (int)split;
     s.items = blocks * split;
+    s.f16 = magic::attn::use_f16(a) && s.wm == 4 && s.n_split == 1;
     return s;
 }
 
-template <typename T, int DP, int WM, int KG, int KW> int launch(FwdArgs &p, hipStream_t st) {
-    typedef Tile<T, DP, KG * KW> tile;
+template <typename M, int DP, int WM, int KG, int KW> int launch(FwdArgs &p, hipStream_t st) {
+    typedef Tile<M, DP, KG * KW> tile;
     size_t lds = 2 * tile::BYTES + KG * KW * 8;
     const size_t join = (size_t)KG * 32 * WM * 8 + (size_t)32 * WM * ((DP + 31) / 32 * 32 + 1) * 4;
     if (KG > 1 && join > lds) lds = join;
-    if (magic::ensure_dynamic_lds((const void *)k_attn_fwd<T, DP, WM, KG, KW>, lds) != MAGIC_OK) return MAGIC_ERR_RUNTIME;
+    if (magic::ensure_dynamic_lds((const void *)k_attn_fwd<M, DP, WM, KG, KW>, lds) != MAGIC_OK) return MAGIC_ERR_RUNTIME;
     const int64_t grid = xcd_grid(p.items, 16);
     if (grid > 0x7fffffffLL) return MAGIC_ERR_UNSUPPORTED;
-    MAGIC_LAUNCH("attn_fwd", (k_attn_fwd<T, DP, WM, KG, KW>), (int)grid, 64 * WM * KG, lds, st, p);
+    MAGIC_LAUNCH(M::SCALED ? "attn_fwd_f16x2" : "attn_fwd", (k_attn_fwd<M, DP, WM, KG, KW>), (int)grid, 64 * WM * KG, lds, st, p);
     return magic::launch_status();
 }
 
-template <typename T> int run(FwdArgs &p, int wm, hipStream_t st) {
+template <typename M> int run_rows(FwdArgs &p, hipStream_t st) {
+    const int D = p.a.head_dim;
+    return D <= 16   ? launch<M, 16, 4, 1, 64>(p, st)
+           : D <= 32 ? launch<M, 32, 4, 1, 64>(p, st)
+           : D <= 64 ? launch<M, 64, 4, 1, 64>(p, st)
+                     : launch<M, 128, 4, 1, M::SCALED ? 32 : 64>(p, st);   // (64 keys would spill registers)
+}
+
+template <typename M> int run(FwdArgs &p, int wm, hipStream_t st) {
     const int D = p.a.head_dim;
     int rc;
     if (wm == 4) {
-        rc = D <= 16 ? launch<T, 16, 4, 1, 64>(p, st) : D <= 32 ? launch<T, 32, 4, 1, 64>(p, st)
-             : D <= 64 ? launch<T, 64, 4, 1, 64>(p, st) : launch<T, 128, 4, 1, 64>(p, st);
+        rc = run_rows<M>(p, st);
     } else {
         // (three planes of 128 keys and 128 columns would not fit the LDS)
-        constexpr int KG128 = Planes<T>::N == 3 ? 2 : 4;
-        rc = D <= 16 ? launch<T, 16, 1, 4, 32>(p, st) : D <= 32 ? launch<T, 32, 1, 4, 32>(p, st)
-             : D <= 64 ? launch<T, 64, 1, 4, 32>(p, st) : launch<T, 128, 1, KG128, 32>(p, st);
+        constexpr int KG128 = M::N == 3 ? 2 : 4;
+        rc = D <= 16   ? launch<M, 16, 1, 4, 32>(p, st)
+             : D <= 32 ? launch<M, 32, 1, 4, 32>(p, st)
+             : D <= 64 ? launch<M, 64, 1, 4, 32>(p, st)
+                       : launch<M, 128, 1, KG128, 32>(p, st);
     }
     if (rc != MAGIC_OK || p.n_split == 1) return rc;
     const int grid = magic::stride_grid(p.a.n_q * p.a.q_heads * (D / 4), 256);
-    MAGIC_LAUNCH("attn_join", k_attn_join<T>, grid, 256, 0, st, p);
+    MAGIC_LAUNCH("attn_join", k_attn_join<typename M::T>, grid, 256, 0, st, p);
     return magic::launch_status();
 }
 
@@ -390,6 +497,7 @@ extern "C" {
 size_t magic_attn_fwd_workspace_bytes(const magic_attn *a) {
     if (check(a) != MAGIC_OK || a->n_q == 0) return 256;
     const Shape s = shape_of(a);
+    if (s.f16) return magic::align_up(magic::attn::range_count(a, false) * sizeof(Range)) + 256;
     if (s.n_split == 1) return 256;
     const size_t rows = (size_t)s.n_split * a->q_heads * a->n_q;
     return magic::align_up(rows * a->head_dim * sizeof(float)) + magic::align_up(rows * sizeof(float)) + 256;
@@ -414,7 +522,20 @@ int magic_attn_fwd(const magic_attn *a, void *out, int64_t ld_out, int64_t hs_ou
         p.part_l = ar.take<float>(rows);
         if (!ar.ok()) return MAGIC_ERR_WORKSPACE;
     }
-    return a->dtype == MAGIC_F32 ? run<float>(p, s.wm, (hipStream_t)stream) : run<bf16_t>(p, s.wm, (hipStream_t)stream);
+    p.rg = Ranges{nullptr, nullptr, nullptr, nullptr, 0, false};
+    if (s.f16) {
+        magic::Arena ar(workspace, workspace_bytes);
+        Range *r = ar.take<Range>(magic::attn::range_count(a, false));
+        if (!ar.ok()) return MAGIC_ERR_WORKSPACE;
+        const int rc = magic::attn::prepare_ranges(a, nullptr, 0, 0, r, p.rg, (hipStream_t)stream);
+        if (rc != MAGIC_OK) return rc;
+        p.rg.want_safe = true;
+        const int rc2 = run_rows<F16x2>(p, (hipStream_t)stream);
+        if (rc2 != MAGIC_OK) return rc2;
+        p.rg.want_safe = false;                // the segments whose rows differ too much in size
+        return run_rows<F32x3>(p, (hipStream_t)stream);
+    }
+    return a->dtype == MAGIC_F32 ? run<F32x3>(p, s.wm, (hipStream_t)stream) : run<BF16>(p, s.wm, (hipStream_t)stream);
 }
 
 }  // extern "C"

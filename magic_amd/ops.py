@@ -468,28 +468,28 @@ _register("readout", "(Tensor feat, Tensor? node_type, int n_types, bool mean) -
 
 # ------------------------------------------------------------------------------------- global-attention block
 # The plan of segment attention travels as its two tile tables and longest segments; operands and results as in ``_lib.attn_fwd``.
-def _attn_plan(q, k, q_tiles, k_tiles, max_q, max_k):
+def _attn_plan(q, k, q_tiles, k_tiles, max_q, max_k, n_seg):
     return SimpleNamespace(q_tiles=q_tiles, k_tiles=k_tiles, n_q=q.shape[0], n_k=k.shape[0], device=q_tiles.device,
-                           max_q=max_q, max_k=max_k)
+                           max_q=max_q, max_k=max_k, n_seg=n_seg)
 
 
-_ATTN = "Tensor q, Tensor k, Tensor v, Tensor q_tiles, Tensor k_tiles, int max_q, int max_k, float scale, float cap, Tensor? slopes, " \
+_ATTN = "Tensor q, Tensor k, Tensor v, Tensor q_tiles, Tensor k_tiles, int max_q, int max_k, int n_seg, float scale, float cap, Tensor? slopes, " \
         "Tensor? q_pos, Tensor? k_pos, Tensor? key_mask"
 _register("attn_fwd", f"({_ATTN}) -> (Tensor, Tensor)",
-          lambda q, k, v, q_tiles, k_tiles, max_q, max_k, scale, cap, slopes, q_pos, k_pos, key_mask:
-          _lib.attn_fwd(q, k, v, _attn_plan(q, k, q_tiles, k_tiles, max_q, max_k), scale, cap, slopes, q_pos, k_pos, key_mask),
-          lambda q, k, v, q_tiles, k_tiles, max_q, max_k, scale, cap, slopes, q_pos, k_pos, key_mask:
+          lambda q, k, v, q_tiles, k_tiles, max_q, max_k, n_seg, scale, cap, slopes, q_pos, k_pos, key_mask:
+          _lib.attn_fwd(q, k, v, _attn_plan(q, k, q_tiles, k_tiles, max_q, max_k, n_seg), scale, cap, slopes, q_pos, k_pos, key_mask),
+          lambda q, k, v, q_tiles, k_tiles, max_q, max_k, n_seg, scale, cap, slopes, q_pos, k_pos, key_mask:
           (q.new_empty(q.shape), q.new_empty((q.shape[1], q.shape[0]), dtype=torch.float32)))
 
 
-def _attn_bwd(q, k, v, q_tiles, k_tiles, max_q: int, max_k: int, scale: float, cap: float, slopes, q_pos, k_pos, key_mask, out, lse, d_out):
-    dq, dk, dv, ds = _lib.attn_bwd(q, k, v, _attn_plan(q, k, q_tiles, k_tiles, max_q, max_k), scale, out, lse, d_out, cap, slopes, q_pos,
+def _attn_bwd(q, k, v, q_tiles, k_tiles, max_q: int, max_k: int, n_seg: int, scale: float, cap: float, slopes, q_pos, k_pos, key_mask, out, lse, d_out):
+    dq, dk, dv, ds = _lib.attn_bwd(q, k, v, _attn_plan(q, k, q_tiles, k_tiles, max_q, max_k, n_seg), scale, out, lse, d_out, cap, slopes, q_pos,
                                    k_pos, key_mask, need_dslopes=slopes is not None)
     return dq, dk, dv, ds if ds is not None else _empty(q)
 
 
 _register("attn_bwd", f"({_ATTN}, Tensor out, Tensor lse, Tensor d_out) -> (Tensor, Tensor, Tensor, Tensor)", _attn_bwd,
-          lambda q, k, v, q_tiles, k_tiles, max_q, max_k, scale, cap, slopes, q_pos, k_pos, key_mask, out, lse, d_out:
+          lambda q, k, v, q_tiles, k_tiles, max_q, max_k, n_seg, scale, cap, slopes, q_pos, k_pos, key_mask, out, lse, d_out:
           (q.new_empty(q.shape), k.new_empty(k.shape), v.new_empty(v.shape),
            q.new_empty(q.shape[1] if slopes is not None else 0, dtype=torch.float32)))
 

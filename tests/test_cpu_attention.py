@@ -15,16 +15,16 @@ def test_plan_tiles_cover_every_row_once():
         for tiles, rows, others in ((plan.q_tiles, ql, kl), (plan.k_tiles, kl, ql)):
             seen = np.zeros(sum(rows), int)
             r0, o0 = np.cumsum([0] + rows), np.cumsum([0] + others)
-            for a, n, b, m in tiles.tolist():
+            for a, n, b, m, g in tiles[:, :5].tolist():
                 assert 1 <= n <= _lib.ATTN_TILE
                 seg = int(np.searchsorted(r0, a, side="right")) - 1
                 while rows[seg] == 0:
                     seg += 1
                 assert r0[seg] <= a and a + n <= r0[seg] + rows[seg]
-                assert (b, m) == (o0[seg], others[seg])
+                assert (b, m, g) == (o0[seg], others[seg], seg)
                 seen[a:a + n] += 1
             assert (seen == 1).all()
-    assert attention_plan([], device="cpu").q_tiles.shape == (0, 4)
+    assert attention_plan([], device="cpu").q_tiles.shape == (0, 8)
 
 
 def test_plan_refusals():

@@ -303,7 +303,7 @@ def test_registered_attention_operators(cuda):
     lens = [45, 80]
     q, k, v, d, kw = make(cuda, lens, lens, 4, 2, 32, torch.float32, seed=31, slopes=True, mask=0.7)
     plan = attention_plan(lens, device=cuda)
-    args = (q, k, v, plan.q_tiles, plan.k_tiles, plan.max_q, plan.max_k, 32 ** -0.5, 4.0, kw["slopes"], kw["q_pos"], kw["k_pos"], kw["key_mask"])
+    args = (q, k, v, plan.q_tiles, plan.k_tiles, plan.max_q, plan.max_k, plan.n_seg, 32 ** -0.5, 4.0, kw["slopes"], kw["q_pos"], kw["k_pos"], kw["key_mask"])
     out, lse = torch.ops.magic.attn_fwd(*args)
     grads = torch.ops.magic.attn_bwd(*args, out, lse, d)
     want = run(q, k, v, d, lens, lens, cap=4.0, **kw)
