@@ -585,7 +585,7 @@ int magic_knn_merge(int64_t n_query, int32_t k, int32_t n_parts,
  *   q_tiles: {first q row, rows (1..MAGIC_ATTN_TILE), first key row of the segment, its keys, segment}
  *   k_tiles: {first key row, keys (1..MAGIC_ATTN_TILE), first q row of the segment, its rows, segment}
  * that cover every row of q (k) exactly once.
- * lse [q_heads, n_q] (natural logarithm) is what _bwd needs beside out.  dq [n_q,q_heads,D],
+ * lse [q_heads, n_q] = log2 sum exp(l) (base 2) is what _bwd needs beside out.  dq [n_q,q_heads,D],
  * dk, dv [n_k,kv_heads,D] contiguous in the operands' type; d_slopes [q_heads] or NULL.  dq may be NULL when it (and
  * d_slopes) is not wanted, dk and dv together likewise.
  * Fixed summation order.

@@ -16,12 +16,12 @@ struct BwdArgs {
     const void *out, *dout;
     int64_t ld_o, hs_o, ld_do, hs_do;
     const float *lse;
-    float *lse2;        // [q_heads][n_q] lse in base 2, +inf for rows that see no key (their probabilities become zeros)
+    float *lse2;        // [q_heads][n_q] lse, +inf for rows that see no key (their probabilities become zeros)
     float *delta;       // [q_heads][n_q]
     void *dq, *dk, *dv;
-    float *slope_part;  // [n_q tiles][q_heads] or NULL
+    double *slope_part; // [n_q tiles][q_heads] or NULL
     int64_t items;
-    Ranges rg;
+    Prepared pr;
     int n_split;        // shares of the rows a key tile's sums are cut into (1: they go straight to dk / dv)
     float *part;        // [n_split][dk | dv][n_k][kv_heads][head_dim]
 };
@@ -51,7 +51,7 @@ template <typename T, int DP> __global__ __launch_bounds__(256) void k_attn_delt
         if (l == 0) {
             const float ls = b.lse[(int64_t)h * a.n_q + row];
             const bool none = ls == -INFINITY;
-            b.lse2[(int64_t)h * a.n_q + row] = none ? INFINITY : ls * LOG2E;
+            b.lse2[(int64_t)h * a.n_q + row] = none ? INFINITY : ls;
             b.delta[(int64_t)h * a.n_q + row] = none ? 0.f : s;
         }
     }
@@ -60,7 +60,7 @@ template <typename T, int DP> __global__ __launch_bounds__(256) void k_attn_delt
 // Powers of two on the operands of a segment and head (1 unless the mode is scaled) and what undoes them
 struct Scales {
     float q = 1.f, k = 1.f, v = 1.f, g = 1.f;
-    float s_in, s_out, dp_in;
+    float s_in, dp_in;
     // heads h .. h + n - 1, which share key head hk, take one kind and one scale
     template <typename M>
     __device__ __forceinline__ bool init(const Ranges &rg, int h, int n, int hk, int seg, const magic_attn &a) {
@@ -75,8 +75,7 @@ struct Scales {
             if ((range_ok(rq) && range_ok(rk) && range_ok(rv) && range_ok(rr)) != rg.want_safe) return false;
             if constexpr (M::SCALED) q = range_scale(rq), k = range_scale(rk), v = range_scale(rv), g = range_scale(rr);
         }
-        s_in = (a.cap > 0.f ? a.scale / a.cap : a.scale * LOG2E) * (1.f / q * (1.f / k));
-        s_out = a.cap * LOG2E;
+        s_in = (a.cap > 0.f ? a.scale / a.cap : a.scale) * (1.f / q * (1.f / k));
         dp_in = 1.f / v * (1.f / g);
         return true;
     }
@@ -134,12 +133,13 @@ __global__ __launch_bounds__(NT, (DP == 128 && M::N > 1) ? 1 : 2) void k_attn_dq
     const int row = wave * 32 + li;
     const bool ok = row < nq;
     const int64_t qr = q0 + (ok ? row : 0);
-    const T *K = (const T *)a.k + k0 * a.ld_k + hk * a.hs_k, *V = (const T *)a.v + k0 * a.ld_v + hk * a.hs_v;
+    const Src<M> K = src_of<M>(a.k, a.ld_k, a.hs_k, p.pr.k, k0, hk, D),
+                 V = src_of<M>(a.v, a.ld_v, a.hs_v, p.pr.v, k0, hk, D);
     const float ls = ok ? p.lse2[(int64_t)h * a.n_q + qr] : INFINITY, dl0 = ok ? p.delta[(int64_t)h * a.n_q + qr] : 0.f;
     const bool live = ls != INFINITY;
 
     Scales sc;
-    if (!sc.init<M>(p.rg, h, 1, hk, t[4], a)) return;          // the other launch's segment
+    if (!sc.init<M>(p.pr.rg, h, 1, hk, t[4], a)) return;          // the other launch's segment
     vec qf[KS][NP], gf[KS][NP];
 #pragma unroll
     for (int ks = 0; ks < KS; ++ks) {
@@ -153,10 +153,14 @@ __global__ __launch_bounds__(NT, (DP == 128 && M::N > 1) ? 1 : 2) void k_attn_dq
         g.planes(gf[ks], sc.g);
     }
     const bool bias = a.slopes != nullptr;
-    const float slope2 = bias ? a.slopes[h] * LOG2E : 0.f;
+    const float slope = bias ? a.slopes[h] : 0.f;
     const uint32_t qpos = bias ? flip(a.q_pos[qr]) : 0u;
     Running run;
-    float dsl = 0.f;
+    // Of the lane's row: sum dl dist, sum dl, sum p dist.  The matrix instructions round their inner sums downwards by
+    // about 2^-27 of the terms; alike for all keys of a row, this changes no gradient but the slope's, where it meets the
+    // mean distance with one sign in every row (4e-5 of d slope over 97,000 rows).  sum dl, zero but for such an offset,
+    // takes it out again.
+    double dsl = 0.0, sdl = 0.0, spd = 0.0;
     f32x16_t acc[DB];
 #pragma unroll
     for (int d = 0; d < DB; ++d)
@@ -168,10 +172,11 @@ __global__ __launch_bounds__(NT, (DP == 128 && M::N > 1) ? 1 : 2) void k_attn_dq
     uint32_t pos = 0;
     float mk = 0.f;
     auto load = [&](int j0) {
-        kst.load(K, a.ld_k, j0, nk, D, tid);
-        vst.load(V, a.ld_v, j0, nk, D, tid);
+        kst.load(K, j0, nk, D, tid);
+        vst.load(V, j0, nk, D, tid);
 #pragma unroll
         for (int i = 0; i < stage::N; ++i) {
+            if (Src<M>::READY) break;
             const int j = j0 + stage::row_of(i, tid);
             keep[i] = j < nk;
             if (a.key_mask && j < nk) keep[i] = a.key_mask[k0 + j];
@@ -186,8 +191,8 @@ __global__ __launch_bounds__(NT, (DP == 128 && M::N > 1) ? 1 : 2) void k_attn_dq
     if (nk > 0) load(0);
     for (int j0 = 0; j0 < nk; j0 += BK) {
         __syncthreads();
-        kst.store(sK, D, tid, sc.k, [&](int i, int) { return keep[i] != 0; });
-        vst.store(sV, D, tid, sc.v, [&](int i, int) { return keep[i] != 0; });
+        kst.store(sK, D, tid, [&](int i) { return keep[i] != 0; });
+        vst.store(sV, D, tid, [&](int i) { return keep[i] != 0; });
         if (tid < BK) sPos[tid] = pos, sMask[tid] = mk;
         const bool masked = a.key_mask != nullptr || j0 + BK > nk;
         __syncthreads();
@@ -206,7 +211,7 @@ __global__ __launch_bounds__(NT, (DP == 128 && M::N > 1) ? 1 : 2) void k_attn_dq
                 mma(dp, g, gf[ks]);
             }
             if (a.cap > 0.f) tanh_tile(s, sc.s_in);
-            float ds[16];
+            float ds[16], t_dsl = 0.f, t_dl = 0.f, t_pd = 0.f;
 #pragma unroll
             for (int g = 0; g < 4; ++g) {
                 const int jr = 32 * b + 8 * g + 4 * hf;
@@ -219,21 +224,27 @@ __global__ __launch_bounds__(NT, (DP == 128 && M::N > 1) ? 1 : 2) void k_attn_dq
                     const int r = 4 * g + e;
                     float f = a.scale, x;
                     if (a.cap > 0.f) {
-                        x = fmaf(s[r], sc.s_out, base[e]);
+                        x = s[r] * a.cap;
                         f -= f * s[r] * s[r];
                     } else {
-                        x = fmaf(s[r], sc.s_in, base[e]);
+                        x = s[r] * sc.s_in;
                     }
                     float dist = 0.f;
                     if (bias) {
                         dist = dist_of((uint32_t)kp[e], qpos);
-                        x = fmaf(-slope2, dist, x);
+                        x = fmaf(-slope, dist, x);
                     }
-                    const float dl = __builtin_amdgcn_exp2f(x) * fmaf(dp[r], sc.dp_in, -dl0);
-                    if (bias) dsl -= dl * dist;
+                    const float pr = __builtin_amdgcn_exp2f(fmaf(x, LOG2E, base[e]));
+                    const float dl = pr * fmaf(dp[r], sc.dp_in, -dl0);
+                    if (bias) {
+                        t_dsl = fmaf(dl, dist, t_dsl);
+                        t_pd = fmaf(pr, dist, t_pd);
+                        t_dl += dl;
+                    }
                     ds[r] = dl * f;
                 }
             }
+            if (bias) dsl += (double)t_dsl, sdl += (double)t_dl, spd += (double)t_pd;
             float u = 1.f;
             if constexpr (M::SCALED) {
                 run.step<DB>(ds, acc);
@@ -269,7 +280,9 @@ __global__ __launch_bounds__(NT, (DP == 128 && M::N > 1) ? 1 : 2) void k_attn_dq
     }
     if (p.slope_part) {
         __syncthreads();
-        float *red = reinterpret_cast<float *>(smem);
+        double *red = reinterpret_cast<double *>(smem);
+        sdl += __shfl_xor(sdl, 32, 64);
+        dsl = sdl * spd - dsl;          // (either half's share of sum p dist)
 #pragma unroll
         for (int k = 32; k > 0; k >>= 1) dsl += __shfl_xor(dsl, k, 64);
         if (lane == 0) red[wave] = dsl;
@@ -306,7 +319,7 @@ __global__ __launch_bounds__(NT, DP == 128 ? 1 : 2) void k_attn_dkv(BwdArgs p) {
     const bool ok = in && (!a.key_mask || a.key_mask[kr]);
 
     Scales sc;
-    if (!sc.init<M>(p.rg, hk * G, G, hk, t[4], a)) return;  // the other launch's segment
+    if (!sc.init<M>(p.pr.rg, hk * G, G, hk, t[4], a)) return;  // the other launch's segment
     vec kf[KS][NP], vf[KS][NP];
 #pragma unroll
     for (int ks = 0; ks < KS; ++ks) {
@@ -332,11 +345,12 @@ __global__ __launch_bounds__(NT, DP == 128 ? 1 : 2) void k_attn_dkv(BwdArgs p) {
     float ls = 0.f, dl0 = 0.f;
     uint32_t pos = 0;
     auto load = [&](int h, int i0) {
-        qst.load((const T *)a.q + q0 * a.ld_q + h * a.hs_q, a.ld_q, i0, nq, D, tid);
-        gst.load((const T *)p.dout + q0 * p.ld_do + h * p.hs_do, p.ld_do, i0, nq, D, tid);
+        qst.load(src_of<M>(a.q, a.ld_q, a.hs_q, p.pr.q, q0, h, D), i0, nq, D, tid);
+        gst.load(src_of<M>(p.dout, p.ld_do, p.hs_do, p.pr.g, q0, h, D), i0, nq, D, tid);
         const float *l2 = p.lse2 + (int64_t)h * a.n_q + q0;
 #pragma unroll
         for (int i = 0; i < stage::N; ++i) {
+            if (Src<M>::READY) break;
             const int r = i0 + stage::row_of(i, tid);
             keep[i] = r < nq && l2[r < nq ? r : 0] != INFINITY;
         }
@@ -354,10 +368,10 @@ __global__ __launch_bounds__(NT, DP == 128 ? 1 : 2) void k_attn_dkv(BwdArgs p) {
     if (s_beg < s_end) load(h, it * BQ);
     for (int st = s_beg; st < s_end; ++st) {
         __syncthreads();
-        qst.store(sQ, D, tid, sc.q, [&](int i, int) { return keep[i] != 0; });
-        gst.store(sG, D, tid, sc.g, [&](int i, int) { return keep[i] != 0; });
+        qst.store(sQ, D, tid, [&](int i) { return keep[i] != 0; });
+        gst.store(sG, D, tid, [&](int i) { return keep[i] != 0; });
         if (tid < BQ) sL[tid] = ls, sD[tid] = dl0, sPos[tid] = pos;
-        const float slope2 = bias ? a.slopes[h] * LOG2E : 0.f;
+        const float slope = bias ? a.slopes[h] : 0.f;
         __syncthreads();
         if (++it == per_h) it = 0, ++h;
         if (st + 1 < s_end) load(h, it * BQ);
@@ -388,13 +402,13 @@ __global__ __launch_bounds__(NT, DP == 128 ? 1 : 2) void k_attn_dkv(BwdArgs p) {
                     const int r = 4 * g + e;
                     float f = a.scale, x;
                     if (a.cap > 0.f) {
-                        x = fmaf(s[r], sc.s_out, l4[e]);
+                        x = s[r] * a.cap;
                         f -= f * s[r] * s[r];
                     } else {
-                        x = fmaf(s[r], sc.s_in, l4[e]);
+                        x = s[r] * sc.s_in;
                     }
-                    if (bias) x = fmaf(-slope2, dist_of((uint32_t)qp[e], kpos), x);
-                    const float q = __builtin_amdgcn_exp2f(x);
+                    if (bias) x = fmaf(-slope, dist_of((uint32_t)qp[e], kpos), x);
+                    const float q = __builtin_amdgcn_exp2f(fmaf(x, LOG2E, l4[e]));
                     pr[r] = M::SCALED ? q * 16384.f : q;
                     ds[r] = q * fmaf(dp[r], sc.dp_in, d4[e]) * f;
                 }
@@ -470,9 +484,9 @@ template <typename T> __global__ __launch_bounds__(256) void k_attn_dkv_join(Bwd
 }
 
 // d slope of a head: the tile sums lane by lane, fixed tree, in double
-__global__ __launch_bounds__(64) void k_attn_dslope(const float *part, int n, int H, float *out) {
+__global__ __launch_bounds__(64) void k_attn_dslope(const double *part, int n, int H, float *out) {
     double s = 0.0;
-    for (int i = threadIdx.x; i < n; i += 64) s += (double)part[(int64_t)i * H + blockIdx.x];
+    for (int i = threadIdx.x; i < n; i += 64) s += part[(int64_t)i * H + blockIdx.x];
 #pragma unroll
     for (int o = 32; o > 0; o >>= 1) s += __shfl_xor(s, o, 64);
     if (threadIdx.x == 0) out[blockIdx.x] = (float)s;
@@ -538,8 +552,8 @@ size_t magic_attn_bwd_workspace_bytes(const magic_attn *a) {
     if (check(a) != MAGIC_OK) return 256;
     const int n = splits(a);
     const size_t part = n > 1 ? (size_t)n * 2 * a->n_k * a->kv_heads * a->head_dim * sizeof(float) : 0;
-    return magic::align_up(part) + (use_f16(a) ? magic::align_up(range_count(a, true) * sizeof(Range)) : 0) + 2 * magic::align_up((size_t)a->n_q * a->q_heads * sizeof(float)) +
-           magic::align_up((size_t)a->n_q_tiles * a->q_heads * sizeof(float)) + 256;
+    return magic::align_up(part) + (use_f16(a) ? prepare_bytes(a, true) : 0) + 2 * magic::align_up((size_t)a->n_q * a->q_heads * sizeof(float)) +
+           magic::align_up((size_t)a->n_q_tiles * a->q_heads * sizeof(double)) + 256;
 }
 
 int magic_attn_bwd(const magic_attn *a, const void *out, int64_t ld_out, int64_t hs_out, const float *lse, const void *d_out,
@@ -561,25 +575,23 @@ int magic_attn_bwd(const magic_attn *a, const void *out, int64_t ld_out, int64_t
     magic::Arena ar(workspace, workspace_bytes);
     b.delta = ar.take<float>((size_t)a->n_q * a->q_heads);
     b.lse2 = ar.take<float>((size_t)a->n_q * a->q_heads);
-    b.slope_part = ar.take<float>((size_t)a->n_q_tiles * a->q_heads);
-    const bool f16 = use_f16(a);
-    Range *ranges = f16 ? ar.take<Range>(range_count(a, true)) : nullptr;
+    b.slope_part = ar.take<double>((size_t)a->n_q_tiles * a->q_heads);
+    const bool f16 = use_f16(a) && a->n_q > 0 && a->n_k > 0;
     b.n_split = dk ? splits(a) : 1;
     b.part = b.n_split > 1 ? ar.take<float>((size_t)b.n_split * 2 * a->n_k * a->kv_heads * a->head_dim) : nullptr;
     if (!ar.ok()) return MAGIC_ERR_WORKSPACE;
     if (!d_slopes) b.slope_part = nullptr;
-    b.rg = Ranges{nullptr, nullptr, nullptr, nullptr, 0, false};
     const bool f32 = a->dtype == MAGIC_F32;
     int rc = MAGIC_OK;
     if (a->n_q > 0) rc = f32 ? delta_of<float>(b, stream) : delta_of<bf16_t>(b, stream);
     if (rc != MAGIC_OK) return rc;
     if (f16) {
-        rc = prepare_ranges(a, d_out, ld_do, hs_do, ranges, b.rg, stream);
+        const GradRows g = {d_out, ld_do, hs_do, b.lse2};
+        rc = prepare(a, &g, ar, b.pr, stream);
         if (rc != MAGIC_OK) return rc;
-        b.rg.want_safe = true;
         rc = sweeps_of<F16x2>(b, stream);
         if (rc != MAGIC_OK) return rc;
-        b.rg.want_safe = false;                // the segments whose rows differ too much in size
+        b.pr.rg.want_safe = false;                // the segments whose rows differ too much in size
     }
     rc = f32 ? sweeps_of<F32x3>(b, stream) : sweeps_of<BF16>(b, stream);
     if (rc != MAGIC_OK) return rc;

@@ -25,7 +25,6 @@ typedef short s16x4_t __attribute__((ext_vector_type(4)));
 typedef __bf16 bf16x4_t __attribute__((ext_vector_type(4)));
 
 constexpr float LOG2E = 1.44269504088896340736f;
-constexpr float LN2 = 0.69314718055994530942f;
 
 // How operands become matrix operands (16-bit planes):
 //   F32x3  float32 as three bf16 pieces, six products; exact pieces for any magnitude
@@ -60,7 +59,9 @@ __device__ __forceinline__ void split_f16(const float (&x)[8], f16x8_t (&p)[2]) 
     for (int j = 0; j < 4; ++j) {
         const f32x2_t v = {x[2 * j], x[2 * j + 1]};
         const f16x2_t h = __builtin_convertvector(v, f16x2_t);
-        const f32x2_t r = {v[0] - (float)h[0], v[1] - (float)h[1]};
+        f32x2_t r;          // v - h, the half read in place (the compiler converts it first)
+        asm("v_fma_mix_f32 %0, %1, -1.0, %2 op_sel:[0,0,0] op_sel_hi:[1,0,0]" : "=v"(r[0]) : "v"(h), "v"(v[0]));
+        asm("v_fma_mix_f32 %0, %1, -1.0, %2 op_sel:[1,0,0] op_sel_hi:[1,0,0]" : "=v"(r[1]) : "v"(h), "v"(v[1]));
         const f16x2_t l = __builtin_convertvector(r, f16x2_t);
         p[0][2 * j] = h[0], p[0][2 * j + 1] = h[1];
         p[1][2 * j] = l[0], p[1][2 * j + 1] = l[1];
@@ -113,6 +114,51 @@ template <> struct Raw<bf16_t> {
     }
 };
 
+struct RawF16 {
+    f16x8_t h, l;
+    __device__ __forceinline__ void zero() {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) h[e] = l[e] = (_Float16)0.f;
+    }
+    __device__ __forceinline__ void planes(f16x8_t (&p)[2]) const { p[0] = h, p[1] = l; }
+};
+
+// Rows of one head that a kernel stages tile by tile.  F16x2 rows come split, scaled and with the rows that take no part
+// as zeros, from the pass that prepares them (a tile's rows are staged once for every 128 rows of the other side).
+template <typename M> struct Src {
+    typedef typename M::T T;
+    struct raw : Raw<T> {
+        __device__ __forceinline__ void planes(typename M::vec (&p)[M::N]) const { Raw<T>::planes(p, 1.f); }
+    };
+    static constexpr bool READY = false;
+    const T *p;
+    int64_t ld;
+    __device__ __forceinline__ void load(raw &r, int64_t row, int col) const { r.load(p + row * ld + col); }
+};
+template <> struct Src<F16x2> {
+    typedef RawF16 raw;
+    static constexpr bool READY = true;
+    const _Float16 *p;
+    int64_t ld, lo;      // lo: from a high piece to its low one
+    __device__ __forceinline__ void load(raw &r, int64_t row, int col) const {
+        r.h = *reinterpret_cast<const f16x8_t *>(p + row * ld + col);
+        r.l = *reinterpret_cast<const f16x8_t *>(p + lo + row * ld + col);
+    }
+};
+// planes of one operand in the workspace: [hi | lo][rows][heads][D]
+struct PlaneSet {
+    const _Float16 *p;
+    int64_t rows;
+    int heads;
+};
+template <typename M>
+__device__ __forceinline__ Src<M> src_of(const void *p, int64_t ld, int64_t hs, const PlaneSet &s, int64_t row, int h, int D) {
+    if constexpr (M::SCALED)
+        return Src<M>{s.p + (row * s.heads + h) * D, (int64_t)s.heads * D, s.rows * s.heads * D};
+    else
+        return Src<M>{(const typename M::T *)p + row * ld + h * hs, ld};
+}
+
 __device__ __forceinline__ void mma(f32x16_t &c, const bf16x8_t (&a)[3], const bf16x8_t (&b)[3]) {
     mfma_split6(c, a[0], a[1], a[2], b[0], b[1], b[2]);
 }
@@ -163,28 +209,32 @@ template <typename M, int DP, int ROWS, int NT> struct Stage {
     static constexpr int CPR = DP / 8;                          // chunks of a row
     static constexpr int TOTAL = ROWS * CPR;
     static constexpr int N = (TOTAL + NT - 1) / NT;
-    Raw<T> r[N];
+    typename Src<M>::raw r[N];
 
-    // rows row0 .. of an operand with `n` valid rows behind `base` (n >= 1): rows past the end are read as the last one
-    __device__ __forceinline__ void load(const T *base, int64_t ld, int row0, int n, int D, int tid) {
+    // rows row0 .. of an operand of `n` rows (n >= 1): rows past the end are read as the last one
+    __device__ __forceinline__ void load(const Src<M> &src, int row0, int n, int D, int tid) {
 #pragma unroll
         for (int i = 0; i < N; ++i) {
             const int c = tid + i * NT;
             const int row = row0 + c / CPR, col = (c % CPR) * 8;
-            const int rc = row < n ? row : n - 1, cc = col < D ? col : 0;
-            r[i].load(base + (int64_t)rc * ld + cc);
+            src.load(r[i], row < n ? row : n - 1, col < D ? col : 0);
         }
     }
-    // keep(row of the tile): false -> zeros, whatever was read
-    template <typename Keep> __device__ __forceinline__ void store(bf16_t *t, int D, int tid, float scale, Keep keep) {
+    // keep(i): false -> zeros, whatever was read.  (Rows past the end of READY sources stay what the last row is: their
+    // probabilities are zeros, and the last row reaches everything that they could.)
+    template <typename Keep> __device__ __forceinline__ void store(bf16_t *t, int D, int tid, Keep keep) {
 #pragma unroll
         for (int i = 0; i < N; ++i) {
             const int c = tid + i * NT;
             const int row = c / CPR, col = (c % CPR) * 8;
             if (TOTAL % NT != 0 && c >= TOTAL) break;
-            if (!(keep(i, row) && col < D)) r[i].zero();
+            if (Src<M>::READY) {
+                if (D < DP && col >= D) r[i].zero();
+            } else if (!(keep(i) && col < D)) {
+                r[i].zero();
+            }
             typename M::vec p[tile::NP];
-            r[i].planes(p, scale);
+            r[i].planes(p);
 #pragma unroll
             for (int k = 0; k < tile::NP; ++k)
                 *reinterpret_cast<typename M::vec *>(t + k * tile::PLANE + row * tile::LDW + col) = p[k];
@@ -224,7 +274,11 @@ __device__ __forceinline__ void tanh_tile(f32x16_t &x, float f) {
 
 // distance of two positions whose sign bit was flipped (order and differences of the unsigned values are theirs)
 __device__ __forceinline__ uint32_t flip(int32_t pos) { return (uint32_t)pos ^ 0x80000000u; }
-__device__ __forceinline__ float dist_of(uint32_t a, uint32_t b) { return (float)(max(a, b) - min(a, b)); }
+__device__ __forceinline__ float dist_of(uint32_t a, uint32_t b) {
+    uint32_t d;
+    asm("v_sad_u32 %0, %1, %2, 0" : "=v"(d) : "v"(a), "v"(b));      // |a - b|
+    return (float)d;
+}
 
 __device__ __forceinline__ float other_half(float x) { return __shfl_xor(x, 32, 64); }
 
@@ -261,11 +315,21 @@ __device__ __forceinline__ float range_scale(Range r) {
     return __uint_as_float((uint32_t)(e + 127) << 23);
 }
 
-// For a float32 call: whether F16x2 is tried, the number of Range entries, and the pass that fills them (with the
-// output's gradient g in backward).
-bool use_f16(const magic_attn *a);
-int64_t range_count(const magic_attn *a, bool grad);
-int prepare_ranges(const magic_attn *a, const void *g, int64_t ld_g, int64_t hs_g, Range *r, Ranges &rg, hipStream_t stream);
+// What F16x2 launches need beside the arguments: the ranges and the planes of the operands they stage
+struct Prepared {
+    Ranges rg = {nullptr, nullptr, nullptr, nullptr, 0, false};
+    PlaneSet q = {}, k = {}, v = {}, g = {};
+};
+// The output's gradient and what marks rows that see no key (lse = +inf there), in backward
+struct GradRows {
+    const void *g;
+    int64_t ld, hs;
+    const float *lse;
+};
+bool use_f16(const magic_attn *a);                                 // whether F16x2 is tried for a call
+size_t prepare_bytes(const magic_attn *a, bool backward);          // its workspace
+// ranges and planes: k, v, and in backward q and the output's gradient
+int prepare(const magic_attn *a, const GradRows *g, Arena &ar, Prepared &out, hipStream_t stream);
 constexpr int TAB = 8;            // int32 words of a tile-table entry
 
 }  // namespace attn

@@ -1,6 +1,6 @@
 // Softmax attention of the rows of a segment over the keys of the same segment, forward (magic_attn_fwd).
 //   s = scale q.k,  c = cap tanh(s / cap) (cap > 0),  l = c - slope_h |pos_q - pos_k|,  p = softmax of l over the
-//   unmasked keys,  o = sum p v;   lse = log sum exp(l), -inf for a row that sees no key (o = 0 then).
+//   unmasked keys,  o = sum p v;   lse = log2 sum exp(l), -inf for a row that sees no key (o = 0 then).
 // One pass over the keys with a running maximum and sum per row; scores are formed transposed (keys x rows), so that a
 // lane owns ONE row's statistics and the probabilities feed the second product from their registers (attn_common.h).
 #include "attn_common.h"
@@ -40,7 +40,7 @@ struct RangeArgs {
     int n_seg;
 };
 
-// block: a 128-row tile of one head of one operand, eight lanes a row.  Finite values only: an infinity or a NaN becomes
+// block: a 128-row tile of one head of one operand, sixteen lanes a row.  Finite values only: an infinity or a NaN becomes
 // one in the planes whatever the scale.  (max and min do not depend on the order of the atomics.)
 __global__ __launch_bounds__(256) void k_range(RangeArgs r) {
     const magic_attn &a = r.a;
@@ -61,22 +61,27 @@ __global__ __launch_bounds__(256) void k_range(RangeArgs r) {
     }
     if ((int)blockIdx.x >= (key ? a.n_k_tiles : a.n_q_tiles)) return;
     const int32_t *t = (key ? a.k_tiles : a.q_tiles) + TAB * (int64_t)blockIdx.x;
-    const int lane = threadIdx.x & 7;
+    constexpr int L = 16;                            // lanes of a row: 16 bytes each, twice for more than 64 columns
+    const int c = 4 * (threadIdx.x & (L - 1));
     uint32_t mx = 0u, mn = 0xffffffffu;
-    for (int i = threadIdx.x >> 3; i < t[1]; i += 32) {
-        const int64_t row = (int64_t)t[0] + i;
-        if (key && a.key_mask && !a.key_mask[row]) continue;
+#pragma unroll 4
+    for (int i = threadIdx.x / L; i < MAGIC_ATTN_TILE; i += 256 / L) {
+        const bool in = i < t[1];
+        const int64_t row = (int64_t)t[0] + (in ? i : 0);
+        const float *x = base + row * ld + y * hs;
+        const bool use = in && !(key && a.key_mask && !a.key_mask[row]);
+        const f32x4_t u = *reinterpret_cast<const f32x4_t *>(x + (c < a.head_dim ? c : 0));
+        f32x4_t v = u;
+        if (a.head_dim > 64) v = *reinterpret_cast<const f32x4_t *>(x + (c + 64 < a.head_dim ? c + 64 : 0));
         uint32_t m = 0u;
-        for (int c = 4 * lane; c < a.head_dim; c += 32) {
-            const f32x4_t x = *reinterpret_cast<const f32x4_t *>(base + row * ld + y * hs + c);
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                const uint32_t b = __float_as_uint(x[e]) & 0x7fffffffu;
-                m = b < 0x7f800000u && b > m ? b : m;
-            }
+        for (int e = 0; e < 4; ++e) {
+            const uint32_t p = __float_as_uint(u[e]) & 0x7fffffffu, q = __float_as_uint(v[e]) & 0x7fffffffu;
+            m = max(m, max(p < 0x7f800000u ? p : 0u, q < 0x7f800000u ? q : 0u));
         }
+        m = use ? m : 0u;
 #pragma unroll
-        for (int o = 4; o > 0; o >>= 1) m = max(m, (uint32_t)__shfl_xor((int)m, o, 8));
+        for (int o = L / 2; o > 0; o >>= 1) m = max(m, (uint32_t)__shfl_xor((int)m, o, L));
         mx = max(mx, m);
         if (m != 0u) mn = min(mn, m);
     }
@@ -85,7 +90,13 @@ __global__ __launch_bounds__(256) void k_range(RangeArgs r) {
         mx = max(mx, (uint32_t)__shfl_xor((int)mx, o, 64));
         mn = min(mn, (uint32_t)__shfl_xor((int)mn, o, 64));
     }
-    if ((threadIdx.x & 63) == 0 && mx != 0u) {
+    // one pair of atomics a block: the tiles of a segment all meet in one place
+    __shared__ uint32_t smx[4], smn[4];
+    if ((threadIdx.x & 63) == 0) smx[threadIdx.x >> 6] = mx, smn[threadIdx.x >> 6] = mn;
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        mx = max(max(smx[0], smx[1]), max(smx[2], smx[3])), mn = min(min(smn[0], smn[1]), min(smn[2], smn[3]));
+        if (mx == 0u) return;
         Range *d = out + (int64_t)y * r.n_seg + t[4];
         atomicMax(&d->max, mx);
         atomicMin(&d->min, mn);
@@ -94,24 +105,101 @@ __global__ __launch_bounds__(256) void k_range(RangeArgs r) {
 
 }  // namespace
 
-// F16x2 needs a pass over the operands first: for float32 calls of enough work to pay for it (measured: see attn_fwd)
-bool use_f16(const magic_attn *a) { return a->dtype == MAGIC_F32 && a->head_dim > 32 && a->max_k >= 512 && a->n_seg > 0; }
+namespace {
 
+struct SplitArgs {
+    magic_attn a;
+    GradRows g;
+    Ranges rg;
+    _Float16 *q, *k, *v, *gr;      // hi planes; the lo ones follow
+};
+
+// block: a 128-row tile of one head of k, v (then q and the gradient, scaled alike for all heads of a key head)
+__global__ __launch_bounds__(256) void k_split(SplitArgs s) {
+    const magic_attn &a = s.a;
+    const int D = a.head_dim, G = a.q_heads / a.kv_heads;
+    int y = blockIdx.y;
+    const float *base;
+    int64_t ld, hs, rows;
+    _Float16 *out;
+    bool key = true;
+    int heads = a.kv_heads;
+    const Range *rg;
+    if (y < a.kv_heads) {
+        base = (const float *)a.k, ld = a.ld_k, hs = a.hs_k, out = s.k, rg = s.rg.k;
+    } else if ((y -= a.kv_heads) < a.kv_heads) {
+        base = (const float *)a.v, ld = a.ld_v, hs = a.hs_v, out = s.v, rg = s.rg.v;
+    } else if ((y -= a.kv_heads, key = false, heads = a.q_heads, y < a.q_heads)) {
+        base = (const float *)a.q, ld = a.ld_q, hs = a.hs_q, out = s.q, rg = s.rg.q;
+    } else {
+        y -= a.q_heads;
+        base = (const float *)s.g.g, ld = s.g.ld, hs = s.g.hs, out = s.gr, rg = s.rg.g;
+    }
+    rows = key ? a.n_k : a.n_q;
+    if ((int)blockIdx.x >= (key ? a.n_k_tiles : a.n_q_tiles)) return;
+    const int32_t *t = (key ? a.k_tiles : a.q_tiles) + TAB * (int64_t)blockIdx.x;
+    Range r = {0u, 0xffffffffu};
+    for (int i = key ? y : y / G * G, e = key ? y + 1 : i + G; i < e; ++i) {
+        const Range x = rg[i * s.rg.n_seg + t[4]];
+        r.max = max(r.max, x.max);
+    }
+    const float scale = range_scale(r);
+    const int cpr = D / 8, n = t[1] * cpr;
+    for (int i = threadIdx.x; i < n; i += 256) {
+        const int64_t row = (int64_t)t[0] + i / cpr;
+        const int c = (i % cpr) * 8;
+        Raw<float> x;
+        x.load(base + row * ld + y * hs + c);
+        const bool use = key ? !a.key_mask || a.key_mask[row] : !s.g.lse || s.g.lse[(int64_t)y * a.n_q + row] != INFINITY;
+        if (!use) x.zero();
+        f16x8_t p[2];
+        x.planes(p, scale);
+        _Float16 *o = out + (row * heads + y) * D + c;
+        *reinterpret_cast<f16x8_t *>(o) = p[0];
+        *reinterpret_cast<f16x8_t *>(o + rows * heads * D) = p[1];
+    }
+}
+
+size_t plane_elems(const magic_attn *a, bool key) {
+    return 2 * (size_t)(key ? a->n_k * a->kv_heads : a->n_q * a->q_heads) * a->head_dim;
+}
 int64_t range_count(const magic_attn *a, bool grad) {
     return ((grad ? 2 : 1) * (int64_t)a->q_heads + 2 * (int64_t)a->kv_heads) * a->n_seg;
 }
 
-int prepare_ranges(const magic_attn *a, const void *g, int64_t ld_g, int64_t hs_g, Range *r, Ranges &rg, hipStream_t stream) {
+}  // namespace
+
+// F16x2 needs two passes over the operands first: for float32 calls of enough work to pay for them
+bool use_f16(const magic_attn *a) { return a->dtype == MAGIC_F32 && a->head_dim > 32 && a->max_k >= 512 && a->n_seg > 0; }
+
+size_t prepare_bytes(const magic_attn *a, bool backward) {
+    const size_t k = align_up(plane_elems(a, true) * 2), q = align_up(plane_elems(a, false) * 2);
+    return align_up(range_count(a, backward) * sizeof(Range)) + 2 * k + (backward ? 2 * q : 0);
+}
+
+int prepare(const magic_attn *a, const GradRows *g, Arena &ar, Prepared &out, hipStream_t stream) {
     const int64_t n = range_count(a, g != nullptr);
+    Range *r = ar.take<Range>(n);
+    SplitArgs s;
+    s.a = *a;
+    s.g = g ? *g : GradRows{nullptr, 0, 0, nullptr};
+    s.k = ar.take<_Float16>(plane_elems(a, true)), s.v = ar.take<_Float16>(plane_elems(a, true));
+    s.q = s.gr = nullptr;
+    if (g) s.q = ar.take<_Float16>(plane_elems(a, false)), s.gr = ar.take<_Float16>(plane_elems(a, false));
+    if (!ar.ok()) return MAGIC_ERR_WORKSPACE;
     RangeArgs ra;
-    ra.a = *a, ra.g = g, ra.ld_g = ld_g, ra.hs_g = hs_g, ra.n_seg = a->n_seg;
+    ra.a = *a, ra.g = s.g.g, ra.ld_g = s.g.ld, ra.hs_g = s.g.hs, ra.n_seg = a->n_seg;
     ra.q = r, ra.k = r + (int64_t)a->q_heads * a->n_seg, ra.v = ra.k + (int64_t)a->kv_heads * a->n_seg,
     ra.gr = ra.v + (int64_t)a->kv_heads * a->n_seg;
-    rg = Ranges{ra.q, ra.k, ra.v, g ? ra.gr : nullptr, a->n_seg, true};
+    out.rg = s.rg = Ranges{ra.q, ra.k, ra.v, g ? ra.gr : nullptr, a->n_seg, true};
+    out.k = {s.k, a->n_k, a->kv_heads}, out.v = {s.v, a->n_k, a->kv_heads};
+    out.q = {s.q, a->n_q, a->q_heads}, out.g = {s.gr, a->n_q, a->q_heads};
     MAGIC_LAUNCH("attn_range_init", k_range_init, magic::stride_grid(n, 256), 256, 0, stream, r, n);
     const int x = a->n_q_tiles > a->n_k_tiles ? a->n_q_tiles : a->n_k_tiles;
-    const int y = a->q_heads * (g ? 2 : 1) + 2 * a->kv_heads;
-    if (x > 0) MAGIC_LAUNCH("attn_range", k_range, dim3(x, y), 256, 0, stream, ra);
+    const int y = a->q_heads * (g ? 2 : 1) + 2 * a->kv_heads, ys = 2 * a->kv_heads + (g ? 2 * a->q_heads : 0);
+    if (y > 65535) return MAGIC_ERR_UNSUPPORTED;
+    MAGIC_LAUNCH("attn_range", k_range, dim3(x, y), 256, 0, stream, ra);
+    MAGIC_LAUNCH("attn_split", k_split, dim3(x, ys), 256, 0, stream, s);
     return magic::launch_status();
 }
 
@@ -136,14 +224,14 @@ struct FwdArgs {
     int sub;              // blocks that share a 128-row tile of the table
     int n_hb;             // head blocks: q_heads / gc
     int64_t items;
-    Ranges rg;
+    Prepared pr;
 };
 
 __device__ __forceinline__ int h_of(const FwdArgs &p, int hb) { return hb * p.gc; }
 
 // WM groups of 32 columns (rows, or rows x heads of one key head), KG groups of KW keys: a block of WM * KG wavefronts
 template <typename M, int DP, int WM, int KG, int KW>
-__global__ __launch_bounds__(64 * WM *KG, (DP == 128 && M::N == 3) ? 1 : 2) void k_attn_fwd(FwdArgs p) {
+__global__ __launch_bounds__(64 * WM *KG, DP == 128 && (M::N == 3 || WM == 1) ? 1 : 2) void k_attn_fwd(FwdArgs p) {
     typedef typename M::T T;
     typedef typename M::vec vec;
     constexpr int NP = M::N, KS = DP / 16, DB = (DP + 31) / 32, BK = KG * KW, NT = 64 * WM * KG, KB = KW / 32;
@@ -175,13 +263,14 @@ __global__ __launch_bounds__(64 * WM *KG, (DP == 128 && M::N == 3) ? 1 : 2) void
     const int row = col / p.gc, h = hb * p.gc + col % p.gc;
     const bool ok = col < p.cols && row < nq && row < p.rows;
     const int hk = hb * p.gc / (a.q_heads / a.kv_heads);
-    const T *K = (const T *)a.k + k0 * a.ld_k + hk * a.hs_k, *V = (const T *)a.v + k0 * a.ld_v + hk * a.hs_v;
+    const Src<M> K = src_of<M>(a.k, a.ld_k, a.hs_k, p.pr.k, k0, hk, a.head_dim),
+                 V = src_of<M>(a.v, a.ld_v, a.hs_v, p.pr.v, k0, hk, a.head_dim);
 
     float sq = 1.f, sk = 1.f, sv = 1.f;
-    if (p.rg.q) {
-        const Range rq = p.rg.q[h_of(p, hb) * p.rg.n_seg + t[4]], rk = p.rg.k[hk * p.rg.n_seg + t[4]],
-                    rv = p.rg.v[hk * p.rg.n_seg + t[4]];
-        if ((range_ok(rq) && range_ok(rk) && range_ok(rv)) != p.rg.want_safe) return;   // the other launch's segment
+    if (p.pr.rg.q) {
+        const Range rq = p.pr.rg.q[h_of(p, hb) * p.pr.rg.n_seg + t[4]], rk = p.pr.rg.k[hk * p.pr.rg.n_seg + t[4]],
+                    rv = p.pr.rg.v[hk * p.pr.rg.n_seg + t[4]];
+        if ((range_ok(rq) && range_ok(rk) && range_ok(rv)) != p.pr.rg.want_safe) return;   // the other launch's segment
         if constexpr (M::SCALED) sq = range_scale(rq), sk = range_scale(rk), sv = range_scale(rv);
     }
     vec qf[KS][NP];
@@ -197,10 +286,10 @@ __global__ __launch_bounds__(64 * WM *KG, (DP == 128 && M::N == 3) ? 1 : 2) void
         }
     }
     const bool bias = a.slopes != nullptr;
-    const float slope2 = bias ? a.slopes[ok ? h : hb * p.gc] * LOG2E : 0.f;
+    const float slope = bias ? a.slopes[ok ? h : hb * p.gc] : 0.f;
     const uint32_t qpos = bias ? flip(a.q_pos[q0 + (ok ? row : 0)]) : 0u;
     const float unscale = 1.f / sq * (1.f / sk);
-    const float s_in = (a.cap > 0.f ? a.scale / a.cap : a.scale * LOG2E) * unscale, s_out = a.cap * LOG2E;
+    const float s_in = (a.cap > 0.f ? a.scale / a.cap : a.scale) * unscale;
     constexpr float P_EXP = M::SCALED ? 14.f : 0.f;       // probabilities are formed times 2^14
 
     f32x16_t o[DB];
@@ -208,7 +297,10 @@ __global__ __launch_bounds__(64 * WM *KG, (DP == 128 && M::N == 3) ? 1 : 2) void
     for (int d = 0; d < DB; ++d)
 #pragma unroll
         for (int r = 0; r < 16; ++r) o[d][r] = 0.f;
-    float m = -INFINITY, l = 0.f;  // of this lane's keys: the two halves of a wavefront share m and add l at the end
+    // Of this lane's keys: the two halves of a wavefront share m and add l at the end.  m is the largest logit times
+    // log2 e, rounded: a probability is 2^(logit log2 e - m) in ONE fused step, so its error is that of the small
+    // difference, not of the two large terms.
+    float m = -INFINITY, l = 0.f;
 
     stage kst, vst;
     uint8_t keep[stage::N];
@@ -216,10 +308,11 @@ __global__ __launch_bounds__(64 * WM *KG, (DP == 128 && M::N == 3) ? 1 : 2) void
     float mk = 0.f;
     auto load = [&](int tt) {
         const int j0 = tt * BK;
-        kst.load(K, a.ld_k, j0, nk, D, tid);
-        vst.load(V, a.ld_v, j0, nk, D, tid);
+        kst.load(K, j0, nk, D, tid);
+        vst.load(V, j0, nk, D, tid);
 #pragma unroll
         for (int i = 0; i < stage::N; ++i) {
+            if (Src<M>::READY) break;
             const int j = j0 + stage::row_of(i, tid);
             keep[i] = j < nk;
             if (a.key_mask && j < nk) keep[i] = a.key_mask[k0 + j];
@@ -234,8 +327,8 @@ __global__ __launch_bounds__(64 * WM *KG, (DP == 128 && M::N == 3) ? 1 : 2) void
     if (t_beg < t_end) load(t_beg);
     for (int tt = t_beg; tt < t_end; ++tt) {
         __syncthreads();  // the reads of the tile before are done
-        kst.store(sK, D, tid, sk, [&](int i, int) { return keep[i] != 0; });
-        vst.store(sV, D, tid, sv, [&](int i, int) { return keep[i] != 0; });
+        kst.store(sK, D, tid, [&](int i) { return keep[i] != 0; });
+        vst.store(sV, D, tid, [&](int i) { return keep[i] != 0; });
         if (tid < BK) sPos[tid] = pos, sMask[tid] = mk;
         const bool masked = a.key_mask != nullptr || (tt + 1) * BK > nk;
         __syncthreads();
@@ -254,10 +347,10 @@ __global__ __launch_bounds__(64 * WM *KG, (DP == 128 && M::N == 3) ? 1 : 2) void
                 tile::frag(sK, kg * KW + 32 * b + li, 16 * ks + 8 * hf, f);
                 mma(s[b], f, qf[ks]);
             }
-        // logits in base 2; a masked key's zero score gets -inf
+        // logits; a masked key's zero score gets -inf
 #pragma unroll
         for (int b = 0; b < KB; ++b) {
-            const float f = a.cap > 0.f ? s_out : s_in;
+            const float f = a.cap > 0.f ? a.cap : s_in;
             if (a.cap > 0.f) tanh_tile(s[b], s_in);
             if (masked) {
 #pragma unroll
@@ -275,50 +368,50 @@ __global__ __launch_bounds__(64 * WM *KG, (DP == 128 && M::N == 3) ? 1 : 2) void
                 for (int g = 0; g < 4; ++g) {
                     const i32x4_t kp = *reinterpret_cast<const i32x4_t *>(sPos + kg * KW + 32 * b + 8 * g + 4 * hf);
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) s[b][4 * g + e] = fmaf(-slope2, dist_of((uint32_t)kp[e], qpos), s[b][4 * g + e]);
+                    for (int e = 0; e < 4; ++e) s[b][4 * g + e] = fmaf(-slope, dist_of((uint32_t)kp[e], qpos), s[b][4 * g + e]);
                 }
             }
         }
-        float mx = m;
+        float mx = -INFINITY;
 #pragma unroll
         for (int b = 0; b < KB; ++b)
 #pragma unroll
             for (int r = 0; r < 16; ++r) mx = fmaxf(mx, s[b][r]);
-        mx = fmaxf(mx, other_half(mx));
+        mx = fmaxf(m, fmaxf(mx, other_half(mx)) * LOG2E);
         const float ms = mx == -INFINITY ? 0.f : mx;
-        if (__any(mx != m)) {
-            const float al = __builtin_amdgcn_exp2f(m - ms);
-            l *= al;
-#pragma unroll
-            for (int d = 0; d < DB; ++d)
-#pragma unroll
-                for (int r = 0; r < 16; ++r) o[d][r] *= al;
-            m = mx;
-        }
-        const float mo = ms - P_EXP;
-#pragma unroll
-        for (int b = 0; b < KB; ++b)
-#pragma unroll
-            for (int r = 0; r < 16; ++r) {
-                s[b][r] = __builtin_amdgcn_exp2f(s[b][r] - mo);
-                l += s[b][r];
-            }
+        const float al = __builtin_amdgcn_exp2f(m - ms), mo = P_EXP - ms;
+        m = mx;
+        // The tile's sums are formed by themselves and added once: a long tail of small terms, each below half a unit of
+        // the running sum, would otherwise be lost term by term (3e-6 of the result over 8,000 keys with a distance bias).
+        float tsum = 0.f;
+        vec pf[KB * 2][NP];
 #pragma unroll
         for (int b = 0; b < KB; ++b)
 #pragma unroll
             for (int u = 0; u < 2; ++u) {
                 float x[8];
 #pragma unroll
-                for (int e = 0; e < 8; ++e) x[e] = s[b][8 * u + e];
-                vec pf[NP];
-                to_planes(x, pf);
-#pragma unroll
-                for (int d = 0; d < DB; ++d) {
-                    vec f[NP];
-                    tile::frag_t(sV, kg * KW + 32 * b + 16 * u, 32 * d, lane, f);
-                    mma(o[d], f, pf);
+                for (int e = 0; e < 8; ++e) {
+                    x[e] = __builtin_amdgcn_exp2f(fmaf(s[b][8 * u + e], LOG2E, mo));
+                    tsum += x[e];
                 }
+                to_planes(x, pf[2 * b + u]);
             }
+        l = fmaf(l, al, tsum);
+#pragma unroll
+        for (int d = 0; d < DB; ++d) {
+            f32x16_t c;
+#pragma unroll
+            for (int r = 0; r < 16; ++r) c[r] = 0.f;
+#pragma unroll
+            for (int w = 0; w < KB * 2; ++w) {
+                vec f[NP];
+                tile::frag_t(sV, kg * KW + 16 * w, 32 * d, lane, f);
+                mma(c, f, pf[w]);
+            }
+#pragma unroll
+            for (int r = 0; r < 16; ++r) o[d][r] = fmaf(o[d][r], al, c[r]);
+        }
     }
     l += other_half(l);
     if constexpr (KG > 1) {
@@ -381,38 +474,43 @@ __global__ __launch_bounds__(64 * WM *KG, (DP == 128 && M::N == 3) ? 1 : 2) void
             const float x[4] = {o[d][4 * g] * inv, o[d][4 * g + 1] * inv, o[d][4 * g + 2] * inv, o[d][4 * g + 3] * inv};
             magic::store_vec<T, 4>(out + c, c < D, x);
         }
-    if (hf == 0) p.lse[(int64_t)h * a.n_q + q0 + row] = ls * LN2;
+    if (hf == 0) p.lse[(int64_t)h * a.n_q + q0 + row] = ls;
 }
 
-// the key ranges of a row joined in order: o = sum_s 2^(l_s - l) o_s
-template <typename T> __global__ __launch_bounds__(256) void k_attn_join(FwdArgs p) {
+// The key ranges of a row joined: o = sum_s 2^(l_s - l) o_s.  A block takes a row and head; CPR lanes hold its columns
+// and the 256 / CPR lane groups take the ranges in turn, added in group order.
+template <typename T, int CPR> __global__ __launch_bounds__(256) void k_attn_join(FwdArgs p) {
+    constexpr int NG = 256 / CPR;
+    __shared__ float w[256], red[256];
+    __shared__ f32x4_t so[256];
     const magic_attn &a = p.a;
-    const int cpr = a.head_dim / 4;
-    const int64_t total = a.n_q * a.q_heads * cpr, plane = a.n_q * a.q_heads;
-    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < total; i += (int64_t)gridDim.x * 256) {
-        const int64_t hr = i / cpr;                     // head * n_q + row
-        const int c = (int)(i - hr * cpr) * 4;
-        float m = -INFINITY;
-        for (int s = 0; s < p.n_split; ++s) {
-            const float x = p.part_l[s * plane + hr];
-            m = x > m || x != x ? x : m;
-        }
-        const float ms = m == -INFINITY ? 0.f : m;
-        float l = 0.f, o[4] = {0.f, 0.f, 0.f, 0.f};
-        for (int s = 0; s < p.n_split; ++s) {
-            const float w = __builtin_amdgcn_exp2f(p.part_l[s * plane + hr] - ms);
-            const f32x4_t x = *reinterpret_cast<const f32x4_t *>(p.part_o + (s * plane + hr) * a.head_dim + c);
-            l += w;
-#pragma unroll
-            for (int e = 0; e < 4; ++e) o[e] += w * x[e];
-        }
-        const float inv = l > 0.f || l != l ? 1.f / l : 0.f;
-#pragma unroll
-        for (int e = 0; e < 4; ++e) o[e] *= inv;
-        const int64_t h = hr / a.n_q, row = hr - h * a.n_q;
-        magic::store_vec<T, 4>((T *)p.out + row * p.ld_o + h * p.hs_o + c, true, o);
-        if (c == 0) p.lse[hr] = m == -INFINITY ? -INFINITY : (ms + __builtin_amdgcn_logf(l)) * LN2;
-    }
+    const int64_t plane = a.n_q * a.q_heads;
+    const int tid = threadIdx.x, g = tid / CPR, c = (tid % CPR) * 4;
+    const int64_t hr = blockIdx.x;                  // head * n_q + row
+    const float mine = tid < p.n_split ? p.part_l[tid * plane + hr] : -INFINITY;
+    red[tid] = mine;
+    __syncthreads();
+    float m = -INFINITY;                            // (a NaN is the largest of all: it has to reach the result)
+    for (int s = 0; s < p.n_split; ++s) m = red[s] > m || red[s] != red[s] ? red[s] : m;
+    const float ms = m == -INFINITY ? 0.f : m;
+    w[tid] = __builtin_amdgcn_exp2f(mine - ms);
+    __syncthreads();
+    float l = 0.f;
+    for (int s = 0; s < p.n_split; ++s) l += w[s];
+    f32x4_t o = {0.f, 0.f, 0.f, 0.f};
+    if (c < a.head_dim)
+        for (int s = g; s < p.n_split; s += NG)
+            o += w[s] * *reinterpret_cast<const f32x4_t *>(p.part_o + (s * plane + hr) * a.head_dim + c);
+    so[tid] = o;
+    __syncthreads();
+    if (g != 0 || c >= a.head_dim) return;
+    const int n = p.n_split < NG ? p.n_split : NG;
+    for (int i = 1; i < n; ++i) o += so[i * CPR + tid];
+    const float inv = l > 0.f || l != l ? 1.f / l : 0.f;
+    const float x[4] = {o[0] * inv, o[1] * inv, o[2] * inv, o[3] * inv};
+    const int64_t h = hr / a.n_q, row = hr - h * a.n_q;
+    magic::store_vec<T, 4>((T *)p.out + row * p.ld_o + h * p.hs_o + c, true, x);
+    if (c == 0) p.lse[hr] = m == -INFINITY ? -INFINITY : ms + __builtin_amdgcn_logf(l);
 }
 
 struct Shape {
@@ -440,7 +538,7 @@ Shape shape_of(const magic_attn *a) {
     if (s.sub < 1) s.sub = 1;
     s.n_hb = a->q_heads / s.gc;
     const int64_t blocks = (int64_t)a->n_q_tiles * s.sub * s.n_hb;
-    int64_t split = (512 + blocks - 1) / blocks;
+    int64_t split = 512 / blocks;                      // two resident blocks a CU, all running at once
     const int64_t most = (a->max_k + 511) / 512;
     if (split > most) split = most;
     if (split > 256) split = 256;
@@ -477,16 +575,25 @@ template <typename M> int run(FwdArgs &p, int wm, hipStream_t st) {
     if (wm == 4) {
         rc = run_rows<M>(p, st);
     } else {
-        // (three planes of 128 keys and 128 columns would not fit the LDS)
-        constexpr int KG128 = M::N == 3 ? 2 : 4;
+        // wavefronts of a block: as many as leave the LDS room for two blocks a CU
+        constexpr int KG64 = M::N == 3 ? 2 : 4, KG128 = M::N == 3 ? 1 : 2;
         rc = D <= 16   ? launch<M, 16, 1, 4, 32>(p, st)
              : D <= 32 ? launch<M, 32, 1, 4, 32>(p, st)
-             : D <= 64 ? launch<M, 64, 1, 4, 32>(p, st)
+             : D <= 64 ? launch<M, 64, 1, KG64, 32>(p, st)
                        : launch<M, 128, 1, KG128, 32>(p, st);
     }
     if (rc != MAGIC_OK || p.n_split == 1) return rc;
-    const int grid = magic::stride_grid(p.a.n_q * p.a.q_heads * (D / 4), 256);
-    MAGIC_LAUNCH("attn_join", k_attn_join<typename M::T>, grid, 256, 0, st, p);
+    typedef typename M::T T;
+    const int64_t grid = p.a.n_q * p.a.q_heads;
+    if (grid > 0x7fffffffLL) return MAGIC_ERR_UNSUPPORTED;
+    if (D <= 16)
+        MAGIC_LAUNCH("attn_join", (k_attn_join<T, 4>), (int)grid, 256, 0, st, p);
+    else if (D <= 32)
+        MAGIC_LAUNCH("attn_join", (k_attn_join<T, 8>), (int)grid, 256, 0, st, p);
+    else if (D <= 64)
+        MAGIC_LAUNCH("attn_join", (k_attn_join<T, 16>), (int)grid, 256, 0, st, p);
+    else
+        MAGIC_LAUNCH("attn_join", (k_attn_join<T, 32>), (int)grid, 256, 0, st, p);
     return magic::launch_status();
 }
 
@@ -497,7 +604,7 @@ extern "C" {
 size_t magic_attn_fwd_workspace_bytes(const magic_attn *a) {
     if (check(a) != MAGIC_OK || a->n_q == 0) return 256;
     const Shape s = shape_of(a);
-    if (s.f16) return magic::align_up(magic::attn::range_count(a, false) * sizeof(Range)) + 256;
+    if (s.f16) return magic::attn::prepare_bytes(a, false) + 256;
     if (s.n_split == 1) return 256;
     const size_t rows = (size_t)s.n_split * a->q_heads * a->n_q;
     return magic::align_up(rows * a->head_dim * sizeof(float)) + magic::align_up(rows * sizeof(float)) + 256;
@@ -522,17 +629,13 @@ int magic_attn_fwd(const magic_attn *a, void *out, int64_t ld_out, int64_t hs_ou
         p.part_l = ar.take<float>(rows);
         if (!ar.ok()) return MAGIC_ERR_WORKSPACE;
     }
-    p.rg = Ranges{nullptr, nullptr, nullptr, nullptr, 0, false};
     if (s.f16) {
         magic::Arena ar(workspace, workspace_bytes);
-        Range *r = ar.take<Range>(magic::attn::range_count(a, false));
-        if (!ar.ok()) return MAGIC_ERR_WORKSPACE;
-        const int rc = magic::attn::prepare_ranges(a, nullptr, 0, 0, r, p.rg, (hipStream_t)stream);
+        const int rc = magic::attn::prepare(a, nullptr, ar, p.pr, (hipStream_t)stream);
         if (rc != MAGIC_OK) return rc;
-        p.rg.want_safe = true;
         const int rc2 = run_rows<F16x2>(p, (hipStream_t)stream);
         if (rc2 != MAGIC_OK) return rc2;
-        p.rg.want_safe = false;                // the segments whose rows differ too much in size
+        p.pr.rg.want_safe = false;             // the segments whose rows differ too much in size
         return run_rows<F32x3>(p, (hipStream_t)stream);
     }
     return a->dtype == MAGIC_F32 ? run<F32x3>(p, s.wm, (hipStream_t)stream) : run<BF16>(p, s.wm, (hipStream_t)stream);

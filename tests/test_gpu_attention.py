@@ -211,6 +211,51 @@ def test_attention_strides(cuda, dtype):
     check(one, q, k, v, torch.ones(n, h, D, device=cuda, dtype=dtype), lens, lens)
 
 
+@pytest.mark.parametrize("D,hq,hk", [(64, 16, 16), (40, 12, 6), (128, 16, 8)])
+@pytest.mark.parametrize("opts", ["plain", "all"])
+def test_attention_large_float32(cuda, D, hq, hk, opts):
+    """Enough rows and heads for the launches that split float32 into two fp16 pieces, forward and backward, with
+    segments next to each other that they do not serve: one whose rows differ by 2^20 in size, one with zero rows only in
+    v, one of zeros, one with an infinity.  The bounds are the ones of the other kernels."""
+    q_lens = kv_lens = [1030, 520, 129, 33, 600, 70]
+    q, k, v, d, kw = make(cuda, q_lens, kv_lens, hq, hk, D, torch.float32, seed=D + hq, slopes=opts == "all",
+                          mask=0.7 if opts == "all" else None)
+    cap = 9.0 if opts == "all" else 0.0
+    k[1030:1550:7] *= 2.0 ** -10
+    v[1030:1550:5] *= 2.0 ** -20
+    d[1030:1550:3] *= 2.0 ** 12
+    v[1550:1679] = 0.0
+    q[1679:1712] = 0.0
+    d[1712:2312:2] = 0.0                                       # rows without a gradient
+    check(run(q, k, v, d, q_lens, kv_lens, cap=cap, **kw), q, k, v, d, q_lens, kv_lens, cap=cap, **kw)
+    v2 = v.clone()
+    v2[2320, 0, 3] = float("inf")                              # the last segment
+    if opts == "plain":
+        a, b = run(q, k, v, d, q_lens, kv_lens), run(q, k, v2, d, q_lens, kv_lens)
+        assert torch.equal(a["out"][:2312], b["out"][:2312]) and torch.equal(a["dk"][:2312], b["dk"][:2312])
+        assert not torch.isfinite(b["out"][2312:, :hq // hk, 3]).any()
+        assert torch.isfinite(b["out"][2312:, hq // hk:]).all()
+
+
+def test_attention_long_tail_of_small_probabilities(cuda):
+    """A distance bias leaves thousands of keys whose terms are each below half a unit of the running sums: together they
+    count.  Relative 2-norm error of a float32 result, as small as one formed with whole-row sums."""
+    from magic_amd.model.attention import attention_plan, segment_attention
+    n, h, D = 6000, 8, 64
+    gen = torch.Generator(device=cuda).manual_seed(1)
+    q, k, v = (torch.randn(n, h, D, generator=gen, device=cuda) for _ in range(3))
+    v += 1.0
+    pos = torch.arange(n, device=cuda, dtype=torch.int32)
+    slopes = torch.full((h,), 0.003, device=cuda)
+    out = segment_attention(q, k, v, attention_plan([n], device=cuda), slopes=slopes, q_pos=pos, k_pos=pos)
+    dist = (pos.double()[:, None] - pos.double()[None]).abs()
+    for j in (0, 5):
+        p = torch.softmax(q[:, j].double() @ k[:, j].double().T / 8 - slopes[j].double() * dist, 1)
+        want = p @ v[:, j].double()
+        # logits off by (D + 8) u |q||k| / 8 at most, 1/50 of it as a 2-norm of random signs; sums of 6,000 terms
+        assert float((out[:, j].double() - want).norm() / want.norm()) < 1e-6
+
+
 def test_attention_gradient_against_differences(cuda):
     """Central differences of the 64-bit definition along random directions against the kernel's gradients."""
     lens = [37, 66]
