@@ -155,6 +155,7 @@ __global__ __launch_bounds__(NT, (DP == 128 && M::N > 1) ? 1 : 2) void k_attn_dq
     const bool bias = a.slopes != nullptr;
     const float slope = bias ? a.slopes[h] : 0.f;
     const uint32_t qpos = bias ? flip(a.q_pos[qr]) : 0u;
+    const float f_cap = a.cap > 0.f ? -a.scale / a.cap / a.cap : 0.f;      // scale (1 - tanh^2) from the capped score
     Running run;
     // Of the lane's row: sum dl dist, sum dl, sum p dist.  The matrix instructions round their inner sums downwards by
     // about 2^-27 of the terms; alike for all keys of a row, this changes no gradient but the slope's, where it meets the
@@ -169,8 +170,8 @@ __global__ __launch_bounds__(NT, (DP == 128 && M::N > 1) ? 1 : 2) void k_attn_dq
 
     stage kst, vst;
     uint8_t keep[stage::N];
-    uint32_t pos = 0;
-    float mk = 0.f;
+    int pos = 0;             // (taken as loaded: a use here would wait for the whole tile)
+    uint8_t mk = 0;
     auto load = [&](int j0) {
         kst.load(K, j0, nk, D, tid);
         vst.load(V, j0, nk, D, tid);
@@ -184,8 +185,8 @@ __global__ __launch_bounds__(NT, (DP == 128 && M::N > 1) ? 1 : 2) void k_attn_dq
         if (tid < BK) {
             const int j = j0 + tid;
             const bool in = j < nk;
-            mk = in && (!a.key_mask || a.key_mask[k0 + (in ? j : 0)]) ? 0.f : -INFINITY;
-            pos = bias && in ? flip(a.k_pos[k0 + j]) : 0u;
+            mk = in && a.key_mask ? a.key_mask[k0 + j] : in;
+            pos = bias && in ? a.k_pos[k0 + j] : 0;
         }
     };
     if (nk > 0) load(0);
@@ -193,7 +194,7 @@ __global__ __launch_bounds__(NT, (DP == 128 && M::N > 1) ? 1 : 2) void k_attn_dq
         __syncthreads();
         kst.store(sK, D, tid, [&](int i) { return keep[i] != 0; });
         vst.store(sV, D, tid, [&](int i) { return keep[i] != 0; });
-        if (tid < BK) sPos[tid] = pos, sMask[tid] = mk;
+        if (tid < BK) sPos[tid] = flip(pos), sMask[tid] = mk ? 0.f : -INFINITY;
         const bool masked = a.key_mask != nullptr || j0 + BK > nk;
         __syncthreads();
         if (j0 + BK < nk) load(j0 + BK);
@@ -210,7 +211,8 @@ __global__ __launch_bounds__(NT, (DP == 128 && M::N > 1) ? 1 : 2) void k_attn_dq
                 mma(s, f, qf[ks]);
                 mma(dp, g, gf[ks]);
             }
-            if (a.cap > 0.f) tanh_tile(s, sc.s_in);
+            feed<2 * NP, 2 * PRODUCTS<M>, KS>();
+            if (a.cap > 0.f) cap_tile<M::N == 1>(s, sc.s_in, a.cap);
             float ds[16], t_dsl = 0.f, t_dl = 0.f, t_pd = 0.f;
 #pragma unroll
             for (int g = 0; g < 4; ++g) {
@@ -224,8 +226,8 @@ __global__ __launch_bounds__(NT, (DP == 128 && M::N > 1) ? 1 : 2) void k_attn_dq
                     const int r = 4 * g + e;
                     float f = a.scale, x;
                     if (a.cap > 0.f) {
-                        x = s[r] * a.cap;
-                        f -= f * s[r] * s[r];
+                        x = s[r];
+                        f = fmaf(x * x, f_cap, f);
                     } else {
                         x = s[r] * sc.s_in;
                     }
@@ -264,6 +266,7 @@ __global__ __launch_bounds__(NT, (DP == 128 && M::N > 1) ? 1 : 2) void k_attn_dq
                     mma(acc[d], f, pf);
                 }
             }
+            feed<2 * NP, PRODUCTS<M>, 2 * DB>();
         }
     }
     const float undo = M::SCALED ? run.undo() * (1.f / sc.k) : 1.f;
@@ -333,6 +336,7 @@ __global__ __launch_bounds__(NT, DP == 128 ? 1 : 2) void k_attn_dkv(BwdArgs p) {
     }
     const bool bias = a.slopes != nullptr;
     const uint32_t kpos = bias ? flip(a.k_pos[kr]) : 0u;
+    const float f_cap = a.cap > 0.f ? -a.scale / a.cap / a.cap : 0.f;      // scale (1 - tanh^2) from the capped score
     Running run;
     f32x16_t gk[DB], gv[DB];
 #pragma unroll
@@ -343,7 +347,7 @@ __global__ __launch_bounds__(NT, DP == 128 ? 1 : 2) void k_attn_dkv(BwdArgs p) {
     stage qst, gst;
     uint8_t keep[stage::N];
     float ls = 0.f, dl0 = 0.f;
-    uint32_t pos = 0;
+    int pos = 0;             // (all taken as loaded: a use here would wait for the whole tile)
     auto load = [&](int h, int i0) {
         qst.load(src_of<M>(a.q, a.ld_q, a.hs_q, p.pr.q, q0, h, D), i0, nq, D, tid);
         gst.load(src_of<M>(p.dout, p.ld_do, p.hs_do, p.pr.g, q0, h, D), i0, nq, D, tid);
@@ -356,9 +360,9 @@ __global__ __launch_bounds__(NT, DP == 128 ? 1 : 2) void k_attn_dkv(BwdArgs p) {
         }
         if (tid < BQ) {
             const int r = i0 + tid;
-            ls = r < nq ? -l2[r] : -INFINITY;
-            dl0 = r < nq ? -p.delta[(int64_t)h * a.n_q + q0 + r] : 0.f;
-            pos = bias && r < nq ? flip(a.q_pos[q0 + r]) : 0u;
+            ls = r < nq ? l2[r] : INFINITY;
+            dl0 = r < nq ? p.delta[(int64_t)h * a.n_q + q0 + r] : 0.f;
+            pos = bias && r < nq ? a.q_pos[q0 + r] : 0;
         }
     };
     // this block's share of the steps (heads that share the key head, tiles of their rows)
@@ -370,7 +374,7 @@ __global__ __launch_bounds__(NT, DP == 128 ? 1 : 2) void k_attn_dkv(BwdArgs p) {
         __syncthreads();
         qst.store(sQ, D, tid, [&](int i) { return keep[i] != 0; });
         gst.store(sG, D, tid, [&](int i) { return keep[i] != 0; });
-        if (tid < BQ) sL[tid] = ls, sD[tid] = dl0, sPos[tid] = pos;
+        if (tid < BQ) sL[tid] = -ls, sD[tid] = -dl0, sPos[tid] = flip(pos);
         const float slope = bias ? a.slopes[h] : 0.f;
         __syncthreads();
         if (++it == per_h) it = 0, ++h;
@@ -388,7 +392,8 @@ __global__ __launch_bounds__(NT, DP == 128 ? 1 : 2) void k_attn_dkv(BwdArgs p) {
                 mma(s, f, kf[ks]);
                 mma(dp, g, vf[ks]);
             }
-            if (a.cap > 0.f) tanh_tile(s, sc.s_in);
+            feed<2 * NP, 2 * PRODUCTS<M>, KS>();
+            if (a.cap > 0.f) cap_tile<M::N == 1>(s, sc.s_in, a.cap);
             float pr[16], ds[16];
 #pragma unroll
             for (int g = 0; g < 4; ++g) {
@@ -402,8 +407,8 @@ __global__ __launch_bounds__(NT, DP == 128 ? 1 : 2) void k_attn_dkv(BwdArgs p) {
                     const int r = 4 * g + e;
                     float f = a.scale, x;
                     if (a.cap > 0.f) {
-                        x = s[r] * a.cap;
-                        f -= f * s[r] * s[r];
+                        x = s[r];
+                        f = fmaf(x * x, f_cap, f);
                     } else {
                         x = s[r] * sc.s_in;
                     }
@@ -435,6 +440,7 @@ __global__ __launch_bounds__(NT, DP == 128 ? 1 : 2) void k_attn_dkv(BwdArgs p) {
                     mma(gk[d], f, sf);
                 }
             }
+            feed<2 * NP, PRODUCTS<M>, 4 * DB>();
         }
     }
     if (!in) return;

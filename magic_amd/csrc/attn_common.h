@@ -171,6 +171,19 @@ __device__ __forceinline__ void mma(f32x16_t &c, const bf16x8_t (&a)[1], const b
     c = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a[0], b[0], c, 0, 0, 0);
 }
 
+// Order of a run of matrix instructions and the LDS reads that feed them: STEPS steps of READS reads and MFMAS
+// instructions, the reads of AHEAD steps before the first.  (Left alone, the compiler reads, waits and multiplies in turn:
+// a trip to the LDS before every product.)
+template <int READS, int MFMAS, int STEPS, int AHEAD = 2> __device__ __forceinline__ void feed() {
+    __builtin_amdgcn_sched_group_barrier(0x100, READS * AHEAD, 0);
+#pragma unroll
+    for (int i = 0; i < STEPS; ++i) {
+        __builtin_amdgcn_sched_group_barrier(0x8, MFMAS, 0);
+        if (i + AHEAD < STEPS) __builtin_amdgcn_sched_group_barrier(0x100, READS, 0);
+    }
+}
+template <typename M> constexpr int PRODUCTS = M::N == 3 ? 6 : M::N == 2 ? 3 : 1;
+
 // A tile of ROWS operand rows in LDS: planes of [ROWS][LDW] bf16, rows padded by 16 bytes (reads of one column range by
 // 32 rows then spread over the banks).
 template <typename M, int DP, int ROWS> struct Tile {
@@ -243,20 +256,20 @@ template <typename M, int DP, int ROWS, int NT> struct Stage {
     __device__ __forceinline__ static int row_of(int i, int tid) { return (tid + i * NT) / CPR; }
 };
 
-// tanh to a few units of float32 relative: odd series below TANH_SMALL, (1 - e) / (1 + e) elsewhere
+// Capped scores of a tile: x[i] = cap tanh(x[i] f).  tanh by its odd series below TANH_SMALL -- to a few units of
+// float32, or to 5e-6 relative where the probabilities are rounded to bfloat16 (SHORT) -- and as (1 - e) / (1 + e)
+// elsewhere.  A cap is far above most scores: the series serves alone where no score of the wavefront leaves it.
 constexpr float TANH_SMALL = 0.35f;
-__device__ __forceinline__ float tanh_series(float x) {
+template <bool SHORT> __device__ __forceinline__ float tanh_series(float x, float cap) {     // times cap
     const float z = x * x;
-    return x * (1.f + z * (-0.333333333f + z * (0.133333333f + z * (-0.0539682540f + z * (0.0218694885f - z * 0.00886323553f)))));
+    float p = SHORT ? -0.0539682540f * cap : (0.0218694885f - z * 0.00886323553f) * cap;
+    if (!SHORT) p = fmaf(z, p, -0.0539682540f * cap);
+    p = fmaf(z, p, 0.133333333f * cap);
+    p = fmaf(z, p, -0.333333333f * cap);
+    p = fmaf(z, p, cap);
+    return x * p;
 }
-__device__ __forceinline__ float tanh_f(float x) {
-    const float a = fabsf(x);
-    const float e = __builtin_amdgcn_exp2f(-2.f * LOG2E * a);
-    const float b = (1.f - e) * __builtin_amdgcn_rcpf(1.f + e);
-    return a < TANH_SMALL ? tanh_series(x) : copysignf(b, x);
-}
-// x[i] = tanh(x[i] * f) of a tile; the series alone where no score of the wavefront leaves it (a cap is far above most scores)
-__device__ __forceinline__ void tanh_tile(f32x16_t &x, float f) {
+template <bool SHORT> __device__ __forceinline__ void cap_tile(f32x16_t &x, float f, float cap) {
     float m = 0.f;
 #pragma unroll
     for (int r = 0; r < 16; ++r) {
@@ -265,10 +278,16 @@ __device__ __forceinline__ void tanh_tile(f32x16_t &x, float f) {
     }
     if (__any(m >= TANH_SMALL)) {
 #pragma unroll
-        for (int r = 0; r < 16; ++r) x[r] = tanh_f(x[r]);
+        for (int r = 0; r < 16; ++r) {
+            const float a = fabsf(x[r]);
+            const float e = __builtin_amdgcn_exp2f(-2.f * LOG2E * a);
+            float b = copysignf(cap * (1.f - e) * __builtin_amdgcn_rcpf(1.f + e), x[r]);
+            asm("" : "+v"(b));          // (a select between two values, not a branch around one)
+            x[r] = a < TANH_SMALL ? tanh_series<SHORT>(x[r], cap) : b;
+        }
     } else {
 #pragma unroll
-        for (int r = 0; r < 16; ++r) x[r] = tanh_series(x[r]);
+        for (int r = 0; r < 16; ++r) x[r] = tanh_series<SHORT>(x[r], cap);
     }
 }
 

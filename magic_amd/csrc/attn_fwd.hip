@@ -304,8 +304,8 @@ __global__ __launch_bounds__(64 * WM *KG, DP == 128 && (M::N == 3 || WM == 1) ? 
 
     stage kst, vst;
     uint8_t keep[stage::N];
-    uint32_t pos = 0;
-    float mk = 0.f;
+    int pos = 0;             // (taken as loaded: a use here would wait for the whole tile)
+    uint8_t mk = 0;
     auto load = [&](int tt) {
         const int j0 = tt * BK;
         kst.load(K, j0, nk, D, tid);
@@ -320,8 +320,8 @@ __global__ __launch_bounds__(64 * WM *KG, DP == 128 && (M::N == 3 || WM == 1) ? 
         if (tid < BK) {
             const int j = j0 + tid;
             const bool in = j < nk;
-            mk = in && (!a.key_mask || a.key_mask[k0 + (in ? j : 0)]) ? 0.f : -INFINITY;
-            pos = bias && in ? flip(a.k_pos[k0 + j]) : 0u;
+            mk = in && a.key_mask ? a.key_mask[k0 + j] : in;
+            pos = bias && in ? a.k_pos[k0 + j] : 0;
         }
     };
     if (t_beg < t_end) load(t_beg);
@@ -329,7 +329,7 @@ __global__ __launch_bounds__(64 * WM *KG, DP == 128 && (M::N == 3 || WM == 1) ? 
         __syncthreads();  // the reads of the tile before are done
         kst.store(sK, D, tid, [&](int i) { return keep[i] != 0; });
         vst.store(sV, D, tid, [&](int i) { return keep[i] != 0; });
-        if (tid < BK) sPos[tid] = pos, sMask[tid] = mk;
+        if (tid < BK) sPos[tid] = flip(pos), sMask[tid] = mk ? 0.f : -INFINITY;
         const bool masked = a.key_mask != nullptr || (tt + 1) * BK > nk;
         __syncthreads();
         if (tt + 1 < t_end) load(tt + 1);
@@ -347,21 +347,23 @@ __global__ __launch_bounds__(64 * WM *KG, DP == 128 && (M::N == 3 || WM == 1) ? 
                 tile::frag(sK, kg * KW + 32 * b + li, 16 * ks + 8 * hf, f);
                 mma(s[b], f, qf[ks]);
             }
+        feed<NP * KB, PRODUCTS<M> * KB, KS>();
         // logits; a masked key's zero score gets -inf
 #pragma unroll
         for (int b = 0; b < KB; ++b) {
-            const float f = a.cap > 0.f ? a.cap : s_in;
-            if (a.cap > 0.f) tanh_tile(s[b], s_in);
+            if (a.cap > 0.f) {
+                cap_tile<M::N == 1>(s[b], s_in, a.cap);
+            } else {
+#pragma unroll
+                for (int r = 0; r < 16; ++r) s[b][r] *= s_in;
+            }
             if (masked) {
 #pragma unroll
                 for (int g = 0; g < 4; ++g) {
                     const f32x4_t km = *reinterpret_cast<const f32x4_t *>(sMask + kg * KW + 32 * b + 8 * g + 4 * hf);
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) s[b][4 * g + e] = fmaf(s[b][4 * g + e], f, km[e]);
+                    for (int e = 0; e < 4; ++e) s[b][4 * g + e] += km[e];
                 }
-            } else {
-#pragma unroll
-                for (int r = 0; r < 16; ++r) s[b][r] *= f;
             }
             if (bias) {
 #pragma unroll
@@ -383,6 +385,14 @@ __global__ __launch_bounds__(64 * WM *KG, DP == 128 && (M::N == 3 || WM == 1) ? 
         m = mx;
         // The tile's sums are formed by themselves and added once: a long tail of small terms, each below half a unit of
         // the running sum, would otherwise be lost term by term (3e-6 of the result over 8,000 keys with a distance bias).
+        // bfloat16 results do not see that: their sums run on, and are scaled where a maximum moves.
+        constexpr bool TILE_SUM = M::N > 1;
+        if (!TILE_SUM && __any(al != 1.f)) {
+#pragma unroll
+            for (int d = 0; d < DB; ++d)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) o[d][r] *= al;
+        }
         float tsum = 0.f;
         vec pf[KB * 2][NP];
 #pragma unroll
@@ -400,17 +410,24 @@ __global__ __launch_bounds__(64 * WM *KG, DP == 128 && (M::N == 3 || WM == 1) ? 
         l = fmaf(l, al, tsum);
 #pragma unroll
         for (int d = 0; d < DB; ++d) {
-            f32x16_t c;
+            f32x16_t c = o[d];
+            if (TILE_SUM) {
 #pragma unroll
-            for (int r = 0; r < 16; ++r) c[r] = 0.f;
+                for (int r = 0; r < 16; ++r) c[r] = 0.f;
+            }
 #pragma unroll
             for (int w = 0; w < KB * 2; ++w) {
                 vec f[NP];
                 tile::frag_t(sV, kg * KW + 16 * w, 32 * d, lane, f);
                 mma(c, f, pf[w]);
             }
+            feed<2 * NP, PRODUCTS<M>, KB * 2>();
+            if (TILE_SUM) {
 #pragma unroll
-            for (int r = 0; r < 16; ++r) o[d][r] = fmaf(o[d][r], al, c[r]);
+                for (int r = 0; r < 16; ++r) o[d][r] = fmaf(o[d][r], al, c[r]);
+            } else {
+                o[d] = c;
+            }
         }
     }
     l += other_half(l);
