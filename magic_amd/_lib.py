@@ -930,7 +930,7 @@ def knn_merge(part_dist: torch.Tensor, part_idx: torch.Tensor):
 # ------------------------------------------------------------------------------------- segment attention
 # These operators take their scratch from torch's allocator at every call (not from ``workspace``): calls on several
 # streams, and captured graphs, never share it.
-ATTN_MAX_DIM, ATTN_TILE = 128, 128
+ATTN_MAX_DIM, ATTN_TILE, ATTN_MAX_LD = 128, 128, 1 << 22
 _ATTN_DTYPE = {torch.float32: 0, torch.bfloat16: 1}
 
 
@@ -959,7 +959,8 @@ def _scratch(nbytes: int, device) -> torch.Tensor:
 def _head_rows(t: torch.Tensor) -> torch.Tensor:
     """[rows, heads, head_dim] operand with unit inner stride, other strides and address in whole 16 bytes."""
     per = 16 // t.element_size()
-    if t.stride(2) == 1 and t.stride(0) % per == 0 and t.stride(1) % per == 0 and t.data_ptr() % 16 == 0:
+    if t.stride(2) == 1 and t.stride(0) % per == 0 and t.stride(1) % per == 0 and t.data_ptr() % 16 == 0 \
+            and t.stride(0) <= ATTN_MAX_LD:
         return t
     t = t.contiguous()
     return t if t.data_ptr() % 16 == 0 else t.clone()

@@ -107,6 +107,79 @@ struct Running {
     __device__ __forceinline__ float undo() const { return u == 0.f ? 0.f : 1.f / u; }
 };
 
+// What a lane knows of its row in the dq sweep
+struct RowSide {
+    float s_in, dp_in, scale, cap, f_cap, slope;   // f_cap: -scale / cap^2, for scale (1 - tanh^2) from the capped score
+    uint32_t pos;
+    float lse, delta;
+};
+// Of the lane's row: sum dl dist, sum dl, sum p dist.  The matrix instructions round their inner sums downwards by about
+// 2^-27 of the terms; alike for all keys of a row, this changes no gradient but the slope's, where it meets the mean
+// distance with one sign in every row (4e-5 of d slope over 97,000 rows).  sum dl, zero but for such an offset, takes it
+// out again.  In double: long sums of both signs.
+struct SlopeSums {
+    double dl_dist = 0.0, dl = 0.0, pd = 0.0;
+};
+
+// Scores and do.v of 32 keys by 32 rows -> gradients of the scores (before the scale of dq); km, kp: the keys' masks
+// (0 / -inf) and positions, four for every group of registers
+template <typename M, bool CAP, bool BIAS, bool MASK>
+__device__ __forceinline__ void score_grad(f32x16_t &s, const f32x16_t &dp, const RowSide &c, const f32x4_t *km,
+                                           const i32x4_t *kp, float (&ds)[16], SlopeSums &sums) {
+    if (CAP) cap_tile<M::N == 1>(s, c.s_in, c.cap);
+    float t_dsl = 0.f, t_dl = 0.f, t_pd = 0.f;
+#pragma unroll
+    for (int g = 0; g < 4; ++g) {
+        f32x4_t base = {-c.lse, -c.lse, -c.lse, -c.lse};       // -inf for masked keys: their probabilities are zeros
+        if (MASK) base += km[2 * g];
+        i32x4_t pos;
+        if (BIAS) pos = kp[2 * g];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            const int r = 4 * g + e;
+            float x = CAP ? s[r] : s[r] * c.s_in, dist;
+            const float f = CAP ? fmaf(x * x, c.f_cap, c.scale) : c.scale;
+            if (BIAS) {
+                dist = dist_of((uint32_t)pos[e], c.pos);
+                x = fmaf(-c.slope, dist, x);
+            }
+            const float pr = __builtin_amdgcn_exp2f(fmaf(x, LOG2E, base[e]));
+            const float dl = pr * fmaf(dp[r], c.dp_in, -c.delta);
+            if (BIAS) {
+                t_dsl = fmaf(dl, dist, t_dsl);
+                t_pd = fmaf(pr, dist, t_pd);
+                t_dl += dl;
+            }
+            ds[r] = dl * f;
+        }
+    }
+    if (BIAS) sums.dl_dist += (double)t_dsl, sums.dl += (double)t_dl, sums.pd += (double)t_pd;
+}
+
+// The same with the keys in the lanes: probabilities (times 2^14 in the scaled mode) and score gradients; l, d: minus lse
+// and minus D of the rows, qp their positions
+template <typename M, bool CAP, bool BIAS>
+__device__ __forceinline__ void prob_grad(f32x16_t &s, const f32x16_t &dp, const RowSide &c, const f32x4_t *l, const f32x4_t *d,
+                                          const i32x4_t *qp, float (&pr)[16], float (&ds)[16]) {
+    if (CAP) cap_tile<M::N == 1>(s, c.s_in, c.cap);
+#pragma unroll
+    for (int g = 0; g < 4; ++g) {
+        const f32x4_t l4 = l[2 * g], d4 = d[2 * g];
+        i32x4_t pos;
+        if (BIAS) pos = qp[2 * g];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            const int r = 4 * g + e;
+            float x = CAP ? s[r] : s[r] * c.s_in;
+            const float f = CAP ? fmaf(x * x, c.f_cap, c.scale) : c.scale;
+            if (BIAS) x = fmaf(-c.slope, dist_of((uint32_t)pos[e], c.pos), x);
+            const float q = __builtin_amdgcn_exp2f(fmaf(x, LOG2E, l4[e]));
+            pr[r] = M::SCALED ? q * 16384.f : q;
+            ds[r] = q * fmaf(dp[r], c.dp_in, d4[e]) * f;
+        }
+    }
+}
+
 constexpr int NT = 256;
 
 template <typename M, int DP, int BK>
@@ -155,20 +228,18 @@ __global__ __launch_bounds__(NT, (DP == 128 && M::N > 1) ? 1 : 2) void k_attn_dq
     const bool bias = a.slopes != nullptr;
     const float slope = bias ? a.slopes[h] : 0.f;
     const uint32_t qpos = bias ? flip(a.q_pos[qr]) : 0u;
-    const float f_cap = a.cap > 0.f ? -a.scale / a.cap / a.cap : 0.f;      // scale (1 - tanh^2) from the capped score
+    const float f_cap = a.cap > 0.f ? -a.scale / a.cap / a.cap : 0.f;
     Running run;
-    // Of the lane's row: sum dl dist, sum dl, sum p dist.  The matrix instructions round their inner sums downwards by
-    // about 2^-27 of the terms; alike for all keys of a row, this changes no gradient but the slope's, where it meets the
-    // mean distance with one sign in every row (4e-5 of d slope over 97,000 rows).  sum dl, zero but for such an offset,
-    // takes it out again.
-    double dsl = 0.0, sdl = 0.0, spd = 0.0;
+    SlopeSums sums;
     f32x16_t acc[DB];
 #pragma unroll
     for (int d = 0; d < DB; ++d)
 #pragma unroll
         for (int r = 0; r < 16; ++r) acc[d][r] = 0.f;
 
+    uint32_t plain = tile::lane_plain(lane), turned = tile::lane_turned(lane);
     stage kst, vst;
+    kst.init(K, D, tid), vst.init(V, D, tid);
     uint8_t keep[stage::N];
     int pos = 0;             // (taken as loaded: a use here would wait for the whole tile)
     uint8_t mk = 0;
@@ -177,10 +248,9 @@ __global__ __launch_bounds__(NT, (DP == 128 && M::N > 1) ? 1 : 2) void k_attn_dq
         vst.load(V, j0, nk, D, tid);
 #pragma unroll
         for (int i = 0; i < stage::N; ++i) {
-            if (Src<M>::READY) break;
             const int j = j0 + stage::row_of(i, tid);
             keep[i] = j < nk;
-            if (a.key_mask && j < nk) keep[i] = a.key_mask[k0 + j];
+            if (!Src<M>::READY && a.key_mask && j < nk) keep[i] = a.key_mask[k0 + j];
         }
         if (tid < BK) {
             const int j = j0 + tid;
@@ -192,61 +262,42 @@ __global__ __launch_bounds__(NT, (DP == 128 && M::N > 1) ? 1 : 2) void k_attn_dq
     if (nk > 0) load(0);
     for (int j0 = 0; j0 < nk; j0 += BK) {
         __syncthreads();
-        kst.store(sK, D, tid, [&](int i) { return keep[i] != 0; });
-        vst.store(sV, D, tid, [&](int i) { return keep[i] != 0; });
-        if (tid < BK) sPos[tid] = flip(pos), sMask[tid] = mk ? 0.f : -INFINITY;
         const bool masked = a.key_mask != nullptr || j0 + BK > nk;
+        kst.store(sK, D, tid, masked, [&](int i) { return keep[i] != 0; });
+        vst.store(sV, D, tid, masked, [&](int i) { return keep[i] != 0; });
+        if (tid < BK) sPos[tid] = flip(pos), sMask[tid] = mk ? 0.f : -INFINITY;
         __syncthreads();
         if (j0 + BK < nk) load(j0 + BK);
 #pragma unroll 1
         for (int b = 0; b < BK / 32; ++b) {
+            stay(plain), stay(turned);
             f32x16_t s, dp;
 #pragma unroll
             for (int r = 0; r < 16; ++r) s[r] = 0.f, dp[r] = 0.f;
 #pragma unroll
             for (int ks = 0; ks < KS; ++ks) {
                 vec f[NP], g[NP];
-                tile::frag(sK, 32 * b + li, 16 * ks + 8 * hf, f);
-                tile::frag(sV, 32 * b + li, 16 * ks + 8 * hf, g);
+                tile::frag(sK, plain, 32 * b, ks, f);
+                tile::frag(sV, plain, 32 * b, ks, g);
                 mma(s, f, qf[ks]);
                 mma(dp, g, gf[ks]);
             }
             feed<2 * NP, 2 * PRODUCTS<M>, KS>();
-            if (a.cap > 0.f) cap_tile<M::N == 1>(s, sc.s_in, a.cap);
-            float ds[16], t_dsl = 0.f, t_dl = 0.f, t_pd = 0.f;
-#pragma unroll
-            for (int g = 0; g < 4; ++g) {
-                const int jr = 32 * b + 8 * g + 4 * hf;
-                f32x4_t base = {-ls, -ls, -ls, -ls};       // -inf for masked keys: their probabilities are zeros
-                if (masked) base += *reinterpret_cast<const f32x4_t *>(sMask + jr);
-                i32x4_t kp = {0, 0, 0, 0};
-                if (bias) kp = *reinterpret_cast<const i32x4_t *>(sPos + jr);
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    const int r = 4 * g + e;
-                    float f = a.scale, x;
-                    if (a.cap > 0.f) {
-                        x = s[r];
-                        f = fmaf(x * x, f_cap, f);
-                    } else {
-                        x = s[r] * sc.s_in;
-                    }
-                    float dist = 0.f;
-                    if (bias) {
-                        dist = dist_of((uint32_t)kp[e], qpos);
-                        x = fmaf(-slope, dist, x);
-                    }
-                    const float pr = __builtin_amdgcn_exp2f(fmaf(x, LOG2E, base[e]));
-                    const float dl = pr * fmaf(dp[r], sc.dp_in, -dl0);
-                    if (bias) {
-                        t_dsl = fmaf(dl, dist, t_dsl);
-                        t_pd = fmaf(pr, dist, t_pd);
-                        t_dl += dl;
-                    }
-                    ds[r] = dl * f;
-                }
+            float ds[16];
+            const RowSide rs = {sc.s_in, sc.dp_in, a.scale, a.cap, f_cap, slope, qpos, ls, dl0};
+            const f32x4_t *km = reinterpret_cast<const f32x4_t *>(sMask + 32 * b + 4 * hf);
+            const i32x4_t *kp = reinterpret_cast<const i32x4_t *>(sPos + 32 * b + 4 * hf);
+            if (a.cap > 0.f) {
+                if (bias)
+                    masked ? score_grad<M, true, true, true>(s, dp, rs, km, kp, ds, sums) : score_grad<M, true, true, false>(s, dp, rs, km, kp, ds, sums);
+                else
+                    masked ? score_grad<M, true, false, true>(s, dp, rs, km, kp, ds, sums) : score_grad<M, true, false, false>(s, dp, rs, km, kp, ds, sums);
+            } else {
+                if (bias)
+                    masked ? score_grad<M, false, true, true>(s, dp, rs, km, kp, ds, sums) : score_grad<M, false, true, false>(s, dp, rs, km, kp, ds, sums);
+                else
+                    masked ? score_grad<M, false, false, true>(s, dp, rs, km, kp, ds, sums) : score_grad<M, false, false, false>(s, dp, rs, km, kp, ds, sums);
             }
-            if (bias) dsl += (double)t_dsl, sdl += (double)t_dl, spd += (double)t_pd;
             float u = 1.f;
             if constexpr (M::SCALED) {
                 run.step<DB>(ds, acc);
@@ -262,7 +313,7 @@ __global__ __launch_bounds__(NT, (DP == 128 && M::N > 1) ? 1 : 2) void k_attn_dq
 #pragma unroll
                 for (int d = 0; d < DB; ++d) {
                     vec f[NP];
-                    tile::frag_t(sK, 32 * b + 16 * w, 32 * d, lane, f);
+                    tile::frag_t(sK, turned, 32 * b + 16 * w, d, f);
                     mma(acc[d], f, pf);
                 }
             }
@@ -284,8 +335,8 @@ __global__ __launch_bounds__(NT, (DP == 128 && M::N > 1) ? 1 : 2) void k_attn_dq
     if (p.slope_part) {
         __syncthreads();
         double *red = reinterpret_cast<double *>(smem);
-        sdl += __shfl_xor(sdl, 32, 64);
-        dsl = sdl * spd - dsl;          // (either half's share of sum p dist)
+        sums.dl += __shfl_xor(sums.dl, 32, 64);
+        double dsl = sums.dl * sums.pd - sums.dl_dist;          // (either half's share of sum p dist)
 #pragma unroll
         for (int k = 32; k > 0; k >>= 1) dsl += __shfl_xor(dsl, k, 64);
         if (lane == 0) red[wave] = dsl;
@@ -336,7 +387,7 @@ __global__ __launch_bounds__(NT, DP == 128 ? 1 : 2) void k_attn_dkv(BwdArgs p) {
     }
     const bool bias = a.slopes != nullptr;
     const uint32_t kpos = bias ? flip(a.k_pos[kr]) : 0u;
-    const float f_cap = a.cap > 0.f ? -a.scale / a.cap / a.cap : 0.f;      // scale (1 - tanh^2) from the capped score
+    const float f_cap = a.cap > 0.f ? -a.scale / a.cap / a.cap : 0.f;
     Running run;
     f32x16_t gk[DB], gv[DB];
 #pragma unroll
@@ -344,20 +395,18 @@ __global__ __launch_bounds__(NT, DP == 128 ? 1 : 2) void k_attn_dkv(BwdArgs p) {
 #pragma unroll
         for (int r = 0; r < 16; ++r) gk[d][r] = 0.f, gv[d][r] = 0.f;
 
+    uint32_t plain = tile::lane_plain(lane), turned = tile::lane_turned(lane);
     stage qst, gst;
-    uint8_t keep[stage::N];
+    qst.init(src_of<M>(a.q, a.ld_q, a.hs_q, p.pr.q, q0, 0, D), D, tid);
+    gst.init(src_of<M>(p.dout, p.ld_do, p.hs_do, p.pr.g, q0, 0, D), D, tid);
+    int staged = 0;          // rows of the segment behind the staged tile's first
     float ls = 0.f, dl0 = 0.f;
     int pos = 0;             // (all taken as loaded: a use here would wait for the whole tile)
     auto load = [&](int h, int i0) {
         qst.load(src_of<M>(a.q, a.ld_q, a.hs_q, p.pr.q, q0, h, D), i0, nq, D, tid);
         gst.load(src_of<M>(p.dout, p.ld_do, p.hs_do, p.pr.g, q0, h, D), i0, nq, D, tid);
         const float *l2 = p.lse2 + (int64_t)h * a.n_q + q0;
-#pragma unroll
-        for (int i = 0; i < stage::N; ++i) {
-            if (Src<M>::READY) break;
-            const int r = i0 + stage::row_of(i, tid);
-            keep[i] = r < nq && l2[r < nq ? r : 0] != INFINITY;
-        }
+        staged = nq - i0;
         if (tid < BQ) {
             const int r = i0 + tid;
             ls = r < nq ? l2[r] : INFINITY;
@@ -372,8 +421,11 @@ __global__ __launch_bounds__(NT, DP == 128 ? 1 : 2) void k_attn_dkv(BwdArgs p) {
     if (s_beg < s_end) load(h, it * BQ);
     for (int st = s_beg; st < s_end; ++st) {
         __syncthreads();
-        qst.store(sQ, D, tid, [&](int i) { return keep[i] != 0; });
-        gst.store(sG, D, tid, [&](int i) { return keep[i] != 0; });
+        // (a row that sees no key belongs to a segment without any: its dk and dv are written as zeros whatever it holds)
+        const bool part = staged < BQ;
+        const int rows = staged;
+        qst.store(sQ, D, tid, part, [&](int i) { return stage::row_of(i, tid) < rows; });
+        gst.store(sG, D, tid, part, [&](int i) { return stage::row_of(i, tid) < rows; });
         if (tid < BQ) sL[tid] = -ls, sD[tid] = -dl0, sPos[tid] = flip(pos);
         const float slope = bias ? a.slopes[h] : 0.f;
         __syncthreads();
@@ -381,43 +433,28 @@ __global__ __launch_bounds__(NT, DP == 128 ? 1 : 2) void k_attn_dkv(BwdArgs p) {
         if (st + 1 < s_end) load(h, it * BQ);
 #pragma unroll 1
         for (int b = 0; b < BQ / 32; ++b) {
+            stay(plain), stay(turned);
             f32x16_t s, dp;
 #pragma unroll
             for (int r = 0; r < 16; ++r) s[r] = 0.f, dp[r] = 0.f;
 #pragma unroll
             for (int ks = 0; ks < KS; ++ks) {
                 vec f[NP], g[NP];
-                tile::frag(sQ, 32 * b + li, 16 * ks + 8 * hf, f);
-                tile::frag(sG, 32 * b + li, 16 * ks + 8 * hf, g);
+                tile::frag(sQ, plain, 32 * b, ks, f);
+                tile::frag(sG, plain, 32 * b, ks, g);
                 mma(s, f, kf[ks]);
                 mma(dp, g, vf[ks]);
             }
             feed<2 * NP, 2 * PRODUCTS<M>, KS>();
-            if (a.cap > 0.f) cap_tile<M::N == 1>(s, sc.s_in, a.cap);
             float pr[16], ds[16];
-#pragma unroll
-            for (int g = 0; g < 4; ++g) {
-                const int ir = 32 * b + 8 * g + 4 * hf;
-                const f32x4_t l4 = *reinterpret_cast<const f32x4_t *>(sL + ir);      // -lse, -D of the rows
-                const f32x4_t d4 = *reinterpret_cast<const f32x4_t *>(sD + ir);
-                i32x4_t qp = {0, 0, 0, 0};
-                if (bias) qp = *reinterpret_cast<const i32x4_t *>(sPos + ir);
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    const int r = 4 * g + e;
-                    float f = a.scale, x;
-                    if (a.cap > 0.f) {
-                        x = s[r];
-                        f = fmaf(x * x, f_cap, f);
-                    } else {
-                        x = s[r] * sc.s_in;
-                    }
-                    if (bias) x = fmaf(-slope, dist_of((uint32_t)qp[e], kpos), x);
-                    const float q = __builtin_amdgcn_exp2f(fmaf(x, LOG2E, l4[e]));
-                    pr[r] = M::SCALED ? q * 16384.f : q;
-                    ds[r] = q * fmaf(dp[r], sc.dp_in, d4[e]) * f;
-                }
-            }
+            const RowSide ks = {sc.s_in, sc.dp_in, a.scale, a.cap, f_cap, slope, kpos, 0.f, 0.f};
+            const f32x4_t *l4 = reinterpret_cast<const f32x4_t *>(sL + 32 * b + 4 * hf);
+            const f32x4_t *d4 = reinterpret_cast<const f32x4_t *>(sD + 32 * b + 4 * hf);
+            const i32x4_t *qp = reinterpret_cast<const i32x4_t *>(sPos + 32 * b + 4 * hf);
+            if (a.cap > 0.f)
+                bias ? prob_grad<M, true, true>(s, dp, ks, l4, d4, qp, pr, ds) : prob_grad<M, true, false>(s, dp, ks, l4, d4, qp, pr, ds);
+            else
+                bias ? prob_grad<M, false, true>(s, dp, ks, l4, d4, qp, pr, ds) : prob_grad<M, false, false>(s, dp, ks, l4, d4, qp, pr, ds);
             float u = 1.f;
             if constexpr (M::SCALED) {
                 run.step<DB>(ds, gk);
@@ -434,9 +471,9 @@ __global__ __launch_bounds__(NT, DP == 128 ? 1 : 2) void k_attn_dkv(BwdArgs p) {
 #pragma unroll
                 for (int d = 0; d < DB; ++d) {
                     vec f[NP];
-                    tile::frag_t(sG, 32 * b + 16 * w, 32 * d, lane, f);
+                    tile::frag_t(sG, turned, 32 * b + 16 * w, d, f);
                     mma(gv[d], f, pf);
-                    tile::frag_t(sQ, 32 * b + 16 * w, 32 * d, lane, f);
+                    tile::frag_t(sQ, turned, 32 * b + 16 * w, d, f);
                     mma(gk[d], f, sf);
                 }
             }
@@ -573,6 +610,7 @@ int magic_attn_bwd(const magic_attn *a, const void *out, int64_t ld_out, int64_t
     if (d_slopes && !a->slopes) return MAGIC_ERR_INVALID_ARG;
     const int per = a->dtype == MAGIC_F32 ? 4 : 8;
     if (((uintptr_t)out | (uintptr_t)d_out | (uintptr_t)dq | (uintptr_t)dk | (uintptr_t)dv) & 15) return MAGIC_ERR_INVALID_ARG;
+    if (ld_do > MAX_LD) return MAGIC_ERR_UNSUPPORTED;
     if (ld_out < 0 || hs_out < 0 || ld_do < 0 || hs_do < 0 || (ld_out | hs_out | ld_do | hs_do) % per) return MAGIC_ERR_INVALID_ARG;
     BwdArgs b;
     b.a = *a;

@@ -133,16 +133,21 @@ template <typename M> struct Src {
     static constexpr bool READY = false;
     const T *p;
     int64_t ld;
-    __device__ __forceinline__ void load(raw &r, int64_t row, int col) const { r.load(p + row * ld + col); }
+    __device__ __forceinline__ Src from(int64_t row) const { return {p + row * ld, ld}; }
+    __device__ __forceinline__ void load(raw &r, uint32_t off) const {
+        r.load(reinterpret_cast<const T *>(reinterpret_cast<const char *>(p) + off * (uint32_t)sizeof(T)));
+    }
 };
 template <> struct Src<F16x2> {
     typedef RawF16 raw;
     static constexpr bool READY = true;
     const _Float16 *p;
     int64_t ld, lo;      // lo: from a high piece to its low one
-    __device__ __forceinline__ void load(raw &r, int64_t row, int col) const {
-        r.h = *reinterpret_cast<const f16x8_t *>(p + row * ld + col);
-        r.l = *reinterpret_cast<const f16x8_t *>(p + lo + row * ld + col);
+    __device__ __forceinline__ Src from(int64_t row) const { return {p + row * ld, ld, lo}; }
+    __device__ __forceinline__ void load(raw &r, uint32_t off) const {
+        const char *b = reinterpret_cast<const char *>(p);
+        r.h = *reinterpret_cast<const f16x8_t *>(b + off * 2u);
+        r.l = *reinterpret_cast<const f16x8_t *>(b + 2 * lo + off * 2u);
     }
 };
 // planes of one operand in the workspace: [hi | lo][rows][heads][D]
@@ -184,23 +189,41 @@ template <int READS, int MFMAS, int STEPS, int AHEAD = 2> __device__ __forceinli
 }
 template <typename M> constexpr int PRODUCTS = M::N == 3 ? 6 : M::N == 2 ? 3 : 1;
 
-// A tile of ROWS operand rows in LDS: planes of [ROWS][LDW] bf16, rows padded by 16 bytes (reads of one column range by
-// 32 rows then spread over the banks).
+// A tile of ROWS operand rows in LDS: planes of [ROWS][W] 16-bit values.  The 16-byte chunks of a row are permuted by its
+// number (swz): sixteen rows at one column range, what a plain fragment reads, and four rows at a 64-byte range, what a
+// transposed one reads, then lie on different banks (padded rows serve only one of the two: 45 % of the LDS cycles at
+// 128 columns were conflicts).
 template <typename M, int DP, int ROWS> struct Tile {
     typedef typename M::vec vec;
     static constexpr int NP = M::N;
     static constexpr int W = DP < 32 ? 32 : DP;      // a transposed read covers 32 columns
-    static constexpr int LDW = W + 8;
-    static constexpr int PLANE = ROWS * LDW;
+    static constexpr int PLANE = ROWS * W;
     static constexpr size_t BYTES = (size_t)NP * PLANE * 2;
 
-    static __device__ __forceinline__ void frag(const bf16_t *t, int row, int col, vec (&f)[NP]) {
-#pragma unroll
-        for (int p = 0; p < NP; ++p) f[p] = *reinterpret_cast<const vec *>(t + p * PLANE + row * LDW + col);
+    static __device__ __forceinline__ int swz(int row) {
+        return W == 128  ? ((row & 3) << 2) | ((row >> 2) & 3)
+               : W == 64 ? ((row & 2) << 1) | ((row >> 2) & 3)
+                         : (row >> 2) & 3;
     }
-    // transpose of rows r0 .. r0 + 15, columns c0 .. c0 + 31, inner order as described above
-    static __device__ __forceinline__ void frag_t(const bf16_t *t, int r0, int c0, int lane, vec (&f)[NP]) {
-        const int off = (r0 + 4 * (lane >> 5) + ((lane & 15) >> 2)) * LDW + c0 + 16 * ((lane >> 4) & 1) + 4 * (lane & 3);
+    static __device__ __forceinline__ int at(int row, int chunk) { return row * W + (chunk ^ swz(row)) * 8; }
+
+    // A lane's byte offsets: the plain fragment of rows 0 .. 31 at columns 0 .. 15, and the transposed one of rows 0 .. 15 at
+    // columns 0 .. 31.  Further columns flip bits of them (a chunk is 16 bytes and a row a power of two), further rows
+    // (multiples of 16) and planes are added.
+    static __device__ __forceinline__ uint32_t lane_plain(int lane) { return 2u * at(lane & 31, lane >> 5); }
+    static __device__ __forceinline__ uint32_t lane_turned(int lane) {
+        return 2u * (at(4 * (lane >> 5) + ((lane & 15) >> 2), 2 * ((lane >> 4) & 1) + ((lane & 3) >> 1)) + 4 * (lane & 1));
+    }
+    // columns 16 ks .. + 15 of rows r0 .. r0 + 31
+    static __device__ __forceinline__ void frag(const bf16_t *t, uint32_t plain, int r0, int ks, vec (&f)[NP]) {
+        const char *q = reinterpret_cast<const char *>(t) + (plain ^ (uint32_t)(32 * ks));
+#pragma unroll
+        for (int p = 0; p < NP; ++p) f[p] = *reinterpret_cast<const vec *>(q + 2 * (p * PLANE + r0 * W));
+    }
+    // transpose of rows r0 .. r0 + 15, columns 32 d .. + 31, inner order as described above
+    static __device__ __forceinline__ void frag_t(const bf16_t *t, uint32_t turned, int r0, int d, vec (&f)[NP]) {
+        const char *q = reinterpret_cast<const char *>(t) + (turned ^ (uint32_t)(64 * d));
+        const char *q8 = reinterpret_cast<const char *>(t) + (turned ^ (uint32_t)(64 * d + 32));
 #pragma unroll
         for (int p = 0; p < NP; ++p) {
             typedef __attribute__((address_space(3))) s16x4_t *lds_ptr;
@@ -208,14 +231,18 @@ template <typename M, int DP, int ROWS> struct Tile {
                 s16x4_t s[2];
                 vec h;
             } u;
-            u.s[0] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_ptr)(t + p * PLANE + off));
-            u.s[1] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_ptr)(t + p * PLANE + off + 8 * LDW));
+            u.s[0] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_ptr)(q + 2 * (p * PLANE + r0 * W)));
+            u.s[1] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_ptr)(q8 + 2 * (p * PLANE + (r0 + 8) * W)));
             f[p] = u.h;
         }
     }
 };
+// Keeps what is formed from x inside the loop: dozens of addresses would be held in registers instead of one flip each
+__device__ __forceinline__ void stay(uint32_t &x) { asm volatile("" : "+v"(x)); }
 
-// Staging of a tile by NT threads: rows of DP columns (zeros behind D) in chunks of eight elements.
+// Staging of a tile by NT threads: rows of DP columns (zeros behind D) in chunks of eight elements.  A chunk's place is a
+// 32-bit offset (MAX_LD bounds it) from the tile's first row, which is the same for all threads.
+constexpr int64_t MAX_LD = 1 << 22;
 template <typename M, int DP, int ROWS, int NT> struct Stage {
     typedef typename M::T T;
     typedef Tile<M, DP, ROWS> tile;
@@ -223,37 +250,57 @@ template <typename M, int DP, int ROWS, int NT> struct Stage {
     static constexpr int TOTAL = ROWS * CPR;
     static constexpr int N = (TOTAL + NT - 1) / NT;
     typename Src<M>::raw r[N];
+    uint32_t off[N];
 
-    // rows row0 .. of an operand of `n` rows (n >= 1): rows past the end are read as the last one
-    __device__ __forceinline__ void load(const Src<M> &src, int row0, int n, int D, int tid) {
+    static __device__ __forceinline__ int chunk(int i, int tid) {
+        const int c = tid + i * NT;
+        return TOTAL % NT != 0 && c >= TOTAL ? 0 : c;
+    }
+    static __device__ __forceinline__ int row_of(int i, int tid) { return chunk(i, tid) / CPR; }
+    __device__ __forceinline__ void init(const Src<M> &src, int D, int tid) {
 #pragma unroll
         for (int i = 0; i < N; ++i) {
-            const int c = tid + i * NT;
-            const int row = row0 + c / CPR, col = (c % CPR) * 8;
-            src.load(r[i], row < n ? row : n - 1, col < D ? col : 0);
+            const int c = chunk(i, tid), col = (c % CPR) * 8;
+            off[i] = (uint32_t)(c / CPR) * (uint32_t)src.ld + (uint32_t)(col < D ? col : 0);
         }
     }
-    // keep(i): false -> zeros, whatever was read.  (Rows past the end of READY sources stay what the last row is: their
-    // probabilities are zeros, and the last row reaches everything that they could.)
-    template <typename Keep> __device__ __forceinline__ void store(bf16_t *t, int D, int tid, Keep keep) {
+    // rows row0 .. of an operand of `n` rows (n >= 1): rows past the end are read as the last one
+    __device__ __forceinline__ void load(const Src<M> &src, int row0, int n, int D, int tid) {
+        if (row0 + ROWS <= n) {
+            const Src<M> s = src.from(row0);
+#pragma unroll
+            for (int i = 0; i < N; ++i) s.load(r[i], off[i]);
+        } else {
+#pragma unroll
+            for (int i = 0; i < N; ++i) {
+                const int c = chunk(i, tid), row = row0 + c / CPR, col = (c % CPR) * 8;
+                src.from(row < n ? row : n - 1).load(r[i], col < D ? col : 0);
+            }
+        }
+    }
+    // some: rows may have to become zeros, those with keep(i) false
+    template <typename Keep> __device__ __forceinline__ void store(bf16_t *t, int D, int tid, bool some, Keep keep) {
+        if (some) {
+#pragma unroll
+            for (int i = 0; i < N; ++i)
+                if (!keep(i)) r[i].zero();
+        }
+        if (D < DP) {
+#pragma unroll
+            for (int i = 0; i < N; ++i)
+                if ((chunk(i, tid) % CPR) * 8 >= D) r[i].zero();
+        }
 #pragma unroll
         for (int i = 0; i < N; ++i) {
+            if (TOTAL % NT != 0 && tid + i * NT >= TOTAL) break;
             const int c = tid + i * NT;
-            const int row = c / CPR, col = (c % CPR) * 8;
-            if (TOTAL % NT != 0 && c >= TOTAL) break;
-            if (Src<M>::READY) {
-                if (D < DP && col >= D) r[i].zero();
-            } else if (!(keep(i) && col < D)) {
-                r[i].zero();
-            }
             typename M::vec p[tile::NP];
             r[i].planes(p);
 #pragma unroll
             for (int k = 0; k < tile::NP; ++k)
-                *reinterpret_cast<typename M::vec *>(t + k * tile::PLANE + row * tile::LDW + col) = p[k];
+                *reinterpret_cast<typename M::vec *>(t + k * tile::PLANE + tile::at(c / CPR, c % CPR)) = p[k];
         }
     }
-    __device__ __forceinline__ static int row_of(int i, int tid) { return (tid + i * NT) / CPR; }
 };
 
 // Capped scores of a tile: x[i] = cap tanh(x[i] f).  tanh by its odd series below TANH_SMALL -- to a few units of

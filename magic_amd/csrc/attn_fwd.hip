@@ -17,6 +17,7 @@ int check(const magic_attn *a) {
     if (a->n_q_tiles < 0 || a->n_k_tiles < 0 || a->max_q < 0 || a->max_k < 0 || a->n_seg < 0) return MAGIC_ERR_INVALID_ARG;
     if (a->n_q > 0 && (!a->q || a->n_q_tiles < 1 || !a->q_tiles)) return MAGIC_ERR_INVALID_ARG;
     if (a->n_k > 0 && (!a->k || !a->v)) return MAGIC_ERR_INVALID_ARG;
+    if (a->ld_q > MAX_LD || a->ld_k > MAX_LD || a->ld_v > MAX_LD || (int64_t)a->q_heads * a->head_dim > MAX_LD) return MAGIC_ERR_UNSUPPORTED;
     if (a->ld_q < 0 || a->hs_q < 0 || a->ld_k < 0 || a->hs_k < 0 || a->ld_v < 0 || a->hs_v < 0) return MAGIC_ERR_INVALID_ARG;
     const int per = a->dtype == MAGIC_F32 ? 4 : 8;   // rows and heads start on 16-byte addresses
     if (((uintptr_t)a->q | (uintptr_t)a->k | (uintptr_t)a->v) & 15) return MAGIC_ERR_INVALID_ARG;
@@ -302,7 +303,9 @@ __global__ __launch_bounds__(64 * WM *KG, DP == 128 && (M::N == 3 || WM == 1) ? 
     // difference, not of the two large terms.
     float m = -INFINITY, l = 0.f;
 
+    uint32_t plain = tile::lane_plain(lane) + 2u * kg * KW * tile::W, turned = tile::lane_turned(lane) + 2u * kg * KW * tile::W;
     stage kst, vst;
+    kst.init(K, D, tid), vst.init(V, D, tid);
     uint8_t keep[stage::N];
     int pos = 0;             // (taken as loaded: a use here would wait for the whole tile)
     uint8_t mk = 0;
@@ -312,10 +315,9 @@ __global__ __launch_bounds__(64 * WM *KG, DP == 128 && (M::N == 3 || WM == 1) ? 
         vst.load(V, j0, nk, D, tid);
 #pragma unroll
         for (int i = 0; i < stage::N; ++i) {
-            if (Src<M>::READY) break;
             const int j = j0 + stage::row_of(i, tid);
             keep[i] = j < nk;
-            if (a.key_mask && j < nk) keep[i] = a.key_mask[k0 + j];
+            if (!Src<M>::READY && a.key_mask && j < nk) keep[i] = a.key_mask[k0 + j];
         }
         if (tid < BK) {
             const int j = j0 + tid;
@@ -327,13 +329,14 @@ __global__ __launch_bounds__(64 * WM *KG, DP == 128 && (M::N == 3 || WM == 1) ? 
     if (t_beg < t_end) load(t_beg);
     for (int tt = t_beg; tt < t_end; ++tt) {
         __syncthreads();  // the reads of the tile before are done
-        kst.store(sK, D, tid, [&](int i) { return keep[i] != 0; });
-        vst.store(sV, D, tid, [&](int i) { return keep[i] != 0; });
-        if (tid < BK) sPos[tid] = flip(pos), sMask[tid] = mk ? 0.f : -INFINITY;
         const bool masked = a.key_mask != nullptr || (tt + 1) * BK > nk;
+        kst.store(sK, D, tid, masked, [&](int i) { return keep[i] != 0; });
+        vst.store(sV, D, tid, masked, [&](int i) { return keep[i] != 0; });
+        if (tid < BK) sPos[tid] = flip(pos), sMask[tid] = mk ? 0.f : -INFINITY;
         __syncthreads();
         if (tt + 1 < t_end) load(tt + 1);
 
+        stay(plain), stay(turned);
         f32x16_t s[KB];
 #pragma unroll
         for (int b = 0; b < KB; ++b)
@@ -344,7 +347,7 @@ __global__ __launch_bounds__(64 * WM *KG, DP == 128 && (M::N == 3 || WM == 1) ? 
 #pragma unroll
             for (int b = 0; b < KB; ++b) {
                 vec f[NP];
-                tile::frag(sK, kg * KW + 32 * b + li, 16 * ks + 8 * hf, f);
+                tile::frag(sK, plain, 32 * b, ks, f);
                 mma(s[b], f, qf[ks]);
             }
         feed<NP * KB, PRODUCTS<M> * KB, KS>();
@@ -418,7 +421,7 @@ __global__ __launch_bounds__(64 * WM *KG, DP == 128 && (M::N == 3 || WM == 1) ? 
 #pragma unroll
             for (int w = 0; w < KB * 2; ++w) {
                 vec f[NP];
-                tile::frag_t(sV, kg * KW + 16 * w, 32 * d, lane, f);
+                tile::frag_t(sV, turned, 16 * w, d, f);
                 mma(c, f, pf[w]);
             }
             feed<2 * NP, PRODUCTS<M>, KB * 2>();
