@@ -581,10 +581,12 @@ int magic_knn_merge(int64_t n_query, int32_t k, int32_t n_parts,
  * MAGIC_BF16 (products of bf16 values, probabilities and score gradients rounded to bf16 before
  * their products; every sum and statistic in fp32).  key_mask [n_k]: 0 = the key takes no part
  * (whatever its rows hold).  A row that sees no key gets o = 0, lse = -inf and zero gradients.
- * The work comes as two device tables of the segments' tiles, eight int32 each (the last three are not read):
- *   q_tiles: {first q row, rows (1..MAGIC_ATTN_TILE), first key row of the segment, its keys, segment}
- *   k_tiles: {first key row, keys (1..MAGIC_ATTN_TILE), first q row of the segment, its rows, segment}
- * that cover every row of q (k) exactly once.
+ * The work comes as two device tables of the segments' tiles, eight int32 each (the last is not read):
+ *   q_tiles: {first q row, rows (1..MAGIC_ATTN_TILE), first key row of the segment, its keys, segment,
+ *             first q row of the segment, its rows}
+ *   k_tiles: {first key row, keys (1..MAGIC_ATTN_TILE), first q row of the segment, its rows, segment,
+ *             first key row of the segment, its keys}
+ * that cover every row of q (k) exactly once; the tiles of a segment lie at multiples of MAGIC_ATTN_TILE from its start.
  * lse [q_heads, n_q] = log2 sum exp(l) (base 2) is what _bwd needs beside out.  dq [n_q,q_heads,D],
  * dk, dv [n_k,kv_heads,D] contiguous in the operands' type; d_slopes [q_heads] or NULL.  dq may be NULL when it (and
  * d_slopes) is not wanted, dk and dv together likewise.

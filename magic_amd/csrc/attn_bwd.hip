@@ -202,7 +202,7 @@ __global__ __launch_bounds__(NT, (DP == 128 && M::N > 1) ? 1 : 2) void k_attn_dq
     const int h = (int)(item / a.n_q_tiles), hk = h / (a.q_heads / a.kv_heads);
     const int32_t *t = a.q_tiles + TAB * tl;
     const int64_t q0 = t[0], k0 = t[2];
-    const int nq = t[1], nk = t[3];
+    const int nq = t[1], nk = t[3] > 0 && p.pr.cnt ? p.pr.cnt[t[4]] : t[3];
     const int row = wave * 32 + li;
     const bool ok = row < nq;
     const int64_t qr = q0 + (ok ? row : 0);
@@ -366,11 +366,12 @@ __global__ __launch_bounds__(NT, DP == 128 ? 1 : 2) void k_attn_dkv(BwdArgs p) {
     const int split = (int)(item / ((int64_t)a.n_k_tiles * a.kv_heads));
     const int32_t *t = a.k_tiles + TAB * tl;
     const int64_t k0 = t[0], q0 = t[2];
-    const int nk = t[1], nq = t[3];
+    const int nk = p.pr.cnt ? min(t[1], p.pr.cnt[t[4]] - (t[0] - t[5])) : t[1], nq = t[3];
+    if (nk <= 0) return;                     // (all unmasked keys of the segment are in the tiles before)
     const int col = wave * 32 + li;
     const bool in = col < nk;
-    const int64_t kr = k0 + (in ? col : 0);
-    const bool ok = in && (!a.key_mask || a.key_mask[kr]);
+    const int64_t kr = p.pr.idx ? p.pr.idx[k0 + (in ? col : 0)] : k0 + (in ? col : 0);
+    const bool ok = in && (p.pr.idx || !a.key_mask || a.key_mask[kr]);
 
     Scales sc;
     if (!sc.init<M>(p.pr.rg, hk * G, G, hk, t[4], a)) return;  // the other launch's segment
@@ -519,10 +520,26 @@ template <typename T> __global__ __launch_bounds__(256) void k_attn_dkv_join(Bwd
     const int64_t plane = p.a.n_k * p.a.kv_heads * p.a.head_dim, n4 = 2 * plane / 4;
     for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n4; i += (int64_t)gridDim.x * 256) {
         f32x4_t x = {0.f, 0.f, 0.f, 0.f};
+        // (masked keys: nothing was written for them)
+        const int64_t row = (4 * i < plane ? 4 * i : 4 * i - plane) / ((int64_t)p.a.kv_heads * p.a.head_dim);
+        if (!p.a.key_mask || p.a.key_mask[row])
         for (int s = 0; s < p.n_split; ++s) x += *reinterpret_cast<const f32x4_t *>(p.part + s * 2 * plane + 4 * i);
         const float y[4] = {x[0], x[1], x[2], x[3]};
         const int64_t e = 4 * i;
         magic::store_vec<T, 4>(e < plane ? (T *)p.dk + e : (T *)p.dv + (e - plane), true, y);
+    }
+}
+
+// zeros for the masked keys, which no tile of gathered keys holds
+template <typename T> __global__ __launch_bounds__(256) void k_attn_dkv_masked(BwdArgs p) {
+    const int cpr = p.a.kv_heads * p.a.head_dim / 8;
+    const int64_t total = p.a.n_k * cpr;
+    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < total; i += (int64_t)gridDim.x * 256) {
+        if (p.a.key_mask[i / cpr]) continue;
+        Raw<T> z;
+        z.zero();
+        z.store((T *)p.dk + 8 * i);
+        z.store((T *)p.dv + 8 * i);
     }
 }
 
@@ -540,8 +557,9 @@ template <typename M, int DP> constexpr int BK_OF = 32;
 template <typename M, int DP> constexpr int BQ_OF = DP == 128 && M::N == 1 ? 64 : 32;
 
 template <typename M, int DP> int sweeps(BwdArgs &b, hipStream_t st) {
-    const magic_attn &a = b.a;
+    const magic_attn full = b.a, a = full;
     constexpr int BK = BK_OF<M, DP>, BQ = BQ_OF<M, DP>;
+    b.a = gathered(&full, b.pr);
     if (a.n_q > 0 && b.dq) {
         const size_t lds = 2 * Tile<M, DP, BK>::BYTES + BK * 8;
         if (magic::ensure_dynamic_lds((const void *)k_attn_dq<M, DP, BK>, lds) != MAGIC_OK) return MAGIC_ERR_RUNTIME;
@@ -551,6 +569,7 @@ template <typename M, int DP> int sweeps(BwdArgs &b, hipStream_t st) {
                      lds, st, b);
     }
     if (a.n_k > 0 && b.dk) {
+        b.a = full;                // (a key's own rows are read where they are)
         const size_t lds = 2 * Tile<M, DP, BQ>::BYTES + BQ * 12;
         if (magic::ensure_dynamic_lds((const void *)k_attn_dkv<M, DP, BQ>, lds) != MAGIC_OK) return MAGIC_ERR_RUNTIME;
         b.items = (int64_t)a.n_k_tiles * a.kv_heads * b.n_split;
@@ -558,6 +577,7 @@ template <typename M, int DP> int sweeps(BwdArgs &b, hipStream_t st) {
         MAGIC_LAUNCH(M::SCALED ? "attn_bwd_dkv_f16x2" : "attn_bwd_dkv", (k_attn_dkv<M, DP, BQ>), (int)xcd_grid(b.items, 16), NT,
                      lds, st, b);
     }
+    b.a = full;
     return magic::launch_status();
 }
 
@@ -595,7 +615,7 @@ size_t magic_attn_bwd_workspace_bytes(const magic_attn *a) {
     if (check(a) != MAGIC_OK) return 256;
     const int n = splits(a);
     const size_t part = n > 1 ? (size_t)n * 2 * a->n_k * a->kv_heads * a->head_dim * sizeof(float) : 0;
-    return magic::align_up(part) + (use_f16(a) ? prepare_bytes(a, true) : 0) + 2 * magic::align_up((size_t)a->n_q * a->q_heads * sizeof(float)) +
+    return magic::align_up(part) + prepare_bytes(a, use_f16(a), true) + 2 * magic::align_up((size_t)a->n_q * a->q_heads * sizeof(float)) +
            magic::align_up((size_t)a->n_q_tiles * a->q_heads * sizeof(double)) + 256;
 }
 
@@ -629,16 +649,25 @@ int magic_attn_bwd(const magic_attn *a, const void *out, int64_t ld_out, int64_t
     int rc = MAGIC_OK;
     if (a->n_q > 0) rc = f32 ? delta_of<float>(b, stream) : delta_of<bf16_t>(b, stream);
     if (rc != MAGIC_OK) return rc;
-    if (f16) {
+    if (a->n_q > 0 && a->n_k > 0) {
         const GradRows g = {d_out, ld_do, hs_do, b.lse2};
-        rc = prepare(a, &g, ar, b.pr, stream);
+        rc = prepare(a, f16, &g, ar, b.pr, stream);
         if (rc != MAGIC_OK) return rc;
+    }
+    if (f16) {
         rc = sweeps_of<F16x2>(b, stream);
         if (rc != MAGIC_OK) return rc;
-        b.pr.rg.want_safe = false;                // the segments whose rows differ too much in size
+        b.pr.rg.want_safe = false;             // the segments whose rows differ too much in size
     }
     rc = f32 ? sweeps_of<F32x3>(b, stream) : sweeps_of<BF16>(b, stream);
     if (rc != MAGIC_OK) return rc;
+    if (b.n_split == 1 && dk && b.pr.idx) {
+        const int grid = magic::stride_grid(a->n_k * a->kv_heads * a->head_dim / 8, 256);
+        if (f32)
+            MAGIC_LAUNCH("attn_dkv_masked", k_attn_dkv_masked<float>, grid, 256, 0, stream, b);
+        else
+            MAGIC_LAUNCH("attn_dkv_masked", k_attn_dkv_masked<bf16_t>, grid, 256, 0, stream, b);
+    }
     if (b.n_split > 1 && a->n_k > 0) {
         const int grid = magic::stride_grid(a->n_k * a->kv_heads * a->head_dim / 2, 256);
         if (f32)

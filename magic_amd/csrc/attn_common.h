@@ -86,6 +86,10 @@ template <> struct Raw<float> {
         a = *reinterpret_cast<const f32x4_t *>(p);
         b = *reinterpret_cast<const f32x4_t *>(p + 4);
     }
+    __device__ __forceinline__ void store(float *p) const {
+        *reinterpret_cast<f32x4_t *>(p) = a;
+        *reinterpret_cast<f32x4_t *>(p + 4) = b;
+    }
     __device__ __forceinline__ void zero() { a = b = f32x4_t{0.f, 0.f, 0.f, 0.f}; }
     __device__ __forceinline__ void planes(bf16x8_t (&p)[3], float) const {
         split8(make_float4(a[0], a[1], a[2], a[3]), make_float4(b[0], b[1], b[2], b[3]), p[0], p[1], p[2]);
@@ -103,6 +107,7 @@ template <> struct Raw<float> {
 template <> struct Raw<bf16_t> {
     bf16x8_t v;
     __device__ __forceinline__ void load(const bf16_t *p) { v = *reinterpret_cast<const bf16x8_t *>(p); }
+    __device__ __forceinline__ void store(bf16_t *p) const { *reinterpret_cast<bf16x8_t *>(p) = v; }
     __device__ __forceinline__ void zero() {
 #pragma unroll
         for (int e = 0; e < 8; ++e) v[e] = (bf16_t)0.f;
@@ -381,11 +386,23 @@ __device__ __forceinline__ float range_scale(Range r) {
     return __uint_as_float((uint32_t)(e + 127) << 23);
 }
 
-// What F16x2 launches need beside the arguments: the ranges and the planes of the operands they stage
+// What the launches of a call need beside its arguments: for F16x2 the ranges and the planes of the operands they stage; with
+// a key mask the unmasked keys of every segment -- idx[first key row of the segment + i] is the row of the i-th, cnt[segment]
+// their number.  Masked keys then cost nothing: the staged side walks rows that were gathered (planes, or kc / vc / posc).
 struct Prepared {
     Ranges rg = {nullptr, nullptr, nullptr, nullptr, 0, false};
     PlaneSet q = {}, k = {}, v = {}, g = {};
+    const int32_t *idx = nullptr, *cnt = nullptr, *posc = nullptr;
+    const void *kc = nullptr, *vc = nullptr;
 };
+// the call with the gathered rows in the place of its keys
+inline magic_attn gathered(const magic_attn *a, const Prepared &p) {
+    magic_attn g = *a;
+    if (!p.idx) return g;
+    g.k = p.kc, g.v = p.vc, g.k_pos = p.posc, g.key_mask = nullptr;
+    g.ld_k = g.ld_v = (int64_t)a->kv_heads * a->head_dim, g.hs_k = g.hs_v = a->head_dim;
+    return g;
+}
 // The output's gradient and what marks rows that see no key (lse = +inf there), in backward
 struct GradRows {
     const void *g;
@@ -393,9 +410,10 @@ struct GradRows {
     const float *lse;
 };
 bool use_f16(const magic_attn *a);                                 // whether F16x2 is tried for a call
-size_t prepare_bytes(const magic_attn *a, bool backward);          // its workspace
-// ranges and planes: k, v, and in backward q and the output's gradient
-int prepare(const magic_attn *a, const GradRows *g, Arena &ar, Prepared &out, hipStream_t stream);
+bool use_gather(const magic_attn *a);                              // whether unmasked keys are gathered
+size_t prepare_bytes(const magic_attn *a, bool f16, bool backward);   // workspace of prepare
+// ranges and planes (k, v, and in backward q and the output's gradient) where f16; unmasked keys
+int prepare(const magic_attn *a, bool f16, const GradRows *g, Arena &ar, Prepared &out, hipStream_t stream);
 constexpr int TAB = 8;            // int32 words of a tile-table entry
 
 }  // namespace attn

@@ -108,10 +108,77 @@ __global__ __launch_bounds__(256) void k_range(RangeArgs r) {
 
 namespace {
 
+// Unmasked keys of a segment in ascending order; block: a 128-key tile, which first counts the unmasked keys before it
+__global__ __launch_bounds__(256) void k_compact(magic_attn a, int32_t *idx, int32_t *cnt) {
+    __shared__ int part[4], w[2];
+    const int32_t *t = a.k_tiles + TAB * (int64_t)blockIdx.x;
+    const int64_t first = t[5], row0 = t[0];
+    const int tid = threadIdx.x, lane = tid & 63, before = (int)(row0 - first);
+    const uint8_t *m = a.key_mask + first;
+    int n = 0;
+    // whole words from the first aligned one on, single bytes around them
+    const int head = min(before, (int)((16 - ((uintptr_t)m & 15)) & 15)), words = (before - head) / 16;
+    if (tid < head) n += m[tid] != 0;
+    for (int i = tid; i < words; i += 256) {
+        const uint4 v = *reinterpret_cast<const uint4 *>(m + head + 16 * i);
+        const uint32_t x[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+        for (int e = 0; e < 4; ++e) n += __popc((((x[e] & 0x7f7f7f7fu) + 0x7f7f7f7fu) | x[e]) & 0x80808080u);
+    }
+    const int tail = head + 16 * words + tid;
+    if (tail < before) n += m[tail] != 0;
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) n += __shfl_xor(n, o, 64);
+    if (lane == 0) part[tid >> 6] = n;
+    const bool in = tid < t[1] && a.key_mask[row0 + (tid < t[1] ? tid : 0)] != 0;     // (t[1] <= 128: two wavefronts)
+    const unsigned long long b = __ballot(in);
+    if (lane == 0 && tid < 128) w[tid >> 6] = __popcll(b);
+    __syncthreads();
+    const int base = part[0] + part[1] + part[2] + part[3];
+    if (in) idx[first + base + (tid >= 64 ? w[0] : 0) + __popcll(b & ((1ull << lane) - 1ull))] = (int32_t)(row0 + tid);
+    if (tid == 0 && row0 + t[1] == first + t[6]) cnt[t[4]] = base + w[0] + w[1];
+}
+
+struct GatherArgs {
+    magic_attn a;
+    const int32_t *idx, *cnt;
+    Ranges rg;              // only what the F16x2 launch leaves over, if ranges are given
+    void *kc, *vc;
+    int32_t *posc;
+};
+// rows of the unmasked keys side by side; block: 128 of them, one key head (y) of k or v
+template <typename T> __global__ __launch_bounds__(256) void k_gather(GatherArgs g) {
+    const magic_attn &a = g.a;
+    const int32_t *t = a.k_tiles + TAB * (int64_t)blockIdx.x;
+    const int local = t[0] - t[5], n = min(t[1], g.cnt[t[4]] - local);
+    if (n <= 0) return;
+    const int h = blockIdx.y >> 1, G = a.q_heads / a.kv_heads;
+    const bool v = blockIdx.y & 1;
+    if (blockIdx.y == 0 && a.slopes && threadIdx.x < n) g.posc[t[0] + threadIdx.x] = a.k_pos[g.idx[t[0] + threadIdx.x]];
+    if (g.rg.k) {
+        bool safe = range_ok(g.rg.k[h * g.rg.n_seg + t[4]]) && range_ok(g.rg.v[h * g.rg.n_seg + t[4]]);
+        for (int i = h * G; i < h * G + G; ++i)
+            safe = safe && range_ok(g.rg.q[i * g.rg.n_seg + t[4]]) && (!g.rg.g || range_ok(g.rg.g[i * g.rg.n_seg + t[4]]));
+        if (safe) return;
+    }
+    const T *base = (const T *)(v ? a.v : a.k) + h * (v ? a.hs_v : a.hs_k);
+    const int64_t ld = v ? a.ld_v : a.ld_k;
+    T *out = (T *)(v ? g.vc : g.kc);
+    const int cpr = a.head_dim / 8;
+    for (int i = threadIdx.x; i < n * cpr; i += 256) {
+        const int64_t at = (int64_t)t[0] + i / cpr;
+        const int c = (i % cpr) * 8;
+        Raw<T> x;
+        x.load(base + g.idx[at] * ld + c);
+        x.store(out + (at * a.kv_heads + h) * a.head_dim + c);
+    }
+}
+
 struct SplitArgs {
     magic_attn a;
     GradRows g;
     Ranges rg;
+    const int32_t *idx, *cnt;      // unmasked keys, or NULL
     _Float16 *q, *k, *v, *gr;      // hi planes; the lo ones follow
 };
 
@@ -145,13 +212,13 @@ __global__ __launch_bounds__(256) void k_split(SplitArgs s) {
         r.max = max(r.max, x.max);
     }
     const float scale = range_scale(r);
-    const int cpr = D / 8, n = t[1] * cpr;
+    const int cpr = D / 8, n = (key && s.cnt ? min(t[1], s.cnt[t[4]] - (t[0] - t[5])) : t[1]) * cpr;
     for (int i = threadIdx.x; i < n; i += 256) {
         const int64_t row = (int64_t)t[0] + i / cpr;
         const int c = (i % cpr) * 8;
         Raw<float> x;
-        x.load(base + row * ld + y * hs + c);
-        const bool use = key ? !a.key_mask || a.key_mask[row] : !s.g.lse || s.g.lse[(int64_t)y * a.n_q + row] != INFINITY;
+        x.load(base + (key && s.idx ? s.idx[row] : row) * ld + y * hs + c);
+        const bool use = key || !s.g.lse || s.g.lse[(int64_t)y * a.n_q + row] != INFINITY;
         if (!use) x.zero();
         f16x8_t p[2];
         x.planes(p, scale);
@@ -173,34 +240,66 @@ int64_t range_count(const magic_attn *a, bool grad) {
 // F16x2 needs two passes over the operands first: for float32 calls of enough work to pay for them
 bool use_f16(const magic_attn *a) { return a->dtype == MAGIC_F32 && a->head_dim > 32 && a->max_k >= 512 && a->n_seg > 0; }
 
-size_t prepare_bytes(const magic_attn *a, bool backward) {
-    const size_t k = align_up(plane_elems(a, true) * 2), q = align_up(plane_elems(a, false) * 2);
-    return align_up(range_count(a, backward) * sizeof(Range)) + 2 * k + (backward ? 2 * q : 0);
+// Gathering costs two launches and a copy of the unmasked rows, and saves the masked share of everything else
+bool use_gather(const magic_attn *a) { return a->key_mask && a->max_k >= 512 && a->n_seg > 0 && a->n_k > 0 && a->n_k_tiles > 0; }
+
+size_t prepare_bytes(const magic_attn *a, bool f16, bool backward) {
+    size_t n = 0;
+    if (f16) {
+        const size_t k = align_up(plane_elems(a, true) * 2), q = align_up(plane_elems(a, false) * 2);
+        n += align_up(range_count(a, backward) * sizeof(Range)) + 2 * k + (backward ? 2 * q : 0);
+    }
+    if (use_gather(a))
+        n += 2 * align_up((size_t)a->n_k * 4) + align_up((size_t)a->n_seg * 4) +
+             2 * align_up((size_t)a->n_k * a->kv_heads * a->head_dim * (a->dtype == MAGIC_F32 ? 4 : 2));
+    return n;
 }
 
-int prepare(const magic_attn *a, const GradRows *g, Arena &ar, Prepared &out, hipStream_t stream) {
-    const int64_t n = range_count(a, g != nullptr);
-    Range *r = ar.take<Range>(n);
-    SplitArgs s;
-    s.a = *a;
-    s.g = g ? *g : GradRows{nullptr, 0, 0, nullptr};
-    s.k = ar.take<_Float16>(plane_elems(a, true)), s.v = ar.take<_Float16>(plane_elems(a, true));
-    s.q = s.gr = nullptr;
-    if (g) s.q = ar.take<_Float16>(plane_elems(a, false)), s.gr = ar.take<_Float16>(plane_elems(a, false));
-    if (!ar.ok()) return MAGIC_ERR_WORKSPACE;
-    RangeArgs ra;
-    ra.a = *a, ra.g = s.g.g, ra.ld_g = s.g.ld, ra.hs_g = s.g.hs, ra.n_seg = a->n_seg;
-    ra.q = r, ra.k = r + (int64_t)a->q_heads * a->n_seg, ra.v = ra.k + (int64_t)a->kv_heads * a->n_seg,
-    ra.gr = ra.v + (int64_t)a->kv_heads * a->n_seg;
-    out.rg = s.rg = Ranges{ra.q, ra.k, ra.v, g ? ra.gr : nullptr, a->n_seg, true};
-    out.k = {s.k, a->n_k, a->kv_heads}, out.v = {s.v, a->n_k, a->kv_heads};
-    out.q = {s.q, a->n_q, a->q_heads}, out.g = {s.gr, a->n_q, a->q_heads};
-    MAGIC_LAUNCH("attn_range_init", k_range_init, magic::stride_grid(n, 256), 256, 0, stream, r, n);
+int prepare(const magic_attn *a, bool f16, const GradRows *g, Arena &ar, Prepared &out, hipStream_t stream) {
+    int32_t *idx = nullptr, *cnt = nullptr, *posc = nullptr;
+    unsigned char *kc = nullptr, *vc = nullptr;
     const int x = a->n_q_tiles > a->n_k_tiles ? a->n_q_tiles : a->n_k_tiles;
-    const int y = a->q_heads * (g ? 2 : 1) + 2 * a->kv_heads, ys = 2 * a->kv_heads + (g ? 2 * a->q_heads : 0);
-    if (y > 65535) return MAGIC_ERR_UNSUPPORTED;
-    MAGIC_LAUNCH("attn_range", k_range, dim3(x, y), 256, 0, stream, ra);
-    MAGIC_LAUNCH("attn_split", k_split, dim3(x, ys), 256, 0, stream, s);
+    if (use_gather(a)) {
+        const size_t rows = (size_t)a->n_k * a->kv_heads * a->head_dim * (a->dtype == MAGIC_F32 ? 4 : 2);
+        idx = ar.take<int32_t>(a->n_k), posc = ar.take<int32_t>(a->n_k), cnt = ar.take<int32_t>(a->n_seg);
+        kc = ar.take<unsigned char>(rows), vc = ar.take<unsigned char>(rows);
+        if (!ar.ok()) return MAGIC_ERR_WORKSPACE;
+        out.idx = idx, out.cnt = cnt, out.posc = posc, out.kc = kc, out.vc = vc;
+        MAGIC_LAUNCH("attn_compact", k_compact, a->n_k_tiles, 256, 0, stream, *a, idx, cnt);
+    }
+    if (f16) {
+        const int64_t n = range_count(a, g != nullptr);
+        Range *r = ar.take<Range>(n);
+        SplitArgs s;
+        s.a = *a;
+        s.g = g ? *g : GradRows{nullptr, 0, 0, nullptr};
+        s.idx = idx, s.cnt = cnt;
+        s.k = ar.take<_Float16>(plane_elems(a, true)), s.v = ar.take<_Float16>(plane_elems(a, true));
+        s.q = s.gr = nullptr;
+        if (g) s.q = ar.take<_Float16>(plane_elems(a, false)), s.gr = ar.take<_Float16>(plane_elems(a, false));
+        if (!ar.ok()) return MAGIC_ERR_WORKSPACE;
+        RangeArgs ra;
+        ra.a = *a, ra.g = s.g.g, ra.ld_g = s.g.ld, ra.hs_g = s.g.hs, ra.n_seg = a->n_seg;
+        ra.q = r, ra.k = r + (int64_t)a->q_heads * a->n_seg, ra.v = ra.k + (int64_t)a->kv_heads * a->n_seg,
+        ra.gr = ra.v + (int64_t)a->kv_heads * a->n_seg;
+        out.rg = s.rg = Ranges{ra.q, ra.k, ra.v, g ? ra.gr : nullptr, a->n_seg, true};
+        out.k = {s.k, a->n_k, a->kv_heads}, out.v = {s.v, a->n_k, a->kv_heads};
+        out.q = {s.q, a->n_q, a->q_heads}, out.g = {s.gr, a->n_q, a->q_heads};
+        MAGIC_LAUNCH("attn_range_init", k_range_init, magic::stride_grid(n, 256), 256, 0, stream, r, n);
+        const int y = a->q_heads * (g ? 2 : 1) + 2 * a->kv_heads, ys = 2 * a->kv_heads + (g ? 2 * a->q_heads : 0);
+        if (y > 65535) return MAGIC_ERR_UNSUPPORTED;
+        MAGIC_LAUNCH("attn_range", k_range, dim3(x, y), 256, 0, stream, ra);
+        MAGIC_LAUNCH("attn_split", k_split, dim3(x, ys), 256, 0, stream, s);
+    }
+    if (idx) {
+        const GatherArgs ga = {*a, idx, cnt, out.rg, kc, vc, posc};
+        const dim3 grid(a->n_k_tiles, 2 * a->kv_heads);
+        if (2 * a->kv_heads > 65535) return MAGIC_ERR_UNSUPPORTED;
+        if (a->dtype == MAGIC_F32)
+            MAGIC_LAUNCH("attn_gather", k_gather<float>, grid, 256, 0, stream, ga);
+        else
+            MAGIC_LAUNCH("attn_gather", k_gather<bf16_t>, grid, 256, 0, stream, ga);
+    }
     return magic::launch_status();
 }
 
@@ -232,7 +331,7 @@ __device__ __forceinline__ int h_of(const FwdArgs &p, int hb) { return hb * p.gc
 
 // WM groups of 32 columns (rows, or rows x heads of one key head), KG groups of KW keys: a block of WM * KG wavefronts
 template <typename M, int DP, int WM, int KG, int KW>
-__global__ __launch_bounds__(64 * WM *KG, DP == 128 && (M::N == 3 || WM == 1) ? 1 : 2) void k_attn_fwd(FwdArgs p) {
+__global__ __launch_bounds__(64 * WM *KG, DP == 128 && (M::N > 1 || WM == 1) ? 1 : 2) void k_attn_fwd(FwdArgs p) {
     typedef typename M::T T;
     typedef typename M::vec vec;
     constexpr int NP = M::N, KS = DP / 16, DB = (DP + 31) / 32, BK = KG * KW, NT = 64 * WM * KG, KB = KW / 32;
@@ -255,7 +354,7 @@ __global__ __launch_bounds__(64 * WM *KG, DP == 128 && (M::N == 3 || WM == 1) ? 
     const int nq = t[1] - (int)(ts % p.sub) * p.rows;     // rows left for this block and the ones behind it
     if (nq <= 0) return;
     const int64_t q0 = (int64_t)t[0] + (ts % p.sub) * p.rows, k0 = t[2];
-    const int nk = t[3];
+    const int nk = t[3] > 0 && p.pr.cnt ? p.pr.cnt[t[4]] : t[3];
     // this block's range of keys, in whole tiles
     const int tiles = (nk + BK - 1) / BK, per = (tiles + p.n_split - 1) / p.n_split;
     const int t_beg = split * per, t_end = min(t_beg + per, tiles);
@@ -562,10 +661,11 @@ Shape shape_of(const magic_attn *a) {
     const int64_t most = (a->max_k + 511) / 512;
     if (split > most) split = most;
     if (split > 256) split = 256;
+    if (s.wm == 4) split = 1;
     if (split < 1) split = 1;
     s.n_split = (int)split;
     s.items = blocks * split;
-    s.f16 = magic::attn::use_f16(a) && s.wm == 4 && s.n_split == 1;
+    s.f16 = magic::attn::use_f16(a) && s.wm == 4 && s.n_split == 1 && a->n_k > 0;
     return s;
 }
 
@@ -586,7 +686,7 @@ template <typename M> int run_rows(FwdArgs &p, hipStream_t st) {
     return D <= 16   ? launch<M, 16, 4, 1, 64>(p, st)
            : D <= 32 ? launch<M, 32, 4, 1, 64>(p, st)
            : D <= 64 ? launch<M, 64, 4, 1, 64>(p, st)
-                     : launch<M, 128, 4, 1, M::SCALED ? 32 : 64>(p, st);   // (64 keys would spill registers)
+                     : launch<M, 128, 4, 1, 64>(p, st);
 }
 
 template <typename M> int run(FwdArgs &p, int wm, hipStream_t st) {
@@ -624,8 +724,7 @@ extern "C" {
 size_t magic_attn_fwd_workspace_bytes(const magic_attn *a) {
     if (check(a) != MAGIC_OK || a->n_q == 0) return 256;
     const Shape s = shape_of(a);
-    if (s.f16) return magic::attn::prepare_bytes(a, false) + 256;
-    if (s.n_split == 1) return 256;
+    if (s.n_split == 1) return (s.wm == 4 ? magic::attn::prepare_bytes(a, s.f16, false) : 0) + 256;
     const size_t rows = (size_t)s.n_split * a->q_heads * a->n_q;
     return magic::align_up(rows * a->head_dim * sizeof(float)) + magic::align_up(rows * sizeof(float)) + 256;
 }
@@ -649,14 +748,17 @@ int magic_attn_fwd(const magic_attn *a, void *out, int64_t ld_out, int64_t hs_ou
         p.part_l = ar.take<float>(rows);
         if (!ar.ok()) return MAGIC_ERR_WORKSPACE;
     }
-    if (s.f16) {
+    if (s.wm == 4 && s.n_split == 1) {
         magic::Arena ar(workspace, workspace_bytes);
-        const int rc = magic::attn::prepare(a, nullptr, ar, p.pr, (hipStream_t)stream);
+        int rc = magic::attn::prepare(a, s.f16, nullptr, ar, p.pr, (hipStream_t)stream);
         if (rc != MAGIC_OK) return rc;
-        const int rc2 = run_rows<F16x2>(p, (hipStream_t)stream);
-        if (rc2 != MAGIC_OK) return rc2;
-        p.pr.rg.want_safe = false;             // the segments whose rows differ too much in size
-        return run_rows<F32x3>(p, (hipStream_t)stream);
+        p.a = magic::attn::gathered(a, p.pr);
+        if (s.f16) {
+            rc = run_rows<F16x2>(p, (hipStream_t)stream);
+            if (rc != MAGIC_OK) return rc;
+            p.pr.rg.want_safe = false;         // the segments whose rows differ too much in size
+            return run_rows<F32x3>(p, (hipStream_t)stream);
+        }
     }
     return a->dtype == MAGIC_F32 ? run<F32x3>(p, s.wm, (hipStream_t)stream) : run<BF16>(p, s.wm, (hipStream_t)stream);
 }

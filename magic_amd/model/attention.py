@@ -42,14 +42,14 @@ class AttentionPlan:
 
 
 def _tiles(rows, others):
-    """int32 [tiles, 8]: {first row, rows, first row of the other side, its rows, segment, 0, 0, 0} of every tile of up to
-    ``_lib.ATTN_TILE`` rows, longest segments' tiles first (they take longest; results do not depend on the order)."""
+    """int32 [tiles, 8]: {first row, rows, first row of the other side, its rows, segment, the segment's own first row
+    and rows, 0} of every tile of up to ``_lib.ATTN_TILE`` rows, longest segments' tiles first (they take longest; results do not depend on the order)."""
     rows, others = np.asarray(rows, np.int64), np.asarray(others, np.int64)
     n = -(-rows // _lib.ATTN_TILE)
     seg = np.repeat(np.arange(rows.size), n)
     at = (np.arange(seg.size) - np.repeat(np.cumsum(n) - n, n)) * _lib.ATTN_TILE
     r0, o0 = np.cumsum(rows) - rows, np.cumsum(others) - others
-    t = np.stack([r0[seg] + at, np.minimum(rows[seg] - at, _lib.ATTN_TILE), o0[seg], others[seg], seg, 0 * seg, 0 * seg, 0 * seg], 1)
+    t = np.stack([r0[seg] + at, np.minimum(rows[seg] - at, _lib.ATTN_TILE), o0[seg], others[seg], seg, r0[seg], rows[seg], 0 * seg], 1)
     return t[np.argsort(-others[seg], kind="stable")].astype(np.int32)
 
 

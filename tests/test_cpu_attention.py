@@ -15,13 +15,14 @@ def test_plan_tiles_cover_every_row_once():
         for tiles, rows, others in ((plan.q_tiles, ql, kl), (plan.k_tiles, kl, ql)):
             seen = np.zeros(sum(rows), int)
             r0, o0 = np.cumsum([0] + rows), np.cumsum([0] + others)
-            for a, n, b, m, g in tiles[:, :5].tolist():
+            for a, n, b, m, g, s0, sn, _ in tiles.tolist():
                 assert 1 <= n <= _lib.ATTN_TILE
                 seg = int(np.searchsorted(r0, a, side="right")) - 1
                 while rows[seg] == 0:
                     seg += 1
                 assert r0[seg] <= a and a + n <= r0[seg] + rows[seg]
-                assert (b, m, g) == (o0[seg], others[seg], seg)
+                assert (b, m, g, s0, sn) == (o0[seg], others[seg], seg, r0[seg], rows[seg])
+                assert (a - s0) % _lib.ATTN_TILE == 0
                 seen[a:a + n] += 1
             assert (seen == 1).all()
     assert attention_plan([], device="cpu").q_tiles.shape == (0, 8)

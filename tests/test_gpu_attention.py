@@ -160,6 +160,27 @@ def test_attention_scale_signs_and_large_scores(cuda):
         check(run(q, k, v, d, q_lens, kv_lens, scale=scale), q, k, v, d, q_lens, kv_lens, scale=scale)
 
 
+@pytest.mark.parametrize("dtype,hq,hk,D", [(torch.float32, 4, 2, 64), (torch.float32, 16, 8, 64), (torch.float32, 16, 16, 16),
+                                           (torch.bfloat16, 16, 4, 128)])
+@pytest.mark.parametrize("keep", [0.5, 0.02, 1.0])
+def test_masked_keys_of_long_segments(cuda, dtype, hq, hk, D, keep):
+    """Long enough for the unmasked keys to be gathered; one segment without any, one whose mask starts off a word."""
+    q_lens = kv_lens = [700, 5, 1301, 260, 33]
+    q, k, v, d, kw = make(cuda, q_lens, kv_lens, hq, hk, D, dtype, seed=17, slopes=True, mask=keep)
+    kw["key_mask"][2006:2266] = False
+    kw["key_mask"][705:900] = False
+    mask = kw["key_mask"]
+    got = run(q, k, v, d, q_lens, kv_lens, **kw)
+    check(got, q, k, v, d, q_lens, kv_lens, **kw)
+    assert not got["out"][2006:2266].any() and not got["dq"][2006:2266].any()
+    k2, v2 = k.clone(), v.clone()
+    k2[~mask], v2[~mask] = float("nan"), float("inf")
+    dirty = run(q, k2, v2, d, q_lens, kv_lens, **kw)
+    byte = run(q, k, v, d, q_lens, kv_lens, **dict(kw, key_mask=mask.to(torch.uint8) * 200))
+    for name in got:
+        assert torch.equal(got[name], dirty[name]) and torch.equal(got[name], byte[name]), name
+
+
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=["f32", "bf16"])
 def test_rows_without_a_visible_key_and_what_masked_keys_hold(cuda, dtype):
     """Masked keys may hold NaN, infinities and the type's lowest value; rows behind a segment's end may too (they
