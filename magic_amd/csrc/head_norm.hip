@@ -12,6 +12,8 @@
 
 namespace {
 
+constexpr int MAX_BLOCKS = 2048;   // of the row sweep
+
 struct RopeArgs {
     int64_t n;
     int hq, hk, D, half;      // half = R / 2 rotated pairs
@@ -23,22 +25,27 @@ struct RopeArgs {
     void *yq, *yk;            // forward: [n, h, D] contiguous
     const void *dyq, *dyk;    // backward
     int64_t ld_dyq, hs_dyq, ld_dyk, hs_dyk;
-    float *partial;           // backward: [gridDim.x][2][D]
+    float *partial;           // backward: [2][D][blocks]
     double freq[64];          // base^(-2i/R) / (2 pi)
 };
 
-// item j of a head: j < half / VEC: the pair of chunks at j*VEC and half + j*VEC; above: the plain chunk behind them
+// Item j of a head, two chunks of VEC columns: the rotated pair (j VEC, half + j VEC), or two chunks of the columns behind
+// the rotated ones (b < 0: an odd column left alone)
 template <int VEC> struct Item {
-    int a, b;                 // first columns; b < 0: no partner
-    bool ok;
+    int a, b;
+    bool ok, turn;
 };
 template <int VEC> __device__ __forceinline__ Item<VEC> item(const RopeArgs &p, int j) {
-    const int np = p.half / VEC;
+    const int np = p.half / VEC, plain = p.D - 2 * p.half, ph = (plain / VEC + 1) / 2;   // chunks in the first plain half
     Item<VEC> it;
-    if (j < np) {
+    it.turn = j < np;
+    if (it.turn) {
         it.a = j * VEC, it.b = p.half + j * VEC, it.ok = true;
     } else {
-        it.a = 2 * p.half + (j - np) * VEC, it.b = -1, it.ok = it.a < p.D;
+        const int i = j - np;
+        it.ok = i < ph;
+        it.a = 2 * p.half + i * VEC, it.b = 2 * p.half + (ph + i) * VEC;
+        if (!it.ok || it.b >= p.D) it.b = -1;
     }
     return it;
 }
@@ -49,181 +56,178 @@ template <int GL> __device__ __forceinline__ float group_sum(float v) {
     return v;
 }
 
-template <typename T, int VEC, int GL, int IPL, bool BWD>
-__global__ __launch_bounds__(256) void k_head_norm(RopeArgs p) {
-    constexpr int RPB = 256 / GL;  // rows of a block
-    const int gl = threadIdx.x % GL;
-    Item<VEC> it[IPL];
-    float w[2][IPL][2][VEC];
-    float dw[2][IPL][2][VEC];
-#pragma unroll
-    for (int i = 0; i < IPL; ++i) {
-        it[i] = item<VEC>(p, gl + i * GL);
-#pragma unroll
-        for (int s = 0; s < 2; ++s)
-#pragma unroll
-            for (int e = 0; e < VEC; ++e) {
-                const float *wp = s ? p.wk : p.wq;
-                w[s][i][0][e] = it[i].ok ? wp[it[i].a + e] : 0.f;
-                w[s][i][1][e] = it[i].b >= 0 ? wp[it[i].b + e] : 0.f;
-                dw[s][i][0][e] = dw[s][i][1][e] = 0.f;
-            }
+// A head's chunks as they lie in memory: the next head's are under way while one is worked on
+template <typename T, int VEC, bool BWD> struct Chunks {
+    typename magic::vec_of<T, VEC>::type x[2], g[2];
+    __device__ __forceinline__ void load(const T *xp, const T *gp, const Item<VEC> &it) {
+        typedef typename magic::vec_of<T, VEC>::type vt;
+        const int a = it.ok ? it.a : 0, b = it.b >= 0 ? it.b : 0;    // (lanes without columns read the first ones)
+        x[0] = *reinterpret_cast<const vt *>(xp + a), x[1] = *reinterpret_cast<const vt *>(xp + b);
+        if (BWD) g[0] = *reinterpret_cast<const vt *>(gp + a), g[1] = *reinterpret_cast<const vt *>(gp + b);
     }
+};
+
+template <typename T, int VEC, int GL, bool BWD>
+__global__ __launch_bounds__(256) void k_head_norm(RopeArgs p) {
+    constexpr int RPB = 256 / GL;
+    const int gl = threadIdx.x % GL;
+    const Item<VEC> it = item<VEC>(p, gl);
+    float w[2][2][VEC], dw[2][2][VEC];
+#pragma unroll
+    for (int s = 0; s < 2; ++s)
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) {
+            const float *wp = s ? p.wk : p.wq;
+            w[s][0][e] = it.ok ? wp[it.a + e] : 0.f;
+            w[s][1][e] = it.b >= 0 ? wp[it.b + e] : 0.f;
+            dw[s][0][e] = dw[s][1][e] = 0.f;
+        }
     const float inv_d = 1.f / (float)p.D;
     for (int64_t row = (int64_t)blockIdx.x * RPB + threadIdx.x / GL; row < p.n; row += (int64_t)gridDim.x * RPB) {
-        float sn[IPL][VEC], cs[IPL][VEC];
+        float sn[VEC], cs[VEC];
         const double ps = (double)p.pos[row];
 #pragma unroll
-        for (int i = 0; i < IPL; ++i)
-#pragma unroll
-            for (int e = 0; e < VEC; ++e) {
-                double t = it[i].b >= 0 ? ps * p.freq[it[i].a + e] : 0.0;
-                t -= rint(t);
-                sincospif(2.f * (float)t, &sn[i][e], &cs[i][e]);
-            }
+        for (int e = 0; e < VEC; ++e) {
+            double t = it.turn ? ps * p.freq[it.a + e] : 0.0;
+            t -= rint(t);
+            sincospif(2.f * (float)t, &sn[e], &cs[e]);
+        }
 #pragma unroll
         for (int s = 0; s < 2; ++s) {
             const int nh = s ? p.hk : p.hq;
-            const T *x = (const T *)(s ? p.k : p.q) + row * (s ? p.ld_k : p.ld_q);
+            const T *x0 = (const T *)(s ? p.k : p.q) + row * (s ? p.ld_k : p.ld_q);
             const int64_t hs = s ? p.hs_k : p.hs_q;
-            const T *dy = BWD ? (const T *)(s ? p.dyk : p.dyq) + row * (s ? p.ld_dyk : p.ld_dyq) : nullptr;
+            const T *dy0 = BWD ? (const T *)(s ? p.dyk : p.dyq) + row * (s ? p.ld_dyk : p.ld_dyq) : nullptr;
             const int64_t hsd = s ? p.hs_dyk : p.hs_dyq;
-            T *y = (T *)(s ? p.yk : p.yq) + row * nh * p.D;
-            for (int h = 0; h < nh; ++h, x += hs, y += p.D) {
-                float v[IPL][2][VEC], g[IPL][2][VEC];
+            T *y0 = (T *)(s ? p.yk : p.yq) + row * nh * p.D;
+            Chunks<T, VEC, BWD> cur, next;
+            next.load(x0, dy0, it);
+            for (int h = 0; h < nh; ++h) {
+                cur = next;
+                const int hn = h + 1 < nh ? h + 1 : h;
+                next.load(x0 + hn * hs, BWD ? dy0 + hn * hsd : nullptr, it);
+                float v[2][VEC], g[2][VEC];
                 float ss = 0.f;
 #pragma unroll
-                for (int i = 0; i < IPL; ++i) {
-                    magic::load_vec<T, VEC>(x + it[i].a, it[i].ok, v[i][0]);
-                    magic::load_vec<T, VEC>(x + it[i].b, it[i].b >= 0, v[i][1]);
-                    if (BWD) {
-                        magic::load_vec<T, VEC>(dy + (int64_t)h * hsd + it[i].a, it[i].ok, g[i][0]);
-                        magic::load_vec<T, VEC>(dy + (int64_t)h * hsd + it[i].b, it[i].b >= 0, g[i][1]);
-                    }
+                for (int e = 0; e < VEC; ++e) {
+                    v[0][e] = it.ok ? (float)cur.x[0][e] : 0.f, v[1][e] = it.b >= 0 ? (float)cur.x[1][e] : 0.f;
+                    if (BWD) g[0][e] = it.ok ? (float)cur.g[0][e] : 0.f, g[1][e] = it.b >= 0 ? (float)cur.g[1][e] : 0.f;
+                    ss += v[0][e] * v[0][e] + v[1][e] * v[1][e];
                 }
-#pragma unroll
-                for (int i = 0; i < IPL; ++i)
-#pragma unroll
-                    for (int e = 0; e < VEC; ++e) ss += v[i][0][e] * v[i][0][e] + v[i][1][e] * v[i][1][e];
                 ss = group_sum<GL>(ss);
                 const float r = 1.f / sqrtf(ss * inv_d + p.eps);
-                if (!BWD) {
+                float dot = 0.f;
+                if (BWD) {
 #pragma unroll
-                    for (int i = 0; i < IPL; ++i) {
-                        float o[2][VEC];
-#pragma unroll
-                        for (int e = 0; e < VEC; ++e) {
-                            const float a = v[i][0][e] * r * w[s][i][0][e], b = v[i][1][e] * r * w[s][i][1][e];
-                            o[0][e] = a * cs[i][e] - b * sn[i][e];
-                            o[1][e] = b * cs[i][e] + a * sn[i][e];
-                        }
-                        magic::store_vec<T, VEC>(y + it[i].a, it[i].ok, o[0]);
-                        magic::store_vec<T, VEC>(y + it[i].b, it[i].b >= 0, o[1]);
+                    for (int e = 0; e < VEC; ++e) {
+                        const float a = g[0][e] * cs[e] + g[1][e] * sn[e];
+                        const float b = g[1][e] * cs[e] - g[0][e] * sn[e];
+                        dw[s][0][e] += a * v[0][e] * r;
+                        dw[s][1][e] += b * v[1][e] * r;
+                        g[0][e] = a * w[s][0][e];
+                        g[1][e] = b * w[s][1][e];
+                        dot += g[0][e] * v[0][e] + g[1][e] * v[1][e];
                     }
-                } else {
-                    float dot = 0.f;
-#pragma unroll
-                    for (int i = 0; i < IPL; ++i)
-#pragma unroll
-                        for (int e = 0; e < VEC; ++e) {
-                            const float a = g[i][0][e] * cs[i][e] + g[i][1][e] * sn[i][e];
-                            const float b = g[i][1][e] * cs[i][e] - g[i][0][e] * sn[i][e];
-                            dw[s][i][0][e] += a * v[i][0][e] * r;
-                            dw[s][i][1][e] += b * v[i][1][e] * r;
-                            g[i][0][e] = a * w[s][i][0][e];
-                            g[i][1][e] = b * w[s][i][1][e];
-                            dot += g[i][0][e] * v[i][0][e] + g[i][1][e] * v[i][1][e];
-                        }
                     dot = group_sum<GL>(dot) * inv_d * r * r;
+                }
+                float o[2][VEC];
 #pragma unroll
-                    for (int i = 0; i < IPL; ++i) {
-                        float o[2][VEC];
-#pragma unroll
-                        for (int e = 0; e < VEC; ++e) {
-                            o[0][e] = r * (g[i][0][e] - v[i][0][e] * dot);
-                            o[1][e] = r * (g[i][1][e] - v[i][1][e] * dot);
-                        }
-                        magic::store_vec<T, VEC>(y + it[i].a, it[i].ok, o[0]);
-                        magic::store_vec<T, VEC>(y + it[i].b, it[i].b >= 0, o[1]);
+                for (int e = 0; e < VEC; ++e) {
+                    if (BWD) {
+                        o[0][e] = r * (g[0][e] - v[0][e] * dot);
+                        o[1][e] = r * (g[1][e] - v[1][e] * dot);
+                    } else {
+                        const float a = v[0][e] * r * w[s][0][e], b = v[1][e] * r * w[s][1][e];
+                        o[0][e] = a * cs[e] - b * sn[e];
+                        o[1][e] = b * cs[e] + a * sn[e];
                     }
                 }
+                magic::store_vec<T, VEC>(y0 + h * p.D + it.a, it.ok, o[0]);
+                magic::store_vec<T, VEC>(y0 + h * p.D + it.b, it.b >= 0, o[1]);
             }
         }
     }
     if (BWD) {
-        // the block's weight gradients: row groups added in order through LDS
+        // the block's weight gradients: lanes of a wavefront that hold the same columns first (fixed tree), then the four
+        // wavefronts in order
         __shared__ float red[2][128];
-        for (int t = threadIdx.x; t < 256; t += 256) red[t >> 7][t & 127] = 0.f;
+        red[threadIdx.x >> 7][threadIdx.x & 127] = 0.f;
         __syncthreads();
-        // lanes of a wavefront that hold the same columns first (fixed tree), then the four wavefronts in order
 #pragma unroll
         for (int s = 0; s < 2; ++s)
-#pragma unroll
-            for (int i = 0; i < IPL; ++i)
 #pragma unroll
                 for (int c = 0; c < 2; ++c)
 #pragma unroll
                     for (int e = 0; e < VEC; ++e)
 #pragma unroll
-                        for (int o = 32; o >= GL; o >>= 1) dw[s][i][c][e] += __shfl_xor(dw[s][i][c][e], o, 64);
+                        for (int o = 32; o >= GL; o >>= 1) dw[s][c][e] += __shfl_xor(dw[s][c][e], o, 64);
         for (int wv = 0; wv < 4; ++wv) {
             if ((int)(threadIdx.x >> 6) == wv && (threadIdx.x & 63) < GL) {
 #pragma unroll
                 for (int s = 0; s < 2; ++s)
 #pragma unroll
-                    for (int i = 0; i < IPL; ++i)
-#pragma unroll
                         for (int e = 0; e < VEC; ++e) {
-                            if (it[i].ok) red[s][it[i].a + e] += dw[s][i][0][e];
-                            if (it[i].b >= 0) red[s][it[i].b + e] += dw[s][i][1][e];
+                            if (it.ok) red[s][it.a + e] += dw[s][0][e];
+                            if (it.b >= 0) red[s][it.b + e] += dw[s][1][e];
                         }
             }
             __syncthreads();
         }
         for (int t = threadIdx.x; t < 2 * p.D; t += 256)
-            p.partial[(int64_t)blockIdx.x * 2 * p.D + t] = red[t / p.D][t % p.D];
+            p.partial[(int64_t)t * gridDim.x + blockIdx.x] = red[t / p.D][t % p.D];
     }
 }
 
-// column sums of the block partials, in double: wavefront per output column, blocks lane by lane, fixed tree
-__global__ __launch_bounds__(64) void k_head_norm_dw(const float *partial, int blocks, int D, float *dwq, float *dwk) {
+// column sums of the block partials, in double: a block per output column, fixed tree
+__global__ __launch_bounds__(256) void k_head_norm_dw(const float *partial, int blocks, int D, float *dwq, float *dwk) {
+    __shared__ double red[4];
     const int c = blockIdx.x;
+    float x[MAX_BLOCKS / 256];
+#pragma unroll
+    for (int i = 0; i < MAX_BLOCKS / 256; ++i) {
+        const int b = threadIdx.x + 256 * i;
+        x[i] = b < blocks ? partial[(int64_t)c * blocks + b] : 0.f;
+    }
     double s = 0.0;
-    for (int b = threadIdx.x; b < blocks; b += 64) s += (double)partial[(int64_t)b * 2 * D + c];
+#pragma unroll
+    for (int i = 0; i < MAX_BLOCKS / 256; ++i) s += (double)x[i];
 #pragma unroll
     for (int o = 32; o > 0; o >>= 1) s += __shfl_xor(s, o, 64);
+    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = s;
+    __syncthreads();
     if (threadIdx.x == 0) {
+        s = (red[0] + red[1]) + (red[2] + red[3]);
         if (c < D) dwq[c] = (float)s;
         else dwk[c - D] = (float)s;
     }
 }
 
-int rope_blocks(int64_t n, int gl) { return magic::stride_grid(n, 256 / gl, 1024); }
+int rope_blocks(int64_t n, int gl) { return magic::stride_grid(n, 256 / gl, MAX_BLOCKS); }
 
-template <typename T, int VEC, int GL, int IPL> int run(const RopeArgs &p, bool bwd, hipStream_t st) {
+template <typename T, int VEC, int GL> int run(const RopeArgs &p, bool bwd, hipStream_t st) {
     const int grid = rope_blocks(p.n, GL);
     if (bwd)
-        MAGIC_LAUNCH("head_norm_rope_bwd", (k_head_norm<T, VEC, GL, IPL, true>), grid, 256, 0, st, p);
+        MAGIC_LAUNCH("head_norm_rope_bwd", (k_head_norm<T, VEC, GL, true>), grid, 256, 0, st, p);
     else
-        MAGIC_LAUNCH("head_norm_rope_fwd", (k_head_norm<T, VEC, GL, IPL, false>), grid, 256, 0, st, p);
+        MAGIC_LAUNCH("head_norm_rope_fwd", (k_head_norm<T, VEC, GL, false>), grid, 256, 0, st, p);
     return magic::launch_status();
 }
 
 template <typename T, int VEC> int pick(const RopeArgs &p, bool bwd, hipStream_t st, int *gl_out) {
-    const int items = p.half / VEC + (p.D - 2 * p.half) / VEC;
+    const int items = p.half / VEC + ((p.D - 2 * p.half) / VEC + 1) / 2;
     int gl = 4;
     while (gl < items && gl < 64) gl *= 2;
     if (gl_out) {
         *gl_out = gl;
         return MAGIC_OK;
     }
-    if (gl < items) return run<T, VEC, 64, 2>(p, bwd, st);  // at most 127 items (one pair, 126 plain columns)
+    // (at most 64 items: single columns of heads of 128)
     switch (gl) {
-        case 4: return run<T, VEC, 4, 1>(p, bwd, st);
-        case 8: return run<T, VEC, 8, 1>(p, bwd, st);
-        case 16: return run<T, VEC, 16, 1>(p, bwd, st);
-        case 32: return run<T, VEC, 32, 1>(p, bwd, st);
-        default: return run<T, VEC, 64, 1>(p, bwd, st);
+        case 4: return run<T, VEC, 4>(p, bwd, st);
+        case 8: return run<T, VEC, 8>(p, bwd, st);
+        case 16: return run<T, VEC, 16>(p, bwd, st);
+        case 32: return run<T, VEC, 32>(p, bwd, st);
+        default: return run<T, VEC, 64>(p, bwd, st);
     }
 }
 
@@ -231,14 +235,19 @@ bool mult(const void *p, int64_t ld, int64_t hs, int vec, int size) {
     return (uintptr_t)p % (size_t)(vec * size) == 0 && ld % vec == 0 && hs % vec == 0;
 }
 
-// whole chunks of 4 columns wherever strides, widths and addresses allow them, single columns otherwise
+bool chunks(const RopeArgs &p, bool bwd, int vec, int size) {
+    const bool ok = p.half % vec == 0 && p.D % vec == 0 && mult(p.q, p.ld_q, p.hs_q, vec, size) &&
+                    mult(p.k, p.ld_k, p.hs_k, vec, size) && mult(p.yq, vec, vec, vec, size) && mult(p.yk, vec, vec, vec, size);
+    return ok && (!bwd || (mult(p.dyq, p.ld_dyq, p.hs_dyq, vec, size) && mult(p.dyk, p.ld_dyk, p.hs_dyk, vec, size)));
+}
+
+// chunks of 16 (or 8) bytes wherever strides, widths and addresses allow them, single columns otherwise
 int launch(const RopeArgs &p, int dtype, bool bwd, hipStream_t st, int *gl_out = nullptr) {
-    const int size = dtype == MAGIC_F32 ? 4 : 2;
-    bool v4 = p.half % 4 == 0 && p.D % 4 == 0 && mult(p.q, p.ld_q, p.hs_q, 4, size) && mult(p.k, p.ld_k, p.hs_k, 4, size) &&
-              mult(p.yq, 4, 4, 4, size) && mult(p.yk, 4, 4, 4, size);
-    if (bwd) v4 = v4 && mult(p.dyq, p.ld_dyq, p.hs_dyq, 4, size) && mult(p.dyk, p.ld_dyk, p.hs_dyk, 4, size);
-    if (dtype == MAGIC_F32) return v4 ? pick<float, 4>(p, bwd, st, gl_out) : pick<float, 1>(p, bwd, st, gl_out);
-    return v4 ? pick<magic::bf16_t, 4>(p, bwd, st, gl_out) : pick<magic::bf16_t, 1>(p, bwd, st, gl_out);
+    if (dtype == MAGIC_F32)
+        return chunks(p, bwd, 4, 4) ? pick<float, 4>(p, bwd, st, gl_out) : pick<float, 1>(p, bwd, st, gl_out);
+    return chunks(p, bwd, 8, 2)   ? pick<magic::bf16_t, 8>(p, bwd, st, gl_out)
+           : chunks(p, bwd, 4, 2) ? pick<magic::bf16_t, 4>(p, bwd, st, gl_out)
+                                  : pick<magic::bf16_t, 1>(p, bwd, st, gl_out);
 }
 
 int fill(RopeArgs &p, int64_t n, int hq, int hk, int D, int rot, int dtype, const void *q, int64_t ld_q, int64_t hs_q,
@@ -278,7 +287,7 @@ int magic_head_norm_rope_fwd(int64_t n_rows, int32_t q_heads, int32_t kv_heads, 
 
 size_t magic_head_norm_rope_bwd_workspace_bytes(int64_t n_rows, int32_t head_dim) {
     if (n_rows < 0 || head_dim < 1) return 256;
-    return magic::align_up((size_t)1024 * 2 * head_dim * sizeof(float)) + 256;
+    return magic::align_up((size_t)MAX_BLOCKS * 2 * head_dim * sizeof(float)) + 256;
 }
 
 int magic_head_norm_rope_bwd(int64_t n_rows, int32_t q_heads, int32_t kv_heads, int32_t head_dim, int32_t rotary_dim,
@@ -295,7 +304,7 @@ int magic_head_norm_rope_bwd(int64_t n_rows, int32_t q_heads, int32_t kv_heads, 
     if (!dwq || !dwk) return MAGIC_ERR_INVALID_ARG;
     int grid = 0;
     magic::Arena ar(workspace, workspace_bytes);
-    p.partial = ar.take<float>((size_t)1024 * 2 * head_dim);
+    p.partial = ar.take<float>((size_t)MAX_BLOCKS * 2 * head_dim);
     if (!ar.ok() || !p.partial) return MAGIC_ERR_WORKSPACE;
     if (n_rows > 0) {
         if (!dyq || !dyk || !dq || !dk || ld_dyq < 0 || hs_dyq < 0 || ld_dyk < 0 || hs_dyk < 0) return MAGIC_ERR_INVALID_ARG;
@@ -307,7 +316,7 @@ int magic_head_norm_rope_bwd(int64_t n_rows, int32_t q_heads, int32_t kv_heads, 
         st = launch(p, dtype, true, stream);
         if (st != MAGIC_OK) return st;
     }
-    MAGIC_LAUNCH("head_norm_rope_dw", k_head_norm_dw, 2 * head_dim, 64, 0, stream, p.partial, grid, head_dim, dwq, dwk);
+    MAGIC_LAUNCH("head_norm_rope_dw", k_head_norm_dw, 2 * head_dim, 256, 0, stream, p.partial, grid, head_dim, dwq, dwk);
     return magic::launch_status();
 }
 
