@@ -8,12 +8,14 @@
 // instructions instead of six).  exp = 255 marks a block that held an infinity or a NaN: it reads back as NaN, so a
 // diverging run is not silently repaired.
 #include "common.h"
-#include "bf16_split.h"
+#include "attn_common.h"
 
 namespace {
 
-typedef float float16_t __attribute__((ext_vector_type(16)));
-typedef float f32x4_t __attribute__((ext_vector_type(4)));
+using magic::bf16_t;
+using magic::bf16x8_t;
+using magic::attn::f32x16_t;
+using magic::attn::f32x4_t;
 
 __device__ __forceinline__ float pow2f(int e) {  // 2^e, -126 <= e <= 127
     return __uint_as_float((uint32_t)(e + 127) << 23);
@@ -95,8 +97,11 @@ __global__ __launch_bounds__(256) void k_act8_unpack(int64_t n, int F, const int
     }
 }
 
-// dW[M,F] = dY[N,M]^T . Xhat[N,F]: a wavefront owns a 32 x 32 output tile and a strip of rows; three matrix products
-// (dY in three bf16 pieces, Xhat in its only one) per 16 rows; the strips are added in order by k_act8_dw_reduce.
+// dW[M,F] = dY[N,M]^T . Xhat[N,F].  HBM-bound at the entity-level shapes: a block of four wavefronts owns an output tile as
+// large as its registers hold (64 x 192 covers the whole of the THEIA-shaped decoder input: each operand is read once) and
+// a strip of the rows.  Steps of 32 rows: dY split into three bf16 planes and the codes turned into their one bf16 value go
+// row-major to LDS, where transposed reads deliver eight rows of a column; three 32x32x16 products a tile and 16 rows.  The
+// next step's rows are loaded under the products.  The strips' tiles are added in order by k_act8_dw_reduce.
 struct DwArgs {
     int64_t n;
     int M, F, nb;
@@ -106,68 +111,187 @@ struct DwArgs {
     int64_t ld_c;
     const uint8_t *exps;
     float *partial, *dw;
-    int strips, ft;
-    int64_t rows;  // of a strip, a multiple of 16
+    int strips, mt, ft;   // tiles along M and F
+    int64_t rows;         // of a strip, a multiple of STEP
 };
 
-__global__ __launch_bounds__(64) void k_act8_dw(DwArgs a) {
-    const int lane = threadIdx.x, li = lane & 31, hf = lane >> 5;
-    const int m0 = (blockIdx.y / a.ft) * 32, f0 = (blockIdx.y % a.ft) * 32;
-    const int64_t r0 = (int64_t)blockIdx.x * a.rows;
-    const int64_t r1 = r0 + a.rows < a.n ? r0 + a.rows : a.n;
-    const int mc = m0 + li < a.M ? m0 + li : 0, fc = f0 + li < a.F ? f0 + li : 0;
-    float16_t acc;
+constexpr int STEP = 32, NT = 256;
+
+// tile: TM = 64 MB rows of dW (two wavefronts of 32 MB), 64 FB columns (two of 32 FB)
+template <int MB, int FB, bool ALIGNED> __global__ __launch_bounds__(NT, MB *FB > 4 ? 2 : 3) void k_act8_dw(DwArgs a) {
+    constexpr int TM = 64 * MB, TF = 64 * FB;
+    typedef magic::attn::Tile<magic::attn::F32x3, TM, STEP> ytile;
+    typedef magic::attn::Tile<magic::attn::BF16, 64, STEP> xtile;        // FB of them side by side
+    constexpr int YN = STEP * TM / 8 / NT, XC = STEP * TF / 8, XN = (XC + NT - 1) / NT;
+    __shared__ __align__(16) bf16_t sy[3 * ytile::PLANE], sx[FB * xtile::PLANE];
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, li = lane & 31, hf = lane >> 5;
+    const int wm = wave & 1, wf = wave >> 1;
+    const int m0 = (int)(blockIdx.y / a.ft) * TM, f0 = (int)(blockIdx.y % a.ft) * TF;
+    const int64_t r0 = (int64_t)blockIdx.x * a.rows, r1 = min(r0 + a.rows, a.n);
+    f32x16_t acc[MB][FB];
 #pragma unroll
-    for (int r = 0; r < 16; ++r) acc[r] = 0.f;
-    for (int64_t r = r0; r < r1; r += 16) {
-        float y[8], x[8];
+    for (int i = 0; i < MB; ++i)
 #pragma unroll
-        for (int u = 0; u < 8; ++u) {
-            const int64_t row = r + 8 * hf + u;
-            const int64_t rc = row < a.n ? row : a.n - 1;
-            const float dv = a.dy[rc * a.ld_dy + mc];
-            const float xv = (float)a.codes[rc * a.ld_c + fc] * scale_of(a.exps[rc * a.nb + f0 / 32]);
-            y[u] = row < r1 && m0 + li < a.M ? dv : 0.f;
-            x[u] = row < r1 && f0 + li < a.F ? xv : 0.f;
+        for (int j = 0; j < FB; ++j)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) acc[i][j][r] = 0.f;
+
+    float y[YN][8];
+    uint64_t x[XN];
+    uint8_t ex[XN];
+    auto load = [&](int64_t r) {
+#pragma unroll
+        for (int i = 0; i < YN; ++i) {
+            const int c = tid + i * NT, col = m0 + (c % (TM / 8)) * 8;
+            const int64_t row = min(r + c / (TM / 8), a.n - 1);
+            const float *p = a.dy + row * a.ld_dy;
+            if (ALIGNED) {
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    const f32x4_t v = *reinterpret_cast<const f32x4_t *>(p + (col + 4 * h < a.M ? col + 4 * h : 0));
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) y[i][4 * h + e] = v[e];
+                }
+            } else {
+#pragma unroll
+                for (int e = 0; e < 8; ++e) y[i][e] = p[col + e < a.M ? col + e : 0];
+            }
         }
-        magic::bf16x8_t y1, y2, y3, xb;
-        magic::split8(make_float4(y[0], y[1], y[2], y[3]), make_float4(y[4], y[5], y[6], y[7]), y1, y2, y3);
 #pragma unroll
-        for (int u = 0; u < 8; ++u) xb[u] = (__bf16)x[u];
-        acc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(y3, xb, acc, 0, 0, 0);
-        acc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(y2, xb, acc, 0, 0, 0);
-        acc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(y1, xb, acc, 0, 0, 0);
+        for (int i = 0; i < XN; ++i) {
+            const int c = min(tid + i * NT, XC - 1), col = f0 + (c % (TF / 8)) * 8;
+            const int64_t row = min(r + c / (TF / 8), a.n - 1);
+            const int cc = col < a.ld_c ? col : 0;
+            x[i] = *reinterpret_cast<const uint64_t *>(a.codes + row * a.ld_c + cc);
+            ex[i] = a.exps[row * a.nb + cc / 32];
+        }
+    };
+    auto store = [&](int64_t r) {
+#pragma unroll
+        for (int i = 0; i < YN; ++i) {
+            const int c = tid + i * NT, row = c / (TM / 8), col = m0 + (c % (TM / 8)) * 8;
+            float v[8];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) v[e] = r + row < r1 && col + e < a.M ? y[i][e] : 0.f;
+            bf16x8_t p[3];
+            magic::attn::to_planes(v, p);
+#pragma unroll
+            for (int k = 0; k < 3; ++k)
+                *reinterpret_cast<bf16x8_t *>(sy + k * ytile::PLANE + ytile::at(row, c % (TM / 8))) = p[k];
+        }
+#pragma unroll
+        for (int i = 0; i < XN; ++i) {
+            const int c = tid + i * NT;
+            if (XC % NT != 0 && c >= XC) break;
+            const int row = c / (TF / 8), cx = c % (TF / 8);
+            const bool ok = r + row < r1 && f0 + cx * 8 < a.ld_c;
+            const float s = ok ? scale_of(ex[i]) : 0.f;
+            bf16x8_t v;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) v[e] = (bf16_t)((float)(int8_t)(x[i] >> (8 * e)) * s);      // (exact)
+            *reinterpret_cast<bf16x8_t *>(sx + (cx / 8) * xtile::PLANE + xtile::at(row, cx % 8)) = v;
+        }
+    };
+    const uint32_t ty = ytile::lane_turned(lane), tx = xtile::lane_turned(lane);
+    if (r0 < r1) load(r0);
+    for (int64_t r = r0; r < r1; r += STEP) {
+        __syncthreads();
+        store(r);
+        __syncthreads();
+        if (r + STEP < r1) load(r + STEP);
+#pragma unroll
+        for (int k = 0; k < STEP / 16; ++k) {
+            bf16x8_t fx[FB][1];
+#pragma unroll
+            for (int j = 0; j < FB; ++j) {
+                const int t = wf * FB + j;         // of the tile's 2 FB column blocks of 32
+                xtile::frag_t(sx + (t >> 1) * xtile::PLANE, tx ^ (uint32_t)(64 * (t & 1)), 16 * k, 0, fx[j]);
+            }
+#pragma unroll
+            for (int i = 0; i < MB; ++i) {
+                bf16x8_t fy[3];
+                ytile::frag_t(sy, ty ^ (uint32_t)(64 * (wm * MB)), 16 * k, i, fy);
+#pragma unroll
+                for (int j = 0; j < FB; ++j) {
+                    acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(fy[2], fx[j][0], acc[i][j], 0, 0, 0);
+                    acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(fy[1], fx[j][0], acc[i][j], 0, 0, 0);
+                    acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(fy[0], fx[j][0], acc[i][j], 0, 0, 0);
+                }
+            }
+        }
     }
-    float *out = a.partial + ((int64_t)blockIdx.x * gridDim.y + blockIdx.y) * 1024;
+    float *out = a.partial + ((int64_t)blockIdx.x * gridDim.y + blockIdx.y) * (TM * TF);
 #pragma unroll
-    for (int r = 0; r < 16; ++r) out[((r & 3) + 8 * (r >> 2) + 4 * hf) * 32 + li] = acc[r];
+    for (int i = 0; i < MB; ++i)
+#pragma unroll
+        for (int j = 0; j < FB; ++j)
+#pragma unroll
+            for (int r = 0; r < 16; ++r)
+                out[((wm * MB + i) * 32 + (r & 3) + 8 * (r >> 2) + 4 * hf) * TF + (wf * FB + j) * 32 + li] = acc[i][j][r];
 }
 
-__global__ __launch_bounds__(256) void k_act8_dw_reduce(DwArgs a, int tiles) {
-    const int e = blockIdx.x * 256 + threadIdx.x, tile = blockIdx.y;
-    const int i = (tile / a.ft) * 32 + (e >> 5), j = (tile % a.ft) * 32 + (e & 31);
-    if (i >= a.M || j >= a.F) return;
+// dW from the strips' tiles: 64 consecutive elements a block, its sixteen wavefronts take the strips in turn (strip order
+// within each, eight loads in flight) and are added in order
+__global__ __launch_bounds__(1024) void k_act8_dw_reduce(DwArgs a, int TM, int TF) {
+    __shared__ float red[16][64];
+    const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, tile = blockIdx.y, tiles = gridDim.y;
+    const int e = blockIdx.x * 64 + lane;
+    const int64_t stride = (int64_t)tiles * TM * TF;
+    const float *p = a.partial + (int64_t)tile * TM * TF + e;
     float s = 0.f;
-    for (int k = 0; k < a.strips; ++k) s += a.partial[((int64_t)k * tiles + tile) * 1024 + e];
-    a.dw[(int64_t)i * a.F + j] = s;
+    int k = w;
+    for (; k + 7 * 16 < a.strips; k += 8 * 16) {
+        float v[8];
+#pragma unroll
+        for (int u = 0; u < 8; ++u) v[u] = p[(k + 16 * u) * stride];
+#pragma unroll
+        for (int u = 0; u < 8; ++u) s += v[u];
+    }
+    for (; k < a.strips; k += 16) s += p[k * stride];
+    red[w][lane] = s;
+    __syncthreads();
+    if (w != 0) return;
+#pragma unroll
+    for (int i = 1; i < 16; ++i) s += red[i][lane];
+    const int i = (tile / a.ft) * TM + e / TF, j = (tile % a.ft) * TF + e % TF;
+    if (i < a.M && j < a.F) a.dw[(int64_t)i * a.F + j] = s;
 }
 
 struct DwPlan {
-    int strips, mt, ft;
+    int mb, fb, mt, ft, strips;
     int64_t rows;
     size_t floats;
 };
+// The output tile that reads the least: dY once for every tile column, the codes once for every tile row.
 DwPlan plan(int64_t n, int M, int F) {
+    static const int cand[][2] = {{1, 1}, {1, 2}, {1, 3}, {2, 2}, {2, 3}, {2, 4}};
     DwPlan p;
-    p.mt = (M + 31) / 32, p.ft = (F + 31) / 32;
-    int64_t strips = 4096 / ((int64_t)p.mt * p.ft);
+    double best = -1.0;
+    for (auto &c : cand) {
+        const int mt = (M + 64 * c[0] - 1) / (64 * c[0]), ft = (F + 64 * c[1] - 1) / (64 * c[1]);
+        const double cost = 4.0 * ft * (mt * 64.0 * c[0]) + 1.03 * mt * (ft * 64.0 * c[1]);
+        if (best < 0 || cost < best) best = cost, p.mb = c[0], p.fb = c[1], p.mt = mt, p.ft = ft;
+    }
+    const int64_t tiles = (int64_t)p.mt * p.ft, tile = (int64_t)p.mb * p.fb * 4096;
+    int64_t strips = 768 / tiles;                       // three resident blocks a CU
+    const int64_t fit = (64 << 20) / (tiles * tile);    // at most 256 MB of partial tiles
+    if (strips > fit) strips = fit;
     if (strips < 1) strips = 1;
     int64_t rows = (n + strips - 1) / strips;
-    if (rows < 128) rows = 128;
-    p.rows = (rows + 15) / 16 * 16;
+    if (rows < 4 * STEP) rows = 4 * STEP;
+    p.rows = (rows + STEP - 1) / STEP * STEP;
     p.strips = (int)((n + p.rows - 1) / p.rows);
-    p.floats = (size_t)p.strips * p.mt * p.ft * 1024;
+    p.floats = (size_t)p.strips * tiles * tile;
     return p;
+}
+
+template <int MB, int FB> int run_dw(const DwArgs &a, hipStream_t stream) {
+    const dim3 grid(a.strips, a.mt * a.ft);
+    if (a.M % 4 == 0 && a.ld_dy % 4 == 0 && (uintptr_t)a.dy % 16 == 0)
+        MAGIC_LAUNCH("act8_weight_grad", (k_act8_dw<MB, FB, true>), grid, NT, 0, stream, a);
+    else
+        MAGIC_LAUNCH("act8_weight_grad", (k_act8_dw<MB, FB, false>), grid, NT, 0, stream, a);
+    return magic::launch_status();
 }
 
 }  // namespace
@@ -218,20 +342,27 @@ int magic_act8_weight_grad(int64_t n_rows, int32_t m, int32_t f, const float *dy
     if (n_rows < 0 || m <= 0 || f <= 0 || !dw) return MAGIC_ERR_INVALID_ARG;
     if (n_rows > 0 && (!dy || !codes || !exps || ld_dy < m || (uintptr_t)codes % 16)) return MAGIC_ERR_INVALID_ARG;
     hipStream_t stream = (hipStream_t)stream_;
-    DwPlan p = plan(n_rows, m, f);
+    const DwPlan p = plan(n_rows, m, f);
+    if ((int64_t)p.mt * p.ft > 65535) return MAGIC_ERR_UNSUPPORTED;
     DwArgs a;
     a.n = n_rows, a.M = m, a.F = f, a.nb = (f + 31) / 32;
     a.dy = dy, a.ld_dy = ld_dy, a.codes = codes, a.ld_c = magic_act8_code_stride(f), a.exps = exps;
-    a.dw = dw, a.ft = p.ft, a.rows = p.rows, a.strips = n_rows > 0 ? p.strips : 0;
+    a.dw = dw, a.mt = p.mt, a.ft = p.ft, a.rows = p.rows, a.strips = n_rows > 0 ? p.strips : 0;
     a.partial = nullptr;
-    const int tiles = p.mt * p.ft;
     if (n_rows > 0) {
         magic::Arena ar(workspace, workspace_bytes);
         a.partial = ar.take<float>(p.floats);
         if (!ar.ok() || !a.partial) return MAGIC_ERR_WORKSPACE;
-        MAGIC_LAUNCH("act8_weight_grad", k_act8_dw, dim3(p.strips, tiles), 64, 0, stream, a);
+        const int st = p.mb == 1 ? (p.fb == 1   ? run_dw<1, 1>(a, stream)
+                                    : p.fb == 2 ? run_dw<1, 2>(a, stream)
+                                                : run_dw<1, 3>(a, stream))
+                                 : (p.fb == 2   ? run_dw<2, 2>(a, stream)
+                                    : p.fb == 3 ? run_dw<2, 3>(a, stream)
+                                                : run_dw<2, 4>(a, stream));
+        if (st != MAGIC_OK) return st;
     }
-    MAGIC_LAUNCH("act8_weight_grad_reduce", k_act8_dw_reduce, dim3(4, tiles), 256, 0, stream, a, tiles);
+    const int TM = 64 * p.mb, TF = 64 * p.fb;
+    MAGIC_LAUNCH("act8_weight_grad_reduce", k_act8_dw_reduce, dim3(TM * TF / 64, p.mt * p.ft), 1024, 0, stream, a, TM, TF);
     return magic::launch_status();
 }
 
