@@ -36,43 +36,59 @@ __device__ __forceinline__ int code_of(float x, int e) {         // e: stored ex
 
 __device__ __forceinline__ float scale_of(int e) { return e == 255 ? __uint_as_float(0x7fc00000u) : pow2f(e - 127); }
 
-// eight lanes of four columns (VEC 4) or thirty-two of one (VEC 1) per block
-template <int VEC>
-__global__ __launch_bounds__(256) void k_act8_pack(int64_t n, int F, const float *x, int64_t ld_x, int8_t *codes,
-                                                   int64_t ld_c, uint8_t *exps, int nb) {
-    constexpr int LPB = 32 / VEC;
-    const int64_t total = n * nb;
+// VEC 8: four lanes a block, two float4 each (rows of whole float4s); VEC 1: thirty-two lanes.  U blocks a thread are in
+// flight together.  I: index type of a block (a 64-bit division costs as much as the rest).
+template <int VEC, typename I>
+__global__ __launch_bounds__(256) void k_act8_pack(I total, int F, const float *x, int64_t ld_x, int8_t *codes,
+                                                   int64_t ld_c, uint8_t *exps, I nb) {
+    constexpr int LPB = 32 / VEC, U = 4;
+    constexpr I PER = 256 / LPB;
     const int l = threadIdx.x % LPB;
-    for (int64_t b = (int64_t)blockIdx.x * (256 / LPB) + threadIdx.x / LPB; b < total;
-         b += (int64_t)gridDim.x * (256 / LPB)) {
-        const int64_t row = b / nb;
-        const int blk = (int)(b - row * nb);
-        const int c = blk * 32 + l * VEC;
-        float v[VEC];
-        uint32_t m = 0;
-        if constexpr (VEC == 4) {
-            f32x4_t t = c < F ? *reinterpret_cast<const f32x4_t *>(x + row * ld_x + c) : f32x4_t{0.f, 0.f, 0.f, 0.f};
+    for (I b0 = (I)blockIdx.x * (U * PER) + threadIdx.x / LPB; b0 < total; b0 += (I)gridDim.x * (U * PER)) {
+        float v[U][VEC];
+        int64_t at[U];      // code of the first column
+        int c[U];
 #pragma unroll
-            for (int e = 0; e < 4; ++e) v[e] = t[e];
-        } else {
-            v[0] = c < F ? x[row * ld_x + c] : 0.f;
-        }
+        for (int u = 0; u < U; ++u) {
+            const I b = b0 + u * PER < total ? b0 + u * PER : total - 1;
+            const I row = b / nb;
+            c[u] = (int)(b - row * nb) * 32 + l * VEC;
+            at[u] = (int64_t)row * ld_c + c[u];
+            const float *p = x + (int64_t)row * ld_x;
+            if constexpr (VEC == 8) {
 #pragma unroll
-        for (int e = 0; e < VEC; ++e) m = max(m, __float_as_uint(v[e]) & 0x7fffffffu);
+                for (int h = 0; h < 2; ++h) {
+                    const bool in = c[u] + 4 * h < F;
+                    const f32x4_t t = *reinterpret_cast<const f32x4_t *>(p + (in ? c[u] + 4 * h : 0));
 #pragma unroll
-        for (int o = LPB / 2; o > 0; o >>= 1) m = max(m, (uint32_t)__shfl_xor((int)m, o, LPB));
-        const int ex = block_exp(m);
-        if constexpr (VEC == 4) {
-            uint32_t w = 0;
-            if (ex != 255) {
-#pragma unroll
-                for (int e = 0; e < 4; ++e) w |= ((uint32_t)code_of(v[e], ex) & 0xffu) << (8 * e);
+                    for (int e = 0; e < 4; ++e) v[u][4 * h + e] = in ? t[e] : 0.f;
+                }
+            } else {
+                v[u][0] = c[u] < F ? p[c[u]] : 0.f;
             }
-            if (c < ld_c) *reinterpret_cast<uint32_t *>(codes + row * ld_c + c) = w;
-        } else {
-            if (c < ld_c) codes[row * ld_c + c] = ex == 255 ? (int8_t)0 : (int8_t)code_of(v[0], ex);
         }
-        if (l == 0) exps[b] = (uint8_t)ex;
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const I b = b0 + u * PER;
+            uint32_t m = 0;
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) m = max(m, __float_as_uint(v[u][e]) & 0x7fffffffu);
+#pragma unroll
+            for (int o = LPB / 2; o > 0; o >>= 1) m = max(m, (uint32_t)__shfl_xor((int)m, o, LPB));
+            if (b >= total) continue;          // (whole blocks: the lanes of one agree)
+            const int ex = block_exp(m);
+            if constexpr (VEC == 8) {
+                uint32_t w[2] = {0u, 0u};
+                if (ex != 255) {
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) w[e >> 2] |= ((uint32_t)code_of(v[u][e], ex) & 0xffu) << (8 * (e & 3));
+                }
+                if (c[u] < ld_c) *reinterpret_cast<uint2 *>(codes + at[u]) = make_uint2(w[0], w[1]);
+            } else {
+                if (c[u] < ld_c) codes[at[u]] = ex == 255 ? (int8_t)0 : (int8_t)code_of(v[u][0], ex);
+            }
+            if (l == 0) exps[b] = (uint8_t)ex;
+        }
     }
 }
 
@@ -307,12 +323,21 @@ int magic_act8_pack(int64_t n_rows, int32_t n_cols, const float *x, int64_t ld_x
     if (!x || !codes || !exps || ld_x < n_cols || (uintptr_t)codes % 16) return MAGIC_ERR_INVALID_ARG;
     const int nb = (n_cols + 31) / 32;
     const int64_t ld_c = magic_act8_code_stride(n_cols);
-    if (n_cols % 4 == 0 && ld_x % 4 == 0 && (uintptr_t)x % 16 == 0)
-        MAGIC_LAUNCH("act8_pack", k_act8_pack<4>, magic::stride_grid(n_rows * nb, 32), 256, 0, (hipStream_t)stream, n_rows,
-                     n_cols, x, ld_x, codes, ld_c, exps, nb);
-    else
-        MAGIC_LAUNCH("act8_pack", k_act8_pack<1>, magic::stride_grid(n_rows * nb, 8), 256, 0, (hipStream_t)stream, n_rows,
-                     n_cols, x, ld_x, codes, ld_c, exps, nb);
+    hipStream_t st = (hipStream_t)stream;
+    const int64_t total = n_rows * nb;
+    const bool vec = n_cols % 4 == 0 && ld_x % 4 == 0 && (uintptr_t)x % 16 == 0;
+    const int grid = magic::stride_grid(total, vec ? 256 : 32);
+    if (total < (1 << 30)) {
+        if (vec)
+            MAGIC_LAUNCH("act8_pack", (k_act8_pack<8, uint32_t>), grid, 256, 0, st, (uint32_t)total, n_cols, x, ld_x, codes, ld_c, exps, (uint32_t)nb);
+        else
+            MAGIC_LAUNCH("act8_pack", (k_act8_pack<1, uint32_t>), grid, 256, 0, st, (uint32_t)total, n_cols, x, ld_x, codes, ld_c, exps, (uint32_t)nb);
+    } else {
+        if (vec)
+            MAGIC_LAUNCH("act8_pack", (k_act8_pack<8, int64_t>), grid, 256, 0, st, total, n_cols, x, ld_x, codes, ld_c, exps, (int64_t)nb);
+        else
+            MAGIC_LAUNCH("act8_pack", (k_act8_pack<1, int64_t>), grid, 256, 0, st, total, n_cols, x, ld_x, codes, ld_c, exps, (int64_t)nb);
+    }
     return magic::launch_status();
 }
 
