@@ -133,3 +133,38 @@ def head_norm_rope(q: torch.Tensor, k: torch.Tensor, q_weight: torch.Tensor, k_w
     float32 or bfloat16, any strides, head_dim up to 128, ``pos`` [n] int32.  Differentiable in q, k and the weights."""
     rotary_dim = q.shape[-1] if rotary_dim is None else int(rotary_dim)
     return _HeadNormRopeFn.apply(q, k, q_weight, k_weight, pos, rotary_dim, float(eps), float(base))
+
+
+class GlobalAttention(nn.Module):
+    """Every node attends the nodes of its own component graph: ``x + W_o attention(q, k, W_v x)`` with ``q, k`` = heads
+    of ``W_q x, W_k x`` after RMS norm and rotation by the node's position, scores capped at ``cap`` (0: not), and a
+    learned bias per head that falls with the distance of two positions.  ``W_o`` starts as zeros: the block is the
+    identity until it has learned something.
+
+    ``act_bits=8`` keeps the inputs of its linear layers for the backward pass as 8-bit codes (``act8.py``)."""
+
+    def __init__(self, dim: int, n_heads: int, cap: float = 50.0, act_bits: int = 32):
+        super().__init__()
+        if dim % n_heads or (dim // n_heads) % 8 or dim // n_heads > _lib.ATTN_MAX_DIM:
+            raise _lib.MagicHipError(f"head width {dim} / {n_heads} must be a multiple of 8 up to {_lib.ATTN_MAX_DIM}")
+        if act_bits not in (8, 32):
+            raise _lib.MagicHipError(f"act_bits must be 32 or 8 (got {act_bits})")
+        self.n_heads, self.head_dim, self.cap, self.act_bits = n_heads, dim // n_heads, float(cap), act_bits
+        self.qkv = nn.Linear(dim, 3 * dim, bias=False)
+        self.out = nn.Linear(dim, dim, bias=False)
+        self.q_weight = nn.Parameter(torch.ones(self.head_dim))
+        self.k_weight = nn.Parameter(torch.ones(self.head_dim))
+        # 1/8 of a unit of score per position down to 2^-11, from head to head
+        self.slopes = nn.Parameter(2.0 ** -torch.linspace(3.0, 11.0, n_heads))
+        nn.init.xavier_uniform_(self.qkv.weight)
+        nn.init.zeros_(self.out.weight)
+
+    def forward(self, graph: Graph, x: torch.Tensor, key_mask: Optional[torch.Tensor] = None) -> torch.Tensor:
+        """``key_mask`` [N] bool: nodes that may be attended (all when None)."""
+        n, dim = x.shape
+        plan, pos = graph.component_attention()
+        parts = linear_nobias(x, self.qkv.weight, self.act_bits).split(dim, dim=1)
+        q, k, v = (t.view(n, self.n_heads, self.head_dim) for t in parts)
+        q, k = head_norm_rope(q, k, self.q_weight, self.k_weight, pos)
+        o = segment_attention(q, k, v, plan, cap=self.cap, slopes=self.slopes, q_pos=pos, k_pos=pos, key_mask=key_mask)
+        return x + linear_nobias(o.view(n, dim), self.out.weight, self.act_bits)

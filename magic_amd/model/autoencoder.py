@@ -25,6 +25,7 @@ import torch.nn as nn
 from .. import _lib, ops  # noqa: F401  (ops registers torch.ops.magic.*)
 from ..graph import Graph
 from ..utils.utils import create_norm, sample_range
+from .attention import GlobalAttention
 from .fused import FusedCfg, FusedGMAEFn
 from .gat import GAT, _LinearFn, _pad_head_dim, fold_layers, linear_nobias
 from .loss_func import sce_loss, sce_loss_masked
@@ -35,7 +36,8 @@ def build_model(args):
     return GMAEModel(
         n_dim=args.n_dim, e_dim=args.e_dim, hidden_dim=args.num_hidden, n_layers=args.num_layers,
         n_heads=4, activation="prelu", feat_drop=0.1, negative_slope=args.negative_slope, residual=True,
-        mask_rate=args.mask_rate, norm="BatchNorm", loss_fn="sce", alpha_l=args.alpha_l)
+        mask_rate=args.mask_rate, norm="BatchNorm", loss_fn="sce", alpha_l=args.alpha_l,
+        global_attention=getattr(args, "global_attention", False), act_bits=getattr(args, "act_bits", 32))
 
 
 def _sorted_edge_keys(g: Graph) -> torch.Tensor:
@@ -128,11 +130,20 @@ class _EdgeHeadLossFn(torch.autograd.Function):
 
 
 class GMAEModel(nn.Module):
-    """``model/autoencoder.py:55-305``."""
+    """``model/autoencoder.py:55-305``.
+
+    Two options beyond the reference, off by default (same parameters, same numbers then): ``global_attention=True``
+    puts a ``GlobalAttention`` block behind the encoder's last layer (unmasked nodes are attended while training, all
+    nodes in ``embed``); ``act_bits=8`` keeps the inputs of that block's linear layers, of the edge head's first layer
+    and, on the layer-by-layer path, of ``encoder_to_decoder`` for the backward pass as 8-bit codes."""
 
     def __init__(self, n_dim, e_dim, hidden_dim, n_layers, n_heads, activation, feat_drop, negative_slope,
-                 residual, norm, mask_rate=0.5, loss_fn="sce", alpha_l=2, mask_rng="cpu", alias_clone=True):
+                 residual, norm, mask_rate=0.5, loss_fn="sce", alpha_l=2, mask_rng="cpu", alias_clone=True,
+                 global_attention=False, act_bits=32):
         super().__init__()
+        if act_bits not in (8, 32):
+            raise _lib.MagicHipError(f"act_bits must be 32 or 8 (got {act_bits})")
+        self.act_bits = act_bits
         self.alias_clone = alias_clone
         # run the first encoder layer on code words (node type, masked, dropout bits) when the input is known to
         # be one-hot node types; MAGIC_CODED_INPUT=0 (or this attribute) keeps the dense projection instead
@@ -170,6 +181,8 @@ class GMAEModel(nn.Module):
         self.enc_mask_token = nn.Parameter(torch.zeros(1, n_dim))
         self.encoder_to_decoder = nn.Linear(hidden_dim * n_layers, hidden_dim, bias=False)
         self.criterion = self.setup_loss_fn(loss_fn, alpha_l)
+        # (last: the parameters above are drawn as without it)
+        self.global_attn = GlobalAttention(hidden_dim, n_heads, act_bits=act_bits) if global_attention else None
 
     @property
     def output_hidden_dim(self):
@@ -233,7 +246,7 @@ class GMAEModel(nn.Module):
         that need padding inside the encoder, dense edge attributes ...)."""
         enc, dec = self.encoder.gats, self.decoder.gats
         etype = g.edge_types_csc()
-        if etype is None or len(dec) != 1 or not torch.is_grad_enabled():
+        if etype is None or len(dec) != 1 or not torch.is_grad_enabled() or self.global_attn is not None:
             return None
         H, D = enc[0].n_heads, enc[0].out_feat
         if _pad_head_dim(D) != D or (2 * H) % 4 != 0:
@@ -278,7 +291,7 @@ class GMAEModel(nn.Module):
             neg_valid = torch.as_tensor(neg_valid).to(pairs.device)
             if neg_valid.dtype not in (torch.bool, torch.uint8):
                 neg_valid = neg_valid != 0
-        h = linear_nobias(pairs, fc1.weight)                                   # (the bias joins in the tail)
+        h = linear_nobias(pairs, fc1.weight, self.act_bits)                    # (the bias joins in the tail)
         return _EdgeHeadLossFn.apply(h, fc1.bias, fc2.weight, fc2.bias, neg_valid, n_pos, act.negative_slope)
 
     def _edge_recon(self, pairs):
@@ -353,9 +366,15 @@ class GMAEModel(nn.Module):
         else:
             if drop_masks is not None:
                 raise NotImplementedError("injected dropout masks need the fused chain")
+            if drop_seeds is not None and pre_use_x.is_cuda and torch.cuda.is_current_stream_capturing():
+                raise NotImplementedError("a recorded step draws its dropout masks in the fused chain only")
             enc_rep, all_hidden = self.encoder(use_g, pre_use_x, return_hidden=True)
+            if self.global_attn is not None:
+                seen = torch.ones(g.num_nodes(), dtype=torch.bool, device=g.device)
+                seen.index_fill_(0, mask_nodes, False)
+                all_hidden[-1] = self.global_attn(use_g, all_hidden[-1], key_mask=seen)
             enc_rep = torch.cat(all_hidden, dim=1)
-            rep = linear_nobias(enc_rep, self.encoder_to_decoder.weight)   # autoencoder.py:237
+            rep = linear_nobias(enc_rep, self.encoder_to_decoder.weight, self.act_bits)   # autoencoder.py:237
             recon = recon_p = self.decoder(pre_use_g, rep)
             samples = enc_rep[sample_idx]
         # autoencoder.py:242-245: gather of the masked rows fused into the loss kernel
@@ -389,11 +408,14 @@ class GMAEModel(nn.Module):
     def embed(self, g: Graph):
         """``model/autoencoder.py:269-282``."""
         x = g.ndata["attr"].to(g.device)
-        return self.encoder(g, x, node_types=g.node_types_if_onehot() if self.coded_input else None)
+        h = self.encoder(g, x, node_types=g.node_types_if_onehot() if self.coded_input else None)
+        return h if self.global_attn is None else self.global_attn(g, h)
 
     @property
     def enc_params(self):
-        return self.encoder.parameters()
+        if self.global_attn is None:
+            return self.encoder.parameters()
+        return chain(self.encoder.parameters(), self.global_attn.parameters())
 
     @property
     def dec_params(self):

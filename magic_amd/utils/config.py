@@ -14,4 +14,9 @@ def build_args(argv=None):
     parser.add_argument("--optimizer", type=str, default="adam")
     parser.add_argument("--loss_fn", type=str, default="sce")
     parser.add_argument("--pooling", type=str, default="mean")
+    # beyond the reference (off by default): model/attention.py, model/act8.py
+    parser.add_argument("--global_attention", action="store_true",
+                        help="attention of every node over its own component graph behind the encoder")
+    parser.add_argument("--act_bits", type=int, default=32, choices=(8, 32),
+                        help="bits of the linear layers' inputs kept for the backward pass")
     return parser.parse_args(argv)
