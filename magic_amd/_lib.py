@@ -959,8 +959,8 @@ def _scratch(nbytes: int, device) -> torch.Tensor:
 def _head_rows(t: torch.Tensor) -> torch.Tensor:
     """[rows, heads, head_dim] operand with unit inner stride, other strides and address in whole 16 bytes."""
     per = 16 // t.element_size()
-    if t.stride(2) == 1 and t.stride(0) % per == 0 and t.stride(1) % per == 0 and t.data_ptr() % 16 == 0 \
-            and t.stride(0) <= ATTN_MAX_LD:
+    ld, hs, inner = t.stride()
+    if inner == 1 and ld % per == 0 and hs % per == 0 and ld <= ATTN_MAX_LD and t.data_ptr() % 16 == 0:
         return t
     t = t.contiguous()
     return t if t.data_ptr() % 16 == 0 else t.clone()
@@ -1014,47 +1014,59 @@ def attn_check(q, k, v, n_q, n_k, plan_device, cap, slopes, q_pos, k_pos, key_ma
 
 def _attn_args(q, k, v, plan, scale, cap, slopes, q_pos, k_pos, key_mask) -> MagicAttn:
     a = MagicAttn()
-    a.dtype, a.q_heads, a.kv_heads, a.head_dim = _ATTN_DTYPE[q.dtype], q.shape[1], k.shape[1], q.shape[2]
-    a.n_q, a.n_k = q.shape[0], k.shape[0]
-    a.q, a.ld_q, a.hs_q = q.data_ptr(), q.stride(0), q.stride(1)
-    a.k, a.ld_k, a.hs_k = k.data_ptr(), k.stride(0), k.stride(1)
-    a.v, a.ld_v, a.hs_v = v.data_ptr(), v.stride(0), v.stride(1)
-    a.scale, a.cap = float(scale), float(cap)
+    a.dtype = _ATTN_DTYPE[q.dtype]
+    a.n_q, a.q_heads, a.head_dim = q.shape
+    a.n_k, a.kv_heads, _ = k.shape
+    a.q, (a.ld_q, a.hs_q, _) = q.data_ptr(), q.stride()
+    a.k, (a.ld_k, a.hs_k, _) = k.data_ptr(), k.stride()
+    a.v, (a.ld_v, a.hs_v, _) = v.data_ptr(), v.stride()
+    a.scale, a.cap = scale, cap
     if slopes is not None:
         a.slopes, a.q_pos, a.k_pos = slopes.data_ptr(), q_pos.data_ptr(), k_pos.data_ptr()
     if key_mask is not None:
         a.key_mask = key_mask.data_ptr()
-    a.q_tiles, a.n_q_tiles = plan.q_tiles.data_ptr(), plan.q_tiles.shape[0]
-    a.k_tiles, a.n_k_tiles = plan.k_tiles.data_ptr(), plan.k_tiles.shape[0]
+    qt, kt = plan.q_tiles, plan.k_tiles
+    a.q_tiles, a.n_q_tiles = qt.data_ptr(), qt.shape[0]
+    a.k_tiles, a.n_k_tiles = kt.data_ptr(), kt.shape[0]
     a.max_q, a.max_k, a.n_seg = plan.max_q, plan.max_k, plan.n_seg
     return a
 
 
 def attn_operands(q, k, v, slopes, q_pos, k_pos, key_mask):
     """The operands as the kernels read them (copies only where strides or addresses ask for one)."""
-    c = lambda t: None if t is None else t.contiguous()  # noqa: E731
-    return _head_rows(q), _head_rows(k), _head_rows(v), c(slopes), c(q_pos), c(k_pos), c(key_mask)
+    if slopes is not None:
+        slopes, q_pos, k_pos = slopes.contiguous(), q_pos.contiguous(), k_pos.contiguous()
+    return (_head_rows(q), _head_rows(k), _head_rows(v), slopes, q_pos, k_pos,
+            None if key_mask is None else key_mask.contiguous())
 
 
 def attn_fwd(q, k, v, plan, scale: float, cap: float = 0.0, slopes=None, q_pos=None, k_pos=None, key_mask=None):
     """Segment attention forward: (out [n_q, q_heads, head_dim], lse [q_heads, n_q] float32)."""
-    lib = load()
     attn_check(q, k, v, plan.n_q, plan.n_k, plan.device, cap, slopes, q_pos, k_pos, key_mask)
-    q, k, v, slopes, q_pos, k_pos, key_mask = attn_operands(q, k, v, slopes, q_pos, k_pos, key_mask)
-    out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-    lse = torch.empty(q.shape[1], q.shape[0], dtype=torch.float32, device=q.device)
-    a = _attn_args(q, k, v, plan, scale, cap, slopes, q_pos, k_pos, key_mask)
-    with _on_device(q.device):
-        ws = _scratch(lib.magic_attn_fwd_workspace_bytes(C.byref(a)), q.device)
-        _check(lib.magic_attn_fwd(C.byref(a), out.data_ptr(), out.stride(0), out.stride(1), lse.data_ptr(), ws.data_ptr(),
-                                  ws.numel(), _stream()), "magic_attn_fwd")
+    return attn_fwd_checked(attn_operands(q, k, v, slopes, q_pos, k_pos, key_mask), plan, scale, cap)
+
+
+def attn_fwd_checked(operands, plan, scale, cap):
+    """``attn_fwd`` for operands that ``attn_operands`` returned and arguments that were checked."""
+    lib = load()
+    q = operands[0]
+    dev = q.device
+    n, h, d = q.shape
+    out = torch.empty((n, h, d), dtype=q.dtype, device=dev)
+    lse = torch.empty((h, n), dtype=torch.float32, device=dev)
+    a = _attn_args(q, operands[1], operands[2], plan, scale, cap, *operands[3:])
+    ref = C.byref(a)
+    with _on_device(dev):
+        nbytes = lib.magic_attn_fwd_workspace_bytes(ref)
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
+        _check(lib.magic_attn_fwd(ref, out.data_ptr(), h * d, d, lse.data_ptr(), ws.data_ptr(), nbytes, _stream()),
+               "magic_attn_fwd")
     return out, lse
 
 
 def attn_bwd(q, k, v, plan, scale: float, out, lse, d_out, cap: float = 0.0, slopes=None, q_pos=None, k_pos=None,
              key_mask=None, need_dq: bool = True, need_dkv: bool = True, need_dslopes: bool = False):
     """Gradients of ``attn_fwd``: (dq | None, dk | None, dv | None, d_slopes | None)."""
-    lib = load()
     attn_check(q, k, v, plan.n_q, plan.n_k, plan.device, cap, slopes, q_pos, k_pos, key_mask)
     _heads_check(d_out, "d_out", q)
     _heads_check(out, "out", q)
@@ -1063,19 +1075,32 @@ def attn_bwd(q, k, v, plan, scale: float, out, lse, d_out, cap: float = 0.0, slo
     if lse.shape != (q.shape[1], q.shape[0]) or lse.dtype != torch.float32 or not lse.is_contiguous() \
             or lse.device != q.device:
         raise MagicHipError("lse must be the float32 [q_heads, n_q] tensor of the forward pass")
-    q, k, v, slopes, q_pos, k_pos, key_mask = attn_operands(q, k, v, slopes, q_pos, k_pos, key_mask)
-    out, d_out = _head_rows(out), _head_rows(d_out)
+    ops = attn_operands(q, k, v, slopes, q_pos, k_pos, key_mask)
+    return attn_bwd_checked(ops, plan, scale, cap, _head_rows(out), lse, d_out, need_dq, need_dkv, need_dslopes)
+
+
+def attn_bwd_checked(operands, plan, scale, cap, out, lse, d_out, need_dq, need_dkv, need_dslopes):
+    """``attn_bwd`` for operands that ``attn_operands`` returned and arguments that were checked: what the autograd node
+    calls with the tensors of its forward pass."""
+    lib = load()
+    q, k, v, slopes, q_pos, k_pos, key_mask = operands
+    dev, dtype = q.device, q.dtype
+    d_out = _head_rows(d_out)
     need_dslopes = need_dslopes and slopes is not None
-    new = lambda t: torch.empty(t.shape, dtype=t.dtype, device=t.device)  # noqa: E731
-    dq = new(q) if need_dq or need_dslopes else None
-    dk, dv = (new(k), new(v)) if need_dkv else (None, None)
-    ds = torch.empty(q.shape[1], dtype=torch.float32, device=q.device) if need_dslopes else None
+    dq = torch.empty(q.shape, dtype=dtype, device=dev) if need_dq or need_dslopes else None
+    dk = torch.empty(k.shape, dtype=dtype, device=dev) if need_dkv else None
+    dv = torch.empty(v.shape, dtype=dtype, device=dev) if need_dkv else None
+    ds = torch.empty(q.shape[1], dtype=torch.float32, device=dev) if need_dslopes else None
     a = _attn_args(q, k, v, plan, scale, cap, slopes, q_pos, k_pos, key_mask)
-    with _on_device(q.device):
-        ws = _scratch(lib.magic_attn_bwd_workspace_bytes(C.byref(a)), q.device)
-        _check(lib.magic_attn_bwd(C.byref(a), out.data_ptr(), out.stride(0), out.stride(1), lse.data_ptr(),
-                                  d_out.data_ptr(), d_out.stride(0), d_out.stride(1), _dev(dq), _dev(dk), _dev(dv), _dev(ds),
-                                  ws.data_ptr(), ws.numel(), _stream()), "magic_attn_bwd")
+    ref = C.byref(a)
+    with _on_device(dev):
+        nbytes = lib.magic_attn_bwd_workspace_bytes(ref)
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
+        _check(lib.magic_attn_bwd(ref, out.data_ptr(), out.stride(0), out.stride(1), lse.data_ptr(), d_out.data_ptr(),
+                                  d_out.stride(0), d_out.stride(1), dq.data_ptr() if dq is not None else None,
+                                  dk.data_ptr() if need_dkv else None, dv.data_ptr() if need_dkv else None,
+                                  ds.data_ptr() if need_dslopes else None, ws.data_ptr(), nbytes, _stream()),
+               "magic_attn_bwd")
     return dq, dk, dv, ds
 
 
@@ -1118,12 +1143,17 @@ def head_norm_rope_fwd(q, k, wq, wk, pos, rotary_dim: int, eps: float, base: flo
 
 def head_norm_rope_bwd(q, k, wq, wk, pos, rotary_dim: int, eps: float, base: float, dyq, dyk):
     """(dq, dk, dwq, dwk) of ``head_norm_rope_fwd``."""
-    lib = load()
     _head_norm_check(q, k, wq, wk, pos, rotary_dim, eps, base)
     _heads_check(dyq, "dyq", q)
     _heads_check(dyk, "dyk", q)
     if dyq.shape != q.shape or dyk.shape != k.shape:
         raise MagicHipError("the gradients must have the shapes of the outputs")
+    return head_norm_rope_bwd_checked(q, k, wq, wk, pos, rotary_dim, eps, base, dyq, dyk)
+
+
+def head_norm_rope_bwd_checked(q, k, wq, wk, pos, rotary_dim, eps, base, dyq, dyk):
+    """``head_norm_rope_bwd`` for arguments that were checked (the autograd node's)."""
+    lib = load()
     q, k, wq, wk, pos = _unit_inner(q), _unit_inner(k), wq.contiguous(), wk.contiguous(), pos.contiguous()
     dyq, dyk = _unit_inner(dyq), _unit_inner(dyk)
     dev = q.device

@@ -21,6 +21,11 @@ struct BwdArgs {
     void *dq, *dk, *dv;
     double *slope_part; // [n_q tiles][q_heads] or NULL
     int64_t items;
+    int sub;            // blocks that share a 128-row tile of the table
+    bool make_delta;    // the dq sweep forms lse2 and delta (no pass before it needs them)
+    uint32_t sweep_blocks;   // of the dk / dv sweep; blocks behind them: d slope of one head each, from n_slope sums
+    int64_t n_slope;
+    float *dslopes;
     Prepared pr;
     int n_split;        // shares of the rows a key tile's sums are cut into (1: they go straight to dk / dv)
     float *part;        // [n_split][dk | dv][n_k][kv_heads][head_dim]
@@ -107,6 +112,20 @@ struct Running {
     __device__ __forceinline__ float undo() const { return u == 0.f ? 0.f : 1.f / u; }
 };
 
+// d slope of head h: the tiles' sums, fixed tree (a block of up to four wavefronts)
+__device__ __forceinline__ void sum_slope(const double *part, int64_t n, int H, int h, float *out, double *red) {
+    double s = 0.0;
+    for (int64_t i = threadIdx.x; i < n; i += blockDim.x) s += part[i * H + h];
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) s += __shfl_xor(s, o, 64);
+    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = s;
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        for (int w = 1; w < (int)blockDim.x / 64; ++w) s += red[w];
+        out[h] = (float)s;
+    }
+}
+
 // What a lane knows of its row in the dq sweep
 struct RowSide {
     float s_in, dp_in, scale, cap, f_cap, slope;   // f_cap: -scale / cap^2, for scale (1 - tanh^2) from the capped score
@@ -180,13 +199,14 @@ __device__ __forceinline__ void prob_grad(f32x16_t &s, const f32x16_t &dp, const
     }
 }
 
-constexpr int NT = 256;
 
-template <typename M, int DP, int BK>
-__global__ __launch_bounds__(NT, (DP == 128 && M::N > 1) ? 1 : 2) void k_attn_dq(BwdArgs p) {
+// WM groups of 32 rows, KG groups of 32 keys of a staged tile: a block of WM * KG wavefronts
+template <typename M, int DP, int WM, int KG>
+__global__ __launch_bounds__(64 * WM *KG, (DP == 128 && M::N > 1) || (DP >= 64 && KG > 1) ? 1 : 2) void k_attn_dq(BwdArgs p) {
     typedef typename M::T T;
     typedef typename M::vec vec;
-    constexpr int NP = M::N, KS = DP / 16, DB = (DP + 31) / 32;
+    constexpr int NP = M::N, KS = DP / 16, DB = (DP + 31) / 32, BK = 32 * KG, NT = 64 * WM * KG;
+    static_assert(KG == 1 || !M::SCALED, "the key groups' sums are joined in one unit");
     typedef Stage<M, DP, BK, NT> stage;
     typedef Tile<M, DP, BK> tile;
     extern __shared__ __align__(16) unsigned char smem[];
@@ -198,17 +218,28 @@ __global__ __launch_bounds__(NT, (DP == 128 && M::N > 1) ? 1 : 2) void k_attn_dq
     const int64_t item = xcd_item(blockIdx.x, 16);
     if (item >= p.items) return;
     const int D = a.head_dim, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, li = lane & 31, hf = lane >> 5;
-    const int64_t tl = item % a.n_q_tiles;
-    const int h = (int)(item / a.n_q_tiles), hk = h / (a.q_heads / a.kv_heads);
-    const int32_t *t = a.q_tiles + TAB * tl;
-    const int64_t q0 = t[0], k0 = t[2];
-    const int nq = t[1], nk = t[3] > 0 && p.pr.cnt ? p.pr.cnt[t[4]] : t[3];
-    const int row = wave * 32 + li;
+    const int wm = wave % WM, kg = wave / WM;
+    const int64_t per_h = (int64_t)a.n_q_tiles * p.sub, tl = item % per_h;
+    const int h = (int)(item / per_h), hk = h / (a.q_heads / a.kv_heads);
+    const int32_t *t = a.q_tiles + TAB * (tl / p.sub);
+    const int first = (int)(tl % p.sub) * 32 * WM, nq = t[1] - first;      // this block's rows of the table's tile
+    if (nq <= 0) {
+        if (p.slope_part && tid == 0) p.slope_part[tl * a.q_heads + h] = 0.0;
+        return;
+    }
+    const int64_t q0 = (int64_t)t[0] + first, k0 = t[2];
+    const int nk = t[3] > 0 && p.pr.cnt ? p.pr.cnt[t[4]] : t[3];
+    const int row = wm * 32 + li;
     const bool ok = row < nq;
     const int64_t qr = q0 + (ok ? row : 0);
     const Src<M> K = src_of<M>(a.k, a.ld_k, a.hs_k, p.pr.k, k0, hk, D),
                  V = src_of<M>(a.v, a.ld_v, a.hs_v, p.pr.v, k0, hk, D);
-    const float ls = ok ? p.lse2[(int64_t)h * a.n_q + qr] : INFINITY, dl0 = ok ? p.delta[(int64_t)h * a.n_q + qr] : 0.f;
+    float ls = INFINITY, dl0 = 0.f;
+    if (ok) {
+        ls = (p.make_delta ? p.lse : p.lse2)[(int64_t)h * a.n_q + qr];
+        if (ls == -INFINITY) ls = INFINITY;
+        if (!p.make_delta) dl0 = p.delta[(int64_t)h * a.n_q + qr];
+    }
     const bool live = ls != INFINITY;
 
     Scales sc;
@@ -222,8 +253,21 @@ __global__ __launch_bounds__(NT, (DP == 128 && M::N > 1) ? 1 : 2) void k_attn_dq
         g.load((const T *)p.dout + qr * p.ld_do + h * p.hs_do + cc);
         if (!ok || c >= D) r.zero();
         if (!live || c >= D) g.zero();
+        if (p.make_delta) {
+            float x[8], y[8];
+            Raw<T> o;
+            o.load((const T *)p.out + qr * p.ld_o + h * p.hs_o + cc);
+            if (!live || c >= D) o.zero();
+            o.floats(x), g.floats(y);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) dl0 += x[e] * y[e];
+        }
         r.planes(qf[ks], sc.q);
         g.planes(gf[ks], sc.g);
+    }
+    if (p.make_delta) {      // what the dk / dv sweep reads
+        dl0 += other_half(dl0);
+        if (ok && hf == 0 && kg == 0) p.lse2[(int64_t)h * a.n_q + qr] = ls, p.delta[(int64_t)h * a.n_q + qr] = dl0;
     }
     const bool bias = a.slopes != nullptr;
     const float slope = bias ? a.slopes[h] : 0.f;
@@ -237,7 +281,7 @@ __global__ __launch_bounds__(NT, (DP == 128 && M::N > 1) ? 1 : 2) void k_attn_dq
 #pragma unroll
         for (int r = 0; r < 16; ++r) acc[d][r] = 0.f;
 
-    uint32_t plain = tile::lane_plain(lane), turned = tile::lane_turned(lane);
+    uint32_t plain = tile::lane_plain(lane) + 64u * kg * tile::W, turned = tile::lane_turned(lane) + 64u * kg * tile::W;
     stage kst, vst;
     kst.init(K, D, tid), vst.init(V, D, tid);
     uint8_t keep[stage::N];
@@ -268,8 +312,8 @@ __global__ __launch_bounds__(NT, (DP == 128 && M::N > 1) ? 1 : 2) void k_attn_dq
         if (tid < BK) sPos[tid] = flip(pos), sMask[tid] = mk ? 0.f : -INFINITY;
         __syncthreads();
         if (j0 + BK < nk) load(j0 + BK);
-#pragma unroll 1
-        for (int b = 0; b < BK / 32; ++b) {
+        {
+            const int b = kg;
             stay(plain), stay(turned);
             f32x16_t s, dp;
 #pragma unroll
@@ -277,8 +321,8 @@ __global__ __launch_bounds__(NT, (DP == 128 && M::N > 1) ? 1 : 2) void k_attn_dq
 #pragma unroll
             for (int ks = 0; ks < KS; ++ks) {
                 vec f[NP], g[NP];
-                tile::frag(sK, plain, 32 * b, ks, f);
-                tile::frag(sV, plain, 32 * b, ks, g);
+                tile::frag(sK, plain, 0, ks, f);
+                tile::frag(sV, plain, 0, ks, g);
                 mma(s, f, qf[ks]);
                 mma(dp, g, gf[ks]);
             }
@@ -313,15 +357,39 @@ __global__ __launch_bounds__(NT, (DP == 128 && M::N > 1) ? 1 : 2) void k_attn_dq
 #pragma unroll
                 for (int d = 0; d < DB; ++d) {
                     vec f[NP];
-                    tile::frag_t(sK, turned, 32 * b + 16 * w, d, f);
+                    tile::frag_t(sK, turned, 16 * w, d, f);
                     mma(acc[d], f, pf);
                 }
             }
             feed<2 * NP, PRODUCTS<M>, 2 * DB>();
         }
     }
+    if constexpr (KG > 1) {      // the key groups' sums come together through LDS, in group order
+        float *so = reinterpret_cast<float *>(smem);
+        constexpr int OW = DB * 32 + 1;
+#pragma unroll
+        for (int g = KG - 1; g >= 1; --g) {
+            __syncthreads();
+            if (kg == g) {
+#pragma unroll
+                for (int d = 0; d < DB; ++d)
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) {
+                        float *q = so + (wm * 32 + li) * OW + 32 * d + 8 * (r >> 2) + 4 * hf + (r & 3);
+                        *q = g == KG - 1 ? acc[d][r] : *q + acc[d][r];
+                    }
+            }
+        }
+        __syncthreads();
+        if (kg == 0) {
+#pragma unroll
+            for (int d = 0; d < DB; ++d)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) acc[d][r] += so[(wm * 32 + li) * OW + 32 * d + 8 * (r >> 2) + 4 * hf + (r & 3)];
+        }
+    }
     const float undo = M::SCALED ? run.undo() * (1.f / sc.k) : 1.f;
-    if (ok) {
+    if (ok && kg == 0) {
         T *o = (T *)p.dq + (qr * a.q_heads + h) * D;
 #pragma unroll
         for (int d = 0; d < DB; ++d)
@@ -334,22 +402,33 @@ __global__ __launch_bounds__(NT, (DP == 128 && M::N > 1) ? 1 : 2) void k_attn_dq
     }
     if (p.slope_part) {
         __syncthreads();
-        double *red = reinterpret_cast<double *>(smem);
-        sums.dl += __shfl_xor(sums.dl, 32, 64);
-        double dsl = sums.dl * sums.pd - sums.dl_dist;          // (either half's share of sum p dist)
+        double *red = reinterpret_cast<double *>(smem), *sdl = red + WM * KG;
+        sdl[wave * 64 + lane] = sums.dl;
+        __syncthreads();
+        double all = 0.0;                    // sum dl of the lane's row: both halves, all key groups
+#pragma unroll
+        for (int g = 0; g < KG; ++g) all += sdl[(g * WM + wm) * 64 + li] + sdl[(g * WM + wm) * 64 + li + 32];
+        double dsl = all * sums.pd - sums.dl_dist;          // (with this lane's share of sum p dist)
 #pragma unroll
         for (int k = 32; k > 0; k >>= 1) dsl += __shfl_xor(dsl, k, 64);
         if (lane == 0) red[wave] = dsl;
         __syncthreads();
-        if (tid == 0) p.slope_part[tl * a.q_heads + h] = (red[0] + red[1]) + (red[2] + red[3]);
+        if (tid == 0) {
+            double x = 0.0;
+#pragma unroll
+            for (int w = 0; w < WM * KG; ++w) x += red[w];
+            p.slope_part[tl * a.q_heads + h] = x;
+        }
     }
 }
 
-template <typename M, int DP, int BQ>
-__global__ __launch_bounds__(NT, DP == 128 ? 1 : 2) void k_attn_dkv(BwdArgs p) {
+// WM groups of 32 keys, KG groups of 32 NB rows of a staged tile.  The blocks behind the sweep's add up the slopes' sums.
+template <typename M, int DP, int WM, int KG, int NB>
+__global__ __launch_bounds__(64 * WM *KG, DP == 128 || (DP >= 64 && KG > 1) ? 1 : 2) void k_attn_dkv(BwdArgs p) {
     typedef typename M::T T;
     typedef typename M::vec vec;
-    constexpr int NP = M::N, KS = DP / 16, DB = (DP + 31) / 32;
+    constexpr int NP = M::N, KS = DP / 16, DB = (DP + 31) / 32, BQ = 32 * KG * NB, NT = 64 * WM * KG;
+    static_assert(KG == 1 || !M::SCALED, "the row groups' sums are joined in one unit");
     typedef Stage<M, DP, BQ, NT> stage;
     typedef Tile<M, DP, BQ> tile;
     extern __shared__ __align__(16) unsigned char smem[];
@@ -358,17 +437,23 @@ __global__ __launch_bounds__(NT, DP == 128 ? 1 : 2) void k_attn_dkv(BwdArgs p) {
     uint32_t *sPos = reinterpret_cast<uint32_t *>(sD + BQ);
 
     const magic_attn &a = p.a;
+    if (blockIdx.x >= p.sweep_blocks) {
+        sum_slope(p.slope_part, p.n_slope, a.q_heads, blockIdx.x - p.sweep_blocks, p.dslopes, reinterpret_cast<double *>(smem));
+        return;
+    }
     const int64_t item = xcd_item(blockIdx.x, 16);
     if (item >= p.items) return;
     const int D = a.head_dim, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, li = lane & 31, hf = lane >> 5;
-    const int64_t tl = item % a.n_k_tiles;
-    const int hk = (int)(item / a.n_k_tiles % a.kv_heads), G = a.q_heads / a.kv_heads;
-    const int split = (int)(item / ((int64_t)a.n_k_tiles * a.kv_heads));
-    const int32_t *t = a.k_tiles + TAB * tl;
-    const int64_t k0 = t[0], q0 = t[2];
-    const int nk = p.pr.cnt ? min(t[1], p.pr.cnt[t[4]] - (t[0] - t[5])) : t[1], nq = t[3];
+    const int wm = wave % WM, kg = wave / WM;
+    const int64_t tiles = (int64_t)a.n_k_tiles * p.sub, tl = item % tiles;
+    const int hk = (int)(item / tiles % a.kv_heads), G = a.q_heads / a.kv_heads;
+    const int split = (int)(item / (tiles * a.kv_heads));
+    const int32_t *t = a.k_tiles + TAB * (tl / p.sub);
+    const int first = (int)(tl % p.sub) * 32 * WM;                         // this block's keys of the table's tile
+    const int64_t k0 = (int64_t)t[0] + first, q0 = t[2];
+    const int nk = (p.pr.cnt ? min(t[1], p.pr.cnt[t[4]] - (t[0] - t[5])) : t[1]) - first, nq = t[3];
     if (nk <= 0) return;                     // (all unmasked keys of the segment are in the tiles before)
-    const int col = wave * 32 + li;
+    const int col = wm * 32 + li;
     const bool in = col < nk;
     const int64_t kr = p.pr.idx ? p.pr.idx[k0 + (in ? col : 0)] : k0 + (in ? col : 0);
     const bool ok = in && (p.pr.idx || !a.key_mask || a.key_mask[kr]);
@@ -433,7 +518,8 @@ __global__ __launch_bounds__(NT, DP == 128 ? 1 : 2) void k_attn_dkv(BwdArgs p) {
         if (++it == per_h) it = 0, ++h;
         if (st + 1 < s_end) load(h, it * BQ);
 #pragma unroll 1
-        for (int b = 0; b < BQ / 32; ++b) {
+        for (int nb = 0; nb < NB; ++nb) {
+            const int b = kg * NB + nb;
             stay(plain), stay(turned);
             f32x16_t s, dp;
 #pragma unroll
@@ -480,6 +566,25 @@ __global__ __launch_bounds__(NT, DP == 128 ? 1 : 2) void k_attn_dkv(BwdArgs p) {
             }
             feed<2 * NP, PRODUCTS<M>, 4 * DB>();
         }
+    }
+    if constexpr (KG > 1) {      // the row groups' sums come together through LDS, in group order
+        float *so = reinterpret_cast<float *>(smem);
+        constexpr int OW = 2 * DB * 32 + 1;
+#pragma unroll
+        for (int g = KG - 1; g >= 0; --g) {
+            __syncthreads();
+            if (kg == g) {
+#pragma unroll
+                for (int d = 0; d < DB; ++d)
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) {
+                        float *q = so + (wm * 32 + li) * OW + 64 * d + 8 * (r >> 2) + 4 * hf + (r & 3);
+                        if (g < KG - 1) gk[d][r] += q[0], gv[d][r] += q[32];
+                        if (g > 0) q[0] = gk[d][r], q[32] = gv[d][r];
+                    }
+            }
+        }
+        if (kg != 0) return;
     }
     if (!in) return;
     const float uk = M::SCALED ? run.undo() * (1.f / sc.q) : 1.f, uv = M::SCALED ? 1.f / 16384.f * (1.f / sc.g) : 1.f;
@@ -543,47 +648,88 @@ template <typename T> __global__ __launch_bounds__(256) void k_attn_dkv_masked(B
     }
 }
 
-// d slope of a head: the tile sums lane by lane, fixed tree, in double
-__global__ __launch_bounds__(64) void k_attn_dslope(const double *part, int n, int H, float *out) {
-    double s = 0.0;
-    for (int i = threadIdx.x; i < n; i += 64) s += part[(int64_t)i * H + blockIdx.x];
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1) s += __shfl_xor(s, o, 64);
-    if (threadIdx.x == 0) out[blockIdx.x] = (float)s;
+// d slope of a head where no dk / dv sweep runs
+__global__ __launch_bounds__(256) void k_attn_dslope(const double *part, int64_t n, int H, float *out) {
+    __shared__ double red[4];
+    sum_slope(part, n, H, blockIdx.x, out, red);
 }
 
-// rows of a staged tile: the ones that leave the kernels without register spills
-template <typename M, int DP> constexpr int BK_OF = 32;
-template <typename M, int DP> constexpr int BQ_OF = DP == 128 && M::N == 1 ? 64 : 32;
-
-template <typename M, int DP> int sweeps(BwdArgs &b, hipStream_t st) {
-    const magic_attn full = b.a, a = full;
-    constexpr int BK = BK_OF<M, DP>, BQ = BQ_OF<M, DP>;
-    b.a = gathered(&full, b.pr);
-    if (a.n_q > 0 && b.dq) {
-        const size_t lds = 2 * Tile<M, DP, BK>::BYTES + BK * 8;
-        if (magic::ensure_dynamic_lds((const void *)k_attn_dq<M, DP, BK>, lds) != MAGIC_OK) return MAGIC_ERR_RUNTIME;
-        b.items = (int64_t)a.n_q_tiles * a.q_heads;
-        if (xcd_grid(b.items, 16) > 0x7fffffffLL) return MAGIC_ERR_UNSUPPORTED;
-        MAGIC_LAUNCH(M::SCALED ? "attn_bwd_dq_f16x2" : "attn_bwd_dq", (k_attn_dq<M, DP, BK>), (int)xcd_grid(b.items, 16), NT,
-                     lds, st, b);
-    }
-    if (a.n_k > 0 && b.dk) {
-        b.a = full;                // (a key's own rows are read where they are)
-        const size_t lds = 2 * Tile<M, DP, BQ>::BYTES + BQ * 12;
-        if (magic::ensure_dynamic_lds((const void *)k_attn_dkv<M, DP, BQ>, lds) != MAGIC_OK) return MAGIC_ERR_RUNTIME;
-        b.items = (int64_t)a.n_k_tiles * a.kv_heads * b.n_split;
-        if (xcd_grid(b.items, 16) > 0x7fffffffLL) return MAGIC_ERR_UNSUPPORTED;
-        MAGIC_LAUNCH(M::SCALED ? "attn_bwd_dkv_f16x2" : "attn_bwd_dkv", (k_attn_dkv<M, DP, BQ>), (int)xcd_grid(b.items, 16), NT,
-                     lds, st, b);
-    }
-    b.a = full;
+template <typename M, int DP, int WM, int KG> int run_dq(BwdArgs &b, hipStream_t st) {
+    size_t lds = 2 * Tile<M, DP, 32 * KG>::BYTES + 32 * KG * 8;
+    const size_t sums = (size_t)WM * KG * 65 * 8, join = (size_t)32 * WM * ((DP + 31) / 32 * 32 + 1) * 4;
+    if (lds < sums) lds = sums;
+    if (KG > 1 && lds < join) lds = join;
+    if (magic::ensure_dynamic_lds((const void *)k_attn_dq<M, DP, WM, KG>, lds) != MAGIC_OK) return MAGIC_ERR_RUNTIME;
+    b.items = (int64_t)b.a.n_q_tiles * b.sub * b.a.q_heads;
+    if (xcd_grid(b.items, 16) > 0x7fffffffLL) return MAGIC_ERR_UNSUPPORTED;
+    MAGIC_LAUNCH(M::SCALED ? "attn_bwd_dq_f16x2" : "attn_bwd_dq", (k_attn_dq<M, DP, WM, KG>), (int)xcd_grid(b.items, 16),
+                 64 * WM * KG, lds, st, b);
     return magic::launch_status();
 }
 
-template <typename M> int sweeps_of(BwdArgs &b, hipStream_t st) {
+template <typename M, int DP, int WM, int KG, int NB> int run_dkv(BwdArgs &b, int slope_heads, hipStream_t st) {
+    constexpr int BQ = 32 * KG * NB;
+    size_t lds = 2 * Tile<M, DP, BQ>::BYTES + BQ * 12;
+    const size_t join = (size_t)32 * WM * (2 * ((DP + 31) / 32 * 32) + 1) * 4;
+    if (KG > 1 && lds < join) lds = join;
+    if (magic::ensure_dynamic_lds((const void *)k_attn_dkv<M, DP, WM, KG, NB>, lds) != MAGIC_OK) return MAGIC_ERR_RUNTIME;
+    b.items = (int64_t)b.a.n_k_tiles * b.sub * b.a.kv_heads * b.n_split;
+    const int64_t grid = xcd_grid(b.items, 16);
+    if (grid + slope_heads > 0x7fffffffLL) return MAGIC_ERR_UNSUPPORTED;
+    b.sweep_blocks = (uint32_t)grid;
+    MAGIC_LAUNCH(M::SCALED ? "attn_bwd_dkv_f16x2" : "attn_bwd_dkv", (k_attn_dkv<M, DP, WM, KG, NB>), (int)grid + slope_heads,
+                 64 * WM * KG, lds, st, b);
+    return magic::launch_status();
+}
+
+// 32 rows a block where tiles of 128 would leave most of the chip idle: the wavefronts share the rows and deal out the keys
+bool small_side(int64_t blocks) { return blocks < 256; }
+
+int sub_tiles(int64_t tiles, int heads, int longest) {
+    if (!small_side(tiles * heads)) return 1;
+    const int rows = longest < MAGIC_ATTN_TILE ? longest : MAGIC_ATTN_TILE;
+    return rows > 32 ? (rows + 31) / 32 : 1;
+}
+
+template <typename M, int DP> int sweeps(BwdArgs &b, bool last, hipStream_t st) {
+    const magic_attn full = b.a;
+    constexpr int KG = DP == 128 && M::N == 3 ? 2 : 4;      // (three planes of 128 rows and columns would not fit the LDS)
+    int rc = MAGIC_OK;
+    if (full.n_q > 0 && b.dq) {
+        b.a = gathered(&full, b.pr);
+        b.sub = sub_tiles(full.n_q_tiles, full.q_heads, full.max_q);
+        if constexpr (M::SCALED) {
+            b.sub = 1;
+            rc = run_dq<M, DP, 4, 1>(b, st);
+        } else {
+            const bool few = !b.pr.rg.q && small_side((int64_t)full.n_q_tiles * full.q_heads);
+            if (!few) b.sub = 1;
+            rc = few ? run_dq<M, DP, 1, KG>(b, st) : run_dq<M, DP, 4, 1>(b, st);
+        }
+        b.n_slope = (int64_t)full.n_q_tiles * b.sub;
+    }
+    b.a = full;                    // (a key's own rows are read where they are)
+    if (rc == MAGIC_OK && full.n_k > 0 && b.dk) {
+        const int slopes = last && b.slope_part ? full.q_heads : 0;
+        b.sub = 1;
+        constexpr int NB = DP == 128 && M::N == 1 ? 2 : 1;  // (one more block of rows a step where registers allow it)
+        if constexpr (M::SCALED) {
+            rc = run_dkv<M, DP, 4, 1, NB>(b, slopes, st);
+        } else {
+            const bool few = !b.pr.rg.q && b.n_split == 1 && small_side((int64_t)full.n_k_tiles * full.kv_heads);
+            if (few) b.sub = sub_tiles(full.n_k_tiles, full.kv_heads, full.max_k);
+            rc = few ? run_dkv<M, DP, 1, KG, 1>(b, slopes, st) : run_dkv<M, DP, 4, 1, NB>(b, slopes, st);
+        }
+    }
+    return rc;
+}
+
+template <typename M> int sweeps_of(BwdArgs &b, bool last, hipStream_t st) {
     const int D = b.a.head_dim;
-    return D <= 16 ? sweeps<M, 16>(b, st) : D <= 32 ? sweeps<M, 32>(b, st) : D <= 64 ? sweeps<M, 64>(b, st) : sweeps<M, 128>(b, st);
+    return D <= 16   ? sweeps<M, 16>(b, last, st)
+           : D <= 32 ? sweeps<M, 32>(b, last, st)
+           : D <= 64 ? sweeps<M, 64>(b, last, st)
+                     : sweeps<M, 128>(b, last, st);
 }
 
 template <typename T, int DP> int delta(BwdArgs &b, hipStream_t st) {
@@ -616,7 +762,7 @@ size_t magic_attn_bwd_workspace_bytes(const magic_attn *a) {
     const int n = splits(a);
     const size_t part = n > 1 ? (size_t)n * 2 * a->n_k * a->kv_heads * a->head_dim * sizeof(float) : 0;
     return magic::align_up(part) + prepare_bytes(a, use_f16(a), true) + 2 * magic::align_up((size_t)a->n_q * a->q_heads * sizeof(float)) +
-           magic::align_up((size_t)a->n_q_tiles * a->q_heads * sizeof(double)) + 256;
+           magic::align_up((size_t)a->n_q_tiles * 4 * a->q_heads * sizeof(double)) + 256;
 }
 
 int magic_attn_bwd(const magic_attn *a, const void *out, int64_t ld_out, int64_t hs_out, const float *lse, const void *d_out,
@@ -635,11 +781,12 @@ int magic_attn_bwd(const magic_attn *a, const void *out, int64_t ld_out, int64_t
     BwdArgs b;
     b.a = *a;
     b.out = out, b.dout = d_out, b.ld_o = ld_out, b.hs_o = hs_out, b.ld_do = ld_do, b.hs_do = hs_do;
-    b.lse = lse, b.dq = dq, b.dk = dk, b.dv = dv;
+    b.lse = lse, b.dq = dq, b.dk = dk, b.dv = dv, b.dslopes = d_slopes;
+    b.n_slope = 0, b.sub = 1, b.sweep_blocks = 0;
     magic::Arena ar(workspace, workspace_bytes);
     b.delta = ar.take<float>((size_t)a->n_q * a->q_heads);
     b.lse2 = ar.take<float>((size_t)a->n_q * a->q_heads);
-    b.slope_part = ar.take<double>((size_t)a->n_q_tiles * a->q_heads);
+    b.slope_part = ar.take<double>((size_t)a->n_q_tiles * 4 * a->q_heads);
     const bool f16 = use_f16(a) && a->n_q > 0 && a->n_k > 0;
     b.n_split = dk ? splits(a) : 1;
     b.part = b.n_split > 1 ? ar.take<float>((size_t)b.n_split * 2 * a->n_k * a->kv_heads * a->head_dim) : nullptr;
@@ -647,7 +794,8 @@ int magic_attn_bwd(const magic_attn *a, const void *out, int64_t ld_out, int64_t
     if (!d_slopes) b.slope_part = nullptr;
     const bool f32 = a->dtype == MAGIC_F32;
     int rc = MAGIC_OK;
-    if (a->n_q > 0) rc = f32 ? delta_of<float>(b, stream) : delta_of<bf16_t>(b, stream);
+    b.make_delta = dq && !f16;      // (the planes of the scaled launches are zero where lse2 says so: they need it before)
+    if (a->n_q > 0 && !b.make_delta) rc = f32 ? delta_of<float>(b, stream) : delta_of<bf16_t>(b, stream);
     if (rc != MAGIC_OK) return rc;
     if (a->n_q > 0 && a->n_k > 0) {
         const GradRows g = {d_out, ld_do, hs_do, b.lse2};
@@ -655,11 +803,11 @@ int magic_attn_bwd(const magic_attn *a, const void *out, int64_t ld_out, int64_t
         if (rc != MAGIC_OK) return rc;
     }
     if (f16) {
-        rc = sweeps_of<F16x2>(b, stream);
+        rc = sweeps_of<F16x2>(b, false, stream);
         if (rc != MAGIC_OK) return rc;
         b.pr.rg.want_safe = false;             // the segments whose rows differ too much in size
     }
-    rc = f32 ? sweeps_of<F32x3>(b, stream) : sweeps_of<BF16>(b, stream);
+    rc = f32 ? sweeps_of<F32x3>(b, true, stream) : sweeps_of<BF16>(b, true, stream);
     if (rc != MAGIC_OK) return rc;
     if (b.n_split == 1 && dk && b.pr.idx) {
         const int grid = magic::stride_grid(a->n_k * a->kv_heads * a->head_dim / 8, 256);
@@ -675,9 +823,8 @@ int magic_attn_bwd(const magic_attn *a, const void *out, int64_t ld_out, int64_t
         else
             MAGIC_LAUNCH("attn_dkv_join", k_attn_dkv_join<bf16_t>, grid, 256, 0, stream, b);
     }
-    if (d_slopes)
-        MAGIC_LAUNCH("attn_bwd_dslope", k_attn_dslope, a->q_heads, 64, 0, stream, b.slope_part, a->n_q > 0 ? a->n_q_tiles : 0,
-                     a->q_heads, d_slopes);
+    if (d_slopes && !(dk && a->n_k > 0))
+        MAGIC_LAUNCH("attn_bwd_dslope", k_attn_dslope, a->q_heads, 256, 0, stream, b.slope_part, b.n_slope, a->q_heads, d_slopes);
     return magic::launch_status();
 }
 

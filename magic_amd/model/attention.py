@@ -77,18 +77,20 @@ def attention_plan(q_lens: Sequence[int], kv_lens: Optional[Sequence[int]] = Non
 class _SegmentAttentionFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, v, slopes, plan, scale, cap, q_pos, k_pos, key_mask):
-        out, lse = _lib.attn_fwd(q, k, v, plan, scale, cap, slopes, q_pos, k_pos, key_mask)
-        ctx.save_for_backward(q, k, v, slopes, q_pos, k_pos, key_mask, out, lse)
+        _lib.attn_check(q, k, v, plan.n_q, plan.n_k, plan.device, cap, slopes, q_pos, k_pos, key_mask)
+        operands = _lib.attn_operands(q, k, v, slopes, q_pos, k_pos, key_mask)
+        out, lse = _lib.attn_fwd_checked(operands, plan, scale, cap)
+        ctx.save_for_backward(*operands, out, lse)
         ctx.plan, ctx.scale, ctx.cap = plan, scale, cap
         return out
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, d_out):
-        q, k, v, slopes, q_pos, k_pos, key_mask, out, lse = ctx.saved_tensors
+        *operands, out, lse = ctx.saved_tensors
         need = ctx.needs_input_grad
-        dq, dk, dv, ds = _lib.attn_bwd(q, k, v, ctx.plan, ctx.scale, out, lse, d_out, ctx.cap, slopes, q_pos, k_pos,
-                                       key_mask, need_dq=need[0], need_dkv=need[1] or need[2], need_dslopes=need[3])
+        dq, dk, dv, ds = _lib.attn_bwd_checked(operands, ctx.plan, ctx.scale, ctx.cap, out, lse, d_out, need[0],
+                                               need[1] or need[2], need[3])
         return (dq if need[0] else None, dk if need[1] else None, dv if need[2] else None, ds) + (None,) * 6
 
 
@@ -122,7 +124,7 @@ class _HeadNormRopeFn(torch.autograd.Function):
     @torch.autograd.function.once_differentiable
     def backward(ctx, dyq, dyk):
         q, k, wq, wk, pos = ctx.saved_tensors
-        return _lib.head_norm_rope_bwd(q, k, wq, wk, pos, *ctx.opts, dyq, dyk) + (None,) * 4
+        return _lib.head_norm_rope_bwd_checked(q, k, wq, wk, pos, *ctx.opts, dyq, dyk) + (None,) * 4
 
 
 def head_norm_rope(q: torch.Tensor, k: torch.Tensor, q_weight: torch.Tensor, k_weight: torch.Tensor, pos: torch.Tensor, *,
