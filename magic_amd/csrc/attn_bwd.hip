@@ -726,10 +726,11 @@ template <typename M, int DP> int sweeps(BwdArgs &b, bool last, hipStream_t st) 
 
 template <typename M> int sweeps_of(BwdArgs &b, bool last, hipStream_t st) {
     const int D = b.a.head_dim;
-    return D <= 16   ? sweeps<M, 16>(b, last, st)
-           : D <= 32 ? sweeps<M, 32>(b, last, st)
-           : D <= 64 ? sweeps<M, 64>(b, last, st)
-                     : sweeps<M, 128>(b, last, st);
+    if constexpr (!M::SCALED) {          // (use_f16: wider heads only)
+        if (D <= 16) return sweeps<M, 16>(b, last, st);
+        if (D <= 32) return sweeps<M, 32>(b, last, st);
+    }
+    return D <= 64 ? sweeps<M, 64>(b, last, st) : sweeps<M, 128>(b, last, st);
 }
 
 template <typename T, int DP> int delta(BwdArgs &b, hipStream_t st) {
@@ -772,7 +773,7 @@ int magic_attn_bwd(const magic_attn *a, const void *out, int64_t ld_out, int64_t
     if (st != MAGIC_OK) return st;
     hipStream_t stream = (hipStream_t)stream_;
     if (a->n_q > 0 && (!out || !lse || !d_out || (d_slopes && !dq))) return MAGIC_ERR_INVALID_ARG;
-    if (!dk != !dv || (dk && a->n_k > 0 && (a->n_k_tiles < 1 || !a->k_tiles))) return MAGIC_ERR_INVALID_ARG;
+    if (!dk != !dv) return MAGIC_ERR_INVALID_ARG;
     if (d_slopes && !a->slopes) return MAGIC_ERR_INVALID_ARG;
     const int per = a->dtype == MAGIC_F32 ? 4 : 8;
     if (((uintptr_t)out | (uintptr_t)d_out | (uintptr_t)dq | (uintptr_t)dk | (uintptr_t)dv) & 15) return MAGIC_ERR_INVALID_ARG;

@@ -248,6 +248,8 @@ __device__ __forceinline__ void stay(uint32_t &x) { asm volatile("" : "+v"(x)); 
 // Staging of a tile by NT threads: rows of DP columns (zeros behind D) in chunks of eight elements.  A chunk's place is a
 // 32-bit offset (MAX_LD bounds it) from the tile's first row, which is the same for all threads.
 constexpr int64_t MAX_LD = 1 << 22;
+constexpr int MAX_HEADS = 8192;               // grids' second dimension
+constexpr int64_t MAX_ROWS = 0x7fff0000;      // a tile past the last row still has a 32-bit number
 template <typename M, int DP, int ROWS, int NT> struct Stage {
     typedef typename M::T T;
     typedef Tile<M, DP, ROWS> tile;

@@ -4,6 +4,8 @@
 // One pass over the keys with a running maximum and sum per row; scores are formed transposed (keys x rows), so that a
 // lane owns ONE row's statistics and the probabilities feed the second product from their registers (attn_common.h).
 #include "attn_common.h"
+#include <cmath>
+#include <type_traits>
 
 namespace magic {
 namespace attn {
@@ -12,17 +14,18 @@ int check(const magic_attn *a) {
     if (!a) return MAGIC_ERR_INVALID_ARG;
     if (a->dtype != MAGIC_F32 && a->dtype != MAGIC_BF16) return MAGIC_ERR_UNSUPPORTED;
     if (a->q_heads < 1 || a->kv_heads < 1 || a->q_heads % a->kv_heads || a->head_dim < 1) return MAGIC_ERR_INVALID_ARG;
-    if (a->head_dim > MAGIC_ATTN_MAX_DIM || a->head_dim % 8 || a->q_heads > 65535) return MAGIC_ERR_UNSUPPORTED;
-    if (a->n_q < 0 || a->n_k < 0 || a->n_q > 0x7fffffff || a->n_k > 0x7fffffff) return MAGIC_ERR_INVALID_ARG;
+    if (a->head_dim > MAGIC_ATTN_MAX_DIM || a->head_dim % 8 || a->q_heads > MAX_HEADS) return MAGIC_ERR_UNSUPPORTED;
+    if (a->n_q < 0 || a->n_k < 0 || a->n_q > MAX_ROWS || a->n_k > MAX_ROWS) return MAGIC_ERR_INVALID_ARG;
     if (a->n_q_tiles < 0 || a->n_k_tiles < 0 || a->max_q < 0 || a->max_k < 0 || a->n_seg < 0) return MAGIC_ERR_INVALID_ARG;
     if (a->n_q > 0 && (!a->q || a->n_q_tiles < 1 || !a->q_tiles)) return MAGIC_ERR_INVALID_ARG;
-    if (a->n_k > 0 && (!a->k || !a->v)) return MAGIC_ERR_INVALID_ARG;
+    if (a->n_k > 0 && (!a->k || !a->v || a->n_k_tiles < 1 || !a->k_tiles)) return MAGIC_ERR_INVALID_ARG;
     if (a->ld_q > MAX_LD || a->ld_k > MAX_LD || a->ld_v > MAX_LD || (int64_t)a->q_heads * a->head_dim > MAX_LD) return MAGIC_ERR_UNSUPPORTED;
     if (a->ld_q < 0 || a->hs_q < 0 || a->ld_k < 0 || a->hs_k < 0 || a->ld_v < 0 || a->hs_v < 0) return MAGIC_ERR_INVALID_ARG;
     const int per = a->dtype == MAGIC_F32 ? 4 : 8;   // rows and heads start on 16-byte addresses
     if (((uintptr_t)a->q | (uintptr_t)a->k | (uintptr_t)a->v) & 15) return MAGIC_ERR_INVALID_ARG;
     if ((a->ld_q | a->hs_q | a->ld_k | a->hs_k | a->ld_v | a->hs_v) % per) return MAGIC_ERR_INVALID_ARG;
-    if (!(a->cap >= 0.f) || !(a->scale == a->scale)) return MAGIC_ERR_INVALID_ARG;
+    // (scale / cap and cap times a series' terms stay normal float32 numbers)
+    if (!(a->cap == 0.f || (a->cap >= 1e-3f && a->cap <= 1e30f)) || !std::isfinite(a->scale)) return MAGIC_ERR_INVALID_ARG;
     if (a->slopes && ((a->n_q > 0 && !a->q_pos) || (a->n_k > 0 && !a->k_pos))) return MAGIC_ERR_INVALID_ARG;
     return MAGIC_OK;
 }
@@ -237,11 +240,13 @@ int64_t range_count(const magic_attn *a, bool grad) {
 
 }  // namespace
 
-// F16x2 needs two passes over the operands first: for float32 calls of enough work to pay for them
+// F16x2 needs two passes over the operands first: for float32 calls of enough work to pay for them.  Heads up to 32 wide
+// do not (the softmax takes their time, not the products): 64 ragged graphs of up to 1,516 nodes with masked keys, 4 heads
+// of 16, 121 us with it against 117 us without.
 bool use_f16(const magic_attn *a) { return a->dtype == MAGIC_F32 && a->head_dim > 32 && a->max_k >= 512 && a->n_seg > 0; }
 
 // Gathering costs two launches and a copy of the unmasked rows, and saves the masked share of everything else
-bool use_gather(const magic_attn *a) { return a->key_mask && a->max_k >= 512 && a->n_seg > 0 && a->n_k > 0 && a->n_k_tiles > 0; }
+bool use_gather(const magic_attn *a) { return a->key_mask && a->max_k >= 512 && a->n_seg > 0 && a->n_k > 0; }
 
 size_t prepare_bytes(const magic_attn *a, bool f16, bool backward) {
     size_t n = 0;
@@ -596,6 +601,154 @@ __global__ __launch_bounds__(64 * WM *KG, DP == 128 && (M::N > 1 || WM == 1) ? 1
     if (hf == 0) p.lse[(int64_t)h * a.n_q + q0 + row] = ls;
 }
 
+// sum over LPR neighbouring lanes, the same in all of them
+template <int LPR> __device__ __forceinline__ float lanes_sum(float x) {
+    auto add = [](float v, auto ctrl) {
+        return v + __uint_as_float(__builtin_amdgcn_update_dpp(0, __float_as_uint(v), decltype(ctrl)::value, 0xf, 0xf, true));
+    };
+    if constexpr (LPR >= 2) x = add(x, std::integral_constant<int, 0xB1>{});    // lane ^ 1
+    if constexpr (LPR >= 4) x = add(x, std::integral_constant<int, 0x4E>{});    // lane ^ 2
+    if constexpr (LPR >= 8) x = add(x, std::integral_constant<int, 0x141>{});   // mirrored in eight
+    if constexpr (LPR >= 16) x = add(x, std::integral_constant<int, 0x140>{});  // mirrored in sixteen
+    if constexpr (LPR >= 32) x += __shfl_xor(x, 16, 64);
+    return x;
+}
+
+// Few columns (rows x heads of one key head, at most NC): no tiles, no matrix instructions -- the keys and values stream
+// through registers once.  LPR lanes hold a key row in 16-byte chunks; every such group walks its own keys with its own
+// running maximum, sum and output, four keys at a time with the next four under way; the groups join through LDS.
+// A matrix tile would split 64 float32 keys into planes for one column of thirty-two: 75 us against 36 us for twelve rows
+// over twelve stored graphs of 8,000 nodes (4 heads of 64).
+template <typename T, int DP, int NC> __global__ __launch_bounds__(256) void k_attn_few(FwdArgs p) {
+    constexpr int EPL = 16 / (int)sizeof(T), LPR = DP / EPL, GPB = 256 / LPR, U = 4;
+    typedef typename magic::vec_of<T, EPL>::type vt;
+    __shared__ float sm[GPB][NC], sl[GPB][NC], so[GPB * NC * DP];
+    const magic_attn &a = p.a;
+    const int64_t item = blockIdx.x;
+    const int D = a.head_dim, tid = threadIdx.x, gl = tid % LPR, grp = tid / LPR;
+    const int64_t per_hb = (int64_t)a.n_q_tiles * p.sub;
+    const int64_t ts = item % per_hb;
+    const int hb = (int)(item / per_hb % p.n_hb), split = (int)(item / (per_hb * p.n_hb));
+    const int32_t *t = a.q_tiles + TAB * (ts / p.sub);
+    const int nq = t[1] - (int)(ts % p.sub) * p.rows;
+    if (nq <= 0) return;
+    const int64_t q0 = (int64_t)t[0] + (ts % p.sub) * p.rows, k0 = t[2];
+    const int nk = t[3], per = (nk + p.n_split - 1) / p.n_split;
+    const int beg = min(split * per, nk), end = min(beg + per, nk);
+    const int c0 = gl * EPL;
+    const bool cin = c0 < D;
+    const int hk = hb * p.gc / (a.q_heads / a.kv_heads);
+    const T *K = (const T *)a.k + k0 * a.ld_k + hk * a.hs_k + (cin ? c0 : 0), *V = (const T *)a.v + k0 * a.ld_v + hk * a.hs_v + (cin ? c0 : 0);
+    const bool bias = a.slopes != nullptr;
+
+    float q[NC][EPL], slope[NC], m[NC], l[NC], o[NC][EPL];
+    uint32_t qpos[NC];
+#pragma unroll
+    for (int c = 0; c < NC; ++c) {
+        const int row = c / p.gc, h = hb * p.gc + c % p.gc;
+        const bool ok = c < p.cols && row < nq;
+        const T *qp = (const T *)a.q + (q0 + (ok ? row : 0)) * a.ld_q + (ok ? h : hb * p.gc) * a.hs_q + (cin ? c0 : 0);
+        const vt x = *reinterpret_cast<const vt *>(qp);
+#pragma unroll
+        for (int e = 0; e < EPL; ++e) q[c][e] = ok && cin ? (float)x[e] : 0.f, o[c][e] = 0.f;
+        slope[c] = bias ? a.slopes[ok ? h : hb * p.gc] : 0.f;
+        qpos[c] = bias ? flip(a.q_pos[q0 + (ok ? row : 0)]) : 0u;
+        m[c] = -INFINITY, l[c] = 0.f;
+    }
+    vt kn[U], vn[U];
+    uint8_t keep[U];
+    int pos[U];
+    auto load = [&](int j0) {
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const int j = j0 + u * GPB, jc = j < end ? j : end - 1;
+            kn[u] = *reinterpret_cast<const vt *>(K + (int64_t)jc * a.ld_k);
+            vn[u] = *reinterpret_cast<const vt *>(V + (int64_t)jc * a.ld_v);
+            keep[u] = a.key_mask ? a.key_mask[k0 + jc] : 1;
+            pos[u] = bias ? a.k_pos[k0 + jc] : 0;
+        }
+    };
+    if (beg < end) load(beg + grp);
+    for (int j0 = beg + grp; j0 < end; j0 += U * GPB) {
+        vt kc[U], vc[U];
+        bool in[U];
+        uint32_t kp[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u) kc[u] = kn[u], vc[u] = vn[u], in[u] = j0 + u * GPB < end && keep[u] != 0, kp[u] = flip(pos[u]);
+        load(j0 + U * GPB);
+        float kf[U][EPL], vf[U][EPL];
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+#pragma unroll
+            for (int e = 0; e < EPL; ++e) kf[u][e] = cin ? (float)kc[u][e] : 0.f, vf[u][e] = in[u] && cin ? (float)vc[u][e] : 0.f;
+#pragma unroll
+        for (int c = 0; c < NC; ++c) {
+            float x[U], mx = m[c];
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                float d = 0.f;
+#pragma unroll
+                for (int e = 0; e < EPL; ++e) d = fmaf(q[c][e], kf[u][e], d);
+                x[u] = lanes_sum<LPR>(d) * a.scale;
+            }
+            if (a.cap > 0.f) {
+#pragma unroll
+                for (int u = 0; u < U; ++u) x[u] = a.cap * tanhf(x[u] / a.cap);
+            }
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                if (bias) x[u] = fmaf(-slope[c], dist_of(kp[u], qpos[c]), x[u]);
+                x[u] = in[u] ? x[u] : -INFINITY;
+                mx = fmaxf(mx, x[u] * LOG2E);
+            }
+            const float ms = mx == -INFINITY ? 0.f : mx, al = __builtin_amdgcn_exp2f(m[c] - ms);
+            m[c] = mx;
+            float ps = 0.f, acc[EPL];
+#pragma unroll
+            for (int e = 0; e < EPL; ++e) acc[e] = o[c][e] * al;
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                const float pr = __builtin_amdgcn_exp2f(fmaf(x[u], LOG2E, -ms));
+                ps += pr;
+#pragma unroll
+                for (int e = 0; e < EPL; ++e) acc[e] = fmaf(pr, vf[u][e], acc[e]);
+            }
+            l[c] = fmaf(l[c], al, ps);
+#pragma unroll
+            for (int e = 0; e < EPL; ++e) o[c][e] = acc[e];
+        }
+    }
+#pragma unroll
+    for (int c = 0; c < NC; ++c) {
+        if (gl == 0) sm[grp][c] = m[c], sl[grp][c] = l[c];
+#pragma unroll
+        for (int e = 0; e < EPL; ++e) so[(grp * NC + c) * DP + c0 + e] = o[c][e];
+    }
+    __syncthreads();
+    // a thread per (column, output column): the groups in order
+    for (int i = tid; i < NC * DP; i += 256) {
+        const int c = i / DP, d = i % DP, row = c / p.gc, h = hb * p.gc + c % p.gc;
+        if (c >= p.cols || row >= nq || d >= D) continue;
+        float mt = -INFINITY, lt = 0.f, ot = 0.f;
+        for (int g = 0; g < GPB; ++g) mt = sm[g][c] > mt || sm[g][c] != sm[g][c] ? sm[g][c] : mt;
+        const float ms = mt == -INFINITY ? 0.f : mt;
+        for (int g = 0; g < GPB; ++g) {
+            const float w = __builtin_amdgcn_exp2f(sm[g][c] - ms);
+            lt = fmaf(sl[g][c], w, lt), ot = fmaf(so[(g * NC + c) * DP + d], w, ot);
+        }
+        const float inv = lt > 0.f || lt != lt ? 1.f / lt : 0.f;
+        const float ls = mt == -INFINITY && lt == 0.f ? -INFINITY : mt + __builtin_amdgcn_logf(lt);
+        if (p.n_split > 1) {
+            const int64_t base = ((int64_t)split * a.q_heads + h) * a.n_q + q0 + row;
+            p.part_o[base * D + d] = ot * inv;
+            if (d == 0) p.part_l[base] = ls;
+        } else {
+            ((T *)p.out)[(q0 + row) * p.ld_o + h * p.hs_o + d] = (T)(ot * inv);
+            if (d == 0) p.lse[(int64_t)h * a.n_q + q0 + row] = ls;
+        }
+    }
+}
+
 // The key ranges of a row joined: o = sum_s 2^(l_s - l) o_s.  A block takes a row and head; CPR lanes hold its columns
 // and the 256 / CPR lane groups take the ranges in turn, added in group order.
 template <typename T, int CPR> __global__ __launch_bounds__(256) void k_attn_join(FwdArgs p) {
@@ -632,19 +785,31 @@ template <typename T, int CPR> __global__ __launch_bounds__(256) void k_attn_joi
     if (c == 0) p.lse[hr] = m == -INFINITY ? -INFINITY : ms + __builtin_amdgcn_logf(l);
 }
 
+constexpr int FEW = 4;
+
 struct Shape {
     int wm, n_split, cols, rows, gc, sub, n_hb;
     bool f16;
     int64_t items;
 };
 
-// How a call is cut: 128 rows of one head a block, or 32 (row, head) columns with the keys dealt to its wavefronts; then
-// key ranges until there are enough blocks.
+// How a call is cut: 128 rows of one head a block (wm 4), or 32 (row, head) columns with the keys dealt to its wavefronts
+// (wm 1), or up to four columns without matrix instructions (wm 0); then key ranges until there are enough blocks.
 Shape shape_of(const magic_attn *a) {
     Shape s;
     const int G = a->q_heads / a->kv_heads;
     const int64_t big = (int64_t)a->n_q_tiles * a->q_heads;
     s.wm = big >= 256 && a->max_q > 32 ? 4 : 1;
+    if ((int64_t)a->max_q * G <= FEW) {
+        s.wm = 0, s.gc = G, s.rows = a->max_q > 0 ? a->max_q : 1, s.cols = s.rows * G, s.sub = 1, s.n_hb = a->kv_heads;
+        s.f16 = false;
+        const int64_t blocks = (int64_t)a->n_q_tiles * s.n_hb, most = (a->max_k + 255) / 256;
+        int64_t split = (1024 + blocks - 1) / blocks;
+        if (split > most) split = most;
+        s.n_split = (int)(split > 256 ? 256 : split < 1 ? 1 : split);
+        s.items = blocks * s.n_split;
+        return s;
+    }
     if (s.wm == 4) {
         s.gc = 1, s.cols = s.rows = 128;
     } else {
@@ -683,10 +848,22 @@ template <typename M, int DP, int WM, int KG, int KW> int launch(FwdArgs &p, hip
 
 template <typename M> int run_rows(FwdArgs &p, hipStream_t st) {
     const int D = p.a.head_dim;
-    return D <= 16   ? launch<M, 16, 4, 1, 64>(p, st)
-           : D <= 32 ? launch<M, 32, 4, 1, 64>(p, st)
-           : D <= 64 ? launch<M, 64, 4, 1, 64>(p, st)
-                     : launch<M, 128, 4, 1, 64>(p, st);
+    if constexpr (!M::SCALED) {          // (use_f16: wider heads only)
+        if (D <= 16) return launch<M, 16, 4, 1, 64>(p, st);
+        if (D <= 32) return launch<M, 32, 4, 1, 64>(p, st);
+    }
+    return D <= 64 ? launch<M, 64, 4, 1, 64>(p, st) : launch<M, 128, 4, 1, 64>(p, st);
+}
+
+template <typename T, int DP> int run_few(FwdArgs &p, hipStream_t st) {
+    if (p.items > 0x7fffffffLL) return MAGIC_ERR_UNSUPPORTED;
+    if (p.cols == 1)
+        MAGIC_LAUNCH("attn_few", (k_attn_few<T, DP, 1>), (int)p.items, 256, 0, st, p);
+    else if (p.cols == 2)
+        MAGIC_LAUNCH("attn_few", (k_attn_few<T, DP, 2>), (int)p.items, 256, 0, st, p);
+    else
+        MAGIC_LAUNCH("attn_few", (k_attn_few<T, DP, 4>), (int)p.items, 256, 0, st, p);
+    return magic::launch_status();
 }
 
 template <typename M> int run(FwdArgs &p, int wm, hipStream_t st) {
@@ -694,6 +871,9 @@ template <typename M> int run(FwdArgs &p, int wm, hipStream_t st) {
     int rc;
     if (wm == 4) {
         rc = run_rows<M>(p, st);
+    } else if (wm == 0) {
+        typedef typename M::T T;
+        rc = D <= 16 ? run_few<T, 16>(p, st) : D <= 32 ? run_few<T, 32>(p, st) : D <= 64 ? run_few<T, 64>(p, st) : run_few<T, 128>(p, st);
     } else {
         // wavefronts of a block: as many as leave the LDS room for two blocks a CU
         constexpr int KG64 = M::N == 3 ? 2 : 4, KG128 = M::N == 3 ? 1 : 2;
