@@ -1002,8 +1002,8 @@ def attn_check(q, k, v, n_q, n_k, plan_device, cap, slopes, q_pos, k_pos, key_ma
         raise MagicHipError(f"the plan is for {n_q} query and {n_k} key rows, got {q.shape[0]} and {k.shape[0]}")
     if plan_device != q.device:
         raise MagicHipError(f"the plan lives on {plan_device}, the operands on {q.device}")
-    if not cap >= 0.0 or cap == float("inf"):
-        raise MagicHipError(f"cap must be finite and >= 0, 0 for none (got {cap})")
+    if not (cap == 0.0 or 1e-3 <= cap <= 1e30):
+        raise MagicHipError(f"cap must be 0 (none) or 1e-3 to 1e30 (got {cap})")
     _vec_check(slopes, "slopes", hq, (torch.float32,), q.device)
     if slopes is not None and (q_pos is None or k_pos is None):
         raise MagicHipError("slopes need q_pos and k_pos")
@@ -1171,13 +1171,18 @@ def head_norm_rope_bwd_checked(q, k, wq, wk, pos, rotary_dim, eps, base, dyq, dy
 
 
 # ------------------------------------------------------------------------------------- 8-bit activation checkpoints
+def full_rows(t: torch.Tensor) -> torch.Tensor:
+    """2-D operand with unit inner stride whose rows do not overlap (an expanded one is copied)."""
+    return t if t.stride(1) == 1 and (t.stride(0) >= t.shape[1] or t.shape[0] <= 1) else t.contiguous()
+
+
 def act8_pack(x: torch.Tensor):
     """(codes int8 [N, stride], exps uint8 [N, ceil(F / 32)]) of a float32 [N, F] matrix."""
     lib = load()
     if x.dim() != 2 or x.shape[1] < 1:
         raise MagicHipError(f"x must be a matrix with at least one column (got {tuple(x.shape)})")
     _dev(x, torch.float32, "x")
-    x = _rows(x)
+    x = full_rows(x)
     n, f = x.shape
     codes = torch.empty(n, lib.magic_act8_code_stride(f), dtype=torch.int8, device=x.device)
     exps = torch.empty(n, (f + 31) // 32, dtype=torch.uint8, device=x.device)
@@ -1213,7 +1218,7 @@ def act8_weight_grad(dy: torch.Tensor, codes: torch.Tensor, exps: torch.Tensor, 
     if dy.dim() != 2 or dy.shape[0] != codes.shape[0] or dy.shape[1] < 1 or dy.device != codes.device:
         raise MagicHipError(f"dy must be a [{codes.shape[0]}, M] matrix on {codes.device}")
     _dev(dy, torch.float32, "dy")
-    dy = _rows(dy)
+    dy = full_rows(dy)
     n, m = dy.shape
     dw = torch.empty(m, n_cols, dtype=torch.float32, device=dy.device)
     with _on_device(dy.device):

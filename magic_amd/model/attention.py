@@ -56,20 +56,23 @@ def _tiles(rows, others):
 def attention_plan(q_lens: Sequence[int], kv_lens: Optional[Sequence[int]] = None, device="cuda") -> AttentionPlan:
     """Plan for segments of ``q_lens[i]`` query rows over ``kv_lens[i]`` key rows (host integers, in row order; keys =
     queries when ``kv_lens`` is None).  Lengths may be zero.  A plan serves any heads, types and options, and can be
-    kept as long as the lengths stay the same (all layers of a step, all calls against one stored graph)."""
+    kept as long as the lengths stay the same (all layers of a step, all calls against one stored graph).  Its tables are
+    copied to the device here: build it before recording a graph."""
     q_lens = [int(x) for x in q_lens]
     kv_lens = q_lens if kv_lens is None else [int(x) for x in kv_lens]
     if len(q_lens) != len(kv_lens):
         raise _lib.MagicHipError(f"{len(q_lens)} query segments but {len(kv_lens)} key segments")
     if any(x < 0 for x in q_lens + kv_lens):
         raise _lib.MagicHipError("segment lengths must not be negative")
-    if max(sum(q_lens), sum(kv_lens)) >= 1 << 31:
-        raise _lib.MagicHipError("segment attention serves up to 2^31 - 1 rows")
+    if max(sum(q_lens), sum(kv_lens)) > 0x7fff0000:
+        raise _lib.MagicHipError("segment attention serves up to 2,147,418,112 rows")
     device = torch.device(device)
     if device.type == "cuda" and device.index is None:
         device = torch.device("cuda", torch.cuda.current_device())
     tabs = [torch.from_numpy(_tiles(a, b)) for a, b in ((q_lens, kv_lens), (kv_lens, q_lens))]
     if device.type == "cuda":
+        if torch.cuda.is_current_stream_capturing():
+            raise _lib.MagicHipError("build the plan before the capture: its tables would not outlive it")
         tabs = [t.pin_memory().to(device, non_blocking=True) for t in tabs]
     return AttentionPlan(q_lens, kv_lens, *tabs)
 
@@ -102,8 +105,8 @@ def segment_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, plan: A
 
     q [n_q, q_heads, head_dim]; k, v [n_k, kv_heads, head_dim], query head h reads key head h // (q_heads //
     kv_heads).  float32 or bfloat16, any row and head strides, head_dim a multiple of 8 up to 128.
-    ``s = scale q.k`` (scale: 1 / sqrt(head_dim)); ``cap > 0``: ``cap tanh(s / cap)``; ``slopes`` [q_heads] float32:
-    minus ``slopes[h] |q_pos[i] - k_pos[j]|`` (int32 positions); ``key_mask`` [n_k] bool: False = the key takes no part,
+    ``s = scale q.k`` (scale: 1 / sqrt(head_dim)); ``cap`` (1e-3 to 1e30, 0: none): ``cap tanh(s / cap)``;
+    ``slopes`` [q_heads] float32: minus ``slopes[h] |q_pos[i] - k_pos[j]|`` (int32 positions); ``key_mask`` [n_k] bool: False = the key takes no part,
     whatever its rows hold.  A row that sees no key gets zeros, and zero gradients.
     Differentiable in q, k, v and slopes; the sums have a fixed order."""
     if scale is None:

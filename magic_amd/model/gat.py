@@ -217,6 +217,7 @@ class _LinearAct8Fn(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, x, w):
+        x = _lib.full_rows(x)
         y, _, _ = _lib.proj_fwd(x, w, w.shape[0], 0, 0)
         codes = exps = None
         if ctx.needs_input_grad[1]:
@@ -227,6 +228,7 @@ class _LinearAct8Fn(torch.autograd.Function):
     @staticmethod
     def backward(ctx, dy):
         codes, exps, w = ctx.saved_tensors
+        dy = _lib.full_rows(dy)
         dx = _lib.proj_bwd_input(dy, w)[0] if ctx.needs_input_grad[0] else None
         dw = _lib.act8_weight_grad(dy, codes, exps, w.shape[1]) if ctx.needs_input_grad[1] else None
         return dx, dw

@@ -135,3 +135,23 @@ def test_linear_keeps_a_quarter_of_the_memory(cuda):
         saved = y.grad_fn.saved_tensors
         held[bits] = sum(t.numel() * t.element_size() for t in saved if t.data_ptr() != w.data_ptr())
     assert held == {32: 4 * x.numel(), 8: x.numel() + x.numel() // 32}
+
+
+def test_expanded_and_overlapping_rows(cuda):
+    """Operands whose rows share memory, as broadcasts and their gradients do."""
+    from magic_amd.model.act8 import act8_pack, act8_weight_grad
+    from magic_amd.model.gat import linear_nobias
+    row = torch.randn(1, 40, device=cuda)
+    a, b = act8_pack(row.expand(50, 40)), act8_pack(row.repeat(50, 1))
+    assert torch.equal(a.codes, b.codes) and torch.equal(a.exps, b.exps)
+    dy = torch.randn(1, 12, device=cuda)
+    assert torch.equal(act8_weight_grad(dy.expand(50, 12), a), act8_weight_grad(dy.repeat(50, 1), a))
+    w = torch.randn(12, 40, device=cuda, requires_grad=True)
+    x = torch.randn(50, 40, device=cuda, requires_grad=True)
+    y = linear_nobias(x, w, act_bits=8)
+    got = torch.autograd.grad((y * dy).sum(), (x, w), retain_graph=True)
+    via = torch.autograd.grad(y, (x, w), dy.expand(50, 12))
+    assert all(torch.equal(p, q) for p, q in zip(got, via))
+    window = torch.randn(89, device=cuda).as_strided((50, 40), (1, 1))
+    assert torch.equal(act8_pack(window).codes, act8_pack(window.contiguous()).codes)
+    assert torch.equal(linear_nobias(row.expand(50, 40), w, act_bits=8), linear_nobias(row.repeat(50, 1), w, act_bits=8))

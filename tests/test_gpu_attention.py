@@ -377,6 +377,71 @@ def test_registered_attention_operators(cuda):
         assert torch.equal(x, want[name]), name
 
 
+def test_attention_refusals(cuda):
+    """What the operators do not serve raises before anything is launched."""
+    from magic_amd._lib import MagicHipError
+    from magic_amd.model.attention import attention_plan, head_norm_rope, segment_attention
+    q, k, v, d, kw = make(cuda, [9], [9], 4, 2, 16, torch.float32, slopes=True)
+    plan = attention_plan([9], device=cuda)
+    ok = dict(slopes=kw["slopes"], q_pos=kw["q_pos"], k_pos=kw["k_pos"])
+    segment_attention(q, k, v, plan, **ok)
+    bad = [((q.half(), k.half(), v.half()), {}), ((q, k.bfloat16(), v), {}), ((q[:, :3], k, v), {}), ((q[..., :12], k[..., :12], v[..., :12]), {}),
+           ((q, k[:8], v[:8]), {}), ((q[:8], k, v), {}), ((q, k, v[:, :1]), {}), ((q[0], k, v), {}),
+           ((q, k, v), dict(cap=-1.0)), ((q, k, v), dict(cap=1e-9)), ((q, k, v), dict(cap=float("nan"))),
+           ((q, k, v), dict(scale=float("inf"))), ((q, k, v), dict(slopes=ok["slopes"])),
+           ((q, k, v), dict(ok, slopes=ok["slopes"][:2])), ((q, k, v), dict(ok, q_pos=ok["q_pos"].long())),
+           ((q, k, v), dict(ok, k_pos=ok["k_pos"].cpu())), ((q, k, v), dict(key_mask=torch.ones(8, dtype=torch.bool, device=cuda))),
+           ((q, k, v), dict(key_mask=torch.ones(9, device=cuda)))]
+    for args, opt in bad:
+        with pytest.raises(MagicHipError):
+            segment_attention(*args, plan, **opt)
+    with pytest.raises(MagicHipError):
+        segment_attention(q, k, v, attention_plan([9], device="cpu"))
+    wide = torch.zeros(3, 1, 136, device=cuda)
+    with pytest.raises(MagicHipError):
+        segment_attention(wide, wide, wide, attention_plan([3], device=cuda))
+    w, pos = torch.ones(16, device=cuda), torch.arange(9, device=cuda, dtype=torch.int32)
+    for args, opt in [((q, k, w, w, pos), dict(rotary_dim=15)), ((q, k, w, w, pos), dict(rotary_dim=18)), ((q, k, w[:8], w, pos), {}),
+                      ((q, k, w, w, pos.long()), {}), ((q, k[:8], w, w, pos), {}), ((q, k, w.bfloat16(), w, pos), {}),
+                      ((q, k, w, w, pos), dict(eps=-1.0)), ((q, k, w, w, pos), dict(base=0.0)), ((q.half(), k.half(), w, w, pos), {})]:
+        with pytest.raises(MagicHipError):
+            head_norm_rope(*args, **opt)
+
+
+def test_plan_is_not_built_during_a_capture(cuda):
+    from magic_amd._lib import MagicHipError
+    from magic_amd.model.attention import attention_plan
+    graph, x = torch.cuda.CUDAGraph(), torch.zeros(8, device=cuda)
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph):
+        y = x + 1
+        with pytest.raises(MagicHipError):
+            attention_plan([4], device=cuda)
+    graph.replay()
+    torch.cuda.synchronize()
+    assert (y == 1).all()
+
+
+@pytest.mark.parametrize("cap", [1e-3, 1e6, 1e30])
+def test_caps_far_from_the_scores(cuda, cap):
+    """One far below the scores makes them its sign.  One far above leaves them as they are (tanh takes less than 1e-10
+    of a score off, a two-hundredth of a half step): the reference has none then."""
+    q, k, v, d, _ = make(cuda, [40], [40], 2, 2, 16, torch.float32)
+    got = run(q, k, v, d, [40], [40], cap=cap)
+    check(got, q, k, v, d, [40], [40], cap=cap if cap < 1 else 0.0)
+
+
+def test_attention_serves_without_rows_or_keys(cuda):
+    from magic_amd.model.attention import attention_plan, segment_attention
+    q, k, v, d, _ = make(cuda, [5], [7], 4, 2, 16, torch.float32)
+    out = segment_attention(q[:0], k, v, attention_plan([0], [7], cuda))
+    assert out.shape == (0, 4, 16)
+    got = run(q[:0], k, v, d[:0], [0], [7])
+    assert not got["dk"].any() and not got["dv"].any() and got["dk"].shape == k.shape
+    got = run(q, k[:0], v[:0], d, [5], [0])
+    assert not got["out"].any() and not got["dq"].any()
+
+
 # ------------------------------------------------------------------------------------------- head norm + rotation
 def rope_reference(x, w, pos, rot, eps, base, dy):
     r = _half_step(x.dtype)

@@ -72,7 +72,7 @@ def test_block_matches_float64(cuda, dim, heads, masked, bits):
     # see inputs off by up to half a step, 2^-7 of the largest of 32 values, which is up to four times their root mean
     # square: dY^T E against dY^T X is then at most about 2^-7 * 4 = 2^-5.
     def rel(a, b):
-        return float((a.double() - b).norm() / b.norm())
+        return float((a.detach().double() - b.detach()).norm() / b.detach().norm())
     assert rel(y, want) < 1e-5
     for name, a, b in zip(["x"] + list(params), grads, wg):
         assert rel(a, b) < (2.0 ** -5 if bits == 8 and name in ("qkv.weight", "out.weight") else 2e-5), name
