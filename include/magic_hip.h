@@ -650,6 +650,11 @@ int magic_act8_pack(int64_t n_rows, int32_t n_cols, const float *x, int64_t ld_x
                     void *stream);
 int magic_act8_unpack(int64_t n_rows, int32_t n_cols, const int8_t *codes, const uint8_t *exps, float *x, int64_t ld_x,
                       void *stream);
+/* y = x w^T (magic_proj_fwd's value, bit for bit) and the codes of x from the same pass over it where the shape allows
+ * (n_cols a multiple of 4, at most 96 outputs), else from one of their own; workspace: magic_proj_fwd_workspace_bytes */
+int magic_act8_linear_fwd(int64_t n_rows, int32_t in_dim, int32_t out_dim, const float *x, int64_t ld_x, const float *w,
+                          float *y, int64_t ld_y, int8_t *codes, uint8_t *exps, void *workspace, size_t workspace_bytes,
+                          void *stream);
 size_t magic_act8_weight_grad_workspace_bytes(int64_t n_rows, int32_t m, int32_t f);
 int magic_act8_weight_grad(int64_t n_rows, int32_t m, int32_t f, const float *dy, int64_t ld_dy, const int8_t *codes,
                            const uint8_t *exps, float *dw, void *workspace, size_t workspace_bytes, void *stream);

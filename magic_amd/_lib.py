@@ -126,6 +126,7 @@ SYMBOLS = {
     "magic_act8_code_stride": (c_i64, [c_i32]),
     "magic_act8_pack": (c_i32, [c_i64, c_i32, c_vp, c_i64, c_vp, c_vp, c_vp]),
     "magic_act8_unpack": (c_i32, [c_i64, c_i32, c_vp, c_vp, c_vp, c_i64, c_vp]),
+    "magic_act8_linear_fwd": (c_i32, [c_i64, c_i32, c_i32, c_vp, c_i64, c_vp, c_vp, c_i64, c_vp, c_vp, c_vp, c_sz, c_vp]),
     "magic_act8_weight_grad_workspace_bytes": (c_sz, [c_i64, c_i32, c_i32]),
     "magic_act8_weight_grad": (c_i32, [c_i64, c_i32, c_i32, c_vp, c_i64, c_vp, c_vp, c_vp, c_vp, c_sz, c_vp]),
     "magic_knn_workspace_bytes": (c_sz, [c_i64, c_i64, c_i32, c_i32]),
@@ -1190,6 +1191,25 @@ def act8_pack(x: torch.Tensor):
         _check(lib.magic_act8_pack(n, f, x.data_ptr(), max(x.stride(0), f), codes.data_ptr(), exps.data_ptr(), _stream()),
                "magic_act8_pack")
     return codes, exps
+
+
+def act8_linear_fwd(x: torch.Tensor, w: torch.Tensor):
+    """(x @ w.T, codes, exps) of a float32 [N, F] matrix and a [M, F] weight."""
+    lib = load()
+    _dev(x, torch.float32, "x")
+    _dev(w, torch.float32, "w")
+    x, w = full_rows(x), w.contiguous()
+    n, f = x.shape
+    m = w.shape[0]
+    y = torch.empty(n, m, dtype=torch.float32, device=x.device)
+    codes = torch.empty(n, lib.magic_act8_code_stride(f), dtype=torch.int8, device=x.device)
+    exps = torch.empty(n, (f + 31) // 32, dtype=torch.uint8, device=x.device)
+    with _on_device(x.device):
+        ws = _scratch(lib.magic_proj_fwd_workspace_bytes(f, m), x.device)
+        _check(lib.magic_act8_linear_fwd(n, f, m, x.data_ptr(), max(x.stride(0), f), w.data_ptr(), y.data_ptr(), m,
+                                         codes.data_ptr(), exps.data_ptr(), ws.data_ptr(), ws.numel(), _stream()),
+               "magic_act8_linear_fwd")
+    return y, codes, exps
 
 
 def _act8_check(codes, exps, n_cols):

@@ -9,6 +9,7 @@
 // diverging run is not silently repaired.
 #include "common.h"
 #include "attn_common.h"
+#include "act8.h"
 
 namespace {
 
@@ -17,22 +18,9 @@ using magic::bf16x8_t;
 using magic::attn::f32x16_t;
 using magic::attn::f32x4_t;
 
-__device__ __forceinline__ float pow2f(int e) {  // 2^e, -126 <= e <= 127
-    return __uint_as_float((uint32_t)(e + 127) << 23);
-}
-
-// amax of a block (its bits as an unsigned number: magnitudes compare like integers, NaN above infinity) -> stored exponent
-__device__ __forceinline__ int block_exp(uint32_t amax_bits) {
-    if (amax_bits >= 0x7f800000u) return 255;
-    const int k = (int)(amax_bits >> 23);                        // biased exponent, 0 for subnormals and zero
-    int e = k - 6;
-    if ((amax_bits & 0x7fffffu) >= 0x7f0000u) ++e;               // mantissa >= 127.5 / 64: would round to 128
-    return e < 1 ? 1 : e;
-}
-
-__device__ __forceinline__ int code_of(float x, int e) {         // e: stored exponent, 1 .. 249
-    return (int)rintf(x * pow2f(127 - e));
-}
+using magic::act8::block_exp;
+using magic::act8::codes4;
+using magic::act8::pow2f;
 
 __device__ __forceinline__ float scale_of(int e) { return e == 255 ? __uint_as_float(0x7fc00000u) : pow2f(e - 127); }
 
@@ -78,14 +66,11 @@ __global__ __launch_bounds__(256) void k_act8_pack(I total, int F, const float *
             if (b >= total) continue;          // (whole blocks: the lanes of one agree)
             const int ex = block_exp(m);
             if constexpr (VEC == 8) {
-                uint32_t w[2] = {0u, 0u};
-                if (ex != 255) {
-#pragma unroll
-                    for (int e = 0; e < 8; ++e) w[e >> 2] |= ((uint32_t)code_of(v[u][e], ex) & 0xffu) << (8 * (e & 3));
-                }
-                if (c[u] < ld_c) *reinterpret_cast<uint2 *>(codes + at[u]) = make_uint2(w[0], w[1]);
+                const uint2 w = make_uint2(codes4(v[u][0], v[u][1], v[u][2], v[u][3], ex),
+                                           codes4(v[u][4], v[u][5], v[u][6], v[u][7], ex));
+                if (c[u] < ld_c) *reinterpret_cast<uint2 *>(codes + at[u]) = w;
             } else {
-                if (c[u] < ld_c) codes[at[u]] = ex == 255 ? (int8_t)0 : (int8_t)code_of(v[u][0], ex);
+                if (c[u] < ld_c) codes[at[u]] = (int8_t)codes4(v[u][0], 0.f, 0.f, 0.f, ex);
             }
             if (l == 0) exps[b] = (uint8_t)ex;
         }

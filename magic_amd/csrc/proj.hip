@@ -22,6 +22,7 @@ namespace magic {
 int proj_rows_try(const ProjArgs &a, int64_t *n_part, int *n_win, bool dry_run, hipStream_t stream);
 int proj_gemm_try(const ProjArgs &a, void *planes_ws, int64_t *n_part, int *n_win, bool dry_run, hipStream_t stream,
                   bool relaxed = false);
+bool proj_strip_packs(const ProjArgs &a);
 size_t proj_gemm_workspace_bytes(int F, int M);
 }
 
@@ -495,6 +496,9 @@ void init_args(ProjArgs &a) {
     a.part_col = nullptr;
     a.part_prelu = nullptr;
     a.sc_src = a.sc_dst = nullptr;
+    a.codes = nullptr;
+    a.ld_codes = 0;
+    a.exps = nullptr;
 }
 
 }  // namespace
@@ -504,7 +508,7 @@ extern "C" {
 static int proj_fwd_run(int64_t n_rows, int32_t in_dim, int32_t out_c, int32_t n_score, int32_t res_c, const float *x,
                         int64_t ld_x, const uint8_t *x_mask, float x_scale, const float *w, float *hs, int64_t ld_hs,
                         float *score, float *res, int64_t ld_res, const float *attn_src, const float *attn_dst,
-                        void *workspace, size_t workspace_bytes, void *stream_) {
+                        int8_t *codes, uint8_t *exps, void *workspace, size_t workspace_bytes, void *stream_) {
     if (n_rows < 0 || in_dim <= 0 || out_c <= 0 || n_score < 0 || res_c < 0) return MAGIC_ERR_INVALID_ARG;
     if (n_rows == 0) return MAGIC_OK;
     if (!x || !w || !hs || ld_x < in_dim || ld_hs < out_c) return MAGIC_ERR_INVALID_ARG;
@@ -533,6 +537,17 @@ static int proj_fwd_run(int64_t n_rows, int32_t in_dim, int32_t out_c, int32_t n
     // the block-tiled kernel keeps the split weight in the workspace; without one the other kernels run
     const size_t need = magic::proj_gemm_workspace_bytes(a.F, a.M);
     void *gemm_ws = (need && workspace && workspace_bytes >= need) ? workspace : nullptr;
+    // 8-bit codes beside the product: where the streaming kernel is the one that dispatch takes and packs this shape
+    if (codes) {
+        const int64_t ld_c = magic_act8_code_stride(in_dim);
+        if (magic::proj_strip_packs(a) &&
+            magic::proj_gemm_try(a, gemm_ws, nullptr, nullptr, true, (hipStream_t)stream_) == MAGIC_ERR_UNSUPPORTED) {
+            a.codes = codes, a.ld_codes = ld_c, a.exps = exps;
+        } else {
+            const int st = magic_act8_pack(n_rows, in_dim, x, ld_x, codes, exps, stream_);
+            if (st != MAGIC_OK) return st;
+        }
+    }
     // Wide layers with 64-wide heads and no residual projection: the 2H score columns would cost the block-tiled
     // kernel a third, nearly idle column block (264 outputs: 122 us against 85 us for 256 at 96,000 rows); with the
     // attention vectors given, its epilogue forms them from the 64 outputs of a head, which one wavefront holds.
@@ -552,7 +567,15 @@ int magic_proj_fwd(int64_t n_rows, int32_t in_dim, int32_t out_c, int32_t n_scor
                    int64_t ld_x, const uint8_t *x_mask, float x_scale, const float *w, float *hs, int64_t ld_hs,
                    float *score, float *res, int64_t ld_res, void *workspace, size_t workspace_bytes, void *stream_) {
     return proj_fwd_run(n_rows, in_dim, out_c, n_score, res_c, x, ld_x, x_mask, x_scale, w, hs, ld_hs, score, res, ld_res,
-                        nullptr, nullptr, workspace, workspace_bytes, stream_);
+                        nullptr, nullptr, nullptr, nullptr, workspace, workspace_bytes, stream_);
+}
+
+int magic_act8_linear_fwd(int64_t n_rows, int32_t in_dim, int32_t out_dim, const float *x, int64_t ld_x, const float *w,
+                          float *y, int64_t ld_y, int8_t *codes, uint8_t *exps, void *workspace, size_t workspace_bytes,
+                          void *stream_) {
+    if (n_rows > 0 && (!codes || !exps || (uintptr_t)codes % 16)) return MAGIC_ERR_INVALID_ARG;
+    return proj_fwd_run(n_rows, in_dim, out_dim, 0, 0, x, ld_x, nullptr, 1.f, w, y, ld_y, nullptr, nullptr, 0, nullptr,
+                        nullptr, codes, exps, workspace, workspace_bytes, stream_);
 }
 
 int magic_proj_fwd_attn(int64_t n_rows, int32_t in_dim, int32_t out_c, int32_t n_score, int32_t res_c, const float *x,
@@ -560,7 +583,7 @@ int magic_proj_fwd_attn(int64_t n_rows, int32_t in_dim, int32_t out_c, int32_t n
                         float *score, float *res, int64_t ld_res, const float *attn_src, const float *attn_dst,
                         void *workspace, size_t workspace_bytes, void *stream_) {
     return proj_fwd_run(n_rows, in_dim, out_c, n_score, res_c, x, ld_x, x_mask, x_scale, w, hs, ld_hs, score, res, ld_res,
-                        attn_src, attn_dst, workspace, workspace_bytes, stream_);
+                        attn_src, attn_dst, nullptr, nullptr, workspace, workspace_bytes, stream_);
 }
 
 size_t magic_proj_fwd_workspace_bytes(int32_t in_dim, int32_t out_total) {

@@ -37,6 +37,10 @@ struct ProjArgs {
     // rows: per output column the attention vector entries of the node as a source / as a destination, [C] each.
     // Set by the dispatcher only for the block-tiled kernel with 64-wide heads; M then excludes the score columns.
     const float *sc_src, *sc_dst;
+    // 8-bit codes of x beside the product (act8.hip), written by the streaming kernel: [n, ld_codes], [n, ceil(F / 32)]
+    int8_t *codes;
+    int64_t ld_codes;
+    uint8_t *exps;
 };
 
 }  // namespace magic

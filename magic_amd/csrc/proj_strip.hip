@@ -14,11 +14,15 @@
 //    them with the LDS-resident, pre-split weight.
 //  * The accumulators leave through the same strip (the X block is dead by then) as whole rows of float4, so
 //    the epilogue operands are read and the result written fully coalesced (proj_common.h: epi_store4).
+//  * PACK: the same pieces leave as 8-bit codes too (act8.hip): eight lanes hold the 32 columns of a block, so a K
+//    block of whole blocks (KSB even) has all that their exponents need.  700,000 rows of 192 columns on 64 outputs:
+//    228 us, 855 MB at 3.75 TB/s; the product (179 us) and the pass of its own (126 us) take 305 us
 //  * One block per CU (W is staged once per block), as many wavefronts as the LDS holds, at most 12
 //    (168 VGPRs; 8 for the longest K blocks).
 #include <cstdlib>
 #include "proj_common.h"
 #include "bf16_split.h"
+#include "act8.h"
 
 namespace {
 
@@ -63,7 +67,7 @@ __device__ __forceinline__ void load_unit(const ProjArgs &a, int64_t tile, int k
 }
 
 // ... into the strip: zero past the last row / last column, dropout mask and scale applied
-template <int KSB>
+template <int KSB, bool PACK>
 __device__ __forceinline__ void write_unit(const ProjArgs &a, int64_t tile, int kb, int lane, const Unit<KSB> &u, float *xs) {
     constexpr int KCB = 4 * KSB;
 #pragma unroll
@@ -80,10 +84,22 @@ __device__ __forceinline__ void write_unit(const ProjArgs &a, int64_t tile, int 
         }
         if (tile * 32 + r >= a.n || (kb * KCB + c) * 4 >= a.F) v = make_float4(0.f, 0.f, 0.f, 0.f);
         *reinterpret_cast<float4 *>(xs + (r * (KCB + 1) + c) * 4) = v;
+        if constexpr (PACK) {
+            const uint32_t sign = 0x7fffffffu;
+            const uint32_t m = max(max(__float_as_uint(v.x) & sign, __float_as_uint(v.y) & sign),
+                                   max(__float_as_uint(v.z) & sign, __float_as_uint(v.w) & sign));
+            const int ex = magic::act8::block_exp(magic::act8::max8(m));
+            const uint32_t word = magic::act8::codes4(v.x, v.y, v.z, v.w, ex);
+            const int col = (kb * KCB + c) * 4, nb = (a.F + 31) / 32, ld = (int)a.ld_codes;
+            if (tile * 32 + r < a.n) {      // (a tile's offsets fit 32 bits: the weight in the LDS bounds F)
+                if (col < ld) *reinterpret_cast<uint32_t *>(a.codes + tile * 32 * ld + (r * ld + col)) = word;
+                if (c % 8 == 0 && col / 32 < nb) a.exps[tile * 32 * nb + (r * nb + col / 32)] = (uint8_t)ex;
+            }
+        }
     }
 }
 
-template <int KSB, int NCG, bool EP>
+template <int KSB, int NCG, bool EP, bool PACK>
 __global__ __launch_bounds__(strip_max_waves(KSB) * 64) void k_proj_strip(ProjArgs a, StripPlan p) {
     constexpr int KCB = 4 * KSB;       // 16-byte pieces per row and K block
     constexpr int LDO = NCG * 32 + 4;  // output strip row stride
@@ -135,7 +151,7 @@ __global__ __launch_bounds__(strip_max_waves(KSB) * 64) void k_proj_strip(ProjAr
         while (true) {
             // ---- this unit into the strip; the next one's loads go out before the matrix work starts
             __builtin_amdgcn_wave_barrier();
-            write_unit<KSB>(a, t, kb, lane, u, xs);
+            write_unit<KSB, PACK>(a, t, kb, lane, u, xs);
             int64_t tn = t;
             int kbn = kb + 1;
             if (kbn == p.nkb) kbn = 0, tn = t + t_stride;
@@ -279,13 +295,19 @@ bool choose_strip(const ProjArgs &a, StripChoice &c) {
     return true;
 }
 
-template <int KSB, int NCG, bool EP> int launch_strip(const ProjArgs &a, const StripChoice &c, hipStream_t stream) {
-    if (magic::ensure_dynamic_lds((const void *)k_proj_strip<KSB, NCG, EP>, c.lds) != MAGIC_OK) return MAGIC_ERR_RUNTIME;
-    MAGIC_LAUNCH(a.name, (k_proj_strip<KSB, NCG, EP>), c.grid, c.plan.wpb * 64, c.lds, stream, a, c.plan);
+template <int KSB, int NCG, bool EP, bool PACK = false>
+int launch_strip(const ProjArgs &a, const StripChoice &c, hipStream_t stream) {
+    if (magic::ensure_dynamic_lds((const void *)k_proj_strip<KSB, NCG, EP, PACK>, c.lds) != MAGIC_OK) return MAGIC_ERR_RUNTIME;
+    MAGIC_LAUNCH(a.name, (k_proj_strip<KSB, NCG, EP, PACK>), c.grid, c.plan.wpb * 64, c.lds, stream, a, c.plan);
     return magic::launch_status();
 }
 
 template <int KSB> int launch_ksb(const ProjArgs &a, const StripChoice &c, bool ep, hipStream_t stream) {
+    if constexpr (KSB % 2 == 0) {
+        if (a.codes) return c.ncg == 1   ? launch_strip<KSB, 1, false, true>(a, c, stream)
+                            : c.ncg == 2 ? launch_strip<KSB, 2, false, true>(a, c, stream)
+                                         : launch_strip<KSB, 3, false, true>(a, c, stream);
+    }
     switch (c.ncg) {
         case 1: return ep ? launch_strip<KSB, 1, true>(a, c, stream) : launch_strip<KSB, 1, false>(a, c, stream);
         case 2: return ep ? launch_strip<KSB, 2, true>(a, c, stream) : launch_strip<KSB, 2, false>(a, c, stream);
@@ -303,9 +325,19 @@ namespace magic {
 // `n_part` receives the number of partial-sum rows an epilogue launch writes (one per wave of the grid),
 // `n_win` the number of column windows (always 1 here).  With `dry_run` nothing is launched.
 // MAGIC_PROJ_STRIP=0 in the environment switches the kernel off (A/B timing in one process).
-int proj_strip_try(const ProjArgs &a0, int64_t *n_part, int *n_win, bool dry_run, hipStream_t stream) {
+static bool strip_off() {
     const char *off = std::getenv("MAGIC_PROJ_STRIP");
-    if (off && off[0] == '0') return MAGIC_ERR_UNSUPPORTED;
+    return off && off[0] == '0';
+}
+
+// the streaming kernel takes the shape and can write its 8-bit codes on the way (K blocks of whole 32-column blocks)
+bool proj_strip_packs(const ProjArgs &a) {
+    StripChoice c;
+    return !strip_off() && !has_epilogue(a) && choose_strip(a, c) && c.ksb % 2 == 0;
+}
+
+int proj_strip_try(const ProjArgs &a0, int64_t *n_part, int *n_win, bool dry_run, hipStream_t stream) {
+    if (strip_off()) return MAGIC_ERR_UNSUPPORTED;
     ProjArgs a = a0;
     a.col0 = 0;
     StripChoice c;

@@ -217,11 +217,11 @@ class _LinearAct8Fn(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, x, w):
-        x = _lib.full_rows(x)
-        y, _, _ = _lib.proj_fwd(x, w, w.shape[0], 0, 0)
         codes = exps = None
         if ctx.needs_input_grad[1]:
-            codes, exps = _lib.act8_pack(x)
+            y, codes, exps = _lib.act8_linear_fwd(x, w)
+        else:
+            y, _, _ = _lib.proj_fwd(_lib.full_rows(x), w, w.shape[0], 0, 0)
         ctx.save_for_backward(codes, exps, w)
         return y
 

@@ -155,3 +155,21 @@ def test_expanded_and_overlapping_rows(cuda):
     window = torch.randn(89, device=cuda).as_strided((50, 40), (1, 1))
     assert torch.equal(act8_pack(window).codes, act8_pack(window.contiguous()).codes)
     assert torch.equal(linear_nobias(row.expand(50, 40), w, act_bits=8), linear_nobias(row.repeat(50, 1), w, act_bits=8))
+
+
+@pytest.mark.parametrize("m", [1, 40, 64, 96, 130])
+@pytest.mark.parametrize("n,f,pad", [(1, 32, 0), (33, 64, 0), (700, 176, 0), (259, 192, 4), (64, 52, 12), (97, 96, 0), (65, 100, 3),
+                                     (2000, 256, 0)])
+def test_codes_written_beside_the_product(cuda, n, f, pad, m):
+    """The product's pass over x writes the codes that a pass of its own writes, whichever kernel takes the shape."""
+    from magic_amd import _lib
+    gen = torch.Generator(device=cuda).manual_seed(f + m)
+    x = (torch.randn(n, f + pad, generator=gen, device=cuda) * torch.exp2(torch.randint(-30, 30, (n, 1), generator=gen, device=cuda).float()))[:, :f]
+    x[n // 2, f // 3] = float("inf")
+    x[n - 1, :] = 0.0
+    w = torch.randn(m, f, generator=gen, device=cuda)
+    y, codes, exps = _lib.act8_linear_fwd(x, w)
+    want = _lib.act8_pack(x)
+    assert torch.equal(codes, want[0]) and torch.equal(exps, want[1])
+    assert torch.equal(y.view(torch.int32), _lib.proj_fwd(x, w, m, 0, 0)[0].view(torch.int32))
+    assert torch.ops.magic.act8_unpack(codes, exps, f).shape == (n, f)

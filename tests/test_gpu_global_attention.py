@@ -103,7 +103,7 @@ def test_model_with_global_attention(cuda, bits):
         assert torch.equal(model.embed(make()), plain.embed(make()))      # the block starts as the identity
     # and so does training, up to the order of the layer-by-layer path's sums
     l0, l1 = plain.compute_loss(make(), **kw), model.compute_loss(make(), **kw)
-    assert abs(float(l0) - float(l1)) < 1e-5 * abs(float(l0))
+    assert abs(l0.item() - l1.item()) < 1e-5 * abs(l0.item())
     with torch.no_grad():
         model.global_attn.out.weight.normal_(std=0.1)
     loss, parts = model.compute_loss(make(), return_parts=True, **kw)

@@ -2,6 +2,7 @@
 // Calls the argument checking and the empty-input paths of the C ABI -- every call here must return before a
 // kernel is launched or device memory is touched, so it runs on a machine without a GPU -- and checks the
 // status codes.  What ASan watches is the host code of the wrappers: plan structs, argument copies, name tables.
+#include <cmath>
 #include <cstdio>
 #include <cstring>
 #include <vector>
@@ -144,6 +145,72 @@ int main() {
     EXPECT(magic_knn_topk(100, 4, 64, 200, dummy, 64, dummy, 64, 0, (double *)dummy, (int64_t *)dummy, nullptr, 0, nullptr),
            MAGIC_ERR_INVALID_ARG);  // k > n_train
     EXPECT(magic_knn_merge(4, 0, 2, nullptr, nullptr, nullptr, nullptr, nullptr), MAGIC_ERR_INVALID_ARG);
+    // segment attention: every field that would be read out of bounds, or by no kernel, is refused before a launch
+    const int32_t tab[8] = {0, 4, 0, 4, 0, 0, 4, 0};
+    magic_attn at;
+    std::memset(&at, 0, sizeof at);
+    at.q_heads = 4, at.kv_heads = 2, at.head_dim = 16, at.n_q = at.n_k = 4;
+    at.q = at.k = at.v = dummy;
+    at.ld_q = 64, at.hs_q = 16, at.ld_k = at.ld_v = 32, at.hs_k = at.hs_v = 16;
+    at.scale = 0.25f;
+    at.q_tiles = at.k_tiles = tab, at.n_q_tiles = at.n_k_tiles = 1, at.max_q = at.max_k = 4, at.n_seg = 1;
+    (void)magic_attn_fwd_workspace_bytes(&at);
+    (void)magic_attn_bwd_workspace_bytes(&at);
+    (void)magic_attn_fwd_workspace_bytes(nullptr);
+    EXPECT(magic_attn_fwd(nullptr, dummy, 64, 16, dummy, nullptr, 0, nullptr), MAGIC_ERR_INVALID_ARG);
+    EXPECT(magic_attn_fwd(&at, nullptr, 64, 16, dummy, nullptr, 0, nullptr), MAGIC_ERR_INVALID_ARG);
+    EXPECT(magic_attn_fwd(&at, dummy, 63, 16, dummy, nullptr, 0, nullptr), MAGIC_ERR_INVALID_ARG);
+    auto attn = [&](auto change) {
+        magic_attn b = at;
+        change(b);
+        return magic_attn_fwd(&b, dummy, 64, 16, dummy, nullptr, 0, nullptr);
+    };
+    EXPECT(attn([](magic_attn &b) { b.dtype = 7; }), MAGIC_ERR_UNSUPPORTED);
+    EXPECT(attn([](magic_attn &b) { b.kv_heads = 3; }), MAGIC_ERR_INVALID_ARG);
+    EXPECT(attn([](magic_attn &b) { b.q_heads = 0; }), MAGIC_ERR_INVALID_ARG);
+    EXPECT(attn([](magic_attn &b) { b.q_heads = b.kv_heads = 8200; }), MAGIC_ERR_UNSUPPORTED);
+    EXPECT(attn([](magic_attn &b) { b.head_dim = 12; }), MAGIC_ERR_UNSUPPORTED);
+    EXPECT(attn([](magic_attn &b) { b.head_dim = 136; }), MAGIC_ERR_UNSUPPORTED);
+    EXPECT(attn([](magic_attn &b) { b.n_q = -1; }), MAGIC_ERR_INVALID_ARG);
+    EXPECT(attn([](magic_attn &b) { b.n_k = 0x7fffffff; }), MAGIC_ERR_INVALID_ARG);
+    EXPECT(attn([](magic_attn &b) { b.v = nullptr; }), MAGIC_ERR_INVALID_ARG);
+    EXPECT(attn([](magic_attn &b) { b.k = (const char *)b.k + 4; }), MAGIC_ERR_INVALID_ARG);
+    EXPECT(attn([](magic_attn &b) { b.ld_k = 30; }), MAGIC_ERR_INVALID_ARG);
+    EXPECT(attn([](magic_attn &b) { b.ld_q = (1 << 22) + 4; }), MAGIC_ERR_UNSUPPORTED);
+    EXPECT(attn([](magic_attn &b) { b.q_tiles = nullptr; }), MAGIC_ERR_INVALID_ARG);
+    EXPECT(attn([](magic_attn &b) { b.n_k_tiles = 0; }), MAGIC_ERR_INVALID_ARG);
+    EXPECT(attn([](magic_attn &b) { b.cap = -1.f; }), MAGIC_ERR_INVALID_ARG);
+    EXPECT(attn([](magic_attn &b) { b.cap = 1e-9f; }), MAGIC_ERR_INVALID_ARG);
+    EXPECT(attn([](magic_attn &b) { b.scale = INFINITY; }), MAGIC_ERR_INVALID_ARG);
+    EXPECT(attn([&](magic_attn &b) { b.slopes = dummy; }), MAGIC_ERR_INVALID_ARG);  // no positions
+    EXPECT(magic_attn_bwd(&at, dummy, 64, 16, dummy, dummy, 64, 16, dummy, dummy, nullptr, nullptr, nullptr, 0, nullptr),
+           MAGIC_ERR_INVALID_ARG);  // dk without dv
+    EXPECT(magic_attn_bwd(&at, dummy, 64, 16, dummy, dummy, 64, 16, dummy, dummy, dummy, dummy, nullptr, 0, nullptr),
+           MAGIC_ERR_INVALID_ARG);  // a slope gradient without slopes
+    EXPECT(magic_attn_bwd(&at, dummy, 64, 16, dummy, dummy, 64, 16, dummy, dummy, dummy, nullptr, nullptr, 0, nullptr),
+           MAGIC_ERR_WORKSPACE);
+    // head norm + rotation, 8-bit checkpoints
+    EXPECT(magic_head_norm_rope_fwd(4, 4, 2, 16, 18, MAGIC_F32, dummy, 64, 16, dummy, 32, 16, dummy, dummy, (const int32_t *)dummy,
+                                    1e-6, 1e4, dummy, dummy, nullptr),
+           MAGIC_ERR_INVALID_ARG);  // more turned columns than there are
+    EXPECT(magic_head_norm_rope_fwd(4, 4, 2, 16, 16, MAGIC_F32, nullptr, 64, 16, dummy, 32, 16, dummy, dummy, (const int32_t *)dummy,
+                                    1e-6, 1e4, dummy, dummy, nullptr),
+           MAGIC_ERR_INVALID_ARG);
+    EXPECT(magic_head_norm_rope_bwd(4, 4, 2, 16, 16, MAGIC_F32, dummy, 64, 16, dummy, 32, 16, dummy, dummy, (const int32_t *)dummy,
+                                    1e-6, 1e4, dummy, 64, 16, dummy, 32, 16, dummy, dummy, dummy, dummy, nullptr, 0, nullptr),
+           MAGIC_ERR_WORKSPACE);
+    EXPECT(magic_act8_pack(4, 0, dummy, 40, (int8_t *)dummy, (uint8_t *)dummy, nullptr), MAGIC_ERR_INVALID_ARG);
+    EXPECT(magic_act8_pack(4, 40, dummy, 39, (int8_t *)dummy, (uint8_t *)dummy, nullptr), MAGIC_ERR_INVALID_ARG);
+    EXPECT(magic_act8_pack(4, 40, dummy, 40, (int8_t *)dummy + 1, (uint8_t *)dummy, nullptr), MAGIC_ERR_INVALID_ARG);
+    EXPECT(magic_act8_linear_fwd(4, 40, 8, dummy, 40, dummy, dummy, 8, nullptr, (uint8_t *)dummy, nullptr, 0, nullptr),
+           MAGIC_ERR_INVALID_ARG);
+    EXPECT(magic_act8_linear_fwd(4, 40, 8, dummy, 39, dummy, dummy, 8, (int8_t *)dummy, (uint8_t *)dummy, nullptr, 0, nullptr),
+           MAGIC_ERR_INVALID_ARG);
+    EXPECT(magic_act8_unpack(4, 40, nullptr, (uint8_t *)dummy, dummy, 40, nullptr), MAGIC_ERR_INVALID_ARG);
+    EXPECT(magic_act8_weight_grad(4, 8, 40, dummy, 7, (int8_t *)dummy, (uint8_t *)dummy, dummy, nullptr, 0, nullptr),
+           MAGIC_ERR_INVALID_ARG);
+    EXPECT(magic_act8_weight_grad(4, 8, 40, dummy, 8, (int8_t *)dummy, (uint8_t *)dummy, dummy, nullptr, 0, nullptr),
+           MAGIC_ERR_WORKSPACE);
     std::printf(failures ? "asan_args: %d failure(s)\n" : "asan_args: ok\n", failures);
     return failures ? 1 : 0;
 }
