@@ -128,7 +128,7 @@ __device__ __forceinline__ void sum_slope(const double *part, int64_t n, int H, 
 
 // What a lane knows of its row in the dq sweep
 struct RowSide {
-    float s_in, dp_in, scale, cap, f_cap, slope;   // f_cap: -scale / cap^2, for scale (1 - tanh^2) from the capped score
+    float s_in, dp_in, scale, f_cap, slope;   // f_cap: -scale / cap^2, for scale (1 - tanh^2) from the capped score
     uint32_t pos;
     float lse, delta;
 };
@@ -143,9 +143,9 @@ struct SlopeSums {
 // Scores and do.v of 32 keys by 32 rows -> gradients of the scores (before the scale of dq); km, kp: the keys' masks
 // (0 / -inf) and positions, four for every group of registers
 template <typename M, bool CAP, bool BIAS, bool MASK>
-__device__ __forceinline__ void score_grad(f32x16_t &s, const f32x16_t &dp, const RowSide &c, const f32x4_t *km,
-                                           const i32x4_t *kp, float (&ds)[16], SlopeSums &sums) {
-    if (CAP) cap_tile<M::N == 1>(s, c.s_in, c.cap);
+__device__ __forceinline__ void score_grad(f32x16_t &s, const f32x16_t &dp, const RowSide &c, const Cap<M::N == 1> &cap,
+                                           const f32x4_t *km, const i32x4_t *kp, float (&ds)[16], SlopeSums &sums) {
+    if (CAP) cap_tile(s, cap);
     float t_dsl = 0.f, t_dl = 0.f, t_pd = 0.f;
 #pragma unroll
     for (int g = 0; g < 4; ++g) {
@@ -178,9 +178,9 @@ __device__ __forceinline__ void score_grad(f32x16_t &s, const f32x16_t &dp, cons
 // The same with the keys in the lanes: probabilities (times 2^14 in the scaled mode) and score gradients; l, d: minus lse
 // and minus D of the rows, qp their positions
 template <typename M, bool CAP, bool BIAS>
-__device__ __forceinline__ void prob_grad(f32x16_t &s, const f32x16_t &dp, const RowSide &c, const f32x4_t *l, const f32x4_t *d,
-                                          const i32x4_t *qp, float (&pr)[16], float (&ds)[16]) {
-    if (CAP) cap_tile<M::N == 1>(s, c.s_in, c.cap);
+__device__ __forceinline__ void prob_grad(f32x16_t &s, const f32x16_t &dp, const RowSide &c, const Cap<M::N == 1> &cap,
+                                          const f32x4_t *l, const f32x4_t *d, const i32x4_t *qp, float (&pr)[16], float (&ds)[16]) {
+    if (CAP) cap_tile(s, cap);
 #pragma unroll
     for (int g = 0; g < 4; ++g) {
         const f32x4_t l4 = l[2 * g], d4 = d[2 * g];
@@ -273,6 +273,7 @@ __global__ __launch_bounds__(64 * WM *KG, (DP == 128 && M::N > 1) || (DP >= 64 &
     const float slope = bias ? a.slopes[h] : 0.f;
     const uint32_t qpos = bias ? flip(a.q_pos[qr]) : 0u;
     const float f_cap = a.cap > 0.f ? -a.scale / a.cap / a.cap : 0.f;
+    const Cap<M::N == 1> cap(sc.s_in, a.cap);
     Running run;
     SlopeSums sums;
     f32x16_t acc[DB];
@@ -328,19 +329,19 @@ __global__ __launch_bounds__(64 * WM *KG, (DP == 128 && M::N > 1) || (DP >= 64 &
             }
             feed<2 * NP, 2 * PRODUCTS<M>, KS>();
             float ds[16];
-            const RowSide rs = {sc.s_in, sc.dp_in, a.scale, a.cap, f_cap, slope, qpos, ls, dl0};
+            const RowSide rs = {sc.s_in, sc.dp_in, a.scale, f_cap, slope, qpos, ls, dl0};
             const f32x4_t *km = reinterpret_cast<const f32x4_t *>(sMask + 32 * b + 4 * hf);
             const i32x4_t *kp = reinterpret_cast<const i32x4_t *>(sPos + 32 * b + 4 * hf);
             if (a.cap > 0.f) {
                 if (bias)
-                    masked ? score_grad<M, true, true, true>(s, dp, rs, km, kp, ds, sums) : score_grad<M, true, true, false>(s, dp, rs, km, kp, ds, sums);
+                    masked ? score_grad<M, true, true, true>(s, dp, rs, cap, km, kp, ds, sums) : score_grad<M, true, true, false>(s, dp, rs, cap, km, kp, ds, sums);
                 else
-                    masked ? score_grad<M, true, false, true>(s, dp, rs, km, kp, ds, sums) : score_grad<M, true, false, false>(s, dp, rs, km, kp, ds, sums);
+                    masked ? score_grad<M, true, false, true>(s, dp, rs, cap, km, kp, ds, sums) : score_grad<M, true, false, false>(s, dp, rs, cap, km, kp, ds, sums);
             } else {
                 if (bias)
-                    masked ? score_grad<M, false, true, true>(s, dp, rs, km, kp, ds, sums) : score_grad<M, false, true, false>(s, dp, rs, km, kp, ds, sums);
+                    masked ? score_grad<M, false, true, true>(s, dp, rs, cap, km, kp, ds, sums) : score_grad<M, false, true, false>(s, dp, rs, cap, km, kp, ds, sums);
                 else
-                    masked ? score_grad<M, false, false, true>(s, dp, rs, km, kp, ds, sums) : score_grad<M, false, false, false>(s, dp, rs, km, kp, ds, sums);
+                    masked ? score_grad<M, false, false, true>(s, dp, rs, cap, km, kp, ds, sums) : score_grad<M, false, false, false>(s, dp, rs, cap, km, kp, ds, sums);
             }
             float u = 1.f;
             if constexpr (M::SCALED) {
@@ -474,6 +475,7 @@ __global__ __launch_bounds__(64 * WM *KG, DP == 128 || (DP >= 64 && KG > 1) ? 1 
     const bool bias = a.slopes != nullptr;
     const uint32_t kpos = bias ? flip(a.k_pos[kr]) : 0u;
     const float f_cap = a.cap > 0.f ? -a.scale / a.cap / a.cap : 0.f;
+    const Cap<M::N == 1> cap(sc.s_in, a.cap);
     Running run;
     f32x16_t gk[DB], gv[DB];
 #pragma unroll
@@ -534,14 +536,14 @@ __global__ __launch_bounds__(64 * WM *KG, DP == 128 || (DP >= 64 && KG > 1) ? 1 
             }
             feed<2 * NP, 2 * PRODUCTS<M>, KS>();
             float pr[16], ds[16];
-            const RowSide ks = {sc.s_in, sc.dp_in, a.scale, a.cap, f_cap, slope, kpos, 0.f, 0.f};
+            const RowSide ks = {sc.s_in, sc.dp_in, a.scale, f_cap, slope, kpos, 0.f, 0.f};
             const f32x4_t *l4 = reinterpret_cast<const f32x4_t *>(sL + 32 * b + 4 * hf);
             const f32x4_t *d4 = reinterpret_cast<const f32x4_t *>(sD + 32 * b + 4 * hf);
             const i32x4_t *qp = reinterpret_cast<const i32x4_t *>(sPos + 32 * b + 4 * hf);
             if (a.cap > 0.f)
-                bias ? prob_grad<M, true, true>(s, dp, ks, l4, d4, qp, pr, ds) : prob_grad<M, true, false>(s, dp, ks, l4, d4, qp, pr, ds);
+                bias ? prob_grad<M, true, true>(s, dp, ks, cap, l4, d4, qp, pr, ds) : prob_grad<M, true, false>(s, dp, ks, cap, l4, d4, qp, pr, ds);
             else
-                bias ? prob_grad<M, false, true>(s, dp, ks, l4, d4, qp, pr, ds) : prob_grad<M, false, false>(s, dp, ks, l4, d4, qp, pr, ds);
+                bias ? prob_grad<M, false, true>(s, dp, ks, cap, l4, d4, qp, pr, ds) : prob_grad<M, false, false>(s, dp, ks, cap, l4, d4, qp, pr, ds);
             float u = 1.f;
             if constexpr (M::SCALED) {
                 run.step<DB>(ds, gk);

@@ -24,8 +24,8 @@ int check(const magic_attn *a) {
     const int per = a->dtype == MAGIC_F32 ? 4 : 8;   // rows and heads start on 16-byte addresses
     if (((uintptr_t)a->q | (uintptr_t)a->k | (uintptr_t)a->v) & 15) return MAGIC_ERR_INVALID_ARG;
     if ((a->ld_q | a->hs_q | a->ld_k | a->hs_k | a->ld_v | a->hs_v) % per) return MAGIC_ERR_INVALID_ARG;
-    // (scale / cap and cap times a series' terms stay normal float32 numbers)
-    if (!(a->cap == 0.f || (a->cap >= 1e-3f && a->cap <= 1e30f)) || !std::isfinite(a->scale)) return MAGIC_ERR_INVALID_ARG;
+    // (scale / cap and cap times a polynomial's terms stay normal float32 numbers)
+    if (!(a->cap == 0.f || (a->cap >= 1e-3f && a->cap <= 1e30f)) || !(std::fabs(a->scale) <= 1e30f)) return MAGIC_ERR_INVALID_ARG;
     if (a->slopes && ((a->n_q > 0 && !a->q_pos) || (a->n_k > 0 && !a->k_pos))) return MAGIC_ERR_INVALID_ARG;
     return MAGIC_OK;
 }
@@ -395,6 +395,7 @@ __global__ __launch_bounds__(64 * WM *KG, DP == 128 && (M::N > 1 || WM == 1) ? 1
     const uint32_t qpos = bias ? flip(a.q_pos[q0 + (ok ? row : 0)]) : 0u;
     const float unscale = 1.f / sq * (1.f / sk);
     const float s_in = (a.cap > 0.f ? a.scale / a.cap : a.scale) * unscale;
+    const Cap<M::N == 1> cap(s_in, a.cap);
     constexpr float P_EXP = M::SCALED ? 14.f : 0.f;       // probabilities are formed times 2^14
 
     f32x16_t o[DB];
@@ -459,7 +460,7 @@ __global__ __launch_bounds__(64 * WM *KG, DP == 128 && (M::N > 1 || WM == 1) ? 1
 #pragma unroll
         for (int b = 0; b < KB; ++b) {
             if (a.cap > 0.f) {
-                cap_tile<M::N == 1>(s[b], s_in, a.cap);
+                cap_tile(s[b], cap);
             } else {
 #pragma unroll
                 for (int r = 0; r < 16; ++r) s[b][r] *= s_in;

@@ -111,8 +111,8 @@ def segment_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, plan: A
     Differentiable in q, k, v and slopes; the sums have a fixed order."""
     if scale is None:
         scale = 1.0 / math.sqrt(q.shape[-1])
-    if not math.isfinite(scale):
-        raise _lib.MagicHipError(f"scale must be finite (got {scale})")
+    if not abs(scale) <= 1e30:
+        raise _lib.MagicHipError(f"scale must be at most 1e30 in size (got {scale})")
     return _SegmentAttentionFn.apply(q, k, v, slopes, plan, float(scale), float(cap), q_pos, k_pos, key_mask)
 
 

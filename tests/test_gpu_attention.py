@@ -431,6 +431,24 @@ def test_caps_far_from_the_scores(cuda, cap):
     check(got, q, k, v, d, [40], [40], cap=cap if cap < 1 else 0.0)
 
 
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=["f32", "bf16"])
+@pytest.mark.parametrize("cap", [1e9, 4e9, 1e20])
+def test_capped_scores_of_many_millions(cuda, cap, dtype):
+    """Scores of 4e8 and 2e8, capped at some times as much: one key takes the whole probability (2^-1e8 of it is left for
+    the other, which gets exact zeros).  The output is its value: p v / p, with a rounding for p v, one for the quotient
+    and one for the result's type.  (Nothing is promised of the winning key's gradients: a logit of 4e8 is off by 4 u 4e8 =
+    95, and e^95 = 2^137 is no float32 number.)"""
+    from magic_amd.model.attention import attention_plan, segment_attention
+    q = torch.full((3, 1, 16), 1e4, device=cuda).to(dtype).requires_grad_(True)
+    k = torch.tensor([0.5e4, 1e4], device=cuda).view(2, 1, 1).expand(2, 1, 16).to(dtype).contiguous().requires_grad_(True)
+    v = torch.randn(2, 1, 16, device=cuda).to(dtype).requires_grad_(True)
+    out = segment_attention(q, k, v, attention_plan([3], [2], cuda), cap=cap)
+    want = v.detach()[1:].expand(3, 1, 16).double()
+    assert ((out.double() - want).abs() <= (2.01 * U + torch.finfo(dtype).eps / 2) * want.abs()).all()
+    dq, dk, dv = torch.autograd.grad(out, (q, k, v), torch.ones_like(out))
+    assert not dk[0].any() and not dv[0].any()
+
+
 def test_attention_serves_without_rows_or_keys(cuda):
     from magic_amd.model.attention import attention_plan, segment_attention
     q, k, v, d, _ = make(cuda, [5], [7], 4, 2, 16, torch.float32)
