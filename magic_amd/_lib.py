@@ -1174,7 +1174,9 @@ def head_norm_rope_bwd_checked(q, k, wq, wk, pos, rotary_dim, eps, base, dyq, dy
 # ------------------------------------------------------------------------------------- 8-bit activation checkpoints
 def full_rows(t: torch.Tensor) -> torch.Tensor:
     """2-D operand with unit inner stride whose rows do not overlap (an expanded one is copied)."""
-    return t if t.stride(1) == 1 and (t.stride(0) >= t.shape[1] or t.shape[0] <= 1) else t.contiguous()
+    if t.stride(1) == 1 and t.stride(0) >= t.shape[1]:
+        return t
+    return t.contiguous().as_strided(t.shape, (max(t.shape[1], 1), 1))     # (a single row keeps any stride otherwise)
 
 
 def act8_pack(x: torch.Tensor):

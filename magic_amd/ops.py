@@ -469,6 +469,11 @@ _register("readout", "(Tensor feat, Tensor? node_type, int n_types, bool mean) -
 # ------------------------------------------------------------------------------------- global-attention block
 # The plan of segment attention travels as its two tile tables and longest segments; operands and results as in ``_lib.attn_fwd``.
 def _attn_plan(q, k, q_tiles, k_tiles, max_q, max_k, n_seg):
+    for name, t in (("q_tiles", q_tiles), ("k_tiles", k_tiles)):
+        if t.dtype != torch.int32 or t.dim() != 2 or t.shape[1] != 8 or not t.is_contiguous() or t.device != q.device:
+            raise _lib.MagicHipError(f"{name} must be a contiguous int32 [tiles, 8] table of an AttentionPlan on {q.device}")
+    if min(max_q, max_k, n_seg) < 0 or max_q > q.shape[0] or max_k > k.shape[0]:
+        raise _lib.MagicHipError(f"longest segments {max_q}, {max_k} of {n_seg} do not fit {q.shape[0]} and {k.shape[0]} rows")
     return SimpleNamespace(q_tiles=q_tiles, k_tiles=k_tiles, n_q=q.shape[0], n_k=k.shape[0], device=q_tiles.device,
                            max_q=max_q, max_k=max_k, n_seg=n_seg)
 

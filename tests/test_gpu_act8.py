@@ -173,3 +173,19 @@ def test_codes_written_beside_the_product(cuda, n, f, pad, m):
     assert torch.equal(codes, want[0]) and torch.equal(exps, want[1])
     assert torch.equal(y.view(torch.int32), _lib.proj_fwd(x, w, m, 0, 0)[0].view(torch.int32))
     assert torch.ops.magic.act8_unpack(codes, exps, f).shape == (n, f)
+
+
+def test_linear_of_one_row_and_of_none(cuda):
+    from magic_amd.model.gat import linear_nobias
+    w = torch.randn(6, 40, device=cuda, requires_grad=True)
+    col = torch.randn(40, 1, device=cuda)
+    x = col.t().requires_grad_(True)                     # one row, row stride 1
+    y = linear_nobias(x, w, act_bits=8)
+    dx, dw = torch.autograd.grad(y, (x, w), torch.randn(6, 1, device=cuda).t())
+    assert torch.equal(y.detach(), linear_nobias(col.t().clone().view(1, 40), w.detach())) and torch.isfinite(dx).all() and torch.isfinite(dw).all()
+    with torch.no_grad():
+        assert torch.equal(linear_nobias(col.t(), w, act_bits=8), y)
+    none = torch.zeros(0, 40, device=cuda, requires_grad=True)
+    y = linear_nobias(none, w, act_bits=8)
+    dx, dw = torch.autograd.grad(y.sum(), (none, w))
+    assert y.shape == (0, 6) and dx.shape == (0, 40) and not dw.any()

@@ -449,6 +449,57 @@ def test_capped_scores_of_many_millions(cuda, cap, dtype):
     assert not dk[0].any() and not dv[0].any()
 
 
+def test_registered_operators_check_their_tables(cuda):
+    from magic_amd._lib import MagicHipError
+    from magic_amd.model.attention import attention_plan
+    q, k, v, _, _ = make(cuda, [9], [9], 2, 2, 16, torch.float32)
+    p = attention_plan([9], device=cuda)
+    call = lambda qt, kt, mq, mk, ns: torch.ops.magic.attn_fwd(q, k, v, qt, kt, mq, mk, ns, 0.25, 0.0, None, None, None, None)  # noqa: E731
+    call(p.q_tiles, p.k_tiles, 9, 9, 1)
+    for bad in ((p.q_tiles.long(), p.k_tiles, 9, 9, 1), (p.q_tiles, p.k_tiles[:, :7], 9, 9, 1), (p.q_tiles.cpu(), p.k_tiles, 9, 9, 1),
+                (p.q_tiles[:0], p.k_tiles, 9, 9, 1), (p.q_tiles, p.k_tiles, 10, 9, 1), (p.q_tiles, p.k_tiles, 9, 9, -1)):
+        with pytest.raises(MagicHipError):
+            call(*bad)
+
+
+def test_attention_one_tensor_thrice_broadcast_operands_and_gradients(cuda):
+    """q, k and v the same leaf; slopes, positions and masks as views; the expanded gradient of a sum; no segment."""
+    from magic_amd.model.attention import attention_plan, segment_attention
+    lens = [5, 40, 1]
+    x = torch.randn(46, 2, 16, device=cuda)
+    plan = attention_plan(lens, device=cuda)
+    slopes, pos = torch.full((1,), 0.25, device=cuda), torch.arange(92, device=cuda, dtype=torch.int32)
+    mask = torch.rand(46, 2, device=cuda) < 0.7
+    views = dict(slopes=slopes.expand(2), q_pos=pos[::2], k_pos=pos[::2], key_mask=mask[:, 0])
+    plain = {n: t.contiguous() for n, t in views.items()}
+    leaf = x.clone().requires_grad_(True)
+    segment_attention(leaf, leaf, leaf, plan, **views).sum().backward()
+    parts = [x.clone().requires_grad_(True) for _ in range(3)]
+    out = segment_attention(*parts, plan, **plain)
+    want = torch.autograd.grad(out, parts, torch.ones_like(out))
+    assert torch.allclose(leaf.grad, want[0] + want[1] + want[2], rtol=1e-6, atol=1e-6)       # (sums of three, any order)
+    none = segment_attention(x[:0], x[:0], x[:0], attention_plan([], device=cuda))
+    assert none.shape == (0, 2, 16)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=["f32", "bf16"])
+def test_calls_on_two_streams_at_once(cuda, dtype):
+    """Calls of two streams share no workspace: each gives the result it gives alone."""
+    sets = [([900, 700], 64), ([1, 640, 3], 64)]
+    jobs = [make(cuda, lens, lens, 4, 2, D, dtype, seed=i, slopes=True, mask=0.5) + (lens,) for i, (lens, D) in enumerate(sets)]
+    alone = [run(q, k, v, d, lens, lens, cap=20.0, **kw) for q, k, v, d, kw, lens in jobs]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in jobs]
+    for _ in range(4):
+        got = []
+        for s, (q, k, v, d, kw, lens) in zip(streams, jobs):
+            with torch.cuda.stream(s):
+                got.append(run(q, k, v, d, lens, lens, cap=20.0, **kw))
+        torch.cuda.synchronize()
+        for a, b in zip(got, alone):
+            assert all(torch.equal(a[n], b[n]) for n in b)
+
+
 def test_attention_serves_without_rows_or_keys(cuda):
     from magic_amd.model.attention import attention_plan, segment_attention
     q, k, v, d, _ = make(cuda, [5], [7], 4, 2, 16, torch.float32)
