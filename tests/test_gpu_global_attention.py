@@ -156,3 +156,45 @@ def test_training_loop_and_refusals(cuda):
     for bad in (lambda: GlobalAttention(60, 5), lambda: GlobalAttention(64, 4, act_bits=4)):
         with pytest.raises(_lib.MagicHipError):
             bad()
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_captured_training_step_of_the_block(cuda, bits):
+    """Forward and backward through autograd in a captured graph (scaled planes, gathered keys, rotation, 8-bit linear
+    layers), replayed on new inputs with eager steps between the replays."""
+    import magic_amd as G
+    from magic_amd.model.attention import GlobalAttention
+    torch.manual_seed(4)
+    lens = [650, 1, 90]
+    g = G.batch([G.graph((torch.zeros(1, dtype=torch.long), torch.zeros(1, dtype=torch.long)), num_nodes=n).to(cuda) for n in lens])
+    block = GlobalAttention(256, 4, act_bits=bits).to(cuda)
+    with torch.no_grad():
+        block.out.weight.normal_(std=1 / 16)
+    params = list(block.parameters())
+    draw = lambda: (torch.randn(sum(lens), 256, device=cuda), torch.randn(sum(lens), 256, device=cuda), torch.rand(sum(lens), device=cuda) < 0.6)  # noqa: E731
+
+    def step(x, d, mask):
+        y = block(g, x, key_mask=mask)
+        return [y.detach(), *torch.autograd.grad(y, [x] + params, d)]
+
+    ins = [t.clone() for t in draw()]
+    ins[0].requires_grad_(True)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        for _ in range(2):
+            step(*ins)
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        res = step(*ins)
+    for _ in range(4):
+        new = draw()
+        with torch.no_grad():
+            for a, b in zip(ins, new):
+                a.copy_(b)
+        graph.replay()
+        got = [t.clone() for t in res]
+        eager = step(new[0].requires_grad_(True), *new[1:])
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(got, eager))
