@@ -685,10 +685,15 @@ template <typename M, int DP, int WM, int KG, int NB> int run_dkv(BwdArgs &b, in
 }
 
 // 32 rows a block where tiles of 128 would leave most of the chip idle: the wavefronts share the rows and deal out the keys
-bool small_side(int64_t blocks) { return blocks < 256; }
+// Heads of more than 32 columns leave a CU room for one such block: one round of them at most.  Four heads, us of both
+// sweeps, 32 rows against 128: 64 wide, bfloat16, graphs of 500 nodes, 64 tiles 31 / 48, 80 tiles 52 / 48, one graph of 7,000
+// (220) 499 / 367; float32, 64 tiles 59 / 111, forty graphs of 100 (160) 72 / 47; 128 wide, float32, 64 tiles 160 / 174, 80
+// tiles 301 / 176.  16 wide: one graph of 7,000 503 / 570 in float32 and 216 / 279 in bfloat16, a hundred graphs of 100
+// (400 tiles) 33 / 23.
+bool small_side(const magic_attn &a, int64_t blocks) { return blocks <= (a.head_dim <= 32 ? 255 : 64); }
 
-int sub_tiles(int64_t tiles, int heads, int longest) {
-    if (!small_side(tiles * heads)) return 1;
+int sub_tiles(const magic_attn &a, int64_t tiles, int heads, int longest) {
+    if (!small_side(a, tiles * heads)) return 1;
     const int rows = longest < MAGIC_ATTN_TILE ? longest : MAGIC_ATTN_TILE;
     return rows > 32 ? (rows + 31) / 32 : 1;
 }
@@ -699,12 +704,12 @@ template <typename M, int DP> int sweeps(BwdArgs &b, bool last, hipStream_t st) 
     int rc = MAGIC_OK;
     if (full.n_q > 0 && b.dq) {
         b.a = gathered(&full, b.pr);
-        b.sub = sub_tiles(full.n_q_tiles, full.q_heads, full.max_q);
+        b.sub = sub_tiles(full, full.n_q_tiles, full.q_heads, full.max_q);
         if constexpr (M::SCALED) {
             b.sub = 1;
             rc = run_dq<M, DP, 4, 1>(b, st);
         } else {
-            const bool few = !b.pr.rg.q && small_side((int64_t)full.n_q_tiles * full.q_heads);
+            const bool few = !b.pr.rg.q && small_side(full, (int64_t)full.n_q_tiles * full.q_heads);
             if (!few) b.sub = 1;
             rc = few ? run_dq<M, DP, 1, KG>(b, st) : run_dq<M, DP, 4, 1>(b, st);
         }
@@ -718,8 +723,8 @@ template <typename M, int DP> int sweeps(BwdArgs &b, bool last, hipStream_t st) 
         if constexpr (M::SCALED) {
             rc = run_dkv<M, DP, 4, 1, NB>(b, slopes, st);
         } else {
-            const bool few = !b.pr.rg.q && b.n_split == 1 && small_side((int64_t)full.n_k_tiles * full.kv_heads);
-            if (few) b.sub = sub_tiles(full.n_k_tiles, full.kv_heads, full.max_k);
+            const bool few = !b.pr.rg.q && b.n_split == 1 && small_side(full, (int64_t)full.n_k_tiles * full.kv_heads);
+            if (few) b.sub = sub_tiles(full, full.n_k_tiles, full.kv_heads, full.max_k);
             rc = few ? run_dkv<M, DP, 1, KG, 1>(b, slopes, st) : run_dkv<M, DP, 4, 1, NB>(b, slopes, st);
         }
     }

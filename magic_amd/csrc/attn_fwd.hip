@@ -794,13 +794,26 @@ struct Shape {
     int64_t items;
 };
 
+// Tiles of 128 rows up to which blocks of 32 columns serve better: where those still find the chip empty.  Measured on
+// both sides with 4 heads, us of kernels, 32 columns against 128.  float32, 64 wide: four graphs of 500 nodes (64 tiles)
+// 33 / 36, one of 2,000 (64) 111 / 94, of 4,000 (128) 295 / 144; 128 wide: one of 128 nodes (4) 27 / 22, of 500 (16)
+// 84 / 63.  bfloat16, 64 wide: eight of 500 (128) 15 / 19, one of 4,000 (128) 62 / 59, forty of 100 (160) 16 / 10; 128
+// wide: one of 1,000 (32) 33 / 33, of 2,000 (64) 54 / 40.  Up to 32 wide: one of 7,000 (220), float32 213 / 188, bfloat16
+// 91 / 110, eight of 500 (128) 16 / 21 and 12 / 15, a hundred of 100 (400) 13 / 10 in bfloat16.
+int64_t few_tiles(const magic_attn *a) {
+    const bool f32 = a->dtype == MAGIC_F32;
+    if (a->head_dim <= 32) return 255;
+    if (a->head_dim <= 64) return f32 ? 48 : 128;
+    return f32 ? 0 : 32;
+}
+
 // How a call is cut: 128 rows of one head a block (wm 4), or 32 (row, head) columns with the keys dealt to its wavefronts
 // (wm 1), or up to four columns without matrix instructions (wm 0); then key ranges until there are enough blocks.
 Shape shape_of(const magic_attn *a) {
     Shape s;
     const int G = a->q_heads / a->kv_heads;
     const int64_t big = (int64_t)a->n_q_tiles * a->q_heads;
-    s.wm = big >= 256 && a->max_q > 32 ? 4 : 1;
+    s.wm = big > few_tiles(a) && a->max_q > 32 ? 4 : 1;
     if ((int64_t)a->max_q * G <= FEW) {
         s.wm = 0, s.gc = G, s.rows = a->max_q > 0 ? a->max_q : 1, s.cols = s.rows * G, s.sub = 1, s.n_hb = a->kv_heads;
         s.f16 = false;
@@ -823,15 +836,17 @@ Shape shape_of(const magic_attn *a) {
     if (s.sub < 1) s.sub = 1;
     s.n_hb = a->q_heads / s.gc;
     const int64_t blocks = (int64_t)a->n_q_tiles * s.sub * s.n_hb;
-    int64_t split = 512 / blocks;                      // two resident blocks a CU, all running at once
+    // the blocks that run at once: two a CU, one where their planes and registers fill it (float32 of more than 64 columns:
+    // one graph of 5,500 nodes, 172 tiles, 435 us whole, 458 us in halves)
+    const int64_t resident = a->dtype == MAGIC_F32 && a->head_dim > 64 && s.wm == 4 ? 256 : 512;
+    int64_t split = resident / blocks;
     const int64_t most = (a->max_k + 511) / 512;
     if (split > most) split = most;
     if (split > 256) split = 256;
-    if (s.wm == 4) split = 1;
     if (split < 1) split = 1;
     s.n_split = (int)split;
     s.items = blocks * split;
-    s.f16 = magic::attn::use_f16(a) && s.wm == 4 && s.n_split == 1 && a->n_k > 0;
+    s.f16 = magic::attn::use_f16(a) && s.wm == 4 && a->n_k > 0;
     return s;
 }
 
@@ -869,22 +884,21 @@ template <typename T, int DP> int run_few(FwdArgs &p, hipStream_t st) {
 
 template <typename M> int run(FwdArgs &p, int wm, hipStream_t st) {
     const int D = p.a.head_dim;
-    int rc;
-    if (wm == 4) {
-        rc = run_rows<M>(p, st);
-    } else if (wm == 0) {
+    if (wm == 4) return run_rows<M>(p, st);
+    if (wm == 0) {
         typedef typename M::T T;
-        rc = D <= 16 ? run_few<T, 16>(p, st) : D <= 32 ? run_few<T, 32>(p, st) : D <= 64 ? run_few<T, 64>(p, st) : run_few<T, 128>(p, st);
-    } else {
-        // wavefronts of a block: as many as leave the LDS room for two blocks a CU
-        constexpr int KG64 = M::N == 3 ? 2 : 4, KG128 = M::N == 3 ? 1 : 2;
-        rc = D <= 16   ? launch<M, 16, 1, 4, 32>(p, st)
-             : D <= 32 ? launch<M, 32, 1, 4, 32>(p, st)
-             : D <= 64 ? launch<M, 64, 1, KG64, 32>(p, st)
-                       : launch<M, 128, 1, KG128, 32>(p, st);
+        return D <= 16 ? run_few<T, 16>(p, st) : D <= 32 ? run_few<T, 32>(p, st) : D <= 64 ? run_few<T, 64>(p, st) : run_few<T, 128>(p, st);
     }
-    if (rc != MAGIC_OK || p.n_split == 1) return rc;
-    typedef typename M::T T;
+    // wavefronts of a block: as many as leave the LDS room for two blocks a CU
+    constexpr int KG64 = M::N == 3 ? 2 : 4, KG128 = M::N == 3 ? 1 : 2;
+    return D <= 16   ? launch<M, 16, 1, 4, 32>(p, st)
+           : D <= 32 ? launch<M, 32, 1, 4, 32>(p, st)
+           : D <= 64 ? launch<M, 64, 1, KG64, 32>(p, st)
+                     : launch<M, 128, 1, KG128, 32>(p, st);
+}
+
+template <typename T> int join(FwdArgs &p, hipStream_t st) {
+    const int D = p.a.head_dim;
     const int64_t grid = p.a.n_q * p.a.q_heads;
     if (grid > 0x7fffffffLL) return MAGIC_ERR_UNSUPPORTED;
     if (D <= 16)
@@ -905,9 +919,9 @@ extern "C" {
 size_t magic_attn_fwd_workspace_bytes(const magic_attn *a) {
     if (check(a) != MAGIC_OK || a->n_q == 0) return 256;
     const Shape s = shape_of(a);
-    if (s.n_split == 1) return (s.wm == 4 ? magic::attn::prepare_bytes(a, s.f16, false) : 0) + 256;
-    const size_t rows = (size_t)s.n_split * a->q_heads * a->n_q;
-    return magic::align_up(rows * a->head_dim * sizeof(float)) + magic::align_up(rows * sizeof(float)) + 256;
+    const size_t rows = s.n_split > 1 ? (size_t)s.n_split * a->q_heads * a->n_q : 0;
+    return magic::align_up(rows * a->head_dim * sizeof(float)) + magic::align_up(rows * sizeof(float)) +
+           (s.wm == 4 ? magic::attn::prepare_bytes(a, s.f16, false) : 0) + 256;
 }
 
 int magic_attn_fwd(const magic_attn *a, void *out, int64_t ld_out, int64_t hs_out, float *lse, void *workspace,
@@ -922,26 +936,28 @@ int magic_attn_fwd(const magic_attn *a, void *out, int64_t ld_out, int64_t hs_ou
     p.out = out, p.ld_o = ld_out, p.hs_o = hs_out, p.lse = lse;
     p.n_split = s.n_split, p.cols = s.cols, p.rows = s.rows, p.gc = s.gc, p.sub = s.sub, p.n_hb = s.n_hb, p.items = s.items;
     p.part_o = p.part_l = nullptr;
+    magic::Arena ar(workspace, workspace_bytes);
     if (s.n_split > 1) {
-        magic::Arena ar(workspace, workspace_bytes);
         const size_t rows = (size_t)s.n_split * a->q_heads * a->n_q;
         p.part_o = ar.take<float>(rows * a->head_dim);
         p.part_l = ar.take<float>(rows);
         if (!ar.ok()) return MAGIC_ERR_WORKSPACE;
     }
-    if (s.wm == 4 && s.n_split == 1) {
-        magic::Arena ar(workspace, workspace_bytes);
-        int rc = magic::attn::prepare(a, s.f16, nullptr, ar, p.pr, (hipStream_t)stream);
+    int rc = MAGIC_OK;
+    if (s.wm == 4) {
+        rc = magic::attn::prepare(a, s.f16, nullptr, ar, p.pr, (hipStream_t)stream);
         if (rc != MAGIC_OK) return rc;
         p.a = magic::attn::gathered(a, p.pr);
         if (s.f16) {
             rc = run_rows<F16x2>(p, (hipStream_t)stream);
             if (rc != MAGIC_OK) return rc;
             p.pr.rg.want_safe = false;         // the segments whose rows differ too much in size
-            return run_rows<F32x3>(p, (hipStream_t)stream);
         }
     }
-    return a->dtype == MAGIC_F32 ? run<F32x3>(p, s.wm, (hipStream_t)stream) : run<BF16>(p, s.wm, (hipStream_t)stream);
+    const bool f32 = a->dtype == MAGIC_F32;
+    rc = f32 ? run<F32x3>(p, s.wm, (hipStream_t)stream) : run<BF16>(p, s.wm, (hipStream_t)stream);
+    if (rc != MAGIC_OK || s.n_split == 1) return rc;
+    return f32 ? join<float>(p, (hipStream_t)stream) : join<magic::bf16_t>(p, (hipStream_t)stream);
 }
 
 }  // extern "C"

@@ -258,6 +258,22 @@ def test_attention_large_float32(cuda, D, hq, hk, opts):
         assert torch.isfinite(b["out"][2312:, hq // hk:]).all()
 
 
+@pytest.mark.parametrize("dtype,D,hq,hk", [(torch.float32, 64, 4, 2), (torch.float32, 128, 2, 1), (torch.float32, 40, 4, 4),
+                                           (torch.bfloat16, 128, 4, 4), (torch.bfloat16, 64, 16, 4)])
+@pytest.mark.parametrize("opts", ["plain", "all", "wide_range"])
+def test_few_long_segments(cuda, dtype, D, hq, hk, opts):
+    """Tiles of 128 rows whose keys are cut into ranges, beside a short and an empty segment; rows of very different
+    sizes in one segment (the scaled planes leave it to the other launch) and a segment whose keys are all masked."""
+    q_lens, kv_lens = [1700, 3, 0, 90], [1810, 600, 5, 90]
+    q, k, v, d, kw = make(cuda, q_lens, kv_lens, hq, hk, D, dtype, seed=D + hq, slopes=opts == "all", mask=None if opts == "plain" else 0.6)
+    if opts == "all":
+        kw["cap"] = 30.0
+    if opts == "wide_range":
+        k[:900] *= 2.0 ** -20
+        kw["key_mask"][1810:2410] = False
+    check(run(q, k, v, d, q_lens, kv_lens, **kw), q, k, v, d, q_lens, kv_lens, **kw)
+
+
 def test_attention_long_tail_of_small_probabilities(cuda):
     """A distance bias leaves thousands of keys whose terms are each below half a unit of the running sums: together they
     count.  Relative 2-norm error of a float32 result, as small as one formed with whole-row sums."""
