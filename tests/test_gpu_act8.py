@@ -189,3 +189,14 @@ def test_linear_of_one_row_and_of_none(cuda):
     y = linear_nobias(none, w, act_bits=8)
     dx, dw = torch.autograd.grad(y.sum(), (none, w))
     assert y.shape == (0, 6) and dx.shape == (0, 40) and not dw.any()
+
+
+def test_every_width_up_to_two_blocks(cuda):
+    """Row ends of every kind: the last columns of the last row are the tensor's last."""
+    from magic_amd.model.act8 import act8_pack, act8_unpack
+    for f in range(1, 70):
+        x = torch.randn(5, f, generator=torch.Generator().manual_seed(f))
+        a = act8_pack(x.to(cuda))
+        codes, exps = definition(x)
+        assert np.array_equal(a.codes.cpu().numpy(), codes) and np.array_equal(a.exps.cpu().numpy(), exps), f
+        assert np.array_equal(act8_unpack(a).cpu().double().numpy(), codes[:, :f] * 2.0 ** (np.repeat(exps, 32, 1)[:, :f] - 127.0)), f
