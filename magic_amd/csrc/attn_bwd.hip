@@ -737,11 +737,10 @@ template <typename M, int DP> int sweeps(BwdArgs &b, bool last, hipStream_t st) 
 
 template <typename M> int sweeps_of(BwdArgs &b, bool last, hipStream_t st) {
     const int D = b.a.head_dim;
-    if constexpr (!M::SCALED) {          // (use_f16: wider heads only)
-        if (D <= 16) return sweeps<M, 16>(b, last, st);
-        if (D <= 32) return sweeps<M, 32>(b, last, st);
-    }
-    return D <= 64 ? sweeps<M, 64>(b, last, st) : sweeps<M, 128>(b, last, st);
+    return D <= 16   ? sweeps<M, 16>(b, last, st)
+           : D <= 32 ? sweeps<M, 32>(b, last, st)
+           : D <= 64 ? sweeps<M, 64>(b, last, st)
+                     : sweeps<M, 128>(b, last, st);
 }
 
 template <typename T, int DP> int delta(BwdArgs &b, hipStream_t st) {

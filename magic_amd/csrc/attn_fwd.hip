@@ -246,9 +246,11 @@ int64_t range_count(const magic_attn *a, bool grad) {
 }  // namespace
 
 // F16x2 needs two passes over the operands first: for float32 calls of enough work to pay for them.  Heads up to 32 wide
-// do not (the softmax takes their time, not the products): 64 ragged graphs of up to 1,516 nodes with masked keys, 4 heads
-// of 16, 121 us with it against 117 us without.
-bool use_f16(const magic_attn *a) { return a->dtype == MAGIC_F32 && a->head_dim > 32 && a->max_k >= 512 && a->n_seg > 0; }
+// gain less (the softmax takes much of their time) and need longer segments.  us with those passes, three planes against
+// two: 64 wide, forward and backward, twenty graphs of 600 nodes 295 / 284, ten of 1,200 483 / 405; 16 wide, forward,
+// twenty of 1,500 147 / 141 (half the keys masked: 93 / 109), eight of 3,000 224 / 188 (134 / 135), four of 8,000 827 /
+// 608 (450 / 339); forward and backward, eight of 3,000 861 / 752, four of 8,000 2,912 / 2,356.
+bool use_f16(const magic_attn *a) { return a->dtype == MAGIC_F32 && a->max_k >= (a->head_dim > 32 ? 512 : 2048) && a->n_seg > 0; }
 
 // Gathering costs two launches and a copy of the unmasked rows, and saves the masked share of everything else
 bool use_gather(const magic_attn *a) { return a->key_mask && a->max_k >= 512 && a->n_seg > 0 && a->n_k > 0; }
@@ -869,11 +871,10 @@ template <typename M, int DP, int WM, int KG, int KW> int launch(FwdArgs &p, hip
 
 template <typename M> int run_rows(FwdArgs &p, hipStream_t st) {
     const int D = p.a.head_dim;
-    if constexpr (!M::SCALED) {          // (use_f16: wider heads only)
-        if (D <= 16) return launch<M, 16, 4, 1, 64>(p, st);
-        if (D <= 32) return launch<M, 32, 4, 1, 64>(p, st);
-    }
-    return D <= 64 ? launch<M, 64, 4, 1, 64>(p, st) : launch<M, 128, 4, 1, 64>(p, st);
+    return D <= 16   ? launch<M, 16, 4, 1, 64>(p, st)
+           : D <= 32 ? launch<M, 32, 4, 1, 64>(p, st)
+           : D <= 64 ? launch<M, 64, 4, 1, 64>(p, st)
+                     : launch<M, 128, 4, 1, 64>(p, st);
 }
 
 template <typename T, int DP> int run_few(FwdArgs &p, hipStream_t st) {

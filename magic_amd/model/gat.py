@@ -243,6 +243,8 @@ def linear_nobias(x: torch.Tensor, w: torch.Tensor, act_bits: int = 32) -> torch
         raise _lib.MagicHipError(f"act_bits must be 32 or 8 (got {act_bits})")
     if x.dim() != 2 or w.dim() != 2 or x.shape[1] != w.shape[1]:
         raise _lib.MagicHipError(f"x [N, F] and w [M, F] expected, got {tuple(x.shape)} and {tuple(w.shape)}")
+    if x.device != w.device:
+        raise _lib.MagicHipError(f"x on {x.device}, w on {w.device}")
     return _LinearAct8Fn.apply(x, w)
 
 

@@ -274,6 +274,17 @@ def test_few_long_segments(cuda, dtype, D, hq, hk, opts):
     check(run(q, k, v, d, q_lens, kv_lens, **kw), q, k, v, d, q_lens, kv_lens, **kw)
 
 
+@pytest.mark.parametrize("D,hq,hk,n", [(16, 4, 2, 2100), (24, 2, 2, 4200), (32, 3, 1, 4300)])
+@pytest.mark.parametrize("opts", ["plain", "all"])
+def test_long_segments_of_narrow_heads(cuda, D, hq, hk, n, opts):
+    """From 2,048 keys on narrow heads take their products from two scaled planes too."""
+    lens = [n, 40, 0, 1]
+    q, k, v, d, kw = make(cuda, lens, lens, hq, hk, D, torch.float32, seed=D, slopes=opts == "all", mask=0.7 if opts == "all" else None)
+    if opts == "all":
+        kw["cap"] = 25.0
+    check(run(q, k, v, d, lens, lens, **kw), q, k, v, d, lens, lens, **kw)
+
+
 def test_attention_long_tail_of_small_probabilities(cuda):
     """A distance bias leaves thousands of keys whose terms are each below half a unit of the running sums: together they
     count.  Relative 2-norm error of a float32 result, as small as one formed with whole-row sums."""
