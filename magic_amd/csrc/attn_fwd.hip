@@ -793,6 +793,37 @@ template <typename T, int CPR> __global__ __launch_bounds__(256) void k_attn_joi
     if (c == 0) p.lse[hr] = m == -INFINITY ? -INFINITY : ms + __builtin_amdgcn_logf(l);
 }
 
+// The same for up to MANY ranges of many rows: a thread holds four columns of a (row, head) and walks its ranges.
+// 8,000 rows of 4 heads of 64 in two ranges: 9 us, where a block for every row and head takes 27.
+constexpr int MANY = 16;
+template <typename T> __global__ __launch_bounds__(256) void k_attn_join_rows(FwdArgs p) {
+    const magic_attn &a = p.a;
+    const int cpr = a.head_dim / 4;
+    const int64_t plane = (int64_t)a.q_heads * a.n_q, total = plane * cpr;
+    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < total; i += (int64_t)gridDim.x * 256) {
+        const int64_t hr = i / cpr;
+        const int c = (int)(i - hr * cpr) * 4;
+        float m = -INFINITY;
+        for (int s = 0; s < p.n_split; ++s) {
+            const float x = p.part_l[s * plane + hr];
+            m = x > m || x != x ? x : m;
+        }
+        const float ms = m == -INFINITY ? 0.f : m;
+        float l = 0.f;
+        f32x4_t o = {0.f, 0.f, 0.f, 0.f};
+        for (int s = 0; s < p.n_split; ++s) {
+            const float w = __builtin_amdgcn_exp2f(p.part_l[s * plane + hr] - ms);
+            l += w;
+            o += w * *reinterpret_cast<const f32x4_t *>(p.part_o + (s * plane + hr) * a.head_dim + c);
+        }
+        const float inv = l > 0.f || l != l ? 1.f / l : 0.f;
+        const float x[4] = {o[0] * inv, o[1] * inv, o[2] * inv, o[3] * inv};
+        const int64_t h = hr / a.n_q, row = hr - h * a.n_q;
+        magic::store_vec<T, 4>((T *)p.out + row * p.ld_o + h * p.hs_o + c, true, x);
+        if (c == 0) p.lse[hr] = m == -INFINITY ? -INFINITY : ms + __builtin_amdgcn_logf(l);
+    }
+}
+
 constexpr int FEW = 4;
 
 struct Shape {
@@ -806,12 +837,31 @@ struct Shape {
 // 33 / 36, one of 2,000 (64) 111 / 94, of 4,000 (128) 295 / 144; 128 wide: one of 128 nodes (4) 27 / 22, of 500 (16)
 // 84 / 63.  bfloat16, 64 wide: eight of 500 (128) 15 / 19, one of 4,000 (128) 62 / 59, forty of 100 (160) 16 / 10; 128
 // wide: one of 1,000 (32) 33 / 33, of 2,000 (64) 54 / 40.  Up to 32 wide: one of 7,000 (220), float32 213 / 188, bfloat16
-// 91 / 110, eight of 500 (128) 16 / 21 and 12 / 15, a hundred of 100 (400) 13 / 10 in bfloat16.
+// 91 / 110, eight of 500 (128) 16 / 21 and 12 / 15, a hundred of 100 (400) 13 / 10 in bfloat16; float32 by
+// two planes, one of 4,000 (128) 78 / 92, half masked 81 / 88, of 5,500 (172) 134 / 150, half masked 134 / 117, of 7,000
+// 222 / 183, half masked 222 / 136.
 int64_t few_tiles(const magic_attn *a) {
     const bool f32 = a->dtype == MAGIC_F32;
-    if (a->head_dim <= 32) return 255;
+    if (a->head_dim <= 32) return magic::attn::use_f16(a) ? 144 : 255;
     if (a->head_dim <= 64) return f32 ? 48 : 128;
     return f32 ? 0 : 32;
+}
+
+// Ranges of keys that fill the rounds of blocks best: `slots` of them run at once (two a CU, one where planes and registers
+// fill it), a block takes 1 / ranges of the time, and the fewest ranges within 8 % of the best are taken.  4 heads of 64,
+// one graph, us whole against cut: 10,000 nodes (316 tiles) 515 / 396 in three, 12,000 (376) 620 / 534 in four, twenty graphs
+// of 700 (480) 83 / 97 in two: stay whole; 128 wide in float32, 10,000 nodes 1,276 / 1,002 in two.
+int64_t ranges(int64_t blocks, int64_t slots, int64_t most) {
+    int64_t top = 3 * slots / blocks, best = 1;
+    if (top > most) top = most;
+    if (top > 256) top = 256;
+    double least = 1e30;
+    for (int64_t n = 1; n <= top; ++n) {
+        const double rounds = (double)((blocks * n + slots - 1) / slots) / (double)n;
+        if (rounds < least) least = rounds;
+    }
+    while (best < top && (double)((blocks * best + slots - 1) / slots) > 1.08 * least * (double)best) ++best;
+    return best;
 }
 
 // How a call is cut: 128 rows of one head a block (wm 4), or 32 (row, head) columns with the keys dealt to its wavefronts
@@ -843,11 +893,9 @@ Shape shape_of(const magic_attn *a) {
     if (s.sub < 1) s.sub = 1;
     s.n_hb = a->q_heads / s.gc;
     const int64_t blocks = (int64_t)a->n_q_tiles * s.sub * s.n_hb;
-    // the blocks that run at once: two a CU, one where their planes and registers fill it (float32 of more than 64 columns:
-    // one graph of 5,500 nodes, 172 tiles, 435 us whole, 458 us in halves)
-    const int64_t resident = a->dtype == MAGIC_F32 && a->head_dim > 64 && s.wm == 4 ? 256 : 512;
-    int64_t split = resident / blocks;
     const int64_t most = (a->max_k + 511) / 512;
+    int64_t split = 512 / blocks;
+    if (s.wm == 4) split = ranges(blocks, a->dtype == MAGIC_F32 && a->head_dim > 64 ? 256 : 512, most);
     if (split > most) split = most;
     if (split > 256) split = 256;
     if (split < 1) split = 1;
@@ -905,6 +953,10 @@ template <typename M> int run(FwdArgs &p, int wm, hipStream_t st) {
 
 template <typename T> int join(FwdArgs &p, hipStream_t st) {
     const int D = p.a.head_dim;
+    if (p.n_split <= MANY) {
+        MAGIC_LAUNCH("attn_join", k_attn_join_rows<T>, magic::stride_grid(p.a.n_q * p.a.q_heads * (D / 4), 256, 8192), 256, 0, st, p);
+        return magic::launch_status();
+    }
     const int64_t grid = p.a.n_q * p.a.q_heads;
     if (grid > 0x7fffffffLL) return MAGIC_ERR_UNSUPPORTED;
     if (D <= 16)
