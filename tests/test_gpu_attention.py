@@ -347,17 +347,18 @@ def test_attention_is_reproducible_and_partial_gradients(cuda):
 
 @pytest.mark.parametrize("dtype,D", [(torch.float32, 64), (torch.float32, 16), (torch.bfloat16, 128)])
 def test_partial_gradients_of_a_long_segment(cuda, dtype, D):
-    """Each gradient asked for alone is the one of the full call (ranges of keys and their joins included)."""
+    """Each gradient asked for alone, with its ranges of keys and their joins, within the bounds of the full call.  (Not
+    its bits: where dq is not wanted, another kernel forms do . o of a row, D float32 terms in another order.)"""
     from magic_amd.model.attention import attention_plan, segment_attention
     lens = [4300, 30]
     q, k, v, d, kw = make(cuda, lens, lens, 2, 1, D, dtype, seed=D, slopes=True, mask=0.8)
-    want = run(q, k, v, d, lens, lens, cap=20.0, **kw)
     plan = attention_plan(lens, device=cuda)
-    names = ("dq", "dk", "dv", "ds")
-    for i, name in enumerate(names):
+    got = {}
+    for i, name in enumerate(("dq", "dk", "dv", "ds")):
         ts = [t.detach().requires_grad_(j == i) for j, t in enumerate((q, k, v, kw["slopes"]))]
         out = segment_attention(*ts[:3], plan, cap=20.0, **dict(kw, slopes=ts[3]))
-        assert torch.equal(torch.autograd.grad(out, ts[i], d)[0], want[name]), name
+        got[name] = torch.autograd.grad(out, ts[i], d)[0]
+    check(got, q, k, v, d, lens, lens, cap=20.0, **kw)
 
 
 def test_attention_streams_and_captured_graph(cuda):
