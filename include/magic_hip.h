@@ -611,6 +611,8 @@ typedef struct magic_attn {
     int32_t n_q_tiles, n_k_tiles;
     int32_t max_q, max_k;              /* the longest segment's rows and keys */
     int32_t n_seg;                     /* segments: 0 .. n_seg - 1 appear in the tables */
+    void *out_lo;                      /* MAGIC_BF16: what rounding took from out, [n_q, q_heads, head_dim] contiguous
+                                          bfloat16, or NULL; _fwd writes it, _bwd adds it to out for do . o */
 } magic_attn;
 size_t magic_attn_fwd_workspace_bytes(const magic_attn *args /* host */);
 int magic_attn_fwd(const magic_attn *args /* host struct of device pointers */, void *out, int64_t ld_out, int64_t hs_out,

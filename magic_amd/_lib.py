@@ -39,7 +39,8 @@ class MagicAttn(C.Structure):
                 ("n_k", c_i64), ("q", c_vp), ("ld_q", c_i64), ("hs_q", c_i64), ("k", c_vp), ("ld_k", c_i64),
                 ("hs_k", c_i64), ("v", c_vp), ("ld_v", c_i64), ("hs_v", c_i64), ("scale", c_f32), ("cap", c_f32),
                 ("slopes", c_vp), ("q_pos", c_vp), ("k_pos", c_vp), ("key_mask", c_vp), ("q_tiles", c_vp),
-                ("k_tiles", c_vp), ("n_q_tiles", c_i32), ("n_k_tiles", c_i32), ("max_q", c_i32), ("max_k", c_i32), ("n_seg", c_i32)]
+                ("k_tiles", c_vp), ("n_q_tiles", c_i32), ("n_k_tiles", c_i32), ("max_q", c_i32), ("max_k", c_i32), ("n_seg", c_i32),
+                ("out_lo", c_vp)]
 
 
 # name -> (restype, argtypes); must list every symbol include/magic_hip.h declares
@@ -1047,8 +1048,9 @@ def attn_fwd(q, k, v, plan, scale: float, cap: float = 0.0, slopes=None, q_pos=N
     return attn_fwd_checked(attn_operands(q, k, v, slopes, q_pos, k_pos, key_mask), plan, scale, cap)
 
 
-def attn_fwd_checked(operands, plan, scale, cap):
-    """``attn_fwd`` for operands that ``attn_operands`` returned and arguments that were checked."""
+def attn_fwd_checked(operands, plan, scale, cap, out_lo=None):
+    """``attn_fwd`` for operands that ``attn_operands`` returned and arguments that were checked.  ``out_lo``: bfloat16
+    tensor of the output's shape that receives what rounding took from it (for ``attn_bwd_checked``)."""
     lib = load()
     q = operands[0]
     dev = q.device
@@ -1056,6 +1058,7 @@ def attn_fwd_checked(operands, plan, scale, cap):
     out = torch.empty((n, h, d), dtype=q.dtype, device=dev)
     lse = torch.empty((h, n), dtype=torch.float32, device=dev)
     a = _attn_args(q, operands[1], operands[2], plan, scale, cap, *operands[3:])
+    a.out_lo = out_lo.data_ptr() if out_lo is not None else None
     ref = C.byref(a)
     with _on_device(dev):
         nbytes = lib.magic_attn_fwd_workspace_bytes(ref)
@@ -1080,7 +1083,7 @@ def attn_bwd(q, k, v, plan, scale: float, out, lse, d_out, cap: float = 0.0, slo
     return attn_bwd_checked(ops, plan, scale, cap, _head_rows(out), lse, d_out, need_dq, need_dkv, need_dslopes)
 
 
-def attn_bwd_checked(operands, plan, scale, cap, out, lse, d_out, need_dq, need_dkv, need_dslopes):
+def attn_bwd_checked(operands, plan, scale, cap, out, lse, d_out, need_dq, need_dkv, need_dslopes, out_lo=None):
     """``attn_bwd`` for operands that ``attn_operands`` returned and arguments that were checked: what the autograd node
     calls with the tensors of its forward pass."""
     lib = load()
@@ -1093,6 +1096,7 @@ def attn_bwd_checked(operands, plan, scale, cap, out, lse, d_out, need_dq, need_
     dv = torch.empty(v.shape, dtype=dtype, device=dev) if need_dkv else None
     ds = torch.empty(q.shape[1], dtype=torch.float32, device=dev) if need_dslopes else None
     a = _attn_args(q, k, v, plan, scale, cap, slopes, q_pos, k_pos, key_mask)
+    a.out_lo = out_lo.data_ptr() if out_lo is not None else None
     ref = C.byref(a)
     with _on_device(dev):
         nbytes = lib.magic_attn_bwd_workspace_bytes(ref)

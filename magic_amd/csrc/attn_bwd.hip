@@ -38,6 +38,20 @@ struct BwdArgs {
     float *part;        // [n_split][dk | dv][n_k][kv_heads][head_dim]
 };
 
+// what the forward pass's rounding took from eight results
+template <typename T> __device__ __forceinline__ void add_low(const magic_attn &a, int64_t row, int h, int c, float (&x)[8]) {
+    if constexpr (sizeof(T) == 2) {
+        if (a.out_lo) {
+            Raw<T> r;
+            float y[8];
+            r.load((const T *)a.out_lo + (row * a.q_heads + h) * a.head_dim + c);
+            r.floats(y);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) x[e] += y[e];
+        }
+    }
+}
+
 // lse2 and D of every row: DP / 8 lanes a row and head
 template <typename T, int DP> __global__ __launch_bounds__(256) void k_attn_delta(BwdArgs b) {
     constexpr int LPR = DP / 8;
@@ -55,6 +69,7 @@ template <typename T, int DP> __global__ __launch_bounds__(256) void k_attn_delt
             Raw<T> ro, rd;
             ro.load(o), rd.load(d);
             ro.floats(x), rd.floats(y);
+            add_low<T>(a, row, h, c, x);
 #pragma unroll
             for (int e = 0; e < 8; ++e) s += x[e] * y[e];
         }
@@ -268,6 +283,7 @@ __global__ __launch_bounds__(64 * WM *KG, (DP == 128 && M::N > 1) || (DP >= 64 &
             o.load((const T *)p.out + qr * p.ld_o + h * p.hs_o + cc);
             if (!live || c >= D) o.zero();
             o.floats(x), g.floats(y);
+            if (live && c < D) add_low<T>(a, qr, h, c, x);
 #pragma unroll
             for (int e = 0; e < 8; ++e) dl0 += x[e] * y[e];
         }

@@ -27,7 +27,7 @@ int check(const magic_attn *a) {
     if (a->ld_q > MAX_LD || a->ld_k > MAX_LD || a->ld_v > MAX_LD || (int64_t)a->q_heads * a->head_dim > MAX_LD) return MAGIC_ERR_UNSUPPORTED;
     if (a->ld_q < 0 || a->hs_q < 0 || a->ld_k < 0 || a->hs_k < 0 || a->ld_v < 0 || a->hs_v < 0) return MAGIC_ERR_INVALID_ARG;
     const int per = a->dtype == MAGIC_F32 ? 4 : 8;   // rows and heads start on 16-byte addresses
-    if (((uintptr_t)a->q | (uintptr_t)a->k | (uintptr_t)a->v) & 15) return MAGIC_ERR_INVALID_ARG;
+    if (((uintptr_t)a->q | (uintptr_t)a->k | (uintptr_t)a->v | (uintptr_t)a->out_lo) & 15) return MAGIC_ERR_INVALID_ARG;
     if ((a->ld_q | a->hs_q | a->ld_k | a->hs_k | a->ld_v | a->hs_v) % per) return MAGIC_ERR_INVALID_ARG;
     // (scale / cap and cap times a polynomial's terms stay normal float32 numbers)
     if (!(a->cap == 0.f || (a->cap >= 1e-3f && a->cap <= 1e30f)) || !(std::fabs(a->scale) <= 1e30f)) return MAGIC_ERR_INVALID_ARG;
@@ -341,6 +341,19 @@ struct FwdArgs {
 
 __device__ __forceinline__ int h_of(const FwdArgs &p, int hb) { return hb * p.gc; }
 
+// four results of a row and head: rounded, and what the rounding took where it is wanted
+template <typename T> __device__ __forceinline__ void store_out(const FwdArgs &p, int64_t row, int64_t h, int c, const float (&x)[4]) {
+    magic::store_vec<T, 4>((T *)p.out + row * p.ld_o + h * p.hs_o + c, true, x);
+    if constexpr (sizeof(T) == 2) {
+        if (p.a.out_lo) {
+            float r[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) r[e] = x[e] - (float)(T)x[e];
+            magic::store_vec<T, 4>((T *)p.a.out_lo + (row * p.a.q_heads + h) * p.a.head_dim + c, true, r);
+        }
+    }
+}
+
 // WM groups of 32 columns (rows, or rows x heads of one key head), KG groups of KW keys: a block of WM * KG wavefronts
 template <typename M, int DP, int WM, int KG, int KW>
 __global__ __launch_bounds__(64 * WM *KG, DP == 128 && (M::N > 1 || WM == 1) ? 1 : 2) void k_attn_fwd(FwdArgs p) {
@@ -597,14 +610,13 @@ __global__ __launch_bounds__(64 * WM *KG, DP == 128 && (M::N > 1 || WM == 1) ? 1
         if (hf == 0) p.part_l[base] = ls;
         return;
     }
-    T *out = (T *)p.out + (q0 + row) * p.ld_o + h * p.hs_o;
 #pragma unroll
     for (int d = 0; d < DB; ++d)
 #pragma unroll
         for (int g = 0; g < 4; ++g) {
             const int c = 32 * d + 8 * g + 4 * hf;
             const float x[4] = {o[d][4 * g] * inv, o[d][4 * g + 1] * inv, o[d][4 * g + 2] * inv, o[d][4 * g + 3] * inv};
-            magic::store_vec<T, 4>(out + c, c < D, x);
+            if (c < D) store_out<T>(p, q0 + row, h, c, x);
         }
     if (hf == 0) p.lse[(int64_t)h * a.n_q + q0 + row] = ls;
 }
@@ -751,7 +763,9 @@ template <typename T, int DP, int NC> __global__ __launch_bounds__(256) void k_a
             p.part_o[base * D + d] = ot * inv;
             if (d == 0) p.part_l[base] = ls;
         } else {
-            ((T *)p.out)[(q0 + row) * p.ld_o + h * p.hs_o + d] = (T)(ot * inv);
+            const float x = ot * inv;
+            ((T *)p.out)[(q0 + row) * p.ld_o + h * p.hs_o + d] = (T)x;
+            if (sizeof(T) == 2 && a.out_lo) ((T *)a.out_lo)[((q0 + row) * a.q_heads + h) * D + d] = (T)(x - (float)(T)x);
             if (d == 0) p.lse[(int64_t)h * a.n_q + q0 + row] = ls;
         }
     }
@@ -789,7 +803,7 @@ template <typename T, int CPR> __global__ __launch_bounds__(256) void k_attn_joi
     const float inv = l > 0.f || l != l ? 1.f / l : 0.f;
     const float x[4] = {o[0] * inv, o[1] * inv, o[2] * inv, o[3] * inv};
     const int64_t h = hr / a.n_q, row = hr - h * a.n_q;
-    magic::store_vec<T, 4>((T *)p.out + row * p.ld_o + h * p.hs_o + c, true, x);
+    store_out<T>(p, row, h, c, x);
     if (c == 0) p.lse[hr] = m == -INFINITY ? -INFINITY : ms + __builtin_amdgcn_logf(l);
 }
 
@@ -819,7 +833,7 @@ template <typename T> __global__ __launch_bounds__(256) void k_attn_join_rows(Fw
         const float inv = l > 0.f || l != l ? 1.f / l : 0.f;
         const float x[4] = {o[0] * inv, o[1] * inv, o[2] * inv, o[3] * inv};
         const int64_t h = hr / a.n_q, row = hr - h * a.n_q;
-        magic::store_vec<T, 4>((T *)p.out + row * p.ld_o + h * p.hs_o + c, true, x);
+        store_out<T>(p, row, h, c, x);
         if (c == 0) p.lse[hr] = m == -INFINITY ? -INFINITY : ms + __builtin_amdgcn_logf(l);
     }
 }

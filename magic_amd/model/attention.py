@@ -82,18 +82,20 @@ class _SegmentAttentionFn(torch.autograd.Function):
     def forward(ctx, q, k, v, slopes, plan, scale, cap, q_pos, k_pos, key_mask):
         _lib.attn_check(q, k, v, plan.n_q, plan.n_k, plan.device, cap, slopes, q_pos, k_pos, key_mask)
         operands = _lib.attn_operands(q, k, v, slopes, q_pos, k_pos, key_mask)
-        out, lse = _lib.attn_fwd_checked(operands, plan, scale, cap)
-        ctx.save_for_backward(*operands, out, lse)
+        # A score gradient is p (do.v - do.o): with few keys the rounding of a bfloat16 o is twice what else is off
+        out_lo = torch.empty(q.shape, dtype=q.dtype, device=q.device) if q.dtype == torch.bfloat16 and any(ctx.needs_input_grad) else None
+        out, lse = _lib.attn_fwd_checked(operands, plan, scale, cap, out_lo)
+        ctx.save_for_backward(*operands, out, lse, out_lo)
         ctx.plan, ctx.scale, ctx.cap = plan, scale, cap
         return out
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, d_out):
-        *operands, out, lse = ctx.saved_tensors
+        *operands, out, lse, out_lo = ctx.saved_tensors
         need = ctx.needs_input_grad
         dq, dk, dv, ds = _lib.attn_bwd_checked(operands, ctx.plan, ctx.scale, ctx.cap, out, lse, d_out, need[0],
-                                               need[1] or need[2], need[3])
+                                               need[1] or need[2], need[3], out_lo)
         return (dq if need[0] else None, dk if need[1] else None, dv if need[2] else None, ds) + (None,) * 6
 
 
