@@ -374,9 +374,10 @@ __global__ __launch_bounds__(64 * WM *KG, (DP == 128 && M::N > 1) || (DP >= 64 &
                 u = run.u;
             }
             // Few keys: dq is the difference of a few large terms, and what rounding takes from the score gradients does not
-            // average out (2.5e-3 of the norm over four keys, 1.9e-3 with a second product of the low parts)
+            // average out (2.5e-3 of the norm over four keys, 1.9e-3 with a second product of the low parts).  Narrow heads
+            // (2.6e-3 at worst) take it always: their products are the smaller part of the work.
             if constexpr (M::N == 1) {
-                if (nk <= 64) {
+                if (DP <= 32 || nk <= 64) {
 #pragma unroll
                     for (int w = 0; w < 2; ++w) {
                         float x[8];
@@ -652,13 +653,23 @@ __global__ __launch_bounds__(64 * WM *KG, DP == 128 || (DP >= 64 && KG > 1) ? 1 
                 vec pf[NP], sf[NP];
                 to_planes(x, pf);
                 to_planes(y, sf);
+                constexpr bool LOW = M::N == 1 && DP <= 32;      // low parts too, as in the dq sweep
+                vec pl[NP], sl[NP];
+                if constexpr (LOW) {
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) x[e] -= (float)(bf16_t)x[e], y[e] -= (float)(bf16_t)y[e];
+                    to_planes(x, pl);
+                    to_planes(y, sl);
+                }
 #pragma unroll
                 for (int d = 0; d < DB; ++d) {
                     vec f[NP];
                     tile::frag_t(sG, turned, 32 * b + 16 * w, d, f);
                     mma(gv[d], f, pf);
+                    if constexpr (LOW) mma(gv[d], f, pl);
                     tile::frag_t(sQ, turned, 32 * b + 16 * w, d, f);
                     mma(gk[d], f, sf);
+                    if constexpr (LOW) mma(gk[d], f, sl);
                 }
             }
             feed<2 * NP, PRODUCTS<M>, 4 * DB>();
