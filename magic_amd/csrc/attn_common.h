@@ -311,46 +311,45 @@ template <typename M, int DP, int ROWS, int NT> struct Stage {
 };
 
 // Capped scores of a tile: x[i] = cap tanh(x[i] f).  Below TANH_SMALL tanh(t) / t is a polynomial in t^2 (equal ripples on
-// that range): 3.5e-8 off with four terms, half a rounding of float32, or 2.9e-6 with three where the probabilities are
-// rounded to bfloat16 (SHORT).  Elsewhere tanh is (1 - e) / (1 + e).  A cap is far above most scores: the polynomial serves
-// alone where no score of the wavefront leaves its range.  SHORT has f and cap in its coefficients and starts from the
-// scores themselves, up to RAW_MAX (their powers stay in range; the scaled modes' scores are far larger).
-constexpr float TANH_SMALL = 0.35f, RAW_MAX = 1e6f;
-constexpr float K0 = 0.999997139f, K1 = -0.332909554f, K2 = 0.12395031f;      // of SHORT
-template <bool SHORT> struct Cap {
+// that range): 3.5e-8 off with four terms, half a rounding of float32.  (Three terms, 2.9e-6 off, show in the slopes'
+// gradients of bfloat16 calls, which are float32.)  Elsewhere tanh is (1 - e) / (1 + e).  A cap is far above most scores:
+// the polynomial serves alone where no score of the wavefront leaves its range.  RAW (bfloat16) has f and cap in its coefficients and starts from
+// the scores themselves, up to RAW_MAX (their powers stay in range; the scaled modes' scores are far larger).
+constexpr float TANH_SMALL = 0.35f, RAW_MAX = 1e5f;
+constexpr float K0 = 0.99999994f, K1 = -0.333324224f, K2 = 0.132957995f, K3 = -0.0489582308f;
+template <bool RAW> struct Cap {
     float f, cap, lim, c0, c1, c2, c3;
     __device__ __forceinline__ Cap(float f, float cap) : f(f), cap(cap) {
-        lim = SHORT ? fminf(TANH_SMALL / fabsf(f), RAW_MAX) : TANH_SMALL;
-        if (SHORT) {
+        lim = RAW ? fminf(TANH_SMALL / fabsf(f), RAW_MAX) : TANH_SMALL;
+        if (RAW) {
             const float u = cap * f, f2 = f * f;
-            c0 = K0 * u, c1 = K1 * u * f2, c2 = K2 * u * f2 * f2, c3 = 0.f;
+            c0 = K0 * u, c1 = K1 * u * f2, c2 = K2 * u * f2 * f2, c3 = K3 * u * f2 * f2 * f2;
         } else {
-            c0 = 0.99999994f * cap, c1 = -0.333324224f * cap, c2 = 0.132957995f * cap, c3 = -0.0489582308f * cap;
+            c0 = K0 * cap, c1 = K1 * cap, c2 = K2 * cap, c3 = K3 * cap;
         }
     }
-    // of a score (SHORT) or of a score times f
+    // of a score (RAW) or of a score times f
     __device__ __forceinline__ float poly(float x) const {
         const float z = x * x;
-        const float p = SHORT ? c2 : fmaf(z, c3, c2);
-        return x * fmaf(z, fmaf(z, p, c1), c0);
+        return x * fmaf(z, fmaf(z, fmaf(z, c3, c2), c1), c0);
     }
 };
-template <bool SHORT> __device__ __forceinline__ void cap_tile(f32x16_t &x, const Cap<SHORT> &c) {
+template <bool RAW> __device__ __forceinline__ void cap_tile(f32x16_t &x, const Cap<RAW> &c) {
     float m = 0.f;
 #pragma unroll
     for (int r = 0; r < 16; ++r) {
-        if (!SHORT) x[r] *= c.f;
+        if (!RAW) x[r] *= c.f;
         m = fmaxf(m, fabsf(x[r]));
     }
     if (__any(m >= c.lim)) {
 #pragma unroll
         for (int r = 0; r < 16; ++r) {
-            const float t = SHORT ? x[r] * c.f : x[r], a = fabsf(t);
+            const float t = RAW ? x[r] * c.f : x[r], a = fabsf(t);
             const float e = __builtin_amdgcn_exp2f(-2.f * LOG2E * a);
             float b = copysignf(c.cap * (1.f - e) * __builtin_amdgcn_rcpf(1.f + e), t);
             asm("" : "+v"(b));          // (a select between two values, not a branch around one)
-            // (SHORT: scores above RAW_MAX may still be small ones of a larger cap)
-            const float s = SHORT ? c.cap * (t * fmaf(t * t, fmaf(t * t, K2, K1), K0)) : c.poly(x[r]);
+            // (RAW: scores above RAW_MAX may still be small ones of a larger cap)
+            const float s = RAW ? c.cap * (t * fmaf(t * t, fmaf(t * t, fmaf(t * t, K3, K2), K1), K0)) : c.poly(x[r]);
             x[r] = a < TANH_SMALL ? s : b;
         }
     } else {
