@@ -5,8 +5,8 @@
 // keys (three products), dk and dv with the keys' wavefronts walking the rows of all heads that share them (four).
 // Seven products instead of the five that one sweep with atomic adds would need.
 // Bound like the forward pass.  Twelve graphs of 8,000 nodes, 4 heads of 64, float32: dq 4.2 ms (289 TFLOP/s of its three
-// products), dk and dv 4.8 ms (338); bfloat16, 8 heads of 128 over 2, capped, half the keys masked: 1.48 ms (677) and
-// 2.38 ms (559: 128 accumulators and both operands' rows leave one wavefront a SIMD, which has nothing to put beside its
+// products), dk and dv 4.8 ms (338); bfloat16, 8 heads of 128 over 2, capped, half the keys masked: 1.54 ms (648) and
+// 2.43 ms (548: 128 accumulators and both operands' rows leave one wavefront a SIMD, which has nothing to put beside its
 // own waits).
 #include "attn_common.h"
 
