@@ -375,9 +375,10 @@ __global__ __launch_bounds__(64 * WM *KG, (DP == 128 && M::N > 1) || (DP >= 64 &
             }
             // Few keys: dq is the difference of a few large terms, and what rounding takes from the score gradients does not
             // average out (2.5e-3 of the norm over four keys, 1.9e-3 with a second product of the low parts).  Narrow heads
-            // (2.6e-3 at worst) take it always: their products are the smaller part of the work.
+            // (2.6e-3 at worst) take it always: their products are the smaller part of the work.  So do the blocks of 32 rows, which
+            // wait more than they compute (3.0e-3 at worst).
             if constexpr (M::N == 1) {
-                if (DP <= 32 || nk <= 64) {
+                if (DP <= 32 || KG > 1 || nk <= 64) {
 #pragma unroll
                     for (int w = 0; w < 2; ++w) {
                         float x[8];
@@ -653,7 +654,7 @@ __global__ __launch_bounds__(64 * WM *KG, DP == 128 || (DP >= 64 && KG > 1) ? 1 
                 vec pf[NP], sf[NP];
                 to_planes(x, pf);
                 to_planes(y, sf);
-                constexpr bool LOW = M::N == 1 && DP <= 32;      // low parts too, as in the dq sweep
+                constexpr bool LOW = M::N == 1 && (DP <= 32 || KG > 1);      // low parts too, as in the dq sweep
                 vec pl[NP], sl[NP];
                 if constexpr (LOW) {
 #pragma unroll
@@ -792,7 +793,7 @@ template <typename M, int DP, int WM, int KG, int NB> int run_dkv(BwdArgs &b, in
 
 // 32 rows a block where tiles of 128 would leave most of the chip idle: the wavefronts share the rows and deal out the keys
 // Heads of more than 32 columns leave a CU room for one such block: one round of them at most.  Four heads, us of both
-// sweeps, 32 rows against 128: 64 wide, bfloat16, graphs of 500 nodes, 64 tiles 31 / 48, 80 tiles 52 / 48, one graph of 7,000
+// sweeps, 32 rows against 128: 64 wide, bfloat16, graphs of 500 nodes, 64 tiles 34 / 48, 80 tiles 52 / 48, one graph of 7,000
 // (220) 499 / 367; float32, 64 tiles 59 / 111, forty graphs of 100 (160) 72 / 47; 128 wide, float32, 64 tiles 160 / 174, 80
 // tiles 301 / 176.  16 wide: one graph of 7,000 503 / 570 in float32 and 216 / 279 in bfloat16, a hundred graphs of 100
 // (400 tiles) 33 / 23.
