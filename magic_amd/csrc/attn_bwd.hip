@@ -102,7 +102,7 @@ struct Scales {
             if ((range_ok(rq) && range_ok(rk) && range_ok(rv) && range_ok(rr)) != rg.want_safe) return false;
             if constexpr (M::SCALED) q = range_scale(rq), k = range_scale(rk), v = range_scale(rv), g = range_scale(rr);
         }
-        s_in = (a.cap > 0.f ? a.scale / a.cap : a.scale) * (1.f / q * (1.f / k));
+        s_in = (a.cap > 0.f ? a.scale / a.cap : a.scale * LOG2E) * (1.f / q * (1.f / k));
         dp_in = 1.f / v * (1.f / g);
         return true;
     }
@@ -150,7 +150,7 @@ __device__ __forceinline__ void sum_slope(const double *part, int64_t n, int H, 
 
 // What a lane knows of its row in the dq sweep
 struct RowSide {
-    float s_in, dp_in, scale, f_cap, slope;   // f_cap: -scale / cap^2, for scale (1 - tanh^2) from the capped score
+    float s_in, dp_in, scale, f_cap, slope;   // f_cap: -scale / (cap log2 e)^2, for scale (1 - tanh^2) from the capped score
     uint32_t pos;
     float lse, delta;
 };
@@ -161,6 +161,11 @@ struct RowSide {
 struct SlopeSums {
     double dl_dist = 0.0, dl = 0.0, pd = 0.0;
 };
+
+// No logit is above the row's log-sum.  One recomputed from other planes than the forward pass took, or in another order,
+// can be (by 2^-22 of its products' size): with logits of millions its probability would be no fp16 number.
+// (v_minimum3_f32: a NaN stays one)
+__device__ __forceinline__ float at_most(float x, float top) { return __builtin_elementwise_minimum(x, top); }
 
 // Scores and do.v of 32 keys by 32 rows -> gradients of the scores (before the scale of dq); km, kp: the keys' masks
 // (0 / -inf) and positions, four for every group of registers
@@ -184,7 +189,7 @@ __device__ __forceinline__ void score_grad(f32x16_t &s, const f32x16_t &dp, cons
                 dist = dist_of((uint32_t)pos[e], c.pos);
                 x = fmaf(-c.slope, dist, x);
             }
-            const float pr = __builtin_amdgcn_exp2f(fmaf(x, LOG2E, base[e]));
+            const float pr = __builtin_amdgcn_exp2f(at_most(x, c.lse) + base[e]);
             const float dl = pr * fmaf(dp[r], c.dp_in, -c.delta);
             if (BIAS) {
                 t_dsl = fmaf(dl, dist, t_dsl);
@@ -214,7 +219,7 @@ __device__ __forceinline__ void prob_grad(f32x16_t &s, const f32x16_t &dp, const
             float x = CAP ? s[r] : s[r] * c.s_in;
             const float f = CAP ? fmaf(x * x, c.f_cap, c.scale) : c.scale;
             if (BIAS) x = fmaf(-c.slope, dist_of((uint32_t)pos[e], c.pos), x);
-            const float q = __builtin_amdgcn_exp2f(fmaf(x, LOG2E, l4[e]));
+            const float q = __builtin_amdgcn_exp2f(at_most(x, -l4[e]) + l4[e]);
             pr[r] = M::SCALED ? q * 16384.f : q;
             ds[r] = q * fmaf(dp[r], c.dp_in, d4[e]) * f;
         }
@@ -295,9 +300,9 @@ __global__ __launch_bounds__(64 * WM *KG, (DP == 128 && M::N > 1) || (DP >= 64 &
         if (ok && hf == 0 && kg == 0 && split == 0) p.lse2[(int64_t)h * a.n_q + qr] = ls, p.delta[(int64_t)h * a.n_q + qr] = dl0;
     }
     const bool bias = a.slopes != nullptr;
-    const float slope = bias ? a.slopes[h] : 0.f;
+    const float slope = bias ? a.slopes[h] * LOG2E : 0.f;
     const uint32_t qpos = bias ? flip(a.q_pos[qr]) : 0u;
-    const float f_cap = a.cap > 0.f ? -a.scale / a.cap / a.cap : 0.f;
+    const float f_cap = a.cap > 0.f ? -a.scale / a.cap / a.cap * (1.f / (LOG2E * LOG2E)) : 0.f;
     const Cap<M::N == 1> cap(sc.s_in, a.cap);
     Running run;
     SlopeSums sums;
@@ -571,7 +576,7 @@ __global__ __launch_bounds__(64 * WM *KG, DP == 128 || (DP >= 64 && KG > 1) ? 1 
     }
     const bool bias = a.slopes != nullptr;
     const uint32_t kpos = bias ? flip(a.k_pos[kr]) : 0u;
-    const float f_cap = a.cap > 0.f ? -a.scale / a.cap / a.cap : 0.f;
+    const float f_cap = a.cap > 0.f ? -a.scale / a.cap / a.cap * (1.f / (LOG2E * LOG2E)) : 0.f;
     const Cap<M::N == 1> cap(sc.s_in, a.cap);
     Running run;
     f32x16_t gk[DB], gv[DB];
@@ -612,7 +617,7 @@ __global__ __launch_bounds__(64 * WM *KG, DP == 128 || (DP >= 64 && KG > 1) ? 1 
         qst.store(sQ, D, tid, part, [&](int i) { return stage::row_of(i, tid) < rows; });
         gst.store(sG, D, tid, part, [&](int i) { return stage::row_of(i, tid) < rows; });
         if (tid < BQ) sL[tid] = -ls, sD[tid] = -dl0, sPos[tid] = flip(pos);
-        const float slope = bias ? a.slopes[h] : 0.f;
+        const float slope = bias ? a.slopes[h] * LOG2E : 0.f;
         __syncthreads();
         if (++it == per_h) it = 0, ++h;
         if (st + 1 < s_end) load(h, it * BQ);
@@ -628,7 +633,7 @@ __global__ __launch_bounds__(64 * WM *KG, DP == 128 || (DP >= 64 && KG > 1) ? 1 
                 vec f[NP], g[NP];
                 tile::frag(sQ, plain, 32 * b, ks, f);
                 tile::frag(sG, plain, 32 * b, ks, g);
-                mma(s, f, kf[ks]);
+                mma_turned(s, f, kf[ks]);
                 mma(dp, g, vf[ks]);
             }
             feed<2 * NP, 2 * PRODUCTS<M>, KS>();

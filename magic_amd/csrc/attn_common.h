@@ -181,6 +181,23 @@ __device__ __forceinline__ void mma(f32x16_t &c, const bf16x8_t (&a)[1], const b
     c = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a[0], b[0], c, 0, 0, 0);
 }
 
+// The same sums in the same order with the operands' parts exchanged: scores of rows by keys come out bit for bit like those
+// of keys by rows, and so do the probabilities that the sweeps rebuild from them.
+__device__ __forceinline__ void mma_turned(f32x16_t &c, const bf16x8_t (&a)[3], const bf16x8_t (&b)[3]) {
+    c = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a[0], b[2], c, 0, 0, 0);
+    c = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a[2], b[0], c, 0, 0, 0);
+    c = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a[1], b[1], c, 0, 0, 0);
+    c = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a[0], b[1], c, 0, 0, 0);
+    c = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a[1], b[0], c, 0, 0, 0);
+    c = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a[0], b[0], c, 0, 0, 0);
+}
+__device__ __forceinline__ void mma_turned(f32x16_t &c, const f16x8_t (&a)[2], const f16x8_t (&b)[2]) {
+    c = __builtin_amdgcn_mfma_f32_32x32x16_f16(a[0], b[1], c, 0, 0, 0);
+    c = __builtin_amdgcn_mfma_f32_32x32x16_f16(a[1], b[0], c, 0, 0, 0);
+    c = __builtin_amdgcn_mfma_f32_32x32x16_f16(a[0], b[0], c, 0, 0, 0);
+}
+__device__ __forceinline__ void mma_turned(f32x16_t &c, const bf16x8_t (&a)[1], const bf16x8_t (&b)[1]) { mma(c, a, b); }
+
 // Order of a run of matrix instructions and the LDS reads that feed them: STEPS steps of READS reads and MFMAS
 // instructions, the reads of AHEAD steps before the first.  (Left alone, the compiler reads, waits and multiplies in turn:
 // a trip to the LDS before every product.)
@@ -310,7 +327,9 @@ template <typename M, int DP, int ROWS, int NT> struct Stage {
     }
 };
 
-// Capped scores of a tile: x[i] = cap tanh(x[i] f).  Below TANH_SMALL tanh(t) / t is a polynomial in t^2 (equal ripples on
+// Logits are formed times log2 e (scale, cap and slopes carry it): a probability is 2^(x - m) with m the row's largest x
+// itself, so that x - m is exact where it matters, whatever the logits' size.
+// Capped scores of a tile: x[i] = log2 e cap tanh(x[i] f).  Below TANH_SMALL tanh(t) / t is a polynomial in t^2 (equal ripples on
 // that range): 3.5e-8 off with four terms, half a rounding of float32.  (Three terms, 2.9e-6 off, show in the slopes'
 // gradients of bfloat16 calls, which are float32.)  Elsewhere tanh is (1 - e) / (1 + e).  A cap is far above most scores:
 // the polynomial serves alone where no score of the wavefront leaves its range.  RAW (bfloat16) has f and cap in its coefficients and starts from
@@ -319,7 +338,7 @@ constexpr float TANH_SMALL = 0.35f, RAW_MAX = 1e5f;
 constexpr float K0 = 0.99999994f, K1 = -0.333324224f, K2 = 0.132957995f, K3 = -0.0489582308f;
 template <bool RAW> struct Cap {
     float f, cap, lim, c0, c1, c2, c3;
-    __device__ __forceinline__ Cap(float f, float cap) : f(f), cap(cap) {
+    __device__ __forceinline__ Cap(float f, float cap_e) : f(f), cap(cap_e * LOG2E) {
         lim = RAW ? fminf(TANH_SMALL / fabsf(f), RAW_MAX) : TANH_SMALL;
         if (RAW) {
             const float u = cap * f, f2 = f * f;

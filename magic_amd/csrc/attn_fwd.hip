@@ -411,21 +411,23 @@ __global__ __launch_bounds__(64 * WM *KG, DP == 128 && (M::N > 1 || WM == 1) ? 1
         }
     }
     const bool bias = a.slopes != nullptr;
-    const float slope = bias ? a.slopes[ok ? h : hb * p.gc] : 0.f;
+    const float slope = bias ? a.slopes[ok ? h : hb * p.gc] * LOG2E : 0.f;
     const uint32_t qpos = bias ? flip(a.q_pos[q0 + (ok ? row : 0)]) : 0u;
     const float unscale = 1.f / sq * (1.f / sk);
-    const float s_in = (a.cap > 0.f ? a.scale / a.cap : a.scale) * unscale;
+    const float s_in = (a.cap > 0.f ? a.scale / a.cap : a.scale * LOG2E) * unscale;
     const Cap<M::N == 1> cap(s_in, a.cap);
-    constexpr float P_EXP = M::SCALED ? 14.f : 0.f;       // probabilities are formed times 2^14
+    // A probability is formed as 2^(x - unit(m)).  The scaled mode keeps them times 2^14 and adds 14 - m, rounded, at once:
+    // alike for a row, so the sum takes it out again.  From FAR on that rounding would be off by 1 and more (2^16 is no
+    // fp16 number): there m is taken off first.
+    constexpr float P_EXP = M::SCALED ? 14.f : 0.f, FAR = 1048576.f;
+    auto unit = [&](float m) { return M::SCALED ? (fabsf(m) >= FAR ? (double)m - 14.0 : -(double)(14.f - m)) : (double)m; };
 
     f32x16_t o[DB];
 #pragma unroll
     for (int d = 0; d < DB; ++d)
 #pragma unroll
         for (int r = 0; r < 16; ++r) o[d][r] = 0.f;
-    // Of this lane's keys: the two halves of a wavefront share m and add l at the end.  m is the largest logit times
-    // log2 e, rounded: a probability is 2^(logit log2 e - m) in ONE fused step, so its error is that of the small
-    // difference, not of the two large terms.
+    // Of this lane's keys: the two halves of a wavefront share m, the largest logit so far, and add l at the end.
     float m = -INFINITY, l = 0.f;
 
     uint32_t plain = tile::lane_plain(lane) + 2u * kg * KW * tile::W, turned = tile::lane_turned(lane) + 2u * kg * KW * tile::W;
@@ -507,9 +509,19 @@ __global__ __launch_bounds__(64 * WM *KG, DP == 128 && (M::N > 1 || WM == 1) ? 1
         for (int b = 0; b < KB; ++b)
 #pragma unroll
             for (int r = 0; r < 16; ++r) mx = fmaxf(mx, s[b][r]);
-        mx = fmaxf(m, fmaxf(mx, other_half(mx)) * LOG2E);
+        mx = fmaxf(m, fmaxf(mx, other_half(mx)));
         const float ms = mx == -INFINITY ? 0.f : mx;
-        const float al = __builtin_amdgcn_exp2f(m - ms), mo = P_EXP - ms;
+        float mo = P_EXP - ms;
+        const float al = __builtin_amdgcn_exp2f(M::SCALED ? (float)(unit(m) - unit(ms)) : m - ms);
+        if (M::SCALED && __any(fabsf(ms) >= FAR)) {
+            const bool far = fabsf(ms) >= FAR;
+            const float off = far ? ms : 0.f;
+            if (far) mo = P_EXP;
+#pragma unroll
+            for (int b = 0; b < KB; ++b)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) s[b][r] -= off;
+        }
         m = mx;
         // The tile's sums are formed by themselves and added once: a long tail of small terms, each below half a unit of
         // the running sum, would otherwise be lost term by term (3e-6 of the result over 8,000 keys with a distance bias).
@@ -530,7 +542,7 @@ __global__ __launch_bounds__(64 * WM *KG, DP == 128 && (M::N > 1 || WM == 1) ? 1
                 float x[8];
 #pragma unroll
                 for (int e = 0; e < 8; ++e) {
-                    x[e] = __builtin_amdgcn_exp2f(fmaf(s[b][8 * u + e], LOG2E, mo));
+                    x[e] = __builtin_amdgcn_exp2f(s[b][8 * u + e] + mo);
                     tsum += x[e];
                 }
                 to_planes(x, pf[2 * b + u]);
@@ -595,7 +607,7 @@ __global__ __launch_bounds__(64 * WM *KG, DP == 128 && (M::N > 1 || WM == 1) ? 1
     }
     if (!ok) return;
     const float inv = l > 0.f || l != l ? 1.f / (l * sv) : 0.f;
-    const float ls = m == -INFINITY && l == 0.f ? -INFINITY : m + __builtin_amdgcn_logf(l) - P_EXP;   // base 2
+    const float ls = m == -INFINITY && l == 0.f ? -INFINITY : (float)(unit(m) + (double)__builtin_amdgcn_logf(l));   // base 2
     if (p.n_split > 1) {
         const int64_t base = ((int64_t)split * a.q_heads + h) * a.n_q + q0 + row;
 #pragma unroll
@@ -660,6 +672,7 @@ template <typename T, int DP, int NC> __global__ __launch_bounds__(256) void k_a
     const int hk = hb * p.gc / (a.q_heads / a.kv_heads);
     const T *K = (const T *)a.k + k0 * a.ld_k + hk * a.hs_k + (cin ? c0 : 0), *V = (const T *)a.v + k0 * a.ld_v + hk * a.hs_v + (cin ? c0 : 0);
     const bool bias = a.slopes != nullptr;
+    const float scale = a.cap > 0.f ? a.scale / a.cap : a.scale * LOG2E, cap = a.cap * LOG2E;
 
     float q[NC][EPL], slope[NC], m[NC], l[NC], o[NC][EPL];
     uint32_t qpos[NC];
@@ -671,7 +684,7 @@ template <typename T, int DP, int NC> __global__ __launch_bounds__(256) void k_a
         const vt x = *reinterpret_cast<const vt *>(qp);
 #pragma unroll
         for (int e = 0; e < EPL; ++e) q[c][e] = ok && cin ? (float)x[e] : 0.f, o[c][e] = 0.f;
-        slope[c] = bias ? a.slopes[ok ? h : hb * p.gc] : 0.f;
+        slope[c] = bias ? a.slopes[ok ? h : hb * p.gc] * LOG2E : 0.f;
         qpos[c] = bias ? flip(a.q_pos[q0 + (ok ? row : 0)]) : 0u;
         m[c] = -INFINITY, l[c] = 0.f;
     }
@@ -709,17 +722,17 @@ template <typename T, int DP, int NC> __global__ __launch_bounds__(256) void k_a
                 float d = 0.f;
 #pragma unroll
                 for (int e = 0; e < EPL; ++e) d = fmaf(q[c][e], kf[u][e], d);
-                x[u] = lanes_sum<LPR>(d) * a.scale;
+                x[u] = lanes_sum<LPR>(d) * scale;
             }
             if (a.cap > 0.f) {
 #pragma unroll
-                for (int u = 0; u < U; ++u) x[u] = a.cap * tanhf(x[u] / a.cap);
+                for (int u = 0; u < U; ++u) x[u] = cap * tanhf(x[u]);
             }
 #pragma unroll
             for (int u = 0; u < U; ++u) {
                 if (bias) x[u] = fmaf(-slope[c], dist_of(kp[u], qpos[c]), x[u]);
                 x[u] = in[u] ? x[u] : -INFINITY;
-                mx = fmaxf(mx, x[u] * LOG2E);
+                mx = fmaxf(mx, x[u]);
             }
             const float ms = mx == -INFINITY ? 0.f : mx, al = __builtin_amdgcn_exp2f(m[c] - ms);
             m[c] = mx;
@@ -728,7 +741,7 @@ template <typename T, int DP, int NC> __global__ __launch_bounds__(256) void k_a
             for (int e = 0; e < EPL; ++e) acc[e] = o[c][e] * al;
 #pragma unroll
             for (int u = 0; u < U; ++u) {
-                const float pr = __builtin_amdgcn_exp2f(fmaf(x[u], LOG2E, -ms));
+                const float pr = __builtin_amdgcn_exp2f(x[u] - ms);
                 ps += pr;
 #pragma unroll
                 for (int e = 0; e < EPL; ++e) acc[e] = fmaf(pr, vf[u][e], acc[e]);
