@@ -588,7 +588,7 @@ int magic_knn_merge(int64_t n_query, int32_t k, int32_t n_parts,
  *   k_tiles: {first key row, keys (1..MAGIC_ATTN_TILE), first q row of the segment, its rows, segment,
  *             first key row of the segment, its keys}
  * that cover every row of q (k) exactly once; the tiles of a segment lie at multiples of MAGIC_ATTN_TILE from its start.
- * lse [q_heads, n_q] = log2 sum exp(l) (base 2) is what _bwd needs beside out.  dq [n_q,q_heads,D],
+ * lse [q_heads, n_q] = log2 sum exp(l) (base 2, double) is what _bwd needs beside out.  dq [n_q,q_heads,D],
  * dk, dv [n_k,kv_heads,D] contiguous in the operands' type; d_slopes [q_heads] or NULL.  dq may be NULL when it (and
  * d_slopes) is not wanted, dk and dv together likewise.
  * Fixed summation order.
@@ -616,9 +616,9 @@ typedef struct magic_attn {
 } magic_attn;
 size_t magic_attn_fwd_workspace_bytes(const magic_attn *args /* host */);
 int magic_attn_fwd(const magic_attn *args /* host struct of device pointers */, void *out, int64_t ld_out, int64_t hs_out,
-                   float *lse, void *workspace, size_t workspace_bytes, void *stream);
+                   double *lse, void *workspace, size_t workspace_bytes, void *stream);
 size_t magic_attn_bwd_workspace_bytes(const magic_attn *args);
-int magic_attn_bwd(const magic_attn *args, const void *out, int64_t ld_out, int64_t hs_out, const float *lse,
+int magic_attn_bwd(const magic_attn *args, const void *out, int64_t ld_out, int64_t hs_out, const double *lse,
                    const void *d_out, int64_t ld_do, int64_t hs_do, void *dq, void *dk, void *dv, float *d_slopes,
                    void *workspace, size_t workspace_bytes, void *stream);
 

@@ -1043,7 +1043,7 @@ def attn_operands(q, k, v, slopes, q_pos, k_pos, key_mask):
 
 
 def attn_fwd(q, k, v, plan, scale: float, cap: float = 0.0, slopes=None, q_pos=None, k_pos=None, key_mask=None):
-    """Segment attention forward: (out [n_q, q_heads, head_dim], lse [q_heads, n_q] float32)."""
+    """Segment attention forward: (out [n_q, q_heads, head_dim], lse [q_heads, n_q] float64)."""
     attn_check(q, k, v, plan.n_q, plan.n_k, plan.device, cap, slopes, q_pos, k_pos, key_mask)
     return attn_fwd_checked(attn_operands(q, k, v, slopes, q_pos, k_pos, key_mask), plan, scale, cap)
 
@@ -1056,7 +1056,7 @@ def attn_fwd_checked(operands, plan, scale, cap, out_lo=None):
     dev = q.device
     n, h, d = q.shape
     out = torch.empty((n, h, d), dtype=q.dtype, device=dev)
-    lse = torch.empty((h, n), dtype=torch.float32, device=dev)
+    lse = torch.empty((h, n), dtype=torch.float64, device=dev)
     a = _attn_args(q, operands[1], operands[2], plan, scale, cap, *operands[3:])
     a.out_lo = out_lo.data_ptr() if out_lo is not None else None
     ref = C.byref(a)
@@ -1076,9 +1076,9 @@ def attn_bwd(q, k, v, plan, scale: float, out, lse, d_out, cap: float = 0.0, slo
     _heads_check(out, "out", q)
     if d_out.shape != q.shape or out.shape != q.shape:
         raise MagicHipError(f"out and d_out must have q's shape {tuple(q.shape)}")
-    if lse.shape != (q.shape[1], q.shape[0]) or lse.dtype != torch.float32 or not lse.is_contiguous() \
+    if lse.shape != (q.shape[1], q.shape[0]) or lse.dtype != torch.float64 or not lse.is_contiguous() \
             or lse.device != q.device:
-        raise MagicHipError("lse must be the float32 [q_heads, n_q] tensor of the forward pass")
+        raise MagicHipError("lse must be the float64 [q_heads, n_q] tensor of the forward pass")
     ops = attn_operands(q, k, v, slopes, q_pos, k_pos, key_mask)
     return attn_bwd_checked(ops, plan, scale, cap, _head_rows(out), lse, d_out, need_dq, need_dkv, need_dslopes)
 

@@ -19,8 +19,9 @@ struct BwdArgs {
     magic_attn a;
     const void *out, *dout;
     int64_t ld_o, hs_o, ld_do, hs_do;
-    const float *lse;
-    float *lse2;        // [q_heads][n_q] lse, +inf for rows that see no key (their probabilities become zeros)
+    const double *lse;
+    float *lse2;        // [q_heads][n_q] lse rounded down, +inf for rows that see no key (their probabilities become zeros)
+    float *rest;        // [q_heads][n_q] 2^(lse2 - lse), what the rounding took: p = 2^(l log2 e - lse2) rest, rest <= 1
     float *delta;       // [q_heads][n_q]
     void *dq, *dk, *dv;
     double *slope_part; // [n_q tiles][q_heads] or NULL
@@ -52,7 +53,14 @@ template <typename T> __device__ __forceinline__ void add_low(const magic_attn &
     }
 }
 
-// lse2 and D of every row: DP / 8 lanes a row and head
+__device__ __forceinline__ float round_down(double x) {
+    const float f = (float)x;
+    if (!((double)f > x)) return f;
+    return f > 0.f ? __uint_as_float(__float_as_uint(f) - 1u) : f < 0.f ? __uint_as_float(__float_as_uint(f) + 1u) : -0x1p-149f;
+}
+__device__ __forceinline__ float rest_of(double lse, float lse2) { return __builtin_amdgcn_exp2f((float)((double)lse2 - lse)); }
+
+// lse2, rest and D of every row: DP / 8 lanes a row and head
 template <typename T, int DP> __global__ __launch_bounds__(256) void k_attn_delta(BwdArgs b) {
     constexpr int LPR = DP / 8;
     const magic_attn &a = b.a;
@@ -76,9 +84,11 @@ template <typename T, int DP> __global__ __launch_bounds__(256) void k_attn_delt
 #pragma unroll
         for (int k = LPR / 2; k > 0; k >>= 1) s += __shfl_xor(s, k, LPR);
         if (l == 0) {
-            const float ls = b.lse[(int64_t)h * a.n_q + row];
+            const double ls = b.lse[(int64_t)h * a.n_q + row];
             const bool none = ls == -INFINITY;
-            b.lse2[(int64_t)h * a.n_q + row] = none ? INFINITY : ls;
+            const float lr = round_down(ls);
+            b.lse2[(int64_t)h * a.n_q + row] = none ? INFINITY : lr;
+            b.rest[(int64_t)h * a.n_q + row] = none ? 0.f : rest_of(ls, lr);
             b.delta[(int64_t)h * a.n_q + row] = none ? 0.f : s;
         }
     }
@@ -202,8 +212,8 @@ __device__ __forceinline__ void score_grad(f32x16_t &s, const f32x16_t &dp, cons
     if (BIAS) sums.dl_dist += (double)t_dsl, sums.dl += (double)t_dl, sums.pd += (double)t_pd;
 }
 
-// The same with the keys in the lanes: probabilities (times 2^14 in the scaled mode) and score gradients; l, d: minus lse
-// and minus D of the rows, qp their positions
+// The same with the keys in the lanes: probabilities (times 2^14 in the scaled mode) and score gradients, both still without
+// the row's `rest`; l, d: minus lse2 and minus D of the rows, qp their positions
 template <typename M, bool CAP, bool BIAS>
 __device__ __forceinline__ void prob_grad(f32x16_t &s, const f32x16_t &dp, const RowSide &c, const Cap<M::N == 1> &cap,
                                           const f32x4_t *l, const f32x4_t *d, const i32x4_t *qp, float (&pr)[16], float (&ds)[16]) {
@@ -263,11 +273,15 @@ __global__ __launch_bounds__(64 * WM *KG, (DP == 128 && M::N > 1) || (DP >= 64 &
     const int64_t qr = q0 + (ok ? row : 0);
     const Src<M> K = src_of<M>(a.k, a.ld_k, a.hs_k, p.pr.k, k0, hk, D),
                  V = src_of<M>(a.v, a.ld_v, a.hs_v, p.pr.v, k0, hk, D);
-    float ls = INFINITY, dl0 = 0.f;
+    float ls = INFINITY, rest = 0.f, dl0 = 0.f;
     if (ok) {
-        ls = (p.make_delta ? p.lse : p.lse2)[(int64_t)h * a.n_q + qr];
-        if (ls == -INFINITY) ls = INFINITY;
-        if (!p.make_delta) dl0 = p.delta[(int64_t)h * a.n_q + qr];
+        const int64_t at = (int64_t)h * a.n_q + qr;
+        if (p.make_delta) {
+            const double x = p.lse[at];
+            if (x != -INFINITY) ls = round_down(x), rest = rest_of(x, ls);
+        } else {
+            ls = p.lse2[at], rest = p.rest[at], dl0 = p.delta[at];
+        }
     }
     const bool live = ls != INFINITY;
 
@@ -297,8 +311,13 @@ __global__ __launch_bounds__(64 * WM *KG, (DP == 128 && M::N > 1) || (DP >= 64 &
     }
     if (p.make_delta) {      // what the dk / dv sweep reads
         dl0 += other_half(dl0);
-        if (ok && hf == 0 && kg == 0 && split == 0) p.lse2[(int64_t)h * a.n_q + qr] = ls, p.delta[(int64_t)h * a.n_q + qr] = dl0;
+        if (ok && hf == 0 && kg == 0 && split == 0) {
+            const int64_t at = (int64_t)h * a.n_q + qr;
+            p.lse2[at] = ls, p.rest[at] = rest, p.delta[at] = dl0;
+        }
     }
+    const float dp_in = sc.dp_in * rest;         // `rest` once a row: score_grad's probabilities are without it
+    dl0 *= rest;
     const bool bias = a.slopes != nullptr;
     const float slope = bias ? a.slopes[h] * LOG2E : 0.f;
     const uint32_t qpos = bias ? flip(a.q_pos[qr]) : 0u;
@@ -359,7 +378,7 @@ __global__ __launch_bounds__(64 * WM *KG, (DP == 128 && M::N > 1) || (DP >= 64 &
             }
             feed<2 * NP, 2 * PRODUCTS<M>, KS>();
             float ds[16];
-            const RowSide rs = {sc.s_in, sc.dp_in, a.scale, f_cap, slope, qpos, ls, dl0};
+            const RowSide rs = {sc.s_in, dp_in, a.scale, f_cap, slope, qpos, ls, dl0};
             const f32x4_t *km = reinterpret_cast<const f32x4_t *>(sMask + 32 * b + 4 * hf);
             const i32x4_t *kp = reinterpret_cast<const i32x4_t *>(sPos + 32 * b + 4 * hf);
             if (a.cap > 0.f) {
@@ -441,6 +460,7 @@ __global__ __launch_bounds__(64 * WM *KG, (DP == 128 && M::N > 1) || (DP >= 64 &
                 for (int r = 0; r < 16; ++r) acc[d][r] += so[(wm * 32 + li) * OW + 32 * d + 8 * (r >> 2) + 4 * hf + (r & 3)];
         }
     }
+    sums.pd *= (double)rest;
     const float undo = M::SCALED ? run.undo() * (1.f / sc.k) : 1.f;
     if (p.q_split > 1) {       // (one key group: k_attn_dq_join puts the ranges together)
         if (p.row_sums) {
@@ -536,8 +556,9 @@ __global__ __launch_bounds__(64 * WM *KG, DP == 128 || (DP >= 64 && KG > 1) ? 1 
     typedef Tile<M, DP, BQ> tile;
     extern __shared__ __align__(16) unsigned char smem[];
     bf16_t *sQ = reinterpret_cast<bf16_t *>(smem), *sG = sQ + NP * tile::PLANE;
-    float *sL = reinterpret_cast<float *>(smem + 2 * tile::BYTES), *sD = sL + BQ;
-    uint32_t *sPos = reinterpret_cast<uint32_t *>(sD + BQ);
+    float *sL = reinterpret_cast<float *>(smem + 2 * tile::BYTES), *sD = sL + BQ, *sZ = sD + BQ;
+    uint32_t *sPos = reinterpret_cast<uint32_t *>(sZ + BQ);
+    int *sFar = reinterpret_cast<int *>(sPos + BQ);
 
     const magic_attn &a = p.a;
     if (blockIdx.x >= p.sweep_blocks) {
@@ -577,6 +598,9 @@ __global__ __launch_bounds__(64 * WM *KG, DP == 128 || (DP >= 64 && KG > 1) ? 1 
     const bool bias = a.slopes != nullptr;
     const uint32_t kpos = bias ? flip(a.k_pos[kr]) : 0u;
     const float f_cap = a.cap > 0.f ? -a.scale / a.cap / a.cap * (1.f / (LOG2E * LOG2E)) : 0.f;
+    // Without `rest` a row's probabilities are off by up to |lse2| 2^-24: below that size it is left out.  (The scaled mode has
+    // it in the rows of the gradient.)
+    constexpr float FAR = M::N == 1 ? 256.f : 4.f;
     const Cap<M::N == 1> cap(sc.s_in, a.cap);
     Running run;
     f32x16_t gk[DB], gv[DB];
@@ -590,17 +614,18 @@ __global__ __launch_bounds__(64 * WM *KG, DP == 128 || (DP >= 64 && KG > 1) ? 1 
     qst.init(src_of<M>(a.q, a.ld_q, a.hs_q, p.pr.q, q0, 0, D), D, tid);
     gst.init(src_of<M>(p.dout, p.ld_do, p.hs_do, p.pr.g, q0, 0, D), D, tid);
     int staged = 0;          // rows of the segment behind the staged tile's first
-    float ls = 0.f, dl0 = 0.f;
+    float ls = 0.f, rest = 0.f, dl0 = 0.f;
     int pos = 0;             // (all taken as loaded: a use here would wait for the whole tile)
     auto load = [&](int h, int i0) {
         qst.load(src_of<M>(a.q, a.ld_q, a.hs_q, p.pr.q, q0, h, D), i0, nq, D, tid);
         gst.load(src_of<M>(p.dout, p.ld_do, p.hs_do, p.pr.g, q0, h, D), i0, nq, D, tid);
-        const float *l2 = p.lse2 + (int64_t)h * a.n_q + q0;
+        const int64_t at = (int64_t)h * a.n_q + q0;
         staged = nq - i0;
         if (tid < BQ) {
             const int r = i0 + tid;
-            ls = r < nq ? l2[r] : INFINITY;
-            dl0 = r < nq ? p.delta[(int64_t)h * a.n_q + q0 + r] : 0.f;
+            ls = r < nq ? p.lse2[at + r] : INFINITY;
+            rest = r < nq ? p.rest[at + r] : 0.f;
+            dl0 = r < nq ? p.delta[at + r] : 0.f;
             pos = bias && r < nq ? a.q_pos[q0 + r] : 0;
         }
     };
@@ -616,9 +641,16 @@ __global__ __launch_bounds__(64 * WM *KG, DP == 128 || (DP >= 64 && KG > 1) ? 1 
         const int rows = staged;
         qst.store(sQ, D, tid, part, [&](int i) { return stage::row_of(i, tid) < rows; });
         gst.store(sG, D, tid, part, [&](int i) { return stage::row_of(i, tid) < rows; });
-        if (tid < BQ) sL[tid] = -ls, sD[tid] = -dl0, sPos[tid] = flip(pos);
+        if (tid < BQ) {
+            sL[tid] = -ls, sZ[tid] = rest, sD[tid] = M::SCALED ? -dl0 * rest : -dl0, sPos[tid] = flip(pos);
+            const bool far = __any(fabsf(ls) > FAR && ls != INFINITY);
+            if (lane == 0) sFar[wave] = far;
+        }
         const float slope = bias ? a.slopes[h] * LOG2E : 0.f;
         __syncthreads();
+        int far = M::SCALED ? 0 : sFar[0];
+        if (!M::SCALED && BQ > 64) far |= sFar[1];
+        far = __builtin_amdgcn_readfirstlane(far);
         if (++it == per_h) it = 0, ++h;
         if (st + 1 < s_end) load(h, it * BQ);
 #pragma unroll 1
@@ -646,6 +678,15 @@ __global__ __launch_bounds__(64 * WM *KG, DP == 128 || (DP >= 64 && KG > 1) ? 1 
                 bias ? prob_grad<M, true, true>(s, dp, ks, cap, l4, d4, qp, pr, ds) : prob_grad<M, true, false>(s, dp, ks, cap, l4, d4, qp, pr, ds);
             else
                 bias ? prob_grad<M, false, true>(s, dp, ks, cap, l4, d4, qp, pr, ds) : prob_grad<M, false, false>(s, dp, ks, cap, l4, d4, qp, pr, ds);
+            if (!M::SCALED && far) {
+                const f32x4_t *z4 = reinterpret_cast<const f32x4_t *>(sZ + 32 * b + 4 * hf);
+#pragma unroll
+                for (int g = 0; g < 4; ++g) {
+                    const f32x4_t z = z4[2 * g];
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) pr[4 * g + e] *= z[e], ds[4 * g + e] *= z[e];
+                }
+            }
             float u = 1.f;
             if constexpr (M::SCALED) {
                 run.step<DB>(ds, gk);
@@ -783,7 +824,7 @@ template <typename M, int DP, int WM, int KG> int run_dq(BwdArgs &b, hipStream_t
 
 template <typename M, int DP, int WM, int KG, int NB> int run_dkv(BwdArgs &b, int slope_heads, hipStream_t st) {
     constexpr int BQ = 32 * KG * NB;
-    size_t lds = 2 * Tile<M, DP, BQ>::BYTES + BQ * 12;
+    size_t lds = 2 * Tile<M, DP, BQ>::BYTES + BQ * 16 + 8;
     const size_t join = (size_t)32 * WM * (2 * ((DP + 31) / 32 * 32) + 1) * 4;
     if (KG > 1 && lds < join) lds = join;
     if (magic::ensure_dynamic_lds((const void *)k_attn_dkv<M, DP, WM, KG, NB>, lds) != MAGIC_OK) return MAGIC_ERR_RUNTIME;
@@ -901,11 +942,11 @@ size_t magic_attn_bwd_workspace_bytes(const magic_attn *a) {
     const size_t part = n > 1 ? (size_t)n * 2 * a->n_k * a->kv_heads * a->head_dim * sizeof(float) : 0;
     const int m = q_splits(a);
     const size_t rows = m > 1 ? (size_t)m * a->n_q * a->q_heads : 0;
-    return magic::align_up(part) + magic::align_up(rows * a->head_dim * sizeof(float)) + magic::align_up(rows * 3 * sizeof(double)) + prepare_bytes(a, use_f16(a), true) + 2 * magic::align_up((size_t)a->n_q * a->q_heads * sizeof(float)) +
+    return magic::align_up(part) + magic::align_up(rows * a->head_dim * sizeof(float)) + magic::align_up(rows * 3 * sizeof(double)) + prepare_bytes(a, use_f16(a), true) + 3 * magic::align_up((size_t)a->n_q * a->q_heads * sizeof(float)) +
            magic::align_up((size_t)a->n_q_tiles * 4 * a->q_heads * sizeof(double)) + 256;
 }
 
-int magic_attn_bwd(const magic_attn *a, const void *out, int64_t ld_out, int64_t hs_out, const float *lse, const void *d_out,
+int magic_attn_bwd(const magic_attn *a, const void *out, int64_t ld_out, int64_t hs_out, const double *lse, const void *d_out,
                    int64_t ld_do, int64_t hs_do, void *dq, void *dk, void *dv, float *d_slopes, void *workspace,
                    size_t workspace_bytes, void *stream_) {
     const int st = check(a);
@@ -926,6 +967,7 @@ int magic_attn_bwd(const magic_attn *a, const void *out, int64_t ld_out, int64_t
     magic::Arena ar(workspace, workspace_bytes);
     b.delta = ar.take<float>((size_t)a->n_q * a->q_heads);
     b.lse2 = ar.take<float>((size_t)a->n_q * a->q_heads);
+    b.rest = ar.take<float>((size_t)a->n_q * a->q_heads);
     b.slope_part = ar.take<double>((size_t)a->n_q_tiles * 4 * a->q_heads);
     const bool f16 = use_f16(a) && a->n_q > 0 && a->n_k > 0;
     b.n_split = dk ? splits(a) : 1;
@@ -942,7 +984,7 @@ int magic_attn_bwd(const magic_attn *a, const void *out, int64_t ld_out, int64_t
     if (a->n_q > 0 && !b.make_delta) rc = f32 ? delta_of<float>(b, stream) : delta_of<bf16_t>(b, stream);
     if (rc != MAGIC_OK) return rc;
     if (a->n_q > 0 && a->n_k > 0) {
-        const GradRows g = {d_out, ld_do, hs_do, b.lse2};
+        const GradRows g = {d_out, ld_do, hs_do, b.lse2, b.rest};
         rc = prepare(a, f16, &g, ar, b.pr, stream);
         if (rc != MAGIC_OK) return rc;
     }

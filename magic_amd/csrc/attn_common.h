@@ -385,6 +385,12 @@ __device__ __forceinline__ float dist_of(uint32_t a, uint32_t b) {
     return (float)d;
 }
 
+// log2 of a sum: the hardware's and a step of Newton's method, within 2e-7
+__device__ __forceinline__ double log2_of(float l) {
+    const float y = __builtin_amdgcn_logf(l);
+    return (double)y + (double)(fmaf(l, __builtin_amdgcn_exp2f(-y), -1.f) * LOG2E);
+}
+
 __device__ __forceinline__ float other_half(float x) { return __shfl_xor(x, 32, 64); }
 
 // Block b of a launch runs on XCD b % 8.  Runs of GS consecutive work items (tiles of one segment and head: they read
@@ -437,11 +443,11 @@ inline magic_attn gathered(const magic_attn *a, const Prepared &p) {
     g.ld_k = g.ld_v = (int64_t)a->kv_heads * a->head_dim, g.hs_k = g.hs_v = a->head_dim;
     return g;
 }
-// The output's gradient and what marks rows that see no key (lse = +inf there), in backward
+// The output's gradient, what marks rows that see no key (lse = +inf there) and what lse's rounding took, in backward
 struct GradRows {
     const void *g;
     int64_t ld, hs;
-    const float *lse;
+    const float *lse, *rest;
 };
 bool use_f16(const magic_attn *a);                                 // whether F16x2 is tried for a call
 bool use_gather(const magic_attn *a);                              // whether unmasked keys are gathered

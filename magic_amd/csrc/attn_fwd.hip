@@ -1,6 +1,7 @@
 // Softmax attention of the rows of a segment over the keys of the same segment, forward (magic_attn_fwd).
 //   s = scale q.k,  c = cap tanh(s / cap) (cap > 0),  l = c - slope_h |pos_q - pos_k|,  p = softmax of l over the
-//   unmasked keys,  o = sum p v;   lse = log2 sum exp(l), -inf for a row that sees no key (o = 0 then).
+//   unmasked keys,  o = sum p v;   lse = log2 sum exp(l), -inf for a row that sees no key (o = 0 then).  lse is a double:
+//   p = 2^(l log2 e - lse), which the backward pass forms again, is off by as much as lse is, for a whole row.
 // One pass over the keys with a running maximum and sum per row; scores are formed transposed (keys x rows), so that a
 // lane owns ONE row's statistics and the probabilities feed the second product from their registers (attn_common.h).
 // Bound by the matrix and the vector units together (beside its 4 D flops a score takes some eleven vector instructions:
@@ -228,6 +229,10 @@ __global__ __launch_bounds__(256) void k_split(SplitArgs s) {
         x.load(base + (key && s.idx ? s.idx[row] : row) * ld + y * hs + c);
         const bool use = key || !s.g.lse || s.g.lse[(int64_t)y * a.n_q + row] != INFINITY;
         if (!use) x.zero();
+        if (out == s.gr) {           // (a rounding of float32; the sweep over the keys has no registers left for it)
+            const float z = s.g.rest[(int64_t)y * a.n_q + row];
+            x.a *= z, x.b *= z;
+        }
         f16x8_t p[2];
         x.planes(p, scale);
         _Float16 *o = out + (row * heads + y) * D + c;
@@ -284,7 +289,7 @@ int prepare(const magic_attn *a, bool f16, const GradRows *g, Arena &ar, Prepare
         Range *r = ar.take<Range>(n);
         SplitArgs s;
         s.a = *a;
-        s.g = g ? *g : GradRows{nullptr, 0, 0, nullptr};
+        s.g = g ? *g : GradRows{nullptr, 0, 0, nullptr, nullptr};
         s.idx = idx, s.cnt = cnt;
         s.k = ar.take<_Float16>(plane_elems(a, true)), s.v = ar.take<_Float16>(plane_elems(a, true));
         s.q = s.gr = nullptr;
@@ -328,10 +333,10 @@ struct FwdArgs {
     magic_attn a;
     void *out;
     int64_t ld_o, hs_o;
-    float *lse;
+    double *lse;
     int n_split;          // key ranges of a tile (1: results go straight to out / lse)
     float *part_o;        // [n_split][q_heads][n_q][head_dim], normalised within the range
-    float *part_l;        // [n_split][q_heads][n_q], base-2 log of the range's sum
+    double *part_l;       // [n_split][q_heads][n_q], base-2 log of the range's sum
     int cols, rows, gc;   // columns of a block's tile = rows x gc heads of one key head
     int sub;              // blocks that share a 128-row tile of the table
     int n_hb;             // head blocks: q_heads / gc
@@ -607,7 +612,7 @@ __global__ __launch_bounds__(64 * WM *KG, DP == 128 && (M::N > 1 || WM == 1) ? 1
     }
     if (!ok) return;
     const float inv = l > 0.f || l != l ? 1.f / (l * sv) : 0.f;
-    const float ls = m == -INFINITY && l == 0.f ? -INFINITY : (float)(unit(m) + (double)__builtin_amdgcn_logf(l));   // base 2
+    const double ls = m == -INFINITY && l == 0.f ? -INFINITY : unit(m) + P_EXP + log2_of(M::SCALED ? l * 0x1p-14f : l);   // base 2
     if (p.n_split > 1) {
         const int64_t base = ((int64_t)split * a.q_heads + h) * a.n_q + q0 + row;
 #pragma unroll
@@ -770,7 +775,7 @@ template <typename T, int DP, int NC> __global__ __launch_bounds__(256) void k_a
             lt = fmaf(sl[g][c], w, lt), ot = fmaf(so[(g * NC + c) * DP + d], w, ot);
         }
         const float inv = lt > 0.f || lt != lt ? 1.f / lt : 0.f;
-        const float ls = mt == -INFINITY && lt == 0.f ? -INFINITY : mt + __builtin_amdgcn_logf(lt);
+        const double ls = mt == -INFINITY && lt == 0.f ? -INFINITY : mt + log2_of(lt);
         if (p.n_split > 1) {
             const int64_t base = ((int64_t)split * a.q_heads + h) * a.n_q + q0 + row;
             p.part_o[base * D + d] = ot * inv;
@@ -788,19 +793,20 @@ template <typename T, int DP, int NC> __global__ __launch_bounds__(256) void k_a
 // and the 256 / CPR lane groups take the ranges in turn, added in group order.
 template <typename T, int CPR> __global__ __launch_bounds__(256) void k_attn_join(FwdArgs p) {
     constexpr int NG = 256 / CPR;
-    __shared__ float w[256], red[256];
+    __shared__ float w[256];
+    __shared__ double red[256];
     __shared__ f32x4_t so[256];
     const magic_attn &a = p.a;
     const int64_t plane = a.n_q * a.q_heads;
     const int tid = threadIdx.x, g = tid / CPR, c = (tid % CPR) * 4;
     const int64_t hr = blockIdx.x;                  // head * n_q + row
-    const float mine = tid < p.n_split ? p.part_l[tid * plane + hr] : -INFINITY;
+    const double mine = tid < p.n_split ? p.part_l[tid * plane + hr] : -INFINITY;
     red[tid] = mine;
     __syncthreads();
-    float m = -INFINITY;                            // (a NaN is the largest of all: it has to reach the result)
+    double m = -INFINITY;                           // (a NaN is the largest of all: it has to reach the result)
     for (int s = 0; s < p.n_split; ++s) m = red[s] > m || red[s] != red[s] ? red[s] : m;
-    const float ms = m == -INFINITY ? 0.f : m;
-    w[tid] = __builtin_amdgcn_exp2f(mine - ms);
+    const double ms = m == -INFINITY ? 0.0 : m;
+    w[tid] = __builtin_amdgcn_exp2f((float)(mine - ms));
     __syncthreads();
     float l = 0.f;
     for (int s = 0; s < p.n_split; ++s) l += w[s];
@@ -817,7 +823,7 @@ template <typename T, int CPR> __global__ __launch_bounds__(256) void k_attn_joi
     const float x[4] = {o[0] * inv, o[1] * inv, o[2] * inv, o[3] * inv};
     const int64_t h = hr / a.n_q, row = hr - h * a.n_q;
     store_out<T>(p, row, h, c, x);
-    if (c == 0) p.lse[hr] = m == -INFINITY ? -INFINITY : ms + __builtin_amdgcn_logf(l);
+    if (c == 0) p.lse[hr] = m == -INFINITY ? -INFINITY : ms + log2_of(l);
 }
 
 // The same for up to MANY ranges of many rows: a thread holds four columns of a (row, head) and walks its ranges.
@@ -830,16 +836,16 @@ template <typename T> __global__ __launch_bounds__(256) void k_attn_join_rows(Fw
     for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < total; i += (int64_t)gridDim.x * 256) {
         const int64_t hr = i / cpr;
         const int c = (int)(i - hr * cpr) * 4;
-        float m = -INFINITY;
+        double m = -INFINITY;
         for (int s = 0; s < p.n_split; ++s) {
-            const float x = p.part_l[s * plane + hr];
+            const double x = p.part_l[s * plane + hr];
             m = x > m || x != x ? x : m;
         }
-        const float ms = m == -INFINITY ? 0.f : m;
+        const double ms = m == -INFINITY ? 0.0 : m;
         float l = 0.f;
         f32x4_t o = {0.f, 0.f, 0.f, 0.f};
         for (int s = 0; s < p.n_split; ++s) {
-            const float w = __builtin_amdgcn_exp2f(p.part_l[s * plane + hr] - ms);
+            const float w = __builtin_amdgcn_exp2f((float)(p.part_l[s * plane + hr] - ms));
             l += w;
             o += w * *reinterpret_cast<const f32x4_t *>(p.part_o + (s * plane + hr) * a.head_dim + c);
         }
@@ -847,7 +853,7 @@ template <typename T> __global__ __launch_bounds__(256) void k_attn_join_rows(Fw
         const float x[4] = {o[0] * inv, o[1] * inv, o[2] * inv, o[3] * inv};
         const int64_t h = hr / a.n_q, row = hr - h * a.n_q;
         store_out<T>(p, row, h, c, x);
-        if (c == 0) p.lse[hr] = m == -INFINITY ? -INFINITY : ms + __builtin_amdgcn_logf(l);
+        if (c == 0) p.lse[hr] = m == -INFINITY ? -INFINITY : ms + log2_of(l);
     }
 }
 
@@ -1005,11 +1011,11 @@ size_t magic_attn_fwd_workspace_bytes(const magic_attn *a) {
     if (check(a) != MAGIC_OK || a->n_q == 0) return 256;
     const Shape s = shape_of(a);
     const size_t rows = s.n_split > 1 ? (size_t)s.n_split * a->q_heads * a->n_q : 0;
-    return magic::align_up(rows * a->head_dim * sizeof(float)) + magic::align_up(rows * sizeof(float)) +
+    return magic::align_up(rows * a->head_dim * sizeof(float)) + magic::align_up(rows * sizeof(double)) +
            (s.wm == 4 ? magic::attn::prepare_bytes(a, s.f16, false) : 0) + 256;
 }
 
-int magic_attn_fwd(const magic_attn *a, void *out, int64_t ld_out, int64_t hs_out, float *lse, void *workspace,
+int magic_attn_fwd(const magic_attn *a, void *out, int64_t ld_out, int64_t hs_out, double *lse, void *workspace,
                    size_t workspace_bytes, void *stream) {
     const int st = check(a);
     if (st != MAGIC_OK || a->n_q == 0) return st;
@@ -1020,12 +1026,12 @@ int magic_attn_fwd(const magic_attn *a, void *out, int64_t ld_out, int64_t hs_ou
     p.a = *a;
     p.out = out, p.ld_o = ld_out, p.hs_o = hs_out, p.lse = lse;
     p.n_split = s.n_split, p.cols = s.cols, p.rows = s.rows, p.gc = s.gc, p.sub = s.sub, p.n_hb = s.n_hb, p.items = s.items;
-    p.part_o = p.part_l = nullptr;
+    p.part_o = nullptr, p.part_l = nullptr;
     magic::Arena ar(workspace, workspace_bytes);
     if (s.n_split > 1) {
         const size_t rows = (size_t)s.n_split * a->q_heads * a->n_q;
         p.part_o = ar.take<float>(rows * a->head_dim);
-        p.part_l = ar.take<float>(rows);
+        p.part_l = ar.take<double>(rows);
         if (!ar.ok()) return MAGIC_ERR_WORKSPACE;
     }
     int rc = MAGIC_OK;

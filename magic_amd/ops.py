@@ -484,7 +484,7 @@ _register("attn_fwd", f"({_ATTN}) -> (Tensor, Tensor)",
           lambda q, k, v, q_tiles, k_tiles, max_q, max_k, n_seg, scale, cap, slopes, q_pos, k_pos, key_mask:
           _lib.attn_fwd(q, k, v, _attn_plan(q, k, q_tiles, k_tiles, max_q, max_k, n_seg), scale, cap, slopes, q_pos, k_pos, key_mask),
           lambda q, k, v, q_tiles, k_tiles, max_q, max_k, n_seg, scale, cap, slopes, q_pos, k_pos, key_mask:
-          (q.new_empty(q.shape), q.new_empty((q.shape[1], q.shape[0]), dtype=torch.float32)))
+          (q.new_empty(q.shape), q.new_empty((q.shape[1], q.shape[0]), dtype=torch.float64)))
 
 
 def _attn_bwd(q, k, v, q_tiles, k_tiles, max_q: int, max_k: int, n_seg: int, scale: float, cap: float, slopes, q_pos, k_pos, key_mask, out, lse, d_out):

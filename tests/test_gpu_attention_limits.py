@@ -66,3 +66,55 @@ def test_one_key_takes_everything(cuda, shape, kind, far, dtype):
     assert not got["dv"][lost].any() and not got["dk"][lost].any()
     for name in got:
         assert torch.isfinite(got[name]).all(), name
+
+
+def _half_step(dtype):
+    """What a bfloat16 call rounds inside its products, relative."""
+    return torch.finfo(dtype).eps / 2 if dtype == torch.bfloat16 else 0.0
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=["f32", "bf16"])
+@pytest.mark.parametrize("far", [80, 8000, 80000, 700000, 8000000, 2100000000])
+@pytest.mark.parametrize("shape", list(SHAPES))
+def test_gradients_where_one_key_takes_everything(cuda, shape, far, dtype):
+    """p = 1 in the backward pass too, however far the key is: dv is the sum of the rows' gradients, and dq, dk what is left
+    of do.v - do.o, zero but for rounding.  q and k are quarters up to 2, so that a score is exact in any order."""
+    q_lens, kv_lens, h, D = SHAPES[shape]
+    q, k, v, d, opts, win = _ahead(cuda, q_lens, kv_lens, h, D, dtype, min(far, 2 ** 31 - 1 - 20000 * max(kv_lens)), "positions")
+    q, k = ((t.float() * 4).round().clamp(-8, 8).div(4).to(dtype) for t in (q, k))
+    got = run(q, k, v, d, q_lens, kv_lens, **opts)
+    want = v[win].double()
+    dv, mag = torch.zeros_like(v, dtype=torch.float64), torch.zeros_like(v, dtype=torch.float64)
+    dv.index_add_(0, win, d.double())
+    mag.index_add_(0, win, d.double().abs())
+    _close(got["dv"], dv, mag, n=max(q_lens))
+    # do.v and do.o: D products and sums each; a bfloat16 o and its low part leave half^2 of it, twice with do.v's own part
+    half = _half_step(dtype)
+    size = (d.double().abs() * want.abs()).sum(-1, keepdim=True)
+    bound = (2 * (D + 8) * U + 2 * half * half) * size / math.sqrt(D) * 1.01
+    assert (got["dq"].double().abs() <= bound * k[win].double().abs() + 2.0 ** -120).all()
+    kb = torch.zeros_like(dv)
+    kb.index_add_(0, win, bound * q.double().abs())
+    assert (got["dk"].double().abs() <= kb + 2.0 ** -120).all()
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=["f32", "bf16"])
+@pytest.mark.parametrize("far", [0, 8000, 700000, 100000000])
+@pytest.mark.parametrize("q_lens,kv_lens,h,D", [([40], [90], 2, 32), ([3], [3000], 1, 64), ([700], [700], 16, 64), ([1300], [1300], 2, 64),
+                                                ([2], [9000], 4, 128), ([20], [9000], 4, 128)])
+def test_keys_of_equal_logits_far_away(cuda, q_lens, kv_lens, h, D, far, dtype):
+    """Three keys at one position share everything, one near the first key and two near the last (so that ranges of keys
+    hold one and two of them), the others 1e6 positions behind them: p = 1/3 each, in the output and in dv."""
+    q, k, v, d, _ = make(cuda, q_lens, kv_lens, h, h, D, dtype, seed=8)
+    k[:] = 0                                                  # all scores are zeros: the logits are the positions'
+    n, m = q_lens[0], kv_lens[0]
+    k_pos = torch.full((m,), -1000000, dtype=torch.int32, device=cuda)
+    win = torch.tensor([1, m - 3, m - 2], device=cuda)
+    k_pos[win] = 0
+    slopes = torch.full((h,), 0.125, device=cuda)
+    got = run(q, k, v, d, q_lens, kv_lens, slopes=slopes, k_pos=k_pos, q_pos=torch.full((n,), far, dtype=torch.int32, device=cuda))
+    half = _half_step(dtype)                              # of a probability in a product
+    want, mag = v[win].double().mean(0), v[win].double().abs().mean(0)
+    _close(got["out"], want.expand(n, h, D), (1 + half / U / 8) * mag.expand(n, h, D))
+    dv, dmag = d.double().sum(0) / 3, d.double().abs().sum(0) / 3
+    _close(got["dv"][win], dv.expand(3, h, D), (1 + half / U / 8) * dmag.expand(3, h, D), n=n + 8)
