@@ -343,6 +343,7 @@ template <bool RAW> struct Cap {
         if (RAW) {
             const float u = cap * f, f2 = f * f;
             c0 = K0 * u, c1 = K1 * u * f2, c2 = K2 * u * f2 * f2, c3 = K3 * u * f2 * f2 * f2;
+            if (!(fabsf(c3) < INFINITY)) lim = -1.f;        // a steep cap: never by these coefficients
         } else {
             c0 = K0 * cap, c1 = K1 * cap, c2 = K2 * cap, c3 = K3 * cap;
         }

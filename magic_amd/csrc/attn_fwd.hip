@@ -30,7 +30,7 @@ int check(const magic_attn *a) {
     const int per = a->dtype == MAGIC_F32 ? 4 : 8;   // rows and heads start on 16-byte addresses
     if (((uintptr_t)a->q | (uintptr_t)a->k | (uintptr_t)a->v | (uintptr_t)a->out_lo) & 15) return MAGIC_ERR_INVALID_ARG;
     if ((a->ld_q | a->hs_q | a->ld_k | a->hs_k | a->ld_v | a->hs_v) % per) return MAGIC_ERR_INVALID_ARG;
-    // (scale / cap and cap times a polynomial's terms stay normal float32 numbers)
+    // (scale / cap and cap stay normal float32 numbers)
     if (!(a->cap == 0.f || (a->cap >= 1e-3f && a->cap <= 1e30f)) || !(std::fabs(a->scale) <= 1e30f)) return MAGIC_ERR_INVALID_ARG;
     if (a->slopes && ((a->n_q > 0 && !a->q_pos) || (a->n_k > 0 && !a->k_pos))) return MAGIC_ERR_INVALID_ARG;
     return MAGIC_OK;

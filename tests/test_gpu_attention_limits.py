@@ -118,3 +118,15 @@ def test_keys_of_equal_logits_far_away(cuda, q_lens, kv_lens, h, D, far, dtype):
     _close(got["out"], want.expand(n, h, D), (1 + half / U / 8) * mag.expand(n, h, D))
     dv, dmag = d.double().sum(0) / 3, d.double().abs().sum(0) / 3
     _close(got["dv"][win], dv.expand(3, h, D), (1 + half / U / 8) * dmag.expand(3, h, D), n=n + 8)
+
+
+@pytest.mark.parametrize("cap,scale", [(1e-3, 2e3), (1.0, 1e6), (1e-3, 1e30), (1e30, 1e30)])
+@pytest.mark.parametrize("n", [40, 700])
+def test_zero_rows_under_steep_caps(cuda, cap, scale, n):
+    """A row of zeros scores zero everywhere and gets the mean of the values, whatever scale / cap is."""
+    q, k, v, d, _ = make(cuda, [n], [n], 4, 4, 64, torch.bfloat16, seed=3)
+    q[:] = 0
+    got = run(q, k, v, d, [n], [n], cap=cap, scale=scale)
+    # (a probability of the product is 2^0 before the division by the sum: no bfloat16 rounding)
+    _close(got["out"], v.double().mean(0).expand(n, 4, 64), v.double().abs().mean(0).expand(n, 4, 64), n=n)
+    assert not torch.isnan(got["dk"]).any() and not torch.isnan(got["dv"]).any()
