@@ -294,8 +294,7 @@ __global__ __launch_bounds__(64 * WM *KG, (DP == 128 && M::N > 1) || (DP >= 64 &
         Raw<T> r, g;
         r.load((const T *)a.q + qr * a.ld_q + h * a.hs_q + cc);
         g.load((const T *)p.dout + qr * p.ld_do + h * p.hs_do + cc);
-        if (!ok || c >= D) r.zero();
-        if (!live || c >= D) g.zero();
+        if (!live || c >= D) r.zero(), g.zero();      // (rows that see no key: nothing of them, NaN included)
         if (p.make_delta) {
             float x[8], y[8];
             Raw<T> o;

@@ -370,7 +370,7 @@ __global__ __launch_bounds__(64 * WM *KG, DP == 128 && (M::N > 1 || WM == 1) ? 1
     extern __shared__ __align__(16) unsigned char smem[];
     bf16_t *sK = reinterpret_cast<bf16_t *>(smem), *sV = sK + NP * tile::PLANE;
     uint32_t *sPos = reinterpret_cast<uint32_t *>(smem + 2 * tile::BYTES);
-    float *sMask = reinterpret_cast<float *>(sPos + BK);
+    uint32_t *sMask = sPos + BK;           // all bits of a key that takes part
 
     const magic_attn &a = p.a;
     const int64_t item = xcd_item(blockIdx.x, 16);
@@ -464,7 +464,7 @@ __global__ __launch_bounds__(64 * WM *KG, DP == 128 && (M::N > 1 || WM == 1) ? 1
         const bool masked = a.key_mask != nullptr || (tt + 1) * BK > nk;
         kst.store(sK, D, tid, masked, [&](int i) { return keep[i] != 0; });
         vst.store(sV, D, tid, masked, [&](int i) { return keep[i] != 0; });
-        if (tid < BK) sPos[tid] = flip(pos), sMask[tid] = mk ? 0.f : -INFINITY;
+        if (tid < BK) sPos[tid] = flip(pos), sMask[tid] = mk ? 0xffffffffu : 0u;
         __syncthreads();
         if (tt + 1 < t_end) load(tt + 1);
 
@@ -483,7 +483,7 @@ __global__ __launch_bounds__(64 * WM *KG, DP == 128 && (M::N > 1 || WM == 1) ? 1
                 mma(s[b], f, qf[ks]);
             }
         feed<NP * KB, PRODUCTS<M> * KB, KS>();
-        // logits; a masked key's zero score gets -inf
+        // logits; a masked key's is -inf, whatever its score became (0 times an infinity of q)
 #pragma unroll
         for (int b = 0; b < KB; ++b) {
             if (a.cap > 0.f) {
@@ -495,9 +495,10 @@ __global__ __launch_bounds__(64 * WM *KG, DP == 128 && (M::N > 1 || WM == 1) ? 1
             if (masked) {
 #pragma unroll
                 for (int g = 0; g < 4; ++g) {
-                    const f32x4_t km = *reinterpret_cast<const f32x4_t *>(sMask + kg * KW + 32 * b + 8 * g + 4 * hf);
+                    const i32x4_t km = *reinterpret_cast<const i32x4_t *>(sMask + kg * KW + 32 * b + 8 * g + 4 * hf);
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) s[b][4 * g + e] += km[e];
+                    for (int e = 0; e < 4; ++e)
+                        s[b][4 * g + e] = __uint_as_float((__float_as_uint(s[b][4 * g + e]) & (uint32_t)km[e]) | (0xff800000u & ~(uint32_t)km[e]));
                 }
             }
             if (bias) {

@@ -130,3 +130,26 @@ def test_zero_rows_under_steep_caps(cuda, cap, scale, n):
     # (a probability of the product is 2^0 before the division by the sum: no bfloat16 rounding)
     _close(got["out"], v.double().mean(0).expand(n, 4, 64), v.double().abs().mean(0).expand(n, 4, 64), n=n)
     assert not torch.isnan(got["dk"]).any() and not torch.isnan(got["dv"]).any()
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=["f32", "bf16"])
+@pytest.mark.parametrize("lens,blind,hq,hk,D", [([40, 70, 33], 1, 4, 2, 64), ([700, 600, 33], 1, 16, 8, 64), ([2, 1, 3], 0, 2, 2, 32), ([300], 0, 1, 1, 128)])
+@pytest.mark.parametrize("opts", ["plain", "all"])
+def test_rows_that_see_no_key_may_hold_anything(cuda, lens, blind, hq, hk, D, opts, dtype):
+    """NaN and infinities in q and in the incoming gradient of rows whose keys are all masked: zeros, and nothing of it in
+    any other result."""
+    q, k, v, d, kw = make(cuda, lens, lens, hq, hk, D, dtype, seed=4, slopes=opts == "all", mask=0.7)
+    if opts == "all":
+        kw["cap"] = 9.0
+    at = sum(lens[:blind])
+    rows = slice(at, at + lens[blind])
+    kw["key_mask"][rows] = False
+    clean = run(q, k, v, d, lens, lens, **kw)
+    check(clean, q, k, v, d, lens, lens, **kw)
+    for poison in (float("nan"), float("inf"), -float("inf")):
+        q2, d2 = q.clone(), d.clone()
+        q2[rows], d2[rows] = poison, poison
+        dirty = run(q2, k, v, d2, lens, lens, **kw)
+        assert not dirty["out"][rows].any() and not dirty["dq"][rows].any()
+        for name in clean:
+            assert torch.equal(clean[name], dirty[name]), (name, poison)
