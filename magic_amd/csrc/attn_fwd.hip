@@ -612,7 +612,8 @@ __global__ __launch_bounds__(64 * WM *KG, DP == 128 && (M::N > 1 || WM == 1) ? 1
         m = mt, l = lt;
     }
     if (!ok) return;
-    const float inv = l > 0.f || l != l ? 1.f / (l * sv) : 0.f;
+    // (two factors: l times the scale of tiny values is no float32 number)
+    const float inv = l > 0.f || l != l ? 1.f / l : 0.f, unv = 1.f / sv;
     const double ls = m == -INFINITY && l == 0.f ? -INFINITY : unit(m) + P_EXP + log2_of(M::SCALED ? l * 0x1p-14f : l);   // base 2
     if (p.n_split > 1) {
         const int64_t base = ((int64_t)split * a.q_heads + h) * a.n_q + q0 + row;
@@ -623,7 +624,7 @@ __global__ __launch_bounds__(64 * WM *KG, DP == 128 && (M::N > 1 || WM == 1) ? 1
                 const int c = 32 * d + 8 * g + 4 * hf;
                 if (c < D)
                     *reinterpret_cast<f32x4_t *>(p.part_o + base * D + c) =
-                        f32x4_t{o[d][4 * g] * inv, o[d][4 * g + 1] * inv, o[d][4 * g + 2] * inv, o[d][4 * g + 3] * inv};
+                        f32x4_t{o[d][4 * g] * inv * unv, o[d][4 * g + 1] * inv * unv, o[d][4 * g + 2] * inv * unv, o[d][4 * g + 3] * inv * unv};
             }
         if (hf == 0) p.part_l[base] = ls;
         return;
@@ -633,7 +634,7 @@ __global__ __launch_bounds__(64 * WM *KG, DP == 128 && (M::N > 1 || WM == 1) ? 1
 #pragma unroll
         for (int g = 0; g < 4; ++g) {
             const int c = 32 * d + 8 * g + 4 * hf;
-            const float x[4] = {o[d][4 * g] * inv, o[d][4 * g + 1] * inv, o[d][4 * g + 2] * inv, o[d][4 * g + 3] * inv};
+            const float x[4] = {o[d][4 * g] * inv * unv, o[d][4 * g + 1] * inv * unv, o[d][4 * g + 2] * inv * unv, o[d][4 * g + 3] * inv * unv};
             if (c < D) store_out<T>(p, q0 + row, h, c, x);
         }
     if (hf == 0) p.lse[(int64_t)h * a.n_q + q0 + row] = ls;

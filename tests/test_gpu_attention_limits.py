@@ -153,3 +153,12 @@ def test_rows_that_see_no_key_may_hold_anything(cuda, lens, blind, hq, hk, D, op
         assert not dirty["out"][rows].any() and not dirty["dq"][rows].any()
         for name in clean:
             assert torch.equal(clean[name], dirty[name]), (name, poison)
+
+
+@pytest.mark.parametrize("size", [1e-20, 1e-30, 1e-34])
+def test_tiny_values(cuda, size):
+    """Values far below one, under the two scaled planes: the outputs and gradients are theirs."""
+    lens = [700, 30]
+    q, k, v, d, _ = make(cuda, lens, lens, 16, 16, 64, torch.float32, seed=6)
+    v = v * size
+    check(run(q, k, v, d, lens, lens), q, k, v, d, lens, lens)
