@@ -182,6 +182,11 @@ def _stream() -> int:
     return torch.cuda.current_stream().cuda_stream
 
 
+def stream_on(device) -> int:
+    """Handle of the current HIP stream of ``device`` (with its index)."""
+    return _raw_stream(device.index) if _raw_stream is not None else torch.cuda.current_stream(device).cuda_stream
+
+
 def _dev(t: Optional[torch.Tensor], dtype=None, name="tensor") -> Optional[int]:
     if t is None:
         return None

@@ -352,17 +352,16 @@ class Graph:
     def component_attention(self):
         """(plan, positions) for attention inside the component graphs: the ``model.attention.AttentionPlan`` of
         ``batch_num_nodes()`` and every node's index in its own component (its order of appearance), int32 [N].  Kept
-        with the structure, which never changes."""
+        with the structure, which never changes, for calls on any stream."""
         lens = self.batch_num_nodes()
         kept = getattr(self._s, "_component_attention", None)
         if kept is None or kept[0] != lens:
             from .model.attention import attention_plan
             n = torch.tensor(lens, dtype=torch.int64)
             pos = torch.arange(self.num_nodes()) - torch.repeat_interleave(torch.cumsum(n, 0) - n, n)
-            pos = pos.to(torch.int32)
-            if self.device.type == "cuda":
-                pos = pos.pin_memory().to(self.device, non_blocking=True)
-            kept = self._s._component_attention = (lens, attention_plan(lens, device=self.device), pos)
+            # (the plan first: it refuses to be built during a capture)
+            kept = self._s._component_attention = (lens, attention_plan(lens, device=self.device), pos.to(torch.int32).to(self.device))
+        kept[1].hold(kept[2])
         return kept[1], kept[2]
 
     # ---- helpers used by the HIP operators -------------------------------------------

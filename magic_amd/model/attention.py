@@ -35,10 +35,22 @@ class AttentionPlan:
         self.max_q, self.max_k = max(q_lens, default=0), max(kv_lens, default=0)
         self.n_seg = len(q_lens)
         self.q_tiles, self.k_tiles = q_tiles, k_tiles
+        self._stream = _stream_of(q_tiles.device)
 
     @property
     def device(self):
         return self.q_tiles.device
+
+    def hold(self, *more):
+        """Keeps the memory of the tables (and of ``more`` that came with them) from being handed out again while work of
+        the current stream, if it is not the one they were made on, still reads them."""
+        if _stream_of(self.device) != self._stream:
+            for t in (self.q_tiles, self.k_tiles) + more:
+                t.record_stream(torch.cuda.current_stream(self.device))
+
+
+def _stream_of(device):
+    return _lib.stream_on(device) if device.type == "cuda" else None
 
 
 def _tiles(rows, others):
@@ -56,8 +68,8 @@ def _tiles(rows, others):
 def attention_plan(q_lens: Sequence[int], kv_lens: Optional[Sequence[int]] = None, device="cuda") -> AttentionPlan:
     """Plan for segments of ``q_lens[i]`` query rows over ``kv_lens[i]`` key rows (host integers, in row order; keys =
     queries when ``kv_lens`` is None).  Lengths may be zero.  A plan serves any heads, types and options, and can be
-    kept as long as the lengths stay the same (all layers of a step, all calls against one stored graph).  Its tables are
-    copied to the device here: build it before recording a graph."""
+    kept as long as the lengths stay the same (all layers of a step, all calls against one stored graph), on any stream of
+    its device.  Its tables are on the device when this returns: build it before recording a graph."""
     q_lens = [int(x) for x in q_lens]
     kv_lens = q_lens if kv_lens is None else [int(x) for x in kv_lens]
     if len(q_lens) != len(kv_lens):
@@ -73,7 +85,8 @@ def attention_plan(q_lens: Sequence[int], kv_lens: Optional[Sequence[int]] = Non
     if device.type == "cuda":
         if torch.cuda.is_current_stream_capturing():
             raise _lib.MagicHipError("build the plan before the capture: its tables would not outlive it")
-        tabs = [t.pin_memory().to(device, non_blocking=True) for t in tabs]
+        # (blocking copies: the kernels take the tables' entries as offsets, on whatever stream a call comes)
+        tabs = [t.to(device) for t in tabs]
     return AttentionPlan(q_lens, kv_lens, *tabs)
 
 
@@ -81,6 +94,7 @@ class _SegmentAttentionFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, v, slopes, plan, scale, cap, q_pos, k_pos, key_mask):
         _lib.attn_check(q, k, v, plan.n_q, plan.n_k, plan.device, cap, slopes, q_pos, k_pos, key_mask)
+        plan.hold()
         operands = _lib.attn_operands(q, k, v, slopes, q_pos, k_pos, key_mask)
         # A score gradient is p (do.v - do.o): with few keys the rounding of a bfloat16 o is twice what else is off
         out_lo = torch.empty(q.shape, dtype=q.dtype, device=q.device) if q.dtype == torch.bfloat16 and any(ctx.needs_input_grad) else None

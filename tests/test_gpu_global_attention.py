@@ -198,3 +198,50 @@ def test_captured_training_step_of_the_block(cuda, bits):
         eager = step(new[0].requires_grad_(True), *new[1:])
         torch.cuda.synchronize()
         assert all(torch.equal(a, b) for a, b in zip(got, eager))
+
+
+def _two_component_graphs(cuda, lens):
+    import magic_amd as G
+    edge = torch.zeros(1, dtype=torch.long)
+    return G.batch([G.graph((edge, edge), num_nodes=n).to(cuda) for n in lens])
+
+
+def test_component_plan_made_on_one_stream_and_read_on_another(cuda):
+    """The tables are whole for a second stream although the first, which made them, is busy."""
+    from magic_amd.model.attention import attention_plan
+    lens = [130, 70, 1]
+    g, want = _two_component_graphs(cuda, lens), attention_plan(lens, device="cpu")
+    torch.cuda.synchronize()
+    a, b = torch.cuda.Stream(), torch.cuda.Stream()
+    with torch.cuda.stream(a):
+        torch.cuda._sleep(5_000_000)
+        plan, pos = g.component_attention()
+    with torch.cuda.stream(b):
+        got = plan.q_tiles.clone(), plan.k_tiles.clone(), pos.clone()
+    torch.cuda.synchronize()
+    assert torch.equal(got[0].cpu(), want.q_tiles) and torch.equal(got[1].cpu(), want.k_tiles)
+    assert torch.equal(got[2].cpu(), torch.cat([torch.arange(n, dtype=torch.int32) for n in lens]))
+
+
+def test_component_plan_dropped_while_another_stream_reads_it(cuda):
+    """The plan's stream gets its memory back only behind the work of the other one.  (What that stream writes next is
+    another valid plan of the same size: whichever of the two a call reads, it stays inside its operands.)"""
+    from magic_amd.model.attention import attention_plan, segment_attention
+    lens, other = [130, 70, 1], [1, 70, 130]
+    x = torch.randn(201, 4, 32, device=cuda)
+    want = segment_attention(x, x, x, attention_plan(lens, device=cuda))
+    fill = attention_plan(other, device=cuda).q_tiles
+    torch.cuda.synchronize()
+    a, b = torch.cuda.Stream(), torch.cuda.Stream()
+    g = _two_component_graphs(cuda, lens)
+    torch.cuda.synchronize()
+    with torch.cuda.stream(a):
+        plan, _ = g.component_attention()
+    with torch.cuda.stream(b):
+        torch.cuda._sleep(5_000_000)
+        got = segment_attention(x, x, x, plan)
+    del plan, g
+    with torch.cuda.stream(a):
+        again = [fill.clone() for _ in range(64)]
+    torch.cuda.synchronize()
+    assert torch.equal(got, want) and len(again) == 64
