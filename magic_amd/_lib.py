@@ -970,7 +970,9 @@ def _head_rows(t: torch.Tensor) -> torch.Tensor:
     if inner == 1 and ld % per == 0 and hs % per == 0 and ld <= ATTN_MAX_LD and t.data_ptr() % 16 == 0:
         return t
     t = t.contiguous()
-    return t if t.data_ptr() % 16 == 0 else t.clone()
+    if t.data_ptr() % 16:
+        t = t.clone()
+    return t.as_strided(t.shape, (t.shape[1] * t.shape[2], t.shape[2], 1))     # (a single row or head keeps any stride otherwise)
 
 
 def _heads_check(t: torch.Tensor, name: str, like: Optional[torch.Tensor] = None):

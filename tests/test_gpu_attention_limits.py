@@ -7,7 +7,7 @@ import math
 import pytest
 import torch
 
-from tests.test_gpu_attention import U, check, make, run
+from tests.test_gpu_attention import U, check, make, rope_reference, run
 
 pytestmark = pytest.mark.gpu
 
@@ -162,3 +162,23 @@ def test_tiny_values(cuda, size):
     q, k, v, d, _ = make(cuda, lens, lens, 16, 16, 64, torch.float32, seed=6)
     v = v * size
     check(run(q, k, v, d, lens, lens), q, k, v, d, lens, lens)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=["f32", "bf16"])
+@pytest.mark.parametrize("shape,strides", [((1, 4, 16), (67, 16, 1)), ((1, 4, 16), (2 ** 22 + 72, 16, 1)), ((1, 1, 16), (3, 5, 1)),
+                                           ((6, 1, 16), (64, 7, 1)), ((0, 4, 16), (67, 16, 1)), ((1, 2, 8), (2 ** 23, 8, 1))])
+def test_single_rows_and_heads_of_any_stride(cuda, shape, strides, dtype):
+    """One row cut from a store, one head cut from a row: a stride that is never taken may be any number."""
+    from magic_amd.model.attention import head_norm_rope
+    n, h, D = shape
+    base = torch.randn(8, 4 * D, device=cuda).to(dtype)
+    cut = lambda i: base.flatten()[i * 8:].as_strided(shape, strides) if n * h else base[:0].view(0, h, D)  # noqa: E731
+    rows = [cut(i) for i in range(4)]
+    plain = [t.clone(memory_format=torch.contiguous_format).reshape(-1).clone().view(shape) for t in rows]
+    got, want = (run(*ts, [n], [n]) for ts in (rows, plain))
+    assert all(torch.equal(got[k], want[k]) for k in want)
+    w, pos = torch.rand(D, device=cuda) + 0.5, torch.arange(n, device=cuda, dtype=torch.int32)
+    # (strides that are no whole 16 bytes take single columns there: another order of a row's sum of squares)
+    for got, x in zip(head_norm_rope(rows[0], rows[1], w, w, pos), plain):
+        want, tol = rope_reference(x, w, pos, D, 1e-6, 10000.0, torch.zeros_like(x))[0]
+        assert ((got.double() - want).abs() <= tol).all()
