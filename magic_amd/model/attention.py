@@ -162,7 +162,9 @@ class GlobalAttention(nn.Module):
     learned bias per head that falls with the distance of two positions.  ``W_o`` starts as zeros: the block is the
     identity until it has learned something.
 
-    ``act_bits=8`` keeps the inputs of its linear layers for the backward pass as 8-bit codes (``act8.py``)."""
+    ``act_bits=8`` keeps the input of its first linear layer for the backward pass as 8-bit codes (``act8.py``).  That saves
+    memory where nothing else keeps ``x``; an activation or a graph layer that made it does.  (The input of the last linear
+    layer is the attention's result, which its own backward pass reads in float32.)"""
 
     def __init__(self, dim: int, n_heads: int, cap: float = 50.0, act_bits: int = 32):
         super().__init__()
@@ -188,4 +190,4 @@ class GlobalAttention(nn.Module):
         q, k, v = (t.view(n, self.n_heads, self.head_dim) for t in parts)
         q, k = head_norm_rope(q, k, self.q_weight, self.k_weight, pos)
         o = segment_attention(q, k, v, plan, cap=self.cap, slopes=self.slopes, q_pos=pos, k_pos=pos, key_mask=key_mask)
-        return x + linear_nobias(o.view(n, dim), self.out.weight, self.act_bits)
+        return x + linear_nobias(o.view(n, dim), self.out.weight)

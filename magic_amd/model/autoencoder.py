@@ -134,8 +134,9 @@ class GMAEModel(nn.Module):
 
     Two options beyond the reference, off by default (same parameters, same numbers then): ``global_attention=True``
     puts a ``GlobalAttention`` block behind the encoder's last layer (unmasked nodes are attended while training, all
-    nodes in ``embed``); ``act_bits=8`` keeps the inputs of that block's linear layers, of the edge head's first layer
-    and, on the layer-by-layer path, of ``encoder_to_decoder`` for the backward pass as 8-bit codes."""
+    nodes in ``embed``); ``act_bits=8`` keeps the input of the edge head's first layer and, on the layer-by-layer path
+    (which the block takes), of ``encoder_to_decoder`` for the backward pass as 8-bit codes.  The other layers' inputs are
+    results that the layers before them keep for themselves: codes beside them would cost memory."""
 
     def __init__(self, n_dim, e_dim, hidden_dim, n_layers, n_heads, activation, feat_drop, negative_slope,
                  residual, norm, mask_rate=0.5, loss_fn="sce", alpha_l=2, mask_rng="cpu", alias_clone=True,
@@ -182,7 +183,7 @@ class GMAEModel(nn.Module):
         self.encoder_to_decoder = nn.Linear(hidden_dim * n_layers, hidden_dim, bias=False)
         self.criterion = self.setup_loss_fn(loss_fn, alpha_l)
         # (last: the parameters above are drawn as without it)
-        self.global_attn = GlobalAttention(hidden_dim, n_heads, act_bits=act_bits) if global_attention else None
+        self.global_attn = GlobalAttention(hidden_dim, n_heads) if global_attention else None
 
     @property
     def output_hidden_dim(self):

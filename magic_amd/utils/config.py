@@ -18,5 +18,5 @@ def build_args(argv=None):
     parser.add_argument("--global_attention", action="store_true",
                         help="attention of every node over its own component graph behind the encoder")
     parser.add_argument("--act_bits", type=int, default=32, choices=(8, 32),
-                        help="bits of the linear layers' inputs kept for the backward pass")
+                        help="bits in which linear layers keep an input that no other layer keeps for the backward pass")
     return parser.parse_args(argv)

@@ -245,3 +245,46 @@ def test_component_plan_dropped_while_another_stream_reads_it(cuda):
         again = [fill.clone() for _ in range(64)]
     torch.cuda.synchronize()
     assert torch.equal(got, want) and len(again) == 64
+
+
+def _held(fn, owned):
+    """Bytes of the distinct memory that the backward pass of ``fn()`` holds beside ``owned`` tensors."""
+    seen = {}
+
+    def pack(t):
+        s = t.untyped_storage()
+        seen[s.data_ptr()] = s.nbytes()
+        return t
+
+    with torch.autograd.graph.saved_tensors_hooks(pack, lambda t: t):
+        y = fn()
+    own = {t.untyped_storage().data_ptr() for t in owned}
+    return sum(n for p, n in seen.items() if p not in own), y
+
+
+def test_what_8_bit_checkpoints_save_in_the_block_and_the_model(cuda):
+    """The inputs that only the 8-bit layers keep shrink from 4 to 1 + 1 / 32 bytes an element, and nothing is added
+    anywhere else."""
+    from magic_amd.model.attention import GlobalAttention
+    from magic_amd.model.autoencoder import GMAEModel
+    lens = [130, 200]
+    g, n = _two_component_graphs(cuda, lens), 330
+    x0 = torch.randn(n, 64, device=cuda, requires_grad=True)
+    held = {}
+    for bits in (32, 8):
+        block = GlobalAttention(64, 4, act_bits=bits).to(cuda)
+        held[bits], _ = _held(lambda: block(g, x0 * 2.0), [x0, *block.parameters()])     # (x0 * 2 keeps nothing of its result)
+    assert held[32] - held[8] == n * 64 * 3 - n * 64 // 32
+    n_dim, e_dim, n, e, layers = 5, 7, 300, 1500, 3
+    src, dst, nt, et = small_graph(n, e, n_dim, e_dim, seed=5, hub_deg=90)
+    gen = torch.Generator().manual_seed(1)
+    kw = dict(perm=torch.randperm(n, generator=gen).to(cuda), pos_idx=torch.randperm(src.size, generator=gen)[:n],
+              neg_pairs=tuple(torch.randint(0, n, (2, n), generator=gen)))
+    for bits in (32, 8):
+        torch.manual_seed(0)
+        model = GMAEModel(n_dim, e_dim, 64, layers, 4, "prelu", 0.1, 0.2, True, "BatchNorm", 0.5, "sce", 3,
+                          global_attention=True, act_bits=bits).to(cuda).eval()
+        graph = to_graph(src, dst, n, nt, et, n_dim, e_dim, cuda)
+        held[bits], loss = _held(lambda: model.compute_loss(graph, **kw), model.parameters())
+    elements = n * 64 * layers + 2 * n * 2 * 64 * layers                  # hidden states side by side; rows of 2 n node pairs
+    assert held[32] - held[8] == elements * 3 - elements // 32
