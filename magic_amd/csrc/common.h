@@ -35,6 +35,10 @@ inline int launch_status() {
     return e == hipSuccess ? MAGIC_OK : MAGIC_ERR_LAUNCH;
 }
 
+// `rows` rows of `cols` 32-bit words, `ld` words apart, all set to v; serves inside a graph capture (fill.hip)
+int fill_rows(void *p, uint32_t v, int64_t rows, int64_t cols, int64_t ld, hipStream_t stream);
+inline int fill_words(void *p, uint32_t v, int64_t n, hipStream_t stream) { return fill_rows(p, v, 1, n, n, stream); }
+
 inline size_t align_up(size_t x, size_t a = 256) { return (x + a - 1) / a * a; }
 
 // Bump allocator over the caller's workspace.

@@ -833,8 +833,7 @@ template <int H, int LPH>
 int launch_table(BwdArgs &a, hipStream_t stream) {
     if (!a.etype || !a.d_table) return MAGIC_OK;
     if (a.E == 0) {
-        if (hipMemsetAsync(a.d_table, 0, sizeof(float) * a.e_dim * H, stream) != hipSuccess) return MAGIC_ERR_RUNTIME;
-        return MAGIC_OK;
+        return magic::fill_words(a.d_table, 0u, (int64_t)a.e_dim * H, stream);
     }
     const size_t sh = (size_t)a.e_dim * H * TBL_THREADS * sizeof(float);
     if (magic::ensure_dynamic_lds((const void *)k_bwd_table_partial<H>, sh) != MAGIC_OK) return MAGIC_ERR_RUNTIME;
@@ -853,8 +852,7 @@ int launch_bwd(BwdArgs &a, hipStream_t stream) {
             MAGIC_LAUNCH("gat_bwd_reduce_bias", k_bwd_reduce_bias, C + 1, 256, 0, stream, a, C);
     }
     if (a.E == 0) {  // no edges: d_hs = d_eh = d_et = 0 and an all-zero edge-type table
-        if (hipMemset2DAsync(a.d_y, sizeof(float) * a.ld_dy, 0, sizeof(float) * (C + 2 * H), a.N, stream) != hipSuccess)
-            return MAGIC_ERR_RUNTIME;
+        if (magic::fill_rows(a.d_y, 0u, a.N, C + 2 * H, a.ld_dy, stream) != MAGIC_OK) return MAGIC_ERR_RUNTIME;
         int st0 = launch_table<H, LPH>(a, stream);
         return st0 != MAGIC_OK ? st0 : launch_status();
     }

@@ -482,10 +482,7 @@ int magic_proj_bwd_weight(int64_t n_rows, int32_t m, int32_t f, const float *dy,
     if (n_rows < 0 || m <= 0 || f <= 0) return MAGIC_ERR_INVALID_ARG;
     if (!dw) return MAGIC_ERR_INVALID_ARG;
     hipStream_t stream = (hipStream_t)stream_;
-    if (n_rows == 0) {
-        if (hipMemsetAsync(dw, 0, sizeof(float) * (size_t)m * f, stream) != hipSuccess) return MAGIC_ERR_RUNTIME;
-        return MAGIC_OK;
-    }
+    if (n_rows == 0) return magic::fill_words(dw, 0u, (int64_t)m * f, stream);
     if (!dy || !x || ld_dy < m || ld_x < f) return MAGIC_ERR_INVALID_ARG;
     magic::Arena ar(workspace, workspace_bytes);
     DwArgs a;

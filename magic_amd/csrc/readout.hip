@@ -100,9 +100,7 @@ int magic_readout(int64_t n_rows, int32_t width, const float *feat, int64_t ld_f
         // no rows: the mean over all nodes is NaN as torch's mean of an empty tensor is (utils/poolers.py:58),
         // the sum is 0; per-type read-outs start from zeros (utils/poolers.py:62) and stay zeros
         const bool nan = n_types == 0 && mean;
-        if (hipMemsetD32Async((hipDeviceptr_t)out, nan ? 0x7fc00000 : 0, (size_t)T * width, stream) != hipSuccess)
-            return MAGIC_ERR_RUNTIME;
-        return MAGIC_OK;
+        return magic::fill_words(out, nan ? 0x7fc00000u : 0u, (int64_t)T * width, stream);
     }
     ReadoutArgs a;
     a.n = n_rows;

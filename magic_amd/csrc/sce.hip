@@ -205,7 +205,7 @@ int magic_sce_fwd_bwd(int64_t n_rows, int32_t n_dim, int64_t n_mask, const int64
     a.ws_loss = ar.take<float>(a.grid);
     a.ws_dt = ar.take<float>((size_t)a.grid * n_dim);
     if (!ar.ok() || !a.ws_loss || !a.ws_dt) return MAGIC_ERR_WORKSPACE;
-    if (hipMemsetAsync(d_x, 0, sizeof(float) * (size_t)n_rows * ld_x, stream) != hipSuccess) return MAGIC_ERR_RUNTIME;
+    if (magic::fill_words(d_x, 0u, n_rows * ld_x, stream) != MAGIC_OK) return MAGIC_ERR_RUNTIME;
     if (n_dim <= 8) {
         MAGIC_LAUNCH("sce_fwd_bwd", k_sce<8>, a.grid, 256, 0, stream, a);
     } else if (n_dim <= 16) {
@@ -244,7 +244,7 @@ int magic_sce_fwd_bwd_static(int64_t n_rows, int32_t n_dim, int64_t n_mask, cons
     if (sp != MAGIC_OK) return sp;
     a.ws_loss = base;                 // [grid]          every entry is rewritten by its block below:
     a.ws_dt = base + kStaticGrid;     // [grid, n_dim]   nothing has to start at zero
-    if (hipMemsetAsync(d_x, 0, sizeof(float) * (size_t)n_rows * ld_x, stream) != hipSuccess) return MAGIC_ERR_RUNTIME;
+    if (magic::fill_words(d_x, 0u, n_rows * ld_x, stream) != MAGIC_OK) return MAGIC_ERR_RUNTIME;
     // plain launches: the timing brackets of MAGIC_LAUNCH create events
     if (n_dim <= 8)
         hipLaunchKernelGGL(k_sce<8>, dim3(a.grid), dim3(256), 0, stream, a);
