@@ -19,7 +19,7 @@ static int failures = 0;
     } while (0)
 
 int main() {
-    if (magic_abi_version() < 3) return 2;
+    if (magic_abi_version() < 5) return 2;
     for (int s = 0; s >= -7; --s) (void)std::strlen(magic_status_string(s));
     // profiler tables
     EXPECT(magic_prof_enable(0), MAGIC_OK);
@@ -147,6 +147,7 @@ int main() {
     EXPECT(magic_knn_merge(4, 0, 2, nullptr, nullptr, nullptr, nullptr, nullptr), MAGIC_ERR_INVALID_ARG);
     // segment attention: every field that would be read out of bounds, or by no kernel, is refused before a launch
     const int32_t tab[8] = {0, 4, 0, 4, 0, 0, 4, 0};
+    double *lse = reinterpret_cast<double *>(dummy);
     magic_attn at;
     std::memset(&at, 0, sizeof at);
     at.q_heads = 4, at.kv_heads = 2, at.head_dim = 16, at.n_q = at.n_k = 4;
@@ -157,13 +158,13 @@ int main() {
     (void)magic_attn_fwd_workspace_bytes(&at);
     (void)magic_attn_bwd_workspace_bytes(&at);
     (void)magic_attn_fwd_workspace_bytes(nullptr);
-    EXPECT(magic_attn_fwd(nullptr, dummy, 64, 16, dummy, nullptr, 0, nullptr), MAGIC_ERR_INVALID_ARG);
-    EXPECT(magic_attn_fwd(&at, nullptr, 64, 16, dummy, nullptr, 0, nullptr), MAGIC_ERR_INVALID_ARG);
-    EXPECT(magic_attn_fwd(&at, dummy, 63, 16, dummy, nullptr, 0, nullptr), MAGIC_ERR_INVALID_ARG);
+    EXPECT(magic_attn_fwd(nullptr, dummy, 64, 16, lse, nullptr, 0, nullptr), MAGIC_ERR_INVALID_ARG);
+    EXPECT(magic_attn_fwd(&at, nullptr, 64, 16, lse, nullptr, 0, nullptr), MAGIC_ERR_INVALID_ARG);
+    EXPECT(magic_attn_fwd(&at, dummy, 63, 16, lse, nullptr, 0, nullptr), MAGIC_ERR_INVALID_ARG);
     auto attn = [&](auto change) {
         magic_attn b = at;
         change(b);
-        return magic_attn_fwd(&b, dummy, 64, 16, dummy, nullptr, 0, nullptr);
+        return magic_attn_fwd(&b, dummy, 64, 16, lse, nullptr, 0, nullptr);
     };
     EXPECT(attn([](magic_attn &b) { b.dtype = 7; }), MAGIC_ERR_UNSUPPORTED);
     EXPECT(attn([](magic_attn &b) { b.kv_heads = 3; }), MAGIC_ERR_INVALID_ARG);
@@ -183,11 +184,11 @@ int main() {
     EXPECT(attn([](magic_attn &b) { b.cap = 1e-9f; }), MAGIC_ERR_INVALID_ARG);
     EXPECT(attn([](magic_attn &b) { b.scale = INFINITY; }), MAGIC_ERR_INVALID_ARG);
     EXPECT(attn([&](magic_attn &b) { b.slopes = dummy; }), MAGIC_ERR_INVALID_ARG);  // no positions
-    EXPECT(magic_attn_bwd(&at, dummy, 64, 16, dummy, dummy, 64, 16, dummy, dummy, nullptr, nullptr, nullptr, 0, nullptr),
+    EXPECT(magic_attn_bwd(&at, dummy, 64, 16, lse, dummy, 64, 16, dummy, dummy, nullptr, nullptr, nullptr, 0, nullptr),
            MAGIC_ERR_INVALID_ARG);  // dk without dv
-    EXPECT(magic_attn_bwd(&at, dummy, 64, 16, dummy, dummy, 64, 16, dummy, dummy, dummy, dummy, nullptr, 0, nullptr),
+    EXPECT(magic_attn_bwd(&at, dummy, 64, 16, lse, dummy, 64, 16, dummy, dummy, dummy, dummy, nullptr, 0, nullptr),
            MAGIC_ERR_INVALID_ARG);  // a slope gradient without slopes
-    EXPECT(magic_attn_bwd(&at, dummy, 64, 16, dummy, dummy, 64, 16, dummy, dummy, dummy, nullptr, nullptr, 0, nullptr),
+    EXPECT(magic_attn_bwd(&at, dummy, 64, 16, lse, dummy, 64, 16, dummy, dummy, dummy, nullptr, nullptr, 0, nullptr),
            MAGIC_ERR_WORKSPACE);
     // head norm + rotation, 8-bit checkpoints
     EXPECT(magic_head_norm_rope_fwd(4, 4, 2, 16, 18, MAGIC_F32, dummy, 64, 16, dummy, 32, 16, dummy, dummy, (const int32_t *)dummy,
