@@ -42,6 +42,9 @@ typedef enum magic_status {
 int magic_abi_version(void);
 /* Static, human readable text for a status code. */
 const char *magic_status_string(int status);
+/* Memory-set nodes of a captured, not instantiated hipGraph_t: replays after the first have left old contents where such
+ * nodes should have cleared memory.  The library records none; a caller's other calls may. */
+int magic_graph_memset_nodes(void *graph, int64_t *count /* host */);
 
 /* ------------------------------------------------------------------------------------
  * Per-kernel timing (HIP events on the launch stream).  While enabled, every kernel the

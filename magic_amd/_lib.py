@@ -47,6 +47,7 @@ class MagicAttn(C.Structure):
 SYMBOLS = {
     "magic_abi_version": (c_i32, []),
     "magic_status_string": (C.c_char_p, [c_i32]),
+    "magic_graph_memset_nodes": (c_i32, [c_vp, C.POINTER(c_i64)]),
     "magic_prof_enable": (c_i32, [c_i32]),
     "magic_prof_reset": (c_i32, []),
     "magic_prof_read": (c_i32, [c_i32, C.c_char_p, C.POINTER(c_i64), C.POINTER(C.c_double)]),
@@ -180,6 +181,13 @@ def _stream() -> int:
     if _raw_stream is not None and _raw_device is not None:
         return _raw_stream(_raw_device())
     return torch.cuda.current_stream().cuda_stream
+
+
+def graph_memset_nodes(graph) -> int:
+    """Memory-set nodes of a ``torch.cuda.CUDAGraph(keep_graph=True)``."""
+    n = c_i64(0)
+    _check(load().magic_graph_memset_nodes(graph.raw_cuda_graph(), C.byref(n)), "magic_graph_memset_nodes")
+    return n.value
 
 
 def stream_on(device) -> int:

@@ -1,5 +1,6 @@
 // Constant fills as kernels.  A memset recorded into a HIP graph is a node of its own kind, and such nodes have left old
 // contents standing in replays after the first; a kernel is replayed like any other.
+#include <vector>
 #include "common.h"
 
 namespace {
@@ -39,3 +40,23 @@ int fill_rows(void *p, uint32_t v, int64_t rows, int64_t cols, int64_t ld, hipSt
 }
 
 }  // namespace magic
+
+extern "C" int magic_graph_memset_nodes(void *graph, int64_t *count) {
+    if (!graph || !count) return MAGIC_ERR_INVALID_ARG;
+    size_t n = 0;
+    if (hipGraphGetNodes((hipGraph_t)graph, nullptr, &n) != hipSuccess) return MAGIC_ERR_RUNTIME;
+    std::vector<hipGraphNode_t> nodes;
+    try {
+        nodes.resize(n);
+    } catch (...) {
+        return MAGIC_ERR_RUNTIME;
+    }
+    if (n > 0 && hipGraphGetNodes((hipGraph_t)graph, nodes.data(), &n) != hipSuccess) return MAGIC_ERR_RUNTIME;
+    *count = 0;
+    for (size_t i = 0; i < n; ++i) {
+        hipGraphNodeType t;
+        if (hipGraphNodeGetType(nodes[i], &t) != hipSuccess) return MAGIC_ERR_RUNTIME;
+        *count += t == hipGraphNodeTypeMemset;
+    }
+    return MAGIC_OK;
+}

@@ -129,6 +129,39 @@ class _EdgeHeadLossFn(torch.autograd.Function):
             d_b2.view(ctx.b2_shape), None, None, None
 
 
+class _TokenRowsFn(torch.autograd.Function):
+    """``x`` whose rows ``idx`` hold the mask token already: hands the token the sum of their gradients.  (The library's
+    kernels, as in ``_PickRowsFn``: torch's sums and sorted scatters over many blocks clear memory in a way that goes wrong
+    in replays of a recorded step.)"""
+
+    @staticmethod
+    def forward(ctx, x, token, idx):
+        ctx.save_for_backward(idx)
+        return x.view_as(x)
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dx):
+        idx, = ctx.saved_tensors
+        return None, _lib.readout(dx.index_select(0, idx), None, 0, False), None
+
+
+class _PickRowsFn(torch.autograd.Function):
+    """``x[idx]``; the gradients of a row that is picked more than once are added in a fixed order."""
+
+    @staticmethod
+    def forward(ctx, x, idx):
+        ctx.save_for_backward(idx)
+        ctx.shape = x.shape
+        return x.index_select(0, idx)
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dy):
+        idx, = ctx.saved_tensors
+        return _lib.rows_scatter_add(dy.new_zeros(ctx.shape), idx, dy), None
+
+
 class GMAEModel(nn.Module):
     """``model/autoencoder.py:55-305``.
 
@@ -240,6 +273,15 @@ class GMAEModel(nn.Module):
         # no device synchronisation); the masks themselves are drawn on the GPU
         seeds = torch.randint(0, 2 ** 62, (len(widths),)).tolist()
         return [_lib.dropout_mask((n, w), 1.0 - p, s, device) for w, s in zip(widths, seeds)], 1.0 / (1.0 - p)
+
+    @staticmethod
+    def _layer_drops(layers, n, device, drop_seeds):
+        """(keep mask, scale) of every layer from its word of ``drop_seeds``, as ``_dropout_masks`` draws them; None where
+        dropout is inactive."""
+        assert drop_seeds.numel() >= len(layers) and drop_seeds.dtype == torch.int64
+        return [(_lib.dropout_mask_dev((n, layer.src_feat), 1.0 - layer.feat_drop.p, drop_seeds[i:i + 1], device),
+                 1.0 / (1.0 - layer.feat_drop.p)) if layer.feat_drop.training and 0.0 < layer.feat_drop.p < 1.0 else None
+                for i, layer in enumerate(layers)]
 
     def _fused_cfg(self, g: Graph, drop_masks, drop_seeds=None):
         """Description of the whole encoder -> decoder chain for ``FusedGMAEFn``, or None when a
@@ -367,17 +409,19 @@ class GMAEModel(nn.Module):
         else:
             if drop_masks is not None:
                 raise NotImplementedError("injected dropout masks need the fused chain")
-            if drop_seeds is not None and pre_use_x.is_cuda and torch.cuda.is_current_stream_capturing():
-                raise NotImplementedError("a recorded step draws its dropout masks in the fused chain only")
-            enc_rep, all_hidden = self.encoder(use_g, pre_use_x, return_hidden=True)
+            drops, n_enc = None, len(self.encoder.gats)
+            if drop_seeds is not None:
+                drops = self._layer_drops([*self.encoder.gats, *self.decoder.gats], g.num_nodes(), g.device, drop_seeds)
+            x = pre_use_x if feat_has_grad else _TokenRowsFn.apply(pre_use_x.detach(), self.enc_mask_token, mask_nodes)
+            enc_rep, all_hidden = self.encoder(use_g, x, return_hidden=True, drops=drops and drops[:n_enc])
             if self.global_attn is not None:
                 seen = torch.ones(g.num_nodes(), dtype=torch.bool, device=g.device)
                 seen.index_fill_(0, mask_nodes, False)
                 all_hidden[-1] = self.global_attn(use_g, all_hidden[-1], key_mask=seen)
             enc_rep = torch.cat(all_hidden, dim=1)
             rep = linear_nobias(enc_rep, self.encoder_to_decoder.weight, self.act_bits)   # autoencoder.py:237
-            recon = recon_p = self.decoder(pre_use_g, rep)
-            samples = enc_rep[sample_idx]
+            recon = recon_p = self.decoder(pre_use_g, rep, drops=drops and drops[n_enc:])
+            samples = _PickRowsFn.apply(enc_rep, sample_idx)
         # autoencoder.py:242-245: gather of the masked rows fused into the loss kernel
         x_target = g.ndata["attr"]
         # (the loss kernel takes the head-padded reconstruction as it is and leaves zeros in the

@@ -346,7 +346,8 @@ class GATConv(nn.Module):
                                       self.activation.weight, False)
         return out
 
-    def forward(self, graph: Graph, feat, get_attention=False):
+    def forward(self, graph: Graph, feat, get_attention=False, drop=None):
+        """``drop``: (uint8 keep mask, scale) to take in the place of ``feat_drop``'s own draw."""
         if isinstance(feat, tuple):
             raise NotImplementedError("bipartite (src, dst) inputs are not used by MAGIC and have no HIP kernel")
         if feat.device.type != "cuda":
@@ -358,7 +359,7 @@ class GATConv(nn.Module):
         Dp = _pad_head_dim(D)
         C = H * Dp
         struct = graph.structure.ensure_csr()
-        h = self.feat_drop(feat)                                       # gat.py:283
+        h = self.feat_drop(feat) if drop is None else feat * (drop[0].to(feat.dtype) * drop[1])     # gat.py:283
         res_identity = isinstance(self.res_fc, nn.Identity)
         if res_identity and Dp != D:
             raise _lib.MagicHipError("identity residual with a padded head width is not supported")
@@ -427,16 +428,17 @@ class GAT(nn.Module):
                                      concat_out=self.concat_out))
         self.head = nn.Identity()
 
-    def forward(self, g, input_feature, return_hidden=False, node_types=None):
+    def forward(self, g, input_feature, return_hidden=False, node_types=None, drops=None):
         """``node_types``: the caller's word that ``input_feature`` is ``one_hot(node_types)``; the first layer then
-        reads the types instead of the matrix where it can (inference)."""
+        reads the types instead of the matrix where it can (inference).  ``drops``: ``GATConv.forward``'s ``drop`` of every
+        layer."""
         h = input_feature
         hidden_list = []
         for layer in range(self.n_layers):
             if layer == 0 and node_types is not None and self.n_layers > 1 and self.gats[0].onehot_input_ok(g):
                 h = self.gats[0].forward_onehot(g, node_types)
             else:
-                h = self.gats[layer](g, h)
+                h = self.gats[layer](g, h, drop=drops[layer] if drops is not None else None)
             hidden_list.append(h)
         if return_hidden:
             return self.head(h), hidden_list

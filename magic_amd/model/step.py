@@ -72,7 +72,10 @@ class CapturedTrainStep:
     the device-side kernel boundary, which a replay does not remove), so recording is an option for
     callers whose host thread is busy elsewhere, not the default.  With ``capture=True`` the
     ``optimizer`` must be capturable (:func:`make_adam`) and every step of the model runs on one side
-    stream, eager warm-up calls included."""
+    stream, eager warm-up calls included.  Models outside the fused chain (the global-attention block, other activations)
+    record their layer-by-layer steps, dropout masks from the seeds like the others'; a model whose torch operations would
+    record memory-set nodes (a PReLU behind a normalisation layer) is refused when its step is recorded: replays would give
+    wrong gradients."""
 
     def __init__(self, model, optimizer, g, n_dim: int, loss_scale: float = 1.0, grad_exchange=None,
                  warmup: int = 2, capture: bool = False, capture_optimizer: bool = True):
@@ -86,10 +89,12 @@ class CapturedTrainStep:
             raise ValueError("Sample larger than population or is negative")   # random.sample's own error
         self.ntype = g.ndata["type"].view(-1).long()
         g.structure.ensure_csr()
+        if getattr(model, "global_attn", None) is not None:
+            g.component_attention()              # (its tables cannot be made while a step is recorded)
         # static inputs of the recorded step
         self.perm = torch.zeros(n, dtype=torch.int64, device=dev)
         self.pos = torch.zeros(self.thr, dtype=torch.int64, device=dev)
-        self.n_masks = len(model.encoder.gats) + 1
+        self.n_masks = len(model.encoder.gats) + len(model.decoder.gats)
         self.seeds = torch.zeros(self.n_masks, dtype=torch.int64, device=dev)
         from .autoencoder import negative_candidate_count
         self.n_neg = negative_candidate_count(self.thr)
@@ -141,14 +146,14 @@ class CapturedTrainStep:
             p_.grad = None
         torch.cuda.synchronize()
         if self.exchange is None:
-            gr = torch.cuda.CUDAGraph()
+            gr = torch.cuda.CUDAGraph(keep_graph=True)
             with torch.cuda.graph(gr, pool=_shared_pool(self.model), stream=_shared_stream(self.model), **_CAPTURE):
                 self._forward_backward()
                 if self._capture_opt:
                     self.opt.step()
             graphs = [gr]
         else:
-            ga, gb = torch.cuda.CUDAGraph(), torch.cuda.CUDAGraph()
+            ga, gb = (torch.cuda.CUDAGraph(keep_graph=True) for _ in range(2))
             with torch.cuda.graph(ga, pool=_shared_pool(self.model), stream=_shared_stream(self.model), **_CAPTURE):
                 self._forward_backward()
             with torch.cuda.graph(gb, pool=_shared_pool(self.model), stream=_shared_stream(self.model), **_CAPTURE):
@@ -156,6 +161,12 @@ class CapturedTrainStep:
             graphs = [ga, gb]
         if {k: v.data_ptr() for k, v in _lib._ws_cache.items()} != ws_before:
             raise _lib.MagicHipError("a kernel workspace grew while the step was being recorded")
+        n_memset = sum(map(_lib.graph_memset_nodes, graphs))
+        if n_memset:
+            for p_ in self.model.parameters():           # (they lie in the recording's pool)
+                p_.grad = None
+            raise _lib.MagicHipError(f"the step records {n_memset} memory-set nodes of torch's (a PReLU behind a "
+                                     "normalisation layer does): its replays would give wrong gradients")
         # the recorded launches hold raw pointers into the kernel workspaces: keep those buffers alive
         # even if a later, larger call makes the library replace them
         self._keep = list(_lib._ws_cache.values())

@@ -63,7 +63,7 @@ def test_recorded_training_step_holds_no_memset(cuda, monkeypatch):
     from magic_amd.model.autoencoder import GMAEModel
     from magic_amd.model.step import CapturedTrainStep, make_adam
     whole = torch.cuda.CUDAGraph
-    monkeypatch.setattr(torch.cuda, "CUDAGraph", lambda: whole(keep_graph=True))
+    monkeypatch.setattr(torch.cuda, "CUDAGraph", lambda **kw: whole(keep_graph=True))
     model = GMAEModel(5, 7, 64, 3, 4, "prelu", 0.1, 0.2, True, "BatchNorm", 0.5, "sce", 3).to(cuda)
     src, dst, nt, et = small_graph(9000, 40000, 5, 7, seed=91, hub_deg=300, hub_out=150)
     step = CapturedTrainStep(model, make_adam(model, 1e-3, 5e-4), to_graph(src, dst, 9000, nt, et, 5, 7, cuda), 5, capture=True)

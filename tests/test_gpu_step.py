@@ -266,3 +266,85 @@ def test_fused_adam_equals_torch_adam(cuda):
     cpu_p.grad = torch.ones(3)
     with pytest.raises(Exception, match="GPU"):
         FusedAdam([cpu_p], lr=1e-3).step()
+
+
+@pytest.mark.parametrize("kind,drop", [("attention", 0.1), ("attention", 0.0), ("attention_8_bits", 0.1), ("relu", 0.1), ("relu", 0.0)])
+def test_recorded_step_of_the_layer_by_layer_path(cuda, kind, drop):
+    """Models outside the fused chain (the global-attention block, an activation other than PReLU) record and replay their
+    steps too: losses and parameters equal those of eager steps with the same permutation, samples and dropout seeds."""
+    from magic_amd.model.autoencoder import GMAEModel
+    from magic_amd.model.step import CapturedTrainStep, make_adam
+    torch.manual_seed(7)
+    a = GMAEModel(N_DIM, E_DIM, HIDDEN, LAYERS, 4, "relu" if kind == "relu" else "prelu", drop, 0.2, True, "BatchNorm", 0.5, "sce", 3,
+                  global_attention=kind != "relu", act_bits=8 if kind == "attention_8_bits" else 32).to(cuda)
+    if a.global_attn is not None:
+        with torch.no_grad():
+            a.global_attn.out.weight.normal_(std=0.1)
+    b = copy.deepcopy(a)
+    n, e = 900, 4000
+    src, dst, nt, et = small_graph(n, e, N_DIM, E_DIM, seed=91, hub_deg=300, hub_out=150)
+    sa, sb = (CapturedTrainStep(m, make_adam(m, 1e-3, 5e-4), to_graph(src, dst, n, nt, et, N_DIM, E_DIM, cuda), N_DIM,
+                                capture=capture, warmup=2) for m, capture in ((a, False), (b, True)))
+    gen = torch.Generator().manual_seed(8)
+    losses = []
+    for step in range(7):
+        kw = dict(perm=torch.randperm(n, generator=gen), pos_idx=torch.randperm(src.size, generator=gen)[:n],
+                  seeds=torch.randint(0, 2 ** 62, (LAYERS + 1,), generator=gen),
+                  neg_pairs=(torch.randint(0, n, (n,), generator=gen), torch.randint(0, n, (n,), generator=gen)))
+        la, lb = sa(**kw).clone(), sb(**kw).clone()
+        torch.cuda.synchronize()
+        assert torch.equal(la, lb), step
+        for (k, pa), (_, pb) in zip(a.named_parameters(), b.named_parameters()):
+            assert torch.equal(pa, pb), (step, k)
+        losses.append(float(la))
+    assert sb._graphs is not None and len(set(losses)) == len(losses)
+
+
+def test_entity_level_loop_records_models_with_the_block(cuda):
+    from magic_amd.model.autoencoder import GMAEModel
+    from magic_amd.model.step import make_adam
+    from magic_amd.model.train import entity_level_train
+    torch.manual_seed(3)
+    model = GMAEModel(N_DIM, E_DIM, HIDDEN, LAYERS, 4, "prelu", 0.1, 0.2, True, "BatchNorm", 0.5, "sce", 3, global_attention=True).to(cuda)
+    src, dst, nt, et = small_graph(600, 3000, N_DIM, E_DIM, seed=80, hub_deg=100)
+    g = to_graph(src, dst, 600, nt, et, N_DIM, E_DIM, cuda)
+    before = model.global_attn.out.weight.detach().clone()
+    entity_level_train(model, lambda i: g, 1, make_adam(model, 5e-3, 5e-4), 5, cuda, N_DIM, E_DIM, progress=False, capture=True)
+    assert not torch.equal(before, model.global_attn.out.weight)
+    assert all(bool(torch.isfinite(p).all()) for p in model.parameters())
+
+
+def test_dropout_seeds_draw_the_same_masks_in_both_paths(cuda):
+    """The loss of the fused chain and of the layer-by-layer path under the same seeds, up to the order of their sums; other
+    seeds give another loss."""
+    _, model = _twins(cuda, seed=9)
+    model.train()
+    n, e = 700, 3000
+    src, dst, nt, et = small_graph(n, e, N_DIM, E_DIM, seed=17, hub_deg=100)
+    inj = _inject(n, src.size, HIDDEN, LAYERS, N_DIM, 4)
+    inj.pop("drop_masks")
+    inj["perm"] = inj["perm"].to(cuda)
+    seeds = torch.randint(0, 2 ** 62, (2, LAYERS + 1), generator=torch.Generator().manual_seed(2)).to(cuda)
+    loss = {(i, fused): float(model.compute_loss(to_graph(src, dst, n, nt, et, N_DIM, E_DIM, cuda), drop_seeds=seeds[i], fused=fused, **inj))
+            for i in range(2) for fused in (True, False)}
+    for i in range(2):
+        assert abs(loss[i, True] - loss[i, False]) < 1e-5 * abs(loss[i, True])
+    assert abs(loss[0, True] - loss[1, True]) > 1e-4 * abs(loss[0, True])
+
+
+def test_steps_whose_replays_would_go_wrong_are_refused(cuda):
+    """torch's PReLU (behind a normalisation layer, which no fused kernel serves) clears memory by a memory-set node."""
+    from magic_amd import _lib
+    from magic_amd.model.autoencoder import GMAEModel
+    from magic_amd.model.step import CapturedTrainStep, make_adam
+    torch.manual_seed(1)
+    model = GMAEModel(N_DIM, E_DIM, HIDDEN, LAYERS, 4, "prelu", 0.1, 0.2, True, "layernorm", 0.5, "sce", 3).to(cuda)
+    src, dst, nt, et = small_graph(9000, 40000, N_DIM, E_DIM, seed=91)
+    step = CapturedTrainStep(model, make_adam(model, 1e-3, 5e-4), to_graph(src, dst, 9000, nt, et, N_DIM, E_DIM, cuda), N_DIM,
+                             capture=True, warmup=2)
+    assert all(torch.isfinite(step()) for _ in range(2))
+    before = {k: v.clone() for k, v in model.state_dict().items()}
+    with pytest.raises(_lib.MagicHipError, match="memory-set"):
+        step()
+    torch.cuda.synchronize()
+    assert all(torch.equal(v, before[k]) for k, v in model.state_dict().items())

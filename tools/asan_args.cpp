@@ -21,6 +21,8 @@ static int failures = 0;
 int main() {
     if (magic_abi_version() < 5) return 2;
     for (int s = 0; s >= -7; --s) (void)std::strlen(magic_status_string(s));
+    int64_t memsets = 0;
+    EXPECT(magic_graph_memset_nodes(nullptr, &memsets), MAGIC_ERR_INVALID_ARG);
     // profiler tables
     EXPECT(magic_prof_enable(0), MAGIC_OK);
     EXPECT(magic_prof_reset(), MAGIC_OK);
