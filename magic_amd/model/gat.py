@@ -226,6 +226,7 @@ class _LinearAct8Fn(torch.autograd.Function):
         return y
 
     @staticmethod
+    @torch.autograd.function.once_differentiable
     def backward(ctx, dy):
         codes, exps, w = ctx.saved_tensors
         dy = _lib.full_rows(dy)

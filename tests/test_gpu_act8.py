@@ -200,3 +200,15 @@ def test_every_width_up_to_two_blocks(cuda):
         codes, exps = definition(x)
         assert np.array_equal(a.codes.cpu().numpy(), codes) and np.array_equal(a.exps.cpu().numpy(), exps), f
         assert np.array_equal(act8_unpack(a).cpu().double().numpy(), codes[:, :f] * 2.0 ** (np.repeat(exps, 32, 1)[:, :f] - 127.0)), f
+
+
+def test_second_derivative_is_refused(cuda):
+    """The backward pass forms plain values: a derivative of them raises instead of coming out as a constant's."""
+    from magic_amd.model.gat import linear_nobias
+    x = torch.randn(20, 32, device=cuda, requires_grad=True)
+    w = torch.randn(4, 32, device=cuda, requires_grad=True)
+    dy = torch.randn(20, 4, device=cuda, requires_grad=True)
+    dx, dw = torch.autograd.grad(linear_nobias(x, w, act_bits=8), (x, w), dy, create_graph=True)
+    for g in (dx, dw):
+        with pytest.raises(RuntimeError, match="once_differentiable"):
+            torch.autograd.grad(g.sum(), (x, w, dy), allow_unused=True, retain_graph=True)
