@@ -209,6 +209,6 @@ def test_second_derivative_is_refused(cuda):
     w = torch.randn(4, 32, device=cuda, requires_grad=True)
     dy = torch.randn(20, 4, device=cuda, requires_grad=True)
     dx, dw = torch.autograd.grad(linear_nobias(x, w, act_bits=8), (x, w), dy, create_graph=True)
-    for g in (dx, dw):
+    for g in (dx, dw):                                    # (beside a term that has a derivative)
         with pytest.raises(RuntimeError, match="once_differentiable"):
-            torch.autograd.grad(g.sum(), (x, w, dy), allow_unused=True, retain_graph=True)
+            (g.sum() + x.sum() + w.sum()).backward(retain_graph=True)
