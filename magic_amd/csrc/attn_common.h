@@ -1,7 +1,8 @@
 // Building blocks of the segment-attention kernels (attn_fwd.hip, attn_bwd.hip).
 //
-// All products run on v_mfma_f32_32x32x16_bf16.  float32 operands are split into three bf16 planes and take the six
-// leading cross products (bf16_split.h: fp32-grade); bfloat16 operands are one plane and one product.
+// All products run on v_mfma_f32_32x32x16_bf16 and _f16.  float32 operands are split into three bf16 planes and take the six
+// leading cross products (bf16_split.h: fp32-grade) or, scaled, into two fp16 planes and three products (F16x2 below);
+// bfloat16 operands are one plane and one product.
 // Lane l of a wavefront, li = l & 31, hf = l >> 5:
 //   A [32 x 16]: row li, columns 8 hf .. + 7        B [16 x 32]: rows 8 hf .. + 7, column li
 //   C [32 x 32]: column li, rows 8 (r / 4) + 4 hf + (r & 3), r = 0 .. 15
@@ -330,12 +331,12 @@ template <typename M, int DP, int ROWS, int NT> struct Stage {
 // Logits are formed times log2 e (scale, cap and slopes carry it): a probability is 2^(x - m) with m the row's largest x
 // itself, so that x - m is exact where it matters, whatever the logits' size.
 // Capped scores of a tile: x[i] = log2 e cap tanh(x[i] f).  Below TANH_SMALL tanh(t) / t is a polynomial in t^2 (equal ripples on
-// that range): 3.5e-8 off with four terms, half a rounding of float32.  (Three terms, 2.9e-6 off, show in the slopes'
+// that range, the first one 1): 4.2e-8 off with four terms, less than a rounding of float32.  (Three terms, 2.9e-6 off, show in the slopes'
 // gradients of bfloat16 calls, which are float32.)  Elsewhere tanh is (1 - e) / (1 + e).  A cap is far above most scores:
 // the polynomial serves alone where no score of the wavefront leaves its range.  RAW (bfloat16) has f and cap in its coefficients and starts from
 // the scores themselves, up to RAW_MAX (their powers stay in range; the scaled modes' scores are far larger).
 constexpr float TANH_SMALL = 0.35f, RAW_MAX = 1e5f;
-constexpr float K0 = 0.99999994f, K1 = -0.333324224f, K2 = 0.132957995f, K3 = -0.0489582308f;
+constexpr float K0 = 1.f, K1 = -0.333326638f, K2 = 0.132998258f, K3 = -0.0491485037f;
 template <bool RAW> struct Cap {
     float f, cap, lim, c0, c1, c2, c3;
     __device__ __forceinline__ Cap(float f, float cap_e) : f(f), cap(cap_e * LOG2E) {
