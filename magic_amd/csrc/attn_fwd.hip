@@ -540,7 +540,10 @@ __global__ __launch_bounds__(64 * WM *KG, DP == 128 && (M::N > 1 || WM == 1) ? 1
                 for (int r = 0; r < 16; ++r) o[d][r] *= al;
         }
         float tsum = 0.f;
-        vec pf[KB * 2][NP];
+        // What rounding takes from bfloat16 probabilities goes through a second product where that is the smaller part of the
+        // work: heads up to 32 wide, and blocks of 32 columns, which wait for their keys more than they compute.
+        constexpr bool LOW = M::N == 1 && (DP <= 32 || KG > 1);
+        vec pf[KB * 2][NP], pl[LOW ? KB * 2 : 1][NP];
 #pragma unroll
         for (int b = 0; b < KB; ++b)
 #pragma unroll
@@ -552,6 +555,11 @@ __global__ __launch_bounds__(64 * WM *KG, DP == 128 && (M::N > 1 || WM == 1) ? 1
                     tsum += x[e];
                 }
                 to_planes(x, pf[2 * b + u]);
+                if constexpr (LOW) {
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) x[e] -= (float)pf[2 * b + u][0][e];
+                    to_planes(x, pl[2 * b + u]);
+                }
             }
         l = fmaf(l, al, tsum);
 #pragma unroll
@@ -565,9 +573,10 @@ __global__ __launch_bounds__(64 * WM *KG, DP == 128 && (M::N > 1 || WM == 1) ? 1
             for (int w = 0; w < KB * 2; ++w) {
                 vec f[NP];
                 tile::frag_t(sV, turned, 16 * w, d, f);
+                if constexpr (LOW) mma(c, f, pl[w]);
                 mma(c, f, pf[w]);
             }
-            feed<2 * NP, PRODUCTS<M>, KB * 2>();
+            feed<2 * NP, (LOW ? 2 : 1) * PRODUCTS<M>, KB * 2>();
             if (TILE_SUM) {
 #pragma unroll
                 for (int r = 0; r < 16; ++r) o[d][r] = fmaf(o[d][r], al, c[r]);

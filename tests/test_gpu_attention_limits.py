@@ -182,3 +182,21 @@ def test_single_rows_and_heads_of_any_stride(cuda, shape, strides, dtype):
     for got, x in zip(head_norm_rope(rows[0], rows[1], w, w, pos), plain):
         want, tol = rope_reference(x, w, pos, D, 1e-6, 10000.0, torch.zeros_like(x))[0]
         assert ((got.double() - want).abs() <= tol).all()
+
+
+@pytest.mark.parametrize("nq,nk,hq,hk,D", [(3, 5000, 16, 4, 128), (40, 900, 4, 2, 64), (500, 500, 8, 8, 16), (2000, 700, 4, 4, 32)])
+def test_bfloat16_outputs_where_low_parts_of_probabilities_are_taken(cuda, nq, nk, hq, hk, D):
+    """Few rows and narrow heads: what is left of a probability's rounding is the square of half a step, so that an output is
+    off by its own rounding and the float32 chain: where the sum nearly cancels, by next to nothing.  (Terms as in
+    test_gpu_attention.reference, whose bound holds a whole half step of the probabilities.)"""
+    q, k, v, d, _ = make(cuda, [nq], [nk], hq, hk, D, torch.bfloat16, seed=D)
+    got, r = run(q, k, v, d, [nq], [nk])["out"].double(), 2.0 ** -8
+    for h in range(hq):
+        Q, K, V = q[:, h].double(), k[:, h * hk // hq].double(), v[:, h * hk // hq].double()
+        s, w = Q @ K.T / math.sqrt(D), Q.abs() @ K.abs().T / math.sqrt(D)
+        delta = ((D + 8) * U * w).amax(1, keepdim=True) + 4 * U * s.abs().amax(1, keepdim=True)
+        p = torch.softmax(s, 1)
+        out, ep = p @ V, 2 * delta + (nk + 16) * U
+        tol = (ep + r * r + (nk + 16) * U) * (p @ V.abs()) + r * out.abs()
+        err = (got[:, h] - out).abs()
+        assert (err <= tol).all(), (h, float((err / tol).max()))
