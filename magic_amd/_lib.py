@@ -205,16 +205,22 @@ def _dev(t: Optional[torch.Tensor], dtype=None, name="tensor") -> Optional[int]:
     return t.data_ptr()
 
 
-_ws_cache: Dict[Tuple[int, int], torch.Tensor] = {}
+_ws_cache: Dict[Tuple[int, int, int], torch.Tensor] = {}
+_capturing = getattr(torch._C, "_cuda_isCurrentStreamCapturing", torch.cuda.is_current_stream_capturing)
 
 
 def workspace(nbytes: int, device, slot: int = 0) -> torch.Tensor:
-    """Grow-only scratch buffer per (device, slot); kernels on one stream run in order, so
-    consecutive calls can share it."""
+    """Grow-only scratch buffer per (device, current stream, slot); kernels on one stream run in order, so consecutive
+    calls can share it.  A call that is being recorded gets one of its own from the recording's pool: the graph holds its
+    address, and a later, larger call would replace a shared one."""
     device = torch.device(device)
     if device.type != "cuda":
         raise MagicHipError(f"operands must live on the GPU (got {device}); there is no CPU fallback")
-    key = (device.index if device.index is not None else torch.cuda.current_device(), slot)
+    if _capturing():
+        return torch.empty(max(int(nbytes), 1), dtype=torch.uint8, device=device)
+    if device.index is None:
+        device = torch.device("cuda", torch.cuda.current_device())
+    key = (device.index, stream_on(device), slot)
     buf = _ws_cache.get(key)
     if buf is None or buf.numel() < nbytes:
         buf = torch.empty(max(int(nbytes), 1 << 20), dtype=torch.uint8, device=device)
@@ -943,8 +949,8 @@ def knn_merge(part_dist: torch.Tensor, part_idx: torch.Tensor):
 
 
 # ------------------------------------------------------------------------------------- segment attention
-# These operators take their scratch from torch's allocator at every call (not from ``workspace``): calls on several
-# streams, and captured graphs, never share it.
+# These operators take their scratch from torch's allocator at every call (not from ``workspace``): it is as large as the
+# call needs and not kept.
 ATTN_MAX_DIM, ATTN_TILE, ATTN_MAX_LD = 128, 128, 1 << 22
 _ATTN_DTYPE = {torch.float32: 0, torch.bfloat16: 1}
 

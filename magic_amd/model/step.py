@@ -139,7 +139,6 @@ class CapturedTrainStep:
 
     def _record(self):
         """Record the step (recording launches nothing; the caller replays it afterwards)."""
-        ws_before = {k: v.data_ptr() for k, v in _lib._ws_cache.items()}
         # gradients left by an earlier step may live in another recorded step's memory pool: release
         # them here, not inside the recording
         for p_ in self.model.parameters():
@@ -159,17 +158,12 @@ class CapturedTrainStep:
             with torch.cuda.graph(gb, pool=_shared_pool(self.model), stream=_shared_stream(self.model), **_CAPTURE):
                 self.opt.step()
             graphs = [ga, gb]
-        if {k: v.data_ptr() for k, v in _lib._ws_cache.items()} != ws_before:
-            raise _lib.MagicHipError("a kernel workspace grew while the step was being recorded")
         n_memset = sum(map(_lib.graph_memset_nodes, graphs))
         if n_memset:
             for p_ in self.model.parameters():           # (they lie in the recording's pool)
                 p_.grad = None
             raise _lib.MagicHipError(f"the step records {n_memset} memory-set nodes of torch's (a PReLU behind a "
                                      "normalisation layer does): its replays would give wrong gradients")
-        # the recorded launches hold raw pointers into the kernel workspaces: keep those buffers alive
-        # even if a later, larger call makes the library replace them
-        self._keep = list(_lib._ws_cache.values())
         self._graphs = graphs
 
     # ------------------------------------------------------------------ per-step inputs

@@ -93,3 +93,54 @@ def test_fills_of_every_alignment(cuda, ld, off):
     keep = torch.ones(n, dtype=torch.bool, device=cuda)
     keep[mask] = False
     assert not rows[keep].any() and not rows[:, d:].any() and rows[mask].any()
+
+
+def _linear(n, f, m, bits, seed, cuda):
+    from magic_amd.model.gat import linear_nobias
+    gen = torch.Generator(device=cuda).manual_seed(seed)
+    x, w, dy = (torch.randn(*s, generator=gen, device=cuda) for s in ((n, f), (m, f), (n, m)))
+    x.requires_grad_(True), w.requires_grad_(True)
+
+    def call():
+        y = linear_nobias(x, w, act_bits=bits)
+        return [y.detach(), *torch.autograd.grad(y, (x, w), dy)]
+
+    return call
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_linear_layers_on_two_streams_share_no_scratch(cuda, bits):
+    calls = [_linear(60000, 256, 256, bits, 1, cuda), _linear(50000, 320, 130, bits, 2, cuda)]
+    alone = [c() for c in calls]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in calls]
+    for _ in range(3):
+        got = []
+        for s, call in zip(streams, calls):
+            with torch.cuda.stream(s):
+                got.append([call() for _ in range(4)])
+        torch.cuda.synchronize()
+        for many, want in zip(got, alone):
+            assert all(torch.equal(a, b) for res in many for a, b in zip(res, want))
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_a_graph_keeps_its_scratch_from_later_calls(cuda, bits):
+    """A larger call after the recording, and tensors that take what it gave back: neither reaches the replays, nor they them."""
+    call = _linear(3000, 256, 256, bits, 3, cuda)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        want = call()
+    torch.cuda.current_stream().wait_stream(side)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=side):
+        got = call()
+    for _ in range(3):
+        _linear(90000, 512, 300, bits, 4, cuda)()
+        other = [torch.full((1 << k,), float(k), device=cuda) for k in range(12, 25)]
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
+        assert all((t == float(k)).all() for k, t in zip(range(12, 25), other))
