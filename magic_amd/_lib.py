@@ -8,6 +8,7 @@ the GPU, the call raises.
 from __future__ import annotations
 
 import ctypes as C
+import functools
 import os
 from typing import Dict, Optional, Tuple
 
@@ -946,6 +947,18 @@ def knn_merge(part_dist: torch.Tensor, part_idx: torch.Tensor):
                                _dev(part_idx, torch.int64, "part_idx"), _dev(dist), _dev(idx), _stream()),
            "magic_knn_merge")
     return dist, idx
+
+
+def once_differentiable(fn):
+    """``torch.autograd.function.once_differentiable`` for a backward pass, without its cost of some microseconds a call where
+    no graph of the backward pass is recorded."""
+    once = torch.autograd.function.once_differentiable(fn)
+
+    @functools.wraps(fn)
+    def backward(ctx, *grads):
+        return (once if torch.is_grad_enabled() else fn)(ctx, *grads)
+
+    return backward
 
 
 # ------------------------------------------------------------------------------------- segment attention

@@ -81,13 +81,14 @@ def attention_plan(q_lens: Sequence[int], kv_lens: Optional[Sequence[int]] = Non
     device = torch.device(device)
     if device.type == "cuda" and device.index is None:
         device = torch.device("cuda", torch.cuda.current_device())
-    tabs = [torch.from_numpy(_tiles(a, b)) for a, b in ((q_lens, kv_lens), (kv_lens, q_lens))]
+    sides = ((q_lens, kv_lens), (kv_lens, q_lens))[:1 if kv_lens == q_lens else 2]      # (both sides' tables are one then)
+    tabs = [torch.from_numpy(_tiles(a, b)) for a, b in sides]
     if device.type == "cuda":
         if torch.cuda.is_current_stream_capturing():
             raise _lib.MagicHipError("build the plan before the capture: its tables would not outlive it")
         # (blocking copies: the kernels take the tables' entries as offsets, on whatever stream a call comes)
         tabs = [t.to(device) for t in tabs]
-    return AttentionPlan(q_lens, kv_lens, *tabs)
+    return AttentionPlan(q_lens, kv_lens, tabs[0], tabs[-1])
 
 
 class _SegmentAttentionFn(torch.autograd.Function):
@@ -104,7 +105,7 @@ class _SegmentAttentionFn(torch.autograd.Function):
         return out
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
+    @_lib.once_differentiable
     def backward(ctx, d_out):
         *operands, out, lse, out_lo = ctx.saved_tensors
         need = ctx.needs_input_grad
@@ -140,7 +141,7 @@ class _HeadNormRopeFn(torch.autograd.Function):
         return _lib.head_norm_rope_fwd(q, k, wq, wk, pos, rotary_dim, eps, base)
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
+    @_lib.once_differentiable
     def backward(ctx, dyq, dyk):
         q, k, wq, wk, pos = ctx.saved_tensors
         return _lib.head_norm_rope_bwd_checked(q, k, wq, wk, pos, *ctx.opts, dyq, dyk) + (None,) * 4

@@ -140,7 +140,7 @@ class _TokenRowsFn(torch.autograd.Function):
         return x.view_as(x)
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
+    @_lib.once_differentiable
     def backward(ctx, dx):
         idx, = ctx.saved_tensors
         return None, _lib.readout(dx.index_select(0, idx), None, 0, False), None
@@ -156,7 +156,7 @@ class _PickRowsFn(torch.autograd.Function):
         return x.index_select(0, idx)
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
+    @_lib.once_differentiable
     def backward(ctx, dy):
         idx, = ctx.saved_tensors
         return _lib.rows_scatter_add(dy.new_zeros(ctx.shape), idx, dy), None

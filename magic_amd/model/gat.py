@@ -226,7 +226,7 @@ class _LinearAct8Fn(torch.autograd.Function):
         return y
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
+    @_lib.once_differentiable
     def backward(ctx, dy):
         codes, exps, w = ctx.saved_tensors
         dy = _lib.full_rows(dy)
@@ -247,6 +247,22 @@ def linear_nobias(x: torch.Tensor, w: torch.Tensor, act_bits: int = 32) -> torch
     if x.device != w.device:
         raise _lib.MagicHipError(f"x on {x.device}, w on {w.device}")
     return _LinearAct8Fn.apply(x, w)
+
+
+class _KeepFn(torch.autograd.Function):
+    """Dropout by a given uint8 keep mask, which is all that is held for the backward pass."""
+
+    @staticmethod
+    def forward(ctx, x, mask, scale):
+        ctx.save_for_backward(mask)
+        ctx.scale = scale
+        return x * mask * scale
+
+    @staticmethod
+    @_lib.once_differentiable
+    def backward(ctx, dy):
+        mask, = ctx.saved_tensors
+        return dy * mask * ctx.scale, None, None
 
 
 class GATConv(nn.Module):
@@ -360,7 +376,7 @@ class GATConv(nn.Module):
         Dp = _pad_head_dim(D)
         C = H * Dp
         struct = graph.structure.ensure_csr()
-        h = self.feat_drop(feat) if drop is None else feat * (drop[0].to(feat.dtype) * drop[1])     # gat.py:283
+        h = self.feat_drop(feat) if drop is None else _KeepFn.apply(feat, *drop)     # gat.py:283
         res_identity = isinstance(self.res_fc, nn.Identity)
         if res_identity and Dp != D:
             raise _lib.MagicHipError("identity residual with a padded head width is not supported")
