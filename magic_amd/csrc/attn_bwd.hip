@@ -27,6 +27,7 @@ struct BwdArgs {
     double *slope_part; // [n_q tiles][q_heads] or NULL
     int64_t items;
     int sub;            // blocks that share a 128-row tile of the table
+    bool hold;          // scaled launches: the forward pass's scores may be others (at_most)
     bool make_delta;    // the dq sweep forms lse2 and delta (no pass before it needs them)
     uint32_t sweep_blocks;   // of the dk / dv sweep; blocks behind them: d slope of one head each, from n_slope sums
     int64_t n_slope;
@@ -172,16 +173,20 @@ struct SlopeSums {
     double dl_dist = 0.0, dl = 0.0, pd = 0.0;
 };
 
-// No logit is above the row's log-sum.  One recomputed from other planes than the forward pass took, or in another order,
-// can be (by 2^-22 of its products' size): with logits of millions its probability would be no fp16 number.
-// (v_minimum3_f32: a NaN stays one)
-__device__ __forceinline__ float at_most(float x, float top) { return __builtin_elementwise_minimum(x, top); }
+// No logit is above the row's log-sum.  A float32 one recomputed from other planes than the forward pass took can be (by 2^-22
+// of its products' size): with logits of millions its probability would be no fp16 number.  HOLD takes it down to the sum
+// (v_minimum3_f32: a NaN stays one) wherever the two passes' planes may differ; elsewhere the scores are the same bits, from
+// one order of the products: 4 % of the sweep over the keys.
+template <bool HOLD> __device__ __forceinline__ float at_most(float x, float top) {
+    return HOLD ? __builtin_elementwise_minimum(x, top) : x;
+}
 
 // Scores and do.v of 32 keys by 32 rows -> gradients of the scores (before the scale of dq); km, kp: the keys' masks
 // (0 / -inf) and positions, four for every group of registers
 template <typename M, bool CAP, bool BIAS, bool MASK>
 __device__ __forceinline__ void score_grad(f32x16_t &s, const f32x16_t &dp, const RowSide &c, const Cap<M::N == 1> &cap,
                                            const f32x4_t *km, const i32x4_t *kp, float (&ds)[16], SlopeSums &sums) {
+#pragma clang fp contract(off)      // (a logit is rounded once, for its row's maximum and for its probability alike)
     if (CAP) cap_tile(s, cap);
     float t_dsl = 0.f, t_dl = 0.f, t_pd = 0.f;
 #pragma unroll
@@ -199,7 +204,7 @@ __device__ __forceinline__ void score_grad(f32x16_t &s, const f32x16_t &dp, cons
                 dist = dist_of((uint32_t)pos[e], c.pos);
                 x = fmaf(-c.slope, dist, x);
             }
-            const float pr = __builtin_amdgcn_exp2f(at_most(x, c.lse) + base[e]);
+            const float pr = __builtin_amdgcn_exp2f(at_most<(M::N > 1)>(x, c.lse) + base[e]);
             const float dl = pr * fmaf(dp[r], c.dp_in, -c.delta);
             if (BIAS) {
                 t_dsl = fmaf(dl, dist, t_dsl);
@@ -214,9 +219,10 @@ __device__ __forceinline__ void score_grad(f32x16_t &s, const f32x16_t &dp, cons
 
 // The same with the keys in the lanes: probabilities (times 2^14 in the scaled mode) and score gradients, both still without
 // the row's `rest`; l, d: minus lse2 and minus D of the rows, qp their positions
-template <typename M, bool CAP, bool BIAS>
+template <typename M, bool HOLD, bool CAP, bool BIAS>
 __device__ __forceinline__ void prob_grad(f32x16_t &s, const f32x16_t &dp, const RowSide &c, const Cap<M::N == 1> &cap,
                                           const f32x4_t *l, const f32x4_t *d, const i32x4_t *qp, float (&pr)[16], float (&ds)[16]) {
+#pragma clang fp contract(off)      // (a logit is rounded once, for its row's maximum and for its probability alike)
     if (CAP) cap_tile(s, cap);
 #pragma unroll
     for (int g = 0; g < 4; ++g) {
@@ -229,7 +235,7 @@ __device__ __forceinline__ void prob_grad(f32x16_t &s, const f32x16_t &dp, const
             float x = CAP ? s[r] : s[r] * c.s_in;
             const float f = CAP ? fmaf(x * x, c.f_cap, c.scale) : c.scale;
             if (BIAS) x = fmaf(-c.slope, dist_of((uint32_t)pos[e], c.pos), x);
-            const float q = __builtin_amdgcn_exp2f(at_most(x, -l4[e]) + l4[e]);
+            const float q = __builtin_amdgcn_exp2f(at_most<HOLD>(x, -l4[e]) + l4[e]);
             pr[r] = M::SCALED ? q * 16384.f : q;
             ds[r] = q * fmaf(dp[r], c.dp_in, d4[e]) * f;
         }
@@ -545,7 +551,7 @@ template <typename T> __global__ __launch_bounds__(256) void k_attn_dq_join(BwdA
 }
 
 // WM groups of 32 keys, KG groups of 32 NB rows of a staged tile.  The blocks behind the sweep's add up the slopes' sums.
-template <typename M, int DP, int WM, int KG, int NB>
+template <typename M, int DP, int WM, int KG, int NB, bool HOLD>
 __global__ __launch_bounds__(64 * WM *KG, DP == 128 || (DP >= 64 && KG > 1) ? 1 : 2) void k_attn_dkv(BwdArgs p) {
     typedef typename M::T T;
     typedef typename M::vec vec;
@@ -674,9 +680,9 @@ __global__ __launch_bounds__(64 * WM *KG, DP == 128 || (DP >= 64 && KG > 1) ? 1 
             const f32x4_t *d4 = reinterpret_cast<const f32x4_t *>(sD + 32 * b + 4 * hf);
             const i32x4_t *qp = reinterpret_cast<const i32x4_t *>(sPos + 32 * b + 4 * hf);
             if (a.cap > 0.f)
-                bias ? prob_grad<M, true, true>(s, dp, ks, cap, l4, d4, qp, pr, ds) : prob_grad<M, true, false>(s, dp, ks, cap, l4, d4, qp, pr, ds);
+                bias ? prob_grad<M, HOLD, true, true>(s, dp, ks, cap, l4, d4, qp, pr, ds) : prob_grad<M, HOLD, true, false>(s, dp, ks, cap, l4, d4, qp, pr, ds);
             else
-                bias ? prob_grad<M, false, true>(s, dp, ks, cap, l4, d4, qp, pr, ds) : prob_grad<M, false, false>(s, dp, ks, cap, l4, d4, qp, pr, ds);
+                bias ? prob_grad<M, HOLD, false, true>(s, dp, ks, cap, l4, d4, qp, pr, ds) : prob_grad<M, HOLD, false, false>(s, dp, ks, cap, l4, d4, qp, pr, ds);
             if (!M::SCALED && far) {
                 const f32x4_t *z4 = reinterpret_cast<const f32x4_t *>(sZ + 32 * b + 4 * hf);
 #pragma unroll
@@ -821,17 +827,17 @@ template <typename M, int DP, int WM, int KG> int run_dq(BwdArgs &b, hipStream_t
     return magic::launch_status();
 }
 
-template <typename M, int DP, int WM, int KG, int NB> int run_dkv(BwdArgs &b, int slope_heads, hipStream_t st) {
+template <typename M, int DP, int WM, int KG, int NB, bool HOLD = (M::N > 1)> int run_dkv(BwdArgs &b, int slope_heads, hipStream_t st) {
     constexpr int BQ = 32 * KG * NB;
     size_t lds = 2 * Tile<M, DP, BQ>::BYTES + BQ * 16 + 8;
     const size_t join = (size_t)32 * WM * (2 * ((DP + 31) / 32 * 32) + 1) * 4;
     if (KG > 1 && lds < join) lds = join;
-    if (magic::ensure_dynamic_lds((const void *)k_attn_dkv<M, DP, WM, KG, NB>, lds) != MAGIC_OK) return MAGIC_ERR_RUNTIME;
+    if (magic::ensure_dynamic_lds((const void *)k_attn_dkv<M, DP, WM, KG, NB, HOLD>, lds) != MAGIC_OK) return MAGIC_ERR_RUNTIME;
     b.items = (int64_t)b.a.n_k_tiles * b.sub * b.a.kv_heads * b.n_split;
     const int64_t grid = xcd_grid(b.items, 16);
     if (grid + slope_heads > 0x7fffffffLL) return MAGIC_ERR_UNSUPPORTED;
     b.sweep_blocks = (uint32_t)grid;
-    MAGIC_LAUNCH(M::SCALED ? "attn_bwd_dkv_f16x2" : "attn_bwd_dkv", (k_attn_dkv<M, DP, WM, KG, NB>), (int)grid + slope_heads,
+    MAGIC_LAUNCH(M::SCALED ? "attn_bwd_dkv_f16x2" : "attn_bwd_dkv", (k_attn_dkv<M, DP, WM, KG, NB, HOLD>), (int)grid + slope_heads,
                  64 * WM * KG, lds, st, b);
     return magic::launch_status();
 }
@@ -880,7 +886,7 @@ template <typename M, int DP> int sweeps(BwdArgs &b, bool last, hipStream_t st) 
         b.sub = 1;
         constexpr int NB = DP == 128 && M::N == 1 ? 2 : 1;  // (one more block of rows a step where registers allow it)
         if constexpr (M::SCALED) {
-            rc = run_dkv<M, DP, 4, 1, NB>(b, slopes, st);
+            rc = b.hold ? run_dkv<M, DP, 4, 1, NB, true>(b, slopes, st) : run_dkv<M, DP, 4, 1, NB, false>(b, slopes, st);
         } else {
             const bool few = !b.pr.rg.q && b.n_split == 1 && small_side(full, (int64_t)full.n_k_tiles * full.kv_heads);
             if (few) b.sub = sub_tiles(full, full.n_k_tiles, full.kv_heads, full.max_k);
@@ -979,6 +985,7 @@ int magic_attn_bwd(const magic_attn *a, const void *out, int64_t ld_out, int64_t
     if (!d_slopes) b.slope_part = nullptr;
     const bool f32 = a->dtype == MAGIC_F32;
     int rc = MAGIC_OK;
+    b.hold = !fwd_scores_f16(a);
     b.make_delta = dq && !f16;      // (the planes of the scaled launches are zero where lse2 says so: they need it before)
     if (a->n_q > 0 && !b.make_delta) rc = f32 ? delta_of<float>(b, stream) : delta_of<bf16_t>(b, stream);
     if (rc != MAGIC_OK) return rc;

@@ -452,6 +452,7 @@ struct GradRows {
     const float *lse, *rest;
 };
 bool use_f16(const magic_attn *a);                                 // whether F16x2 is tried for a call
+bool fwd_scores_f16(const magic_attn *a);                          // whether its forward pass takes the scores that way too, scaled as here
 bool use_gather(const magic_attn *a);                              // whether unmasked keys are gathered
 size_t prepare_bytes(const magic_attn *a, bool f16, bool backward);   // workspace of prepare
 // ranges and planes (k, v, and in backward q and the output's gradient) where f16; unmasked keys

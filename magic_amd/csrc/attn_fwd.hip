@@ -362,6 +362,7 @@ template <typename T> __device__ __forceinline__ void store_out(const FwdArgs &p
 // WM groups of 32 columns (rows, or rows x heads of one key head), KG groups of KW keys: a block of WM * KG wavefronts
 template <typename M, int DP, int WM, int KG, int KW>
 __global__ __launch_bounds__(64 * WM *KG, DP == 128 && (M::N > 1 || WM == 1) ? 1 : 2) void k_attn_fwd(FwdArgs p) {
+#pragma clang fp contract(off)      // (a logit is rounded once, for its row's maximum and for its probability alike)
     typedef typename M::T T;
     typedef typename M::vec vec;
     constexpr int NP = M::N, KS = DP / 16, DB = (DP + 31) / 32, BK = KG * KW, NT = 64 * WM * KG, KB = KW / 32;
@@ -668,6 +669,7 @@ template <int LPR> __device__ __forceinline__ float lanes_sum(float x) {
 // A matrix tile would split 64 float32 keys into planes for one column of thirty-two: 75 us against 36 us for twelve rows
 // over twelve stored graphs of 8,000 nodes (4 heads of 64; 199 MB, 5.5 TB/s).
 template <typename T, int DP, int NC> __global__ __launch_bounds__(256) void k_attn_few(FwdArgs p) {
+#pragma clang fp contract(off)      // (a logit is rounded once, for its row's maximum and for its probability alike)
     constexpr int EPL = 16 / (int)sizeof(T), LPR = DP / EPL, GPB = 256 / LPR, U = 4;
     typedef typename magic::vec_of<T, EPL>::type vt;
     __shared__ float sm[GPB][NC], sl[GPB][NC], so[GPB * NC * DP];
@@ -909,13 +911,14 @@ int64_t ranges(int64_t blocks, int64_t slots, int64_t most) {
 }
 
 // How a call is cut: 128 rows of one head a block (wm 4), or 32 (row, head) columns with the keys dealt to its wavefronts
-// (wm 1), or up to four columns without matrix instructions (wm 0); then key ranges until there are enough blocks.
+// (wm 1), or up to four columns without matrix instructions (wm 0; not for bfloat16 training, whose backward pass takes the
+// scores of the matrix instructions to be the forward pass's); then key ranges until there are enough blocks.
 Shape shape_of(const magic_attn *a) {
     Shape s;
     const int G = a->q_heads / a->kv_heads;
     const int64_t big = (int64_t)a->n_q_tiles * a->q_heads;
     s.wm = big > few_tiles(a) && a->max_q > 32 ? 4 : 1;
-    if ((int64_t)a->max_q * G <= FEW) {
+    if ((int64_t)a->max_q * G <= FEW && !a->out_lo) {
         s.wm = 0, s.gc = G, s.rows = a->max_q > 0 ? a->max_q : 1, s.cols = s.rows * G, s.sub = 1, s.n_hb = a->kv_heads;
         s.f16 = false;
         const int64_t blocks = (int64_t)a->n_q_tiles * s.n_hb, most = (a->max_k + 255) / 256;
@@ -948,6 +951,12 @@ Shape shape_of(const magic_attn *a) {
     s.f16 = magic::attn::use_f16(a) && s.wm == 4 && a->n_k > 0;
     return s;
 }
+
+}  // namespace
+
+bool magic::attn::fwd_scores_f16(const magic_attn *a) { return a->n_q_tiles > 0 && shape_of(a).f16 && a->q_heads == a->kv_heads; }
+
+namespace {
 
 template <typename M, int DP, int WM, int KG, int KW> int launch(FwdArgs &p, hipStream_t st) {
     typedef Tile<M, DP, KG * KW> tile;

@@ -23,7 +23,7 @@ def _close(got, want, mag, n=8):
 
 # rows, keys, heads, width: two scaled planes, blocks of 32 rows, columns without tiles, three planes, narrow heads
 SHAPES = {"planes": ([700, 30], [700, 41], 16, 64), "narrow_planes": ([2100], [2100], 16, 16), "small": ([50], [70], 4, 64),
-          "few": ([1, 3], [700, 1100], 1, 32), "wide": ([300], [300], 8, 128), "ranges": ([1300], [1300], 2, 64)}
+          "whole_tiles": ([640], [640], 16, 64), "whole_tiles_of_one": ([64], [128], 4, 128), "few": ([1, 3], [700, 1100], 1, 32), "wide": ([300], [300], 8, 128), "ranges": ([1300], [1300], 2, 64)}
 
 
 def _ahead(cuda, q_lens, kv_lens, h, D, dtype, far, kind):
