@@ -200,3 +200,20 @@ def test_bfloat16_outputs_where_low_parts_of_probabilities_are_taken(cuda, nq, n
         tol = (ep + r * r + (nk + 16) * U) * (p @ V.abs()) + r * out.abs()
         err = (got[:, h] - out).abs()
         assert (err <= tol).all(), (h, float((err / tol).max()))
+
+
+@pytest.mark.parametrize("far", [1e6, 1e8])
+@pytest.mark.parametrize("shape,dtype", [(s, torch.float32) for s in ("planes", "narrow_planes", "small", "whole_tiles", "whole_tiles_of_one", "wide")]
+                         + [(s, torch.bfloat16) for s in SHAPES], ids=str)
+def test_both_passes_take_large_scores_for_the_same_numbers(cuda, shape, dtype, far):
+    """Where the two passes split their operands alike (bfloat16, and these float32 shapes), a score is the same bits in both,
+    and p = 1 in the gradients of a key that is ahead by its scores too."""
+    q_lens, kv_lens, h, D = SHAPES[shape]
+    if dtype == torch.bfloat16:
+        q_lens, kv_lens = q_lens[:1], [min(kv_lens[0], 60)]
+    q, k, v, d, opts, win = _ahead(cuda, q_lens, kv_lens, h, D, dtype, far, "scores")
+    got = run(q, k, v, d, q_lens, kv_lens, **opts)
+    dv, mag = torch.zeros_like(v, dtype=torch.float64), torch.zeros_like(v, dtype=torch.float64)
+    dv.index_add_(0, win, d.double())
+    mag.index_add_(0, win, d.double().abs())
+    _close(got["dv"], dv, mag, n=max(q_lens))
