@@ -186,7 +186,7 @@ def test_single_rows_and_heads_of_any_stride(cuda, shape, strides, dtype):
 
 @pytest.mark.parametrize("nq,nk,hq,hk,D", [(3, 5000, 16, 4, 128), (40, 900, 4, 2, 64), (500, 500, 8, 8, 16), (2000, 700, 4, 4, 32)])
 def test_bfloat16_outputs_where_low_parts_of_probabilities_are_taken(cuda, nq, nk, hq, hk, D):
-    """Few rows and narrow heads: what is left of a probability's rounding is the square of half a step, so that an output is
+    """Blocks of few rows: what is left of a probability's rounding is the square of half a step, so that an output is
     off by its own rounding and the float32 chain: where the sum nearly cancels, by next to nothing.  (Terms as in
     test_gpu_attention.reference, whose bound holds a whole half step of the probabilities.)"""
     q, k, v, d, _ = make(cuda, [nq], [nk], hq, hk, D, torch.bfloat16, seed=D)
