@@ -543,7 +543,7 @@ __global__ __launch_bounds__(64 * WM *KG, DP == 128 && (M::N > 1 || WM == 1) ? 1
         float tsum = 0.f;
         // What rounding takes from bfloat16 probabilities goes through a second product in blocks of 32 columns, which wait for
         // their keys more than they compute: outputs 1.94e-3 -> 1.66e-3 of their norm off, a rounding of the result alone, and
-        // three rows over 262,147 keys 120 -> 124 us.  (Tiles of 128 rows: 24 wide 279 -> 323 us, 128 wide 1,095 -> 1,470.)
+        // three rows over 262,147 keys 120 -> 124 us.  (Tiles of 128 rows: 24 wide 279 -> 323 us, 128 wide 1,095 -> 1,455.)
         constexpr bool LOW = M::N == 1 && KG > 1;
         vec pf[KB * 2][NP], pl[LOW ? KB * 2 : 1][NP];
 #pragma unroll
