@@ -580,7 +580,7 @@ int magic_knn_merge(int64_t n_query, int32_t k, int32_t n_parts,
  * q [n_q, q_heads, head_dim], k and v [n_k, kv_heads, head_dim]; query head h reads key head
  * h / (q_heads / kv_heads).  Row strides ld_*, head strides hs_*, unit stride along head_dim, rows and heads on 16-byte
  * addresses (out, d_out and the gradients too), row strides at most 2^22 elements, at most 0x7fff0000 rows and 8192
- * heads, cap 0 (none) or 1e-3 to 1e30, scale at most 1e30 in size
+ * heads, cap 0 (none) or 1e-3 to 1e30, scale at most 1e30 in size and 0 or, with a cap, at least 2^-126 of it
  * (head_dim % 8 == 0, at most MAGIC_ATTN_MAX_DIM).  dtype: MAGIC_F32 (products fp32-grade) or
  * MAGIC_BF16 (products of bf16 values, probabilities and score gradients rounded to bf16 before
  * their products; every sum and statistic in fp32).  key_mask [n_k]: 0 = the key takes no part

@@ -32,6 +32,7 @@ int check(const magic_attn *a) {
     if ((a->ld_q | a->hs_q | a->ld_k | a->hs_k | a->ld_v | a->hs_v) % per) return MAGIC_ERR_INVALID_ARG;
     // (scale / cap and cap stay normal float32 numbers)
     if (!(a->cap == 0.f || (a->cap >= 1e-3f && a->cap <= 1e30f)) || !(std::fabs(a->scale) <= 1e30f)) return MAGIC_ERR_INVALID_ARG;
+    if (a->cap > 0.f && a->scale != 0.f && !(std::fabs(a->scale / a->cap) >= 0x1p-126f)) return MAGIC_ERR_INVALID_ARG;
     if (a->slopes && ((a->n_q > 0 && !a->q_pos) || (a->n_k > 0 && !a->k_pos))) return MAGIC_ERR_INVALID_ARG;
     return MAGIC_OK;
 }

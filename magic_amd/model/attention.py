@@ -130,6 +130,8 @@ def segment_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, plan: A
         scale = 1.0 / math.sqrt(q.shape[-1])
     if not abs(scale) <= 1e30:
         raise _lib.MagicHipError(f"scale must be at most 1e30 in size (got {scale})")
+    if cap and scale and abs(scale) < cap * 2.0 ** -126:
+        raise _lib.MagicHipError(f"scale must be at least 2^-126 of the cap (got {scale}, {cap})")
     return _SegmentAttentionFn.apply(q, k, v, slopes, plan, float(scale), float(cap), q_pos, k_pos, key_mask)
 
 

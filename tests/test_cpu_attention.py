@@ -93,3 +93,19 @@ def test_cap_polynomial_is_as_close_to_tanh_as_its_comment_says():
     z = t * t
     poly = k[0] + z * (k[1] + z * (k[2] + z * k[3]))
     assert np.abs(poly * t / np.tanh(t) - 1).max() <= 4.2e-8 and k[0] == 1.0
+
+
+def test_scales_far_below_the_cap_are_refused():
+    """scale / cap would be no normal float32 number: capped scores lose bits."""
+    import ctypes as C
+
+    from magic_amd import _lib
+    from magic_amd.model.attention import attention_plan, segment_attention
+    a = _lib.MagicAttn()
+    a.dtype, a.q_heads, a.kv_heads, a.head_dim = 0, 4, 2, 64
+    for cap, scale, want in ((1e30, 1e-7, 0), (1e30, 1e-9, -1), (1e30, 0.0, 0), (0.0, 1e-38, 0), (50.0, 1e-36, 0), (50.0, 1e-37, -1)):      # (1e-36 / 50 = 2e-38, 2^-126 = 1.2e-38)
+        a.cap, a.scale = cap, scale
+        assert _lib.load().magic_attn_fwd(C.byref(a), None, 0, 0, None, None, 0, None) == want, (cap, scale)
+    x = torch.randn(4, 2, 16)
+    with pytest.raises(_lib.MagicHipError, match="of the cap"):
+        segment_attention(x, x, x, attention_plan([4], device="cpu"), cap=1e30, scale=1e-9)

@@ -185,6 +185,7 @@ int main() {
     EXPECT(attn([](magic_attn &b) { b.cap = -1.f; }), MAGIC_ERR_INVALID_ARG);
     EXPECT(attn([](magic_attn &b) { b.cap = 1e-9f; }), MAGIC_ERR_INVALID_ARG);
     EXPECT(attn([](magic_attn &b) { b.scale = INFINITY; }), MAGIC_ERR_INVALID_ARG);
+    EXPECT(attn([](magic_attn &b) { b.cap = 1e30f, b.scale = 1e-9f; }), MAGIC_ERR_INVALID_ARG);
     EXPECT(attn([&](magic_attn &b) { b.slopes = dummy; }), MAGIC_ERR_INVALID_ARG);  // no positions
     EXPECT(magic_attn_bwd(&at, dummy, 64, 16, lse, dummy, 64, 16, dummy, dummy, nullptr, nullptr, nullptr, 0, nullptr),
            MAGIC_ERR_INVALID_ARG);  // dk without dv
