@@ -603,9 +603,9 @@ __global__ __launch_bounds__(64 * WM *KG, DP == 128 || (DP >= 64 && KG > 1) ? 1 
     const bool bias = a.slopes != nullptr;
     const uint32_t kpos = bias ? flip(a.k_pos[kr]) : 0u;
     const float f_cap = a.cap > 0.f ? -a.scale / a.cap / a.cap * (1.f / (LOG2E * LOG2E)) : 0.f;
-    // Without `rest` a row's probabilities are off by up to |lse2| 2^-24: below that size it is left out.  (The scaled mode has
+    // Without `rest` a row's probabilities are off by up to |lse2| 2^-23: up to this size it is left out.  (The scaled mode has
     // it in the rows of the gradient.)
-    constexpr float FAR = M::N == 1 ? 256.f : 4.f;
+    constexpr float FAR = M::N == 1 ? 256.f : 1.f;
     const Cap<M::N == 1> cap(sc.s_in, a.cap);
     Running run;
     f32x16_t gk[DB], gv[DB];
