@@ -4,9 +4,9 @@
 // Two sweeps, so that every sum has one owner and a fixed order (no atomics): dq with the rows' wavefronts walking the
 // keys (three products), dk and dv with the keys' wavefronts walking the rows of all heads that share them (four).
 // Seven products instead of the five that one sweep with atomic adds would need.
-// Bound like the forward pass.  Twelve graphs of 8,000 nodes, 4 heads of 64, float32: dq 4.2 ms (289 TFLOP/s of its three
-// products), dk and dv 4.8 ms (338); bfloat16, 8 heads of 128 over 2, capped, half the keys masked: 1.54 ms (648) and
-// 2.43 ms (548: 128 accumulators and both operands' rows leave one wavefront a SIMD, which has nothing to put beside its
+// Bound like the forward pass.  Twelve graphs of 8,000 nodes, 4 heads of 64, float32: dq 4.33 ms (280 TFLOP/s of its three
+// products), dk and dv 4.95 ms (328); bfloat16, 8 heads of 128 over 2, capped, half the keys masked: 1.65 ms (605) and
+// 2.60 ms (512: 128 accumulators and both operands' rows leave one wavefront a SIMD, which has nothing to put beside its
 // own waits).
 #include "attn_common.h"
 

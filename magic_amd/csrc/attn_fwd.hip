@@ -5,10 +5,10 @@
 // One pass over the keys with a running maximum and sum per row; scores are formed transposed (keys x rows), so that a
 // lane owns ONE row's statistics and the probabilities feed the second product from their registers (attn_common.h).
 // Bound by the matrix and the vector units together (beside its 4 D flops a score takes some eleven vector instructions:
-// cap, exponential, sums, conversion).  Twelve graphs of 8,000 nodes, 4 heads of 64, float32 with a distance bias: 2.76 ms,
-// 292 TFLOP/s; seven graphs of up to 15,001 nodes, 8 bfloat16 heads of 128 over 2, capped, half the keys masked: 1.10 ms,
-// 605 TFLOP/s of the unmasked products.  Three rows over 262,147 keys, 16 heads of 128 over 4: 117 us + 14 to join the
-// ranges, 4.6 TB/s of keys and values while it sweeps them.
+// cap, exponential, sums, conversion).  Twelve graphs of 8,000 nodes, 4 heads of 64, float32 with a distance bias: 2.85 ms,
+// 283 TFLOP/s; seven graphs of up to 15,001 nodes, 8 bfloat16 heads of 128 over 2, capped, half the keys masked: 1.12 ms,
+// 594 TFLOP/s of the unmasked products.  Three rows over 262,147 keys, 16 heads of 128 over 4: 120 us + 13 to join the
+// ranges, 4.5 TB/s of keys and values while it sweeps them.
 #include "attn_common.h"
 #include <cmath>
 #include <type_traits>
