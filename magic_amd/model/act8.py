@@ -1,7 +1,7 @@
 """Activations kept for the backward pass in 8 bits.
 
-Full-graph training keeps the input of every linear layer until its weight gradient is formed; at the entity-level
-sizes that is most of a step's memory.  ``act8_pack`` stores a float32 matrix as signed 8-bit codes with one
+A linear layer keeps its input until its weight gradient is formed.  Where nothing else keeps that matrix, 8 bits save
+three quarters of its memory.  ``act8_pack`` stores a float32 matrix as signed 8-bit codes with one
 power-of-two scale for every 32 columns of a row (1.03 bytes an element instead of 4), ``act8_unpack`` reads it back,
 and ``linear_nobias(x, w, act_bits=8)`` (``gat.py``) forms its weight gradient from the codes.  The rounding is off by
 at most half a step, 2^-7.98 of a block's largest magnitude at worst.  No counterpart in the reference, which keeps
